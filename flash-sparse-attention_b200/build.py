@@ -28,6 +28,7 @@ SOURCES = [
     "fsa_quant.cu",
     "fsa_topk.cu",
     "fsa_kvcache.cu",
+    "fsa_rotary.cu",
     "fsa_peer.cu",
 ]
 

@@ -300,6 +300,112 @@ class FsaKvAppendArgs(ctypes.Structure):
     ]
 
 
+class FsaRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("q_out", c_void_p),
+        ("k_out", c_void_p),
+        ("cos", c_void_p),
+        ("sin", c_void_p),
+        ("cu_seqlens", c_void_p),
+        ("seqlen_offsets", c_void_p),
+        ("position_ids", c_void_p),
+        ("status", c_void_p),
+        ("q_stride_b", c_int64),
+        ("q_stride_s", c_int64),
+        ("q_stride_h", c_int64),
+        ("k_stride_b", c_int64),
+        ("k_stride_s", c_int64),
+        ("k_stride_h", c_int64),
+        ("q_out_stride_b", c_int64),
+        ("q_out_stride_s", c_int64),
+        ("q_out_stride_h", c_int64),
+        ("k_out_stride_b", c_int64),
+        ("k_out_stride_s", c_int64),
+        ("k_out_stride_h", c_int64),
+        ("position_stride_b", c_int64),
+        ("position_stride_s", c_int64),
+        ("table_stride", c_int64),
+        ("batch", c_int32),
+        ("seqlen", c_int32),
+        ("total", c_int32),
+        ("heads_q", c_int32),
+        ("heads_k", c_int32),
+        ("head_dim", c_int32),
+        ("rotary_dim", c_int32),
+        ("table_rows", c_int32),
+        ("offset", c_int32),
+        ("dtype", c_int32),
+        ("table_dtype", c_int32),
+        ("position_ids_int64", c_int32),
+        ("interleaved", c_int32),
+        ("transposed", c_int32),
+    ]
+
+
+class FsaKvAppendRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p),
+        ("k_new", c_void_p),
+        ("v_new", c_void_p),
+        ("q_out", c_void_p),
+        ("k_cache", c_void_p),
+        ("v_cache", c_void_p),
+        ("cos", c_void_p),
+        ("sin", c_void_p),
+        ("seqused_k", c_void_p),
+        ("page_table", c_void_p),
+        ("free_pages", c_void_p),
+        ("free_count", c_void_p),
+        ("cu_seqlens_new", c_void_p),
+        ("seqlen_offsets", c_void_p),
+        ("q_scale", c_void_p),
+        ("k_scale", c_void_p),
+        ("v_scale", c_void_p),
+        ("place_ws", c_void_p),
+        ("status", c_void_p),
+        ("q_stride_b", c_int64),
+        ("q_stride_s", c_int64),
+        ("q_stride_h", c_int64),
+        ("k_stride_b", c_int64),
+        ("k_stride_s", c_int64),
+        ("k_stride_h", c_int64),
+        ("v_stride_b", c_int64),
+        ("v_stride_s", c_int64),
+        ("v_stride_h", c_int64),
+        ("q_out_stride_b", c_int64),
+        ("q_out_stride_s", c_int64),
+        ("q_out_stride_h", c_int64),
+        ("k_cache_stride_b", c_int64),
+        ("k_cache_stride_s", c_int64),
+        ("k_cache_stride_h", c_int64),
+        ("v_cache_stride_b", c_int64),
+        ("v_cache_stride_s", c_int64),
+        ("v_cache_stride_h", c_int64),
+        ("table_stride", c_int64),
+        ("page_table_stride", c_int64),
+        ("batch", c_int32),
+        ("new_tokens", c_int32),
+        ("total", c_int32),
+        ("heads_q", c_int32),
+        ("heads_kv", c_int32),
+        ("head_dim", c_int32),
+        ("rotary_dim", c_int32),
+        ("table_rows", c_int32),
+        ("offset", c_int32),
+        ("capacity", c_int32),
+        ("page_size", c_int32),
+        ("max_pages", c_int32),
+        ("num_pages", c_int32),
+        ("dtype", c_int32),
+        ("cache_dtype", c_int32),
+        ("table_dtype", c_int32),
+        ("interleaved", c_int32),
+        ("advance", c_int32),
+    ]
+
+
 PEER_MAX_RANKS = 16
 
 
@@ -370,6 +476,10 @@ def load():
     lib.fsa_quantize_fp8_blockwise.argtypes = [POINTER(FsaBlockQuantArgs), c_void_p]
     lib.fsa_kv_append.restype = c_int
     lib.fsa_kv_append.argtypes = [POINTER(FsaKvAppendArgs), c_void_p]
+    lib.fsa_rotary.restype = c_int
+    lib.fsa_rotary.argtypes = [POINTER(FsaRotaryArgs), c_void_p]
+    lib.fsa_kv_append_rotary.restype = c_int
+    lib.fsa_kv_append_rotary.argtypes = [POINTER(FsaKvAppendRotaryArgs), c_void_p]
     lib.fsa_localize_indices.restype = c_int
     lib.fsa_localize_indices.argtypes = [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p]
     lib.fsa_peer_region_bytes.restype = c_int

@@ -488,6 +488,93 @@ typedef struct FsaKvAppendArgs {
 } FsaKvAppendArgs;
 int fsa_kv_append(const FsaKvAppendArgs* args, void* stream);
 
+/*
+ * Rotary positions. For every token at position p and every pair i < rotary_dim / 2 of a head's columns - (i, i +
+ * rotary_dim / 2), or (2i, 2i + 1) when `interleaved` -
+ *   y1 = x1 cos[p, i] - x2 sin[p, i],  y2 = x2 cos[p, i] + x1 sin[p, i];
+ * columns from rotary_dim on are copied. `transposed` turns the other way (the gradient). Angles are held in fp32, results
+ * rounded once. The reference leaves positions to its caller.
+ *   tensors   q, q_out [batch, seqlen, heads_q, head_dim], or [total, heads_q, head_dim] with cu_seqlens (strides in
+ *             elements, head_dim contiguous; _b unused then); k, k_out alike. heads_q or heads_k may be 0.
+ *   tables    cos, sin [table_rows, rotary_dim / 2], rows table_stride apart, fp32 or 16 bits (table_dtype)
+ *   position  place in the sequence + offset + seqlen_offsets[sequence] (optional), or position_ids (optional, int32 or
+ *             int64) as they are
+ * Tokens behind the last sequence come out as zeros; so do tokens whose position is outside the tables, which also set the
+ * status word to 5. q_out may be q and k_out may be k (same strides).
+ */
+typedef struct FsaRotaryArgs {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const void* cos;
+  const void* sin;
+  const int32_t* cu_seqlens;     /* [batch + 1] or null */
+  const int32_t* seqlen_offsets; /* [batch] or null */
+  const void* position_ids;      /* or null */
+  int32_t* status;
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  int64_t q_out_stride_b, q_out_stride_s, q_out_stride_h;
+  int64_t k_out_stride_b, k_out_stride_s, k_out_stride_h;
+  int64_t position_stride_b, position_stride_s;
+  int64_t table_stride;
+  int32_t batch, seqlen, total;
+  int32_t heads_q, heads_k, head_dim, rotary_dim;
+  int32_t table_rows, offset;
+  int32_t dtype, table_dtype;
+  int32_t position_ids_int64, interleaved, transposed;
+} FsaRotaryArgs;
+int fsa_rotary(const FsaRotaryArgs* args, void* stream);
+
+/*
+ * fsa_kv_append with the rotation on the way: the new key rows are turned by the position seqused_k[b] + t + offset +
+ * seqlen_offsets[b], the new value rows copied, the query rows turned alike into q_out (heads_q may be 0). New rows are
+ * [batch, new_tokens, heads, head_dim], or [total, heads, head_dim] with cu_seqlens_new. A cache in FP8 (cache_dtype e4m3 or
+ * e5m2) receives value / *_scale rounded and saturated, and so does q_out.
+ * Missing pages (entries < 0) come off the stack free_pages[0 .. free_count) from its top in the order of sequences and slots.
+ * Rows without room - no page left, a page number outside [0, num_pages), the end of the table or of the cache - are not stored
+ * and set the status word to 3, rows whose position is outside the tables to 5; a sequence keeps the rows in front of the first
+ * such one, and the q_out rows of those that are not stored are zeros. With `advance` seqused_k[b] grows by the rows that were
+ * stored; without, the lengths stay (layers that share them advance once). place_ws: 2 * batch int32, written by this call.
+ */
+typedef struct FsaKvAppendRotaryArgs {
+  const void* q;
+  const void* k_new;
+  const void* v_new;
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  const void* cos;
+  const void* sin;
+  int32_t* seqused_k;
+  int32_t* page_table; /* [batch, max_pages] or null */
+  const int32_t* free_pages;
+  int32_t* free_count;
+  const int32_t* cu_seqlens_new; /* [batch + 1] or null */
+  const int32_t* seqlen_offsets; /* [batch] or null */
+  const float* q_scale;
+  const float* k_scale;
+  const float* v_scale;
+  int32_t* place_ws;
+  int32_t* status;
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  int64_t v_stride_b, v_stride_s, v_stride_h;
+  int64_t q_out_stride_b, q_out_stride_s, q_out_stride_h;
+  int64_t k_cache_stride_b, k_cache_stride_s, k_cache_stride_h; /* paged: _b = page stride */
+  int64_t v_cache_stride_b, v_cache_stride_s, v_cache_stride_h;
+  int64_t table_stride, page_table_stride;
+  int32_t batch, new_tokens, total;
+  int32_t heads_q, heads_kv, head_dim, rotary_dim;
+  int32_t table_rows, offset;
+  int32_t capacity; /* contiguous cache: positions per sequence */
+  int32_t page_size, max_pages, num_pages;
+  int32_t dtype, cache_dtype, table_dtype;
+  int32_t interleaved, advance;
+} FsaKvAppendRotaryArgs;
+int fsa_kv_append_rotary(const FsaKvAppendRotaryArgs* args, void* stream);
+
 /* ---- Peer exchange of decode partials (context-parallel decode over the GPUs of one node) -------------------
  * No counterpart in the reference (it has no multi-GPU code). Every rank owns one region (fsa_peer_alloc: cudaMalloc,
  * so that it can be exported), opens the regions of the others (fsa_peer_open on their handles) and then, per step:
