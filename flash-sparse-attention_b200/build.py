@@ -24,6 +24,7 @@ SOURCES = [
     "fsa_fwd_sm100.cu",
     "fsa_bwd_sm100.cu",
     "fsa_dec_sm100.cu",
+    "fsa_prefix_sm100.cu",
     "fsa_static_scratch.cu",
     "fsa_quant.cu",
     "fsa_topk.cu",

@@ -1,5 +1,6 @@
 // Parameter blocks and launchers of the helper kernels (internal).
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include "fsa_params.h"
@@ -103,6 +104,26 @@ struct GateExtParams {
   int B, Hq, Hkv, G, gpack, hgrid, sq, sk, num_m_blocks, n_tiles_k, page_size, pt_stride;
   unsigned flags;  // F_VARLEN_* | F_USED_* | F_PAGED
 };
+// Decode over a prefix that all sequences share: what the prefix kernel and the merge behind it take.
+struct alignas(64) PrefixParams {
+  CUtensorMap map_k, map_v;
+  const void* q;         // [B, Hq, D]
+  const int* used;       // optional [1]: keys of the prefix
+  const int* page_table; // optional [max_pages]
+  void* out;             // [B, Hq, D]
+  float* lse;            // [B, Hq]
+  float* out_partial;    // [slots + splits, B, Hq, D]: pieces of the prefix (two slots each), splits of the sequences' own keys
+  float* lse_partial;    // [slots + splits, Hq, B] base 2
+  int* status;
+  long long q_sb, q_sh, o_sb, o_sh, l_sb, l_sh, op_ss, lp_ss;
+  int B, Hq, Hkv, G, D;
+  int rows, q_tiles;     // of a KV head: B * G, and tiles of 128 of them
+  int keys;              // capacity of the prefix
+  int page_size, num_pages;
+  int ctas, slots, splits;
+  float scale_log2;
+};
+cudaError_t launch_prefix(const PrefixParams& p, int dtype, int head_dim, cudaStream_t stream);
 cudaError_t launch_gate_ext(const GateExtParams& p, int dtype, cudaStream_t stream);
 cudaError_t launch_dq_order(const DqOrderParams& p, cudaStream_t stream);
 cudaError_t launch_flat_sum(const FlatSumParams& p, int dtype, cudaStream_t stream);

@@ -11,6 +11,7 @@ from flash_sparse_attn.ops.triton.interface import (  # noqa: F401
     flash_dense_attn_varlen_func,
     flash_dense_attn_varlen_with_kvcache_func,
     flash_dense_attn_with_kvcache_func,
+    flash_dense_attn_with_shared_prefix_func,
     flash_gated_attn_func,
     flash_gated_attn_varlen_func,
     flash_gated_attn_varlen_with_kvcache_func,

@@ -406,6 +406,35 @@ class FsaKvAppendRotaryArgs(ctypes.Structure):
     ]
 
 
+class FsaSharedPrefixArgs(ctypes.Structure):
+    _fields_ = [
+        ("decode", c_void_p),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("seqused", c_void_p),
+        ("page_table", c_void_p),
+        ("out_partial", c_void_p),
+        ("lse_partial", c_void_p),
+        ("k_stride_p", c_int64),
+        ("k_stride_s", c_int64),
+        ("k_stride_h", c_int64),
+        ("v_stride_p", c_int64),
+        ("v_stride_s", c_int64),
+        ("v_stride_h", c_int64),
+        ("seqlen", c_int32),
+        ("num_pages", c_int32),
+        ("page_size", c_int32),
+        ("max_pages", c_int32),
+    ]
+
+
+class FsaSharedPrefixWorkspace(ctypes.Structure):
+    _fields_ = [
+        ("out_partial", c_size_t),
+        ("lse_partial", c_size_t),
+    ]
+
+
 PEER_MAX_RANKS = 16
 
 
@@ -476,6 +505,10 @@ def load():
     lib.fsa_quantize_fp8_blockwise.argtypes = [POINTER(FsaBlockQuantArgs), c_void_p]
     lib.fsa_kv_append.restype = c_int
     lib.fsa_kv_append.argtypes = [POINTER(FsaKvAppendArgs), c_void_p]
+    lib.fsa_shared_prefix_workspace_bytes.restype = c_int
+    lib.fsa_shared_prefix_workspace_bytes.argtypes = [POINTER(FsaSharedPrefixArgs), POINTER(FsaSharedPrefixWorkspace)]
+    lib.fsa_decode_shared_prefix.restype = c_int
+    lib.fsa_decode_shared_prefix.argtypes = [POINTER(FsaSharedPrefixArgs), c_void_p]
     lib.fsa_rotary.restype = c_int
     lib.fsa_rotary.argtypes = [POINTER(FsaRotaryArgs), c_void_p]
     lib.fsa_kv_append_rotary.restype = c_int

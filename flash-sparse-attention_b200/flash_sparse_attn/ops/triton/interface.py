@@ -18,6 +18,7 @@ from flash_sparse_attn.ops.triton import quant
 from flash_sparse_attn.ops.triton.flash_bwd import attn_backward
 from flash_sparse_attn.ops.triton.flash_dec import attn_decode
 from flash_sparse_attn.ops.triton.flash_fwd import attn_forward
+from flash_sparse_attn.ops.triton.flash_prefix import attn_decode_shared_prefix
 from flash_sparse_attn.ops.triton.utils import ensure_contiguous
 
 _Out = Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]
@@ -505,6 +506,38 @@ def flash_dense_attn_varlen_with_kvcache_func(
     return _decode("dense", query, key, value, None, None, cu_seqlens_k, max_seqlen_k, softmax_scale, query_scale,
                    key_scale, value_scale, window_sizes, None, None, True, is_local, is_quant, num_splits, None,
                    gather_kv_indices, seqused_k, out, lse, is_autotune, tile_mn, skip_checks, return_lse)
+
+
+def flash_dense_attn_with_shared_prefix_func(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    prefix_key: torch.Tensor,
+    prefix_value: torch.Tensor,
+    softmax_scale: Optional[float] = None,
+    num_splits: Optional[int] = None,
+    page_table: Optional[torch.Tensor] = None,
+    seqused_k: Optional[torch.Tensor] = None,
+    prefix_page_table: Optional[torch.Tensor] = None,
+    prefix_seqused: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+    skip_checks: bool = False,
+    return_lse: bool = False,
+) -> _Out:
+    """Dense decode for a batch whose sequences begin with the same keys: ``query [B, Hq, D]`` attends to the prefix
+    ``prefix_key/value [P, Hkv, D]`` and to its sequence's own ``key/value [B, Sk, Hkv, D]`` (``seqused_k [B]`` of them, possibly
+    none). The prefix is read once for the whole batch, not once per sequence; the result is that of
+    ``flash_dense_attn_with_kvcache_func`` on the concatenated keys.
+
+    Paged caches: own keys as pages ``[num_pages, page, Hkv, D]`` + ``page_table [B, max_pages]``, the prefix as pages (of the same pool or
+    another) + ``prefix_page_table [prefix_pages]``; ``prefix_seqused`` (int32, one element) says how many of the prefix's positions
+    count. bf16 / fp16, ``head_dim`` a multiple of 16 up to 128. ``num_splits`` concerns the own keys. A row without any key is 0 with
+    log-sum-exp ``-inf``. Returns ``out [B, Hq, D]`` or ``(out, lse [B, Hq])``; the reference has no such operator."""
+    out, lse = attn_decode_shared_prefix(
+        query, key, value, prefix_key, prefix_value, softmax_scale=softmax_scale, num_splits=num_splits, page_table=page_table,
+        seqused_k=seqused_k, prefix_page_table=prefix_page_table, prefix_seqused=prefix_seqused, out=out, lse=lse, skip_checks=skip_checks)
+    return (out, lse) if return_lse else out
 
 
 def flash_sparse_attn_with_kvcache_func(

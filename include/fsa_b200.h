@@ -332,6 +332,37 @@ int fsa_combine(const float* out_partial, const float* lse_partial, void* out, f
                 int64_t lse_partial_stride, void* stream);
 
 /*
+ * Decode for a batch whose sequences share a prefix: every query attends to the prefix and to its sequence's own keys; the
+ * prefix's keys are read once for the whole batch (tensor-core products of all queries of a KV head with them), the own keys by
+ * fsa_decode, and the partial results are merged. The reference has no such operator.
+ *   decode   query, own keys (contiguous, packed or paged, with seqused_k / cu_seqlens_k as for fsa_decode), out, lse, sizes,
+ *            softmax_scale (> 0), num_splits, status. Dense kind, bf16 / fp16, head_dim a multiple of 8 up to 128, no windows, gathered
+ *            positions or peers; out_partial, lse_partial and partial_only are ignored. seqlen_k may be 0: no own keys.
+ *   k, v     prefix [seqlen, heads_kv, head_dim], or pages [num_pages, page_size, heads_kv, head_dim] with page_table [max_pages]
+ *            (page_size 32, 64, 128 or 256; a page outside the pool that holds keys sets the status word to 3)
+ *   seqused  optional, device: keys of the prefix that count (at most the capacity)
+ *   out_partial, lse_partial   workspaces of fsa_shared_prefix_workspace_bytes()
+ * A row without any key: out 0, lse -inf.
+ */
+typedef struct FsaSharedPrefixArgs {
+  const FsaDecArgs* decode;
+  const void* k;
+  const void* v;
+  const int32_t* seqused;
+  const int32_t* page_table;
+  float* out_partial;
+  float* lse_partial;
+  int64_t k_stride_p, k_stride_s, k_stride_h; /* paged: _p = page stride */
+  int64_t v_stride_p, v_stride_s, v_stride_h;
+  int32_t seqlen, num_pages, page_size, max_pages;
+} FsaSharedPrefixArgs;
+typedef struct FsaSharedPrefixWorkspace {
+  size_t out_partial, lse_partial;
+} FsaSharedPrefixWorkspace;
+int fsa_shared_prefix_workspace_bytes(const FsaSharedPrefixArgs* args, FsaSharedPrefixWorkspace* sizes);
+int fsa_decode_shared_prefix(const FsaSharedPrefixArgs* args, void* stream);
+
+/*
  * Split-KV decode without any caller-provided (or freshly allocated) workspace. This entry point has
  * no counterpart in the reference, whose launcher allocates its partial buffers with torch.empty on
  * every call (flash_sparse_attn/ops/triton/flash_sparse_dec.py:637-646).
