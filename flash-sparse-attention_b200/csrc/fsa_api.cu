@@ -900,107 +900,106 @@ int fsa_decode(const FsaDecArgs* a, void* stream_) {
   return FSA_OK;
 }
 
-// How a call over a shared prefix is cut: CTAs and partial results. The number of CTAs a KV head's items are shared out to follows
-// from the prefix's length, which may be known on the device only; the bound on the pieces of an item does not depend on it.
+// Sizes of a call over a shared prefix, and how it is cut.
 static int prefix_geometry(const FsaSharedPrefixArgs* a, fsa::PrefixParams* p) {
-  const FsaDecArgs* d = a->decode;
-  if (!d || d->batch <= 0 || d->heads_q <= 0 || d->heads_kv <= 0 || d->heads_q % d->heads_kv || !head_dim_ok(d->head_dim)) return FSA_ERR_INVALID_ARG;
-  p->B = d->batch;
-  p->Hq = d->heads_q;
-  p->Hkv = d->heads_kv;
-  p->G = d->heads_q / d->heads_kv;
-  p->D = d->head_dim;
-  if ((long long)p->B * p->G > (1ll << 30)) return FSA_ERR_UNSUPPORTED;
-  p->rows = p->B * p->G;
-  p->q_tiles = cdiv(p->rows, 128);
-  const long long keys = a->page_table ? (long long)a->max_pages * a->page_size : a->seqlen;
-  if (keys < 0 || keys > 0x7fffff00ll) return FSA_ERR_INVALID_ARG;
-  p->keys = (int)keys;
-  const long long work = (long long)p->Hkv * p->q_tiles * ((keys + 127) / 128);
-  const int sms = fsa::device_sm_count();
-  p->ctas = work < sms ? (int)work : sms;
-  const long long weight = p->q_tiles > 1 ? 2 : 1, tiles_per_head = (long long)p->Hkv * p->q_tiles;
-  p->slots = p->ctas > 0 ? 2 * (int)((weight * p->ctas + tiles_per_head - 1) / tiles_per_head + 1) : 0;
-  p->splits = d->seqlen_k > 0 ? (d->num_splits > 0 ? d->num_splits : 1) : 0;
-  p->op_ss = (long long)p->B * p->Hq * p->D;
-  p->lp_ss = (long long)p->B * p->Hq;
+  if (a->batch <= 0 || a->heads_q <= 0 || a->heads_kv <= 0 || a->heads_q % a->heads_kv || !head_dim_ok(a->head_dim)) return FSA_ERR_INVALID_ARG;
+  auto capacity = [](bool paged, int seqlen, int pages, int size, int pool, int* keys) {
+    if (!paged) {
+      *keys = seqlen;
+      return seqlen >= 0 && seqlen <= 0x7fffff00;
+    }
+    if (pages < 0 || pool < 0 || (size != 32 && size != 64 && size != 128 && size != 256)) return false;
+    const long long n = pool > 0 ? (long long)pages * size : 0;
+    *keys = (int)n;
+    return n <= 0x7fffff00ll;
+  };
+  if (!capacity(a->page_table != nullptr, a->seqlen_k, a->max_pages, a->page_size, a->num_pages, &p->own_keys) ||
+      !capacity(a->prefix_page_table != nullptr, a->prefix_seqlen, a->prefix_max_pages, a->prefix_page_size, a->prefix_num_pages, &p->prefix_keys))
+    return FSA_ERR_INVALID_ARG;
+  p->B = a->batch;
+  p->Hq = a->heads_q;
+  p->Hkv = a->heads_kv;
+  p->G = a->heads_q / a->heads_kv;
+  p->D = a->head_dim;
+  if ((long long)p->B * p->Hq > (1ll << 30) || !fsa::prefix_shape(p)) return FSA_ERR_UNSUPPORTED;
   return FSA_OK;
 }
 
 int fsa_shared_prefix_workspace_bytes(const FsaSharedPrefixArgs* a, FsaSharedPrefixWorkspace* w) {
   if (!a || !w) return FSA_ERR_INVALID_ARG;
   memset(w, 0, sizeof(*w));
-  fsa::PrefixParams p = {};
+  fsa::PrefixParams p;
+  memset(&p, 0, sizeof(p));
   const int rc = prefix_geometry(a, &p);
   if (rc != FSA_OK) return rc;
-  w->out_partial = sizeof(float) * (size_t)(p.slots + p.splits) * (size_t)p.op_ss;
-  w->lse_partial = sizeof(float) * (size_t)(p.slots + p.splits) * (size_t)p.lp_ss;
+  w->out_partial = sizeof(float) * (size_t)p.partial_rows * (size_t)p.D;
+  w->lse_partial = sizeof(float) * (((size_t)p.partial_rows + 3) & ~(size_t)3);
+  w->plan_ws = sizeof(int32_t) * (size_t)p.plan_ints;
   return FSA_OK;
 }
 
 int fsa_decode_shared_prefix(const FsaSharedPrefixArgs* a, void* stream_) {
-  if (!a || !a->decode || !a->out_partial || !a->lse_partial) return FSA_ERR_INVALID_ARG;
-  const FsaDecArgs* d = a->decode;
-  if (!d->q || !d->out || !d->lse || !d->status) return FSA_ERR_INVALID_ARG;
-  if (d->kind != FSA_KIND_DENSE || (d->dtype != FSA_DT_BF16 && d->dtype != FSA_DT_FP16) || (d->flags & FSA_F_LOCAL) || d->gather_kv_indices ||
-      d->peers || d->qkv_scale)
-    return FSA_ERR_UNSUPPORTED;
-  if (!(d->softmax_scale > 0.f) || d->softmax_scale > 3.4e38f) return FSA_ERR_INVALID_ARG;
+  if (!a || !a->q || !a->out || !a->lse || !a->status || !a->out_partial || !a->lse_partial || !a->plan_ws) return FSA_ERR_INVALID_ARG;
+  if (a->dtype != FSA_DT_BF16 && a->dtype != FSA_DT_FP16) return FSA_ERR_UNSUPPORTED;
+  if (!(a->softmax_scale > 0.f) || a->softmax_scale > 3.4e38f) return FSA_ERR_INVALID_ARG;
   fsa::PrefixParams p;
   memset(&p, 0, sizeof(p));
   int rc = prefix_geometry(a, &p);
   if (rc != FSA_OK) return rc;
-  if ((reinterpret_cast<uintptr_t>(d->out) & 3) || (d->batch > 1 && d->o_stride_b % 2) || (d->heads_q > 1 && d->o_stride_h % 2))
+  if ((reinterpret_cast<uintptr_t>(a->out) & 3) || (a->batch > 1 && a->o_stride_b % 2) || (a->heads_q > 1 && a->o_stride_h % 2))
     return FSA_ERR_INVALID_ARG;  // rows are written in pieces of 4 bytes
-  if ((reinterpret_cast<uintptr_t>(d->q) & 15) || (d->batch > 1 && d->q_stride_b % 8) || (d->heads_q > 1 && d->q_stride_h % 8))
-    return FSA_ERR_INVALID_ARG;  // and read in pieces of 16
-  const bool paged = a->page_table != nullptr;
-  if (p.keys > 0) {
-    if (!a->k || !a->v) return FSA_ERR_INVALID_ARG;
-    if (paged && (a->num_pages <= 0 || (a->page_size != 32 && a->page_size != 64 && a->page_size != 128 && a->page_size != 256)))
-      return FSA_ERR_INVALID_ARG;
-    const uint64_t D = p.D, H = p.Hkv;
-    auto map = [&](CUtensorMap* m, const void* base, int64_t sp, int64_t ss, int64_t sh) {
-      // (a dimension of one has no stride that matters: one that TMA takes)
-      if (H == 1) sh = D;
-      if (paged) return make_map4(m, d->dtype, base, D, H, sh, (uint64_t)a->page_size, ss, (uint64_t)a->num_pages, a->num_pages > 1 ? sp : 8, 64, 1,
-                                  a->page_size < 128 ? a->page_size : 128);
-      return make_map4(m, d->dtype, base, D, H, sh, (uint64_t)p.keys, p.keys > 1 ? ss : 8, 1, 8, 64, 1, 128);
-    };
-    if ((rc = map(&p.map_k, a->k, a->k_stride_p, a->k_stride_s, a->k_stride_h)) != FSA_OK) return rc;
-    if ((rc = map(&p.map_v, a->v, a->v_stride_p, a->v_stride_s, a->v_stride_h)) != FSA_OK) return rc;
+  if ((reinterpret_cast<uintptr_t>(a->q) & 15) || (a->batch > 1 && a->q_stride_b % 8) || (a->heads_q > 1 && a->q_stride_h % 8))
+    return FSA_ERR_INVALID_ARG;  // and copied by TMA
+  if ((reinterpret_cast<uintptr_t>(a->out_partial) & 15) || (reinterpret_cast<uintptr_t>(a->lse_partial) & 3) ||
+      (reinterpret_cast<uintptr_t>(a->plan_ws) & 7))
+    return FSA_ERR_INVALID_ARG;
+  if ((p.own_keys > 0 && (!a->k || !a->v)) || (p.prefix_keys > 0 && (!a->prefix_k || !a->prefix_v))) return FSA_ERR_INVALID_ARG;
+  // (a dimension of one has no stride that matters: one that TMA takes)
+  auto map = [&](CUtensorMap* m, const void* base, int rows, int64_t ss, int64_t sh, int outer, int64_t so, int box) {
+    return make_map4(m, a->dtype, base, p.D, p.Hkv, p.Hkv > 1 ? sh : 8, rows, rows > 1 ? ss : 8, outer, outer > 1 ? so : 8, 64, 1, box);
+  };
+  if (p.prefix_keys > 0) {
+    const bool paged = a->prefix_page_table != nullptr;
+    const int rows = paged ? a->prefix_page_size : p.prefix_keys, outer = paged ? a->prefix_num_pages : 1, box = paged && rows < 128 ? rows : 128;
+    if ((rc = map(&p.map_pk, a->prefix_k, rows, a->prefix_k_stride_s, a->prefix_k_stride_h, outer, a->prefix_k_stride_p, box)) != FSA_OK) return rc;
+    if ((rc = map(&p.map_pv, a->prefix_v, rows, a->prefix_v_stride_s, a->prefix_v_stride_h, outer, a->prefix_v_stride_p, box)) != FSA_OK) return rc;
   }
-  p.q = d->q;
-  p.used = a->seqused;
+  if (p.own_keys > 0) {
+    const bool paged = a->page_table != nullptr;
+    const int rows = paged ? a->page_size : p.own_keys, outer = paged ? a->num_pages : p.B;
+    for (int i = 0; i < 2; ++i) {
+      const int box = i ? 32 : (paged && rows < 128 ? rows : 128);
+      if ((rc = map(&p.map_k[i], a->k, rows, a->k_stride_s, a->k_stride_h, outer, a->k_stride_b, box)) != FSA_OK) return rc;
+      if ((rc = map(&p.map_v[i], a->v, rows, a->v_stride_s, a->v_stride_h, outer, a->v_stride_b, box)) != FSA_OK) return rc;
+    }
+  }
+  for (int i = 0; i < 2; ++i) {
+    const int64_t sh = p.G > 1 ? a->q_stride_h : 8, sb = p.B > 1 ? a->q_stride_b : 8, sg = p.Hkv > 1 ? p.G * a->q_stride_h : 8;
+    if ((rc = make_map4(i ? &p.map_pq : &p.map_q, a->dtype, a->q, p.D, p.G, sh, p.B, sb, p.Hkv, sg, 64, p.item_rows, i ? p.tile_seqs : 1)) != FSA_OK)
+      return rc;
+  }
+  p.used = a->seqused_k;
   p.page_table = a->page_table;
-  p.out = d->out;
-  p.lse = d->lse;
+  p.prefix_used = a->prefix_seqused;
+  p.prefix_table = a->prefix_page_table;
+  p.out = a->out;
+  p.lse = a->lse;
   p.out_partial = a->out_partial;
   p.lse_partial = a->lse_partial;
-  p.status = d->status;
-  p.q_sb = d->q_stride_b;
-  p.q_sh = d->q_stride_h;
-  p.o_sb = d->o_stride_b;
-  p.o_sh = d->o_stride_h;
-  p.l_sb = d->lse_stride_b;
-  p.l_sh = d->lse_stride_h;
+  p.plan_ws = a->plan_ws;
+  p.status = a->status;
+  p.o_sb = a->o_stride_b;
+  p.o_sh = a->o_stride_h;
+  p.l_sb = a->lse_stride_b;
+  p.l_sh = a->lse_stride_h;
   p.page_size = a->page_size;
+  p.max_pages = a->max_pages;
   p.num_pages = a->num_pages;
-  p.scale_log2 = d->softmax_scale * 1.44269504089f;
-  if (p.splits > 0) {
-    FsaDecArgs own = *d;
-    own.partial_only = 1;
-    own.num_splits = p.splits;
-    own.out_partial = a->out_partial + (size_t)p.slots * p.op_ss;
-    own.lse_partial = a->lse_partial + (size_t)p.slots * p.lp_ss;
-    own.out_partial_stride = own.lse_partial_stride = 0;
-    own.flags &= ~(uint32_t)FSA_F_SCRATCH_PARTIALS;
-    rc = fsa_decode(&own, stream_);
-    if (rc != FSA_OK) return rc;
-  }
-  const cudaError_t e = fsa::launch_prefix(p, d->dtype, head_dim_kernel(p.D), reinterpret_cast<cudaStream_t>(stream_));
+  p.prefix_page_size = a->prefix_page_size;
+  p.prefix_pages = a->prefix_num_pages;
+  p.scale_log2 = a->softmax_scale * 1.44269504089f;
+  const cudaError_t e = fsa::launch_prefix(p, a->dtype, head_dim_kernel(p.D), reinterpret_cast<cudaStream_t>(stream_));
   return e == cudaSuccess ? FSA_OK : FSA_ERR_LAUNCH;
 }
-
 
 }  // extern "C"

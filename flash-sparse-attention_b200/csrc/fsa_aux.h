@@ -104,25 +104,33 @@ struct GateExtParams {
   int B, Hq, Hkv, G, gpack, hgrid, sq, sk, num_m_blocks, n_tiles_k, page_size, pt_stride;
   unsigned flags;  // F_VARLEN_* | F_USED_* | F_PAGED
 };
-// Decode over a prefix that all sequences share: what the prefix kernel and the merge behind it take.
+// Decode over a prefix that all sequences share: what its kernel and the merge behind it take.
 struct alignas(64) PrefixParams {
-  CUtensorMap map_k, map_v;
-  const void* q;         // [B, Hq, D]
-  const int* used;       // optional [1]: keys of the prefix
-  const int* page_table; // optional [max_pages]
-  void* out;             // [B, Hq, D]
-  float* lse;            // [B, Hq]
-  float* out_partial;    // [slots + splits, B, Hq, D]: pieces of the prefix (two slots each), splits of the sequences' own keys
-  float* lse_partial;    // [slots + splits, Hq, B] base 2
+  CUtensorMap map_q, map_pq;   // the query's rows of one sequence and KV head (at most 128), of the sequences of a tile
+  CUtensorMap map_pk, map_pv;  // prefix
+  CUtensorMap map_k[2], map_v[2];  // own keys: boxes of a page (at most 128 rows), and of 32 rows
+  const int* used;             // optional [B]: own keys
+  const int* page_table;       // optional [B, max_pages]
+  const int* prefix_used;      // optional [1]
+  const int* prefix_table;     // optional [prefix_keys / prefix_page_size]
+  void* out;                   // [B, Hq, D]
+  float* lse;                  // [B, Hq]
+  float* out_partial;          // [partial_rows, D]: pieces of the pairs of query tiles, of single ones, of own keys
+  float* lse_partial;          // [partial_rows] base 2
+  int* plan_ws;                // [plan_ints]: first and last piece of every item
   int* status;
-  long long q_sb, q_sh, o_sb, o_sh, l_sb, l_sh, op_ss, lp_ss;
+  long long o_sb, o_sh, l_sb, l_sh;
+  long long single_rows, own_rows, partial_rows, plan_ints;  // where the second and third part begin, and sizes
   int B, Hq, Hkv, G, D;
-  int rows, q_tiles;     // of a KV head: B * G, and tiles of 128 of them
-  int keys;              // capacity of the prefix
-  int page_size, num_pages;
-  int ctas, slots, splits;
+  int tile_seqs, q_tiles, pairs;        // over the prefix: sequences of a query tile, tiles of a KV head, pairs of them
+  int head_tiles, items_b, item_rows;   // own keys: tiles of the group's heads, items of a sequence, rows of an item
+  int q_box, pq_box;                    // bytes of 64 columns of the query rows
+  int own_keys, prefix_keys;            // capacities
+  int page_size, max_pages, num_pages, prefix_page_size, prefix_pages;
+  int ctas;
   float scale_log2;
 };
+bool prefix_shape(PrefixParams* p);  // fills in what follows from sizes and capacities; false: too many units of work
 cudaError_t launch_prefix(const PrefixParams& p, int dtype, int head_dim, cudaStream_t stream);
 cudaError_t launch_gate_ext(const GateExtParams& p, int dtype, cudaStream_t stream);
 cudaError_t launch_dq_order(const DqOrderParams& p, cudaStream_t stream);

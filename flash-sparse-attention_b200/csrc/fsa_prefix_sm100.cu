@@ -1,19 +1,24 @@
-// Attention of a batch of single queries over a prefix that all sequences share, sm_100a.
+// Attention of a batch of single queries over a prefix that all sequences share and over each sequence's own keys, sm_100a.
 //
-//   s[r, n] = q[r] . k[n],  o[r] = sum_n 2^(c (s[r, n] - m)) v[n] / l[r],  c = softmax_scale * log2(e),
+//   s[r, n] = q[r] . k[n],  o[r] = sum_n 2^(c (s[r, n] - m)) v[n] / l[r],  c = softmax_scale * log2(e)
 //
-// for the rows r = (sequence, query head of the group) of one KV head against the same keys: with the batch on the M side the
-// prefix is read once for all sequences and its products run on tcgen05, where a decode of each sequence would read it
-// `batch` times. What it leaves are partial results (normalised, with base-2 log-sum-exps), which prefix_merge_kernel joins
-// with those of the sequences' own keys (dec_kernel).
+// Over the prefix, the rows r = (sequence, query head of the group) of one KV head meet the same keys: with them on the M side of tcgen05 the
+// prefix is read once for all sequences, where a decode of each would read it `batch` times. Over a sequence's own keys only the G heads
+// of the group share them; those tiles run through the same pipeline with G of 128 rows filled: a key tile's 64 KB take an SM's share of
+// HBM about 2900 cycles, its two products and one warp's softmax fewer.
 //
-// One CTA an SM; every CTA takes an equal share of the work, counted in (query tile of 128 rows) x (key tile of 128 keys): the
-// items (KV head, pair of query tiles) lie behind one another, cut into as many pieces as there are CTAs, so a piece may end inside one
-// item and begin the next, and every piece of an item leaves a partial result. Inside a CTA two softmax warpgroups, each with a score
-// tile and an output accumulator in TMEM, alternate on the tensor pipe: on two query tiles that use the same key tile, or, where the item
-// has one query tile, on even and odd key tiles of it.
+// The work is a list of units of one key tile each (128 keys of one KV head):
+//   pairs     prefix tile x two query tiles, for every KV head and pair of query tiles (a tile: the rows of as many sequences as
+//             fit 128, or 128 heads of one)
+//   singles   prefix tile x the last query tile, where their number is odd; own tile x the G rows of its sequence
+// It is cut into shares of equal cost, one per CTA (one CTA an SM), at any unit: a share may end inside an item (the units of the same rows and
+// KV head) and begin the next, and every piece of an item leaves a partial result - normalised, with a base-2 log-sum-exp -
+// that prefix_merge_kernel joins. Lengths live on the device: every CTA works its share out from them.
 //
-// Bound: few rows - the prefix's bytes (64 KB a key tile and KV head); from about 400 rows a KV head on the chain
+// In a CTA two softmax warpgroups, each with a score tile and an accumulator in TMEM, alternate on the tensor pipe. They share the
+// key tile of a pair; of the singles each walks its own half of the share ("stream"), tile by tile in turn.
+//
+// Bound: the keys' bytes, except where many sequences share a prefix (from about 400 rows a KV head): there the chain
 // S -> softmax -> P V of the two groups, as in the forward.
 #include <type_traits>
 
@@ -25,28 +30,61 @@ namespace fsa {
 
 namespace {
 
-constexpr int PM = 128;        // rows of a query tile
-constexpr int PN = 128;        // keys of a key tile
-constexpr int P_THREADS = 384; // two softmax warpgroups, and K producer, MMA issuer, V producer, one idle warp
-constexpr int W_K = 8, W_ISSUE = 9, W_V = 10;
+constexpr int PM = 128;         // rows of a query tile
+constexpr int PN = 128;         // keys of a key tile
+constexpr int OWN_BOX = 32;     // rows of the copies at the end of a sequence's own keys: no more than that is read in vain behind it
+constexpr int P_THREADS = 384;  // two softmax warpgroups, and one warp each that requests K, issues the MMAs, requests V, plans
+constexpr int W_K = 8, W_ISSUE = 9, W_V = 10, W_PLAN = 11;
+constexpr int BATCH = 16;       // steps that the planner works out at a time, one a lane; it is two batches ahead at most
+// What a unit costs, in parts of an SM's time: a pair of the tensor-bound case against a single one bound by its bytes.
+constexpr int COST_PAIR = 4, COST_SINGLE = 3;
 
-template <int HD>
-struct PrefixSmem {
-  static constexpr int kTile = 128 * HD * 2;            // bytes of a Q, K or V tile
-  static constexpr int kStages = HD == 64 ? 4 : 2;      // of K and of V
-  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStages * kTile, kBars = kV + kStages * kTile;
-  static constexpr int kTotal = kBars + 256 + 1024;     // 1024: the base is aligned by hand
+// What a softmax group has to know about the units of one item that it walks.
+struct GroupSegment {
+  int n;     // key tiles; 0: the group is done
+  int keys;  // of the item from the first of these tiles on
+  int rows;  // of the group's query tile that exist: the first ones
+  int row0;  // of the workspaces: the piece's first row
+  int shift; // place of the first row in the tile
+  int gap;   // rows behind row0 at which the next piece is left out (0: it is not)
 };
-
+// A step: one key tile, with word of the segment that it begins, if it does. The planner's lanes work sixteen out at a time, ahead of the
+// copies: step by step in the lane that also requests the tiles, indexes, lengths and pages took 5000 cycles a step, where a tile's bytes
+// take 2900, and by a lane of its own the first came 10 000 cycles after the plan, most of them waits for instructions.
+struct alignas(16) StepRecord {
+  uint32_t info;  // STEP_*, keys in the tile (from bit 8), own: tile of the group's heads (from bit 16)
+  int h, n0;      // KV head; first key
+  int b;          // own: the sequence; prefix: the (first) query tile
+  int page[4];    // of the tile's boxes, or of the one that holds them all
+  int n, keys;    // of the segment, when this is its first step: key tiles; keys from here on
+  int row0, gap;  // first row of its piece in the workspaces; see GroupSegment
+};
+static_assert(sizeof(StepRecord) == 48, "two batches fit");
 struct PrefixBars {
+  StepRecord rec[2 * BATCH];
+  uint64_t rec_full[2], rec_empty[2];
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t v_fixed;                      // rows behind the prefix's end are cleared
-  uint64_t q_full[2], s_full[2], p_full[2], o_final[2];
-  uint64_t done;                         // everything the tensor pipe was given
+  uint64_t seg_full[2][2], s_full[2], p_full[2], o_final[2];
+  GroupSegment seg[2][2];
+  uint64_t done;         // everything the tensor pipe was given
+  uint32_t v_info[4];
   uint32_t tmem_base;
   int abort_flag;
+  // this CTA's share: pairs [a0, a1), singles [s[0], s[1]) and [s[1], s[2]) of the two streams, the sequence in which a stream
+  // begins among the own keys and the tiles in front of it
+  int a0, a1, s[3], b_at[2], cum_at[2];
+  int ctas, tiles, keys, singles_prefix;
+  int warp_sum[16];
 };
-static_assert(sizeof(PrefixBars) <= 256, "fits its room");
+template <int HD>
+struct PrefixSmem {
+  static constexpr int kTile = 128 * HD * 2;        // bytes of a Q, K or V tile
+  static constexpr int kStages = HD == 64 ? 4 : 2;  // of K and of V
+  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStages * kTile, kOut = kV + kStages * kTile, kBars = kOut + 8 * 4096;
+  static constexpr int kTotal = kBars + (int)sizeof(PrefixBars) + 1024;  // 1024: the base is aligned by hand
+};
+
+enum : uint32_t { STEP_FIRST = 1u, STEP_LAST = 2u, STEP_OWN = 4u };  // of a segment; own keys
 
 // Bounded wait that does not look at the abort flag: for what has been started and will come to its end.
 __device__ __forceinline__ void wait_out(uint64_t* bar, uint32_t parity) {
@@ -55,50 +93,79 @@ __device__ __forceinline__ void wait_out(uint64_t* bar, uint32_t parity) {
   }
 }
 
-// The key tiles [t0, t1) of an item that a CTA computes.
-struct PrefixSegment {
-  int hkv, pair, t0, t1;
-};
+__device__ __forceinline__ int own_keys(const PrefixParams& p, int b) { return p.used ? max(0, min(p.used[b], p.own_keys)) : p.own_keys; }
+__device__ __forceinline__ int tiles_of(int keys) { return (keys + PN - 1) / PN; }
 
-// Work is counted in query tiles x key tiles: an item has `tiles` key tiles, each counting as many as the item has query tiles (one or two).
-struct PrefixWork {
-  int q_tiles;      // query tiles of a KV head
-  int pairs;        // items of a KV head
-  int tiles;        // key tiles
-  int ctas;         // CTAs that have work
-  long long total;
-
-  __device__ __forceinline__ PrefixWork(const PrefixParams& p) {
-    const int keys = p.used ? max(0, min(*p.used, p.keys)) : p.keys;
-    q_tiles = p.q_tiles;
-    pairs = (q_tiles + 1) >> 1;
-    tiles = (keys + PN - 1) / PN;
-    total = (long long)p.Hkv * q_tiles * tiles;
-    ctas = (int)min((long long)p.ctas, total);
+// This CTA's share of the work, by all threads.
+__device__ __forceinline__ void make_plan(const PrefixParams& p, PrefixBars* s) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int prefix_keys = tid == 0 && p.prefix_used ? *p.prefix_used : p.prefix_keys;
+  const int chunk = (p.B + P_THREADS - 1) / P_THREADS, b0 = tid * chunk, b1 = min(p.B, b0 + chunk);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += tiles_of(own_keys(p, b));
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
   }
-  __device__ __forceinline__ int weight(int pair) const { return 2 * pair + 1 < q_tiles ? 2 : 1; }
-  __device__ __forceinline__ long long item_start(int item) const {  // item = hkv * pairs + pair
-    return (long long)(item / pairs) * q_tiles * tiles + 2ll * (item % pairs) * tiles;
+  if (lane == 31) s->warp_sum[warp] = incl;
+  __syncthreads();
+  int cum = incl - mine, total_own = 0;
+#pragma unroll
+  for (int w = 0; w < P_THREADS / 32; ++w) {
+    const int v = s->warp_sum[w];
+    if (w < warp) cum += v;
+    total_own += v;
   }
-  __device__ __forceinline__ long long share_start(int cta) const { return total * cta / ctas; }
-  // The first key tile of an item that does not begin before place x; a key tile belongs to the CTA that holds its start.
-  __device__ __forceinline__ int first_tile(int item, long long x) const {
-    const int w = weight(item % pairs);
-    const long long off = x - item_start(item);
-    return off <= 0 ? 0 : (int)min((off + w - 1) / w, (long long)tiles);
+  if (tid == 0) {
+    const int keys = max(0, min(prefix_keys, p.prefix_keys)), tiles = tiles_of(keys);
+    const int pairs = p.Hkv * p.pairs * tiles, odd = (p.q_tiles & 1) ? p.Hkv * tiles : 0, singles = odd + total_own * p.items_b;
+    const long long cost = (long long)COST_PAIR * pairs + (long long)COST_SINGLE * singles;
+    // shares of at least a pair's cost: every share between two that hold units of a kind then holds one of it, too
+    const int ctas = (int)min((long long)p.ctas, max(cost / COST_PAIR, min(cost, 1ll))), cta = blockIdx.x;
+    s->ctas = ctas;
+    s->tiles = tiles;
+    s->keys = keys;
+    s->singles_prefix = odd;
+    s->b_at[0] = s->b_at[1] = 0;  // (a stream that begins in front of the own keys begins them with the first sequence)
+    s->cum_at[0] = s->cum_at[1] = 0;
+    auto bounds = [&](int at_cta, int& a, int& x) {
+      // the quotient of numbers below 2^41 in 64-bit floating point, rounded down: exact, since it is 1 / 256 from the next integer
+      const long long at = (long long)((double)cost * (double)at_cta / (double)ctas), behind = at - (long long)COST_PAIR * pairs;
+      a = behind >= 0 ? pairs : (int)((unsigned)(at + COST_PAIR - 1) / COST_PAIR);
+      x = behind <= 0 ? 0 : (int)((unsigned)(behind + COST_SINGLE - 1) / COST_SINGLE);
+    };
+    if (cta < ctas) {
+      int x0, x1;
+      bounds(cta, s->a0, x0);
+      bounds(cta + 1, s->a1, x1);
+      const int mid = x0 + (x1 - x0 + 1) / 2;
+      s->s[0] = x0;
+      s->s[1] = mid;
+      s->s[2] = x1;
+    }
   }
-  __device__ __forceinline__ int item_at(long long x) const {
-    const long long per_head = (long long)q_tiles * tiles;
-    const int h = (int)(x / per_head);
-    return h * pairs + min((int)((x - h * per_head) / (2ll * tiles)), pairs - 1);
+  __syncthreads();
+  if ((int)blockIdx.x < s->ctas && total_own > 0) {
+    // the sequences in which the streams begin
+    const int at0 = s->s[0] - s->singles_prefix, at1 = s->s[1] - s->singles_prefix;
+    const int c0 = at0 >= 0 ? at0 / p.items_b : -1, c1 = at1 >= 0 ? at1 / p.items_b : -1;
+    int c = cum;
+    for (int b = b0; b < b1; ++b) {
+      const int u = tiles_of(own_keys(p, b));
+      if (c0 >= c && c0 < c + u) s->b_at[0] = b, s->cum_at[0] = c;
+      if (c1 >= c && c1 < c + u) s->b_at[1] = b, s->cum_at[1] = c;
+      c += u;
+    }
   }
-  __device__ __forceinline__ int cta_at(long long x) const { return (int)(((x + 1) * ctas - 1) / total); }  // the share that holds place x
-};
+}
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_constant__ PrefixParams p) {
   using SM = PrefixSmem<HD>;
   constexpr int STAGES = SM::kStages;
+  static_assert(SM::kTotal <= 232448, "shared memory of an SM");
   constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t TMEM_S = 0, TMEM_O = 256;  // two tiles of 128 columns each; O of group q at 256 + 128 q
   after_previous();
@@ -108,109 +175,275 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &bars->abort_flag;
 
-  const PrefixWork work(p);
-  if ((int)blockIdx.x >= work.ctas) return;  // nothing for this CTA: before any barrier or TMEM exists
-  const long long x0 = work.share_start(blockIdx.x), x1 = work.share_start(blockIdx.x + 1);
-  const int item0 = work.item_at(x0), item1 = work.item_at(x1 - 1);
-  const int keys = p.used ? max(0, min(*p.used, p.keys)) : p.keys;
-
-  if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&bars->k_full[s], 1);
-      mbar_init(&bars->k_empty[s], 1);
-      mbar_init(&bars->v_full[s], 1);
-      mbar_init(&bars->v_empty[s], 1);
-    }
-    mbar_init(&bars->v_fixed, 1);
-    mbar_init(&bars->done, 1);
-    for (int q = 0; q < 2; ++q) {
-      mbar_init(&bars->q_full[q], 4);
-      mbar_init(&bars->s_full[q], 1);
-      mbar_init(&bars->p_full[q], 4);
-      mbar_init(&bars->o_final[q], 1);
-    }
-    bars->abort_flag = (*reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
-    mbar_fence_init();
-  }
   if (warp == W_K) {
+    if (lane == 0) {
+      const int given_up = *reinterpret_cast<volatile int*>(p.status);
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&bars->k_full[s], 1);
+        mbar_init(&bars->k_empty[s], 1);
+        mbar_init(&bars->v_full[s], 1);
+        mbar_init(&bars->v_empty[s], 1);
+      }
+      for (int q = 0; q < 2; ++q) {
+        mbar_init(&bars->seg_full[q][0], 1);
+        mbar_init(&bars->seg_full[q][1], 1);
+        mbar_init(&bars->s_full[q], 1);
+        mbar_init(&bars->p_full[q], 4);
+        mbar_init(&bars->o_final[q], 1);
+      }
+      for (int r = 0; r < 2; ++r) {
+        mbar_init(&bars->rec_full[r], 1);
+        mbar_init(&bars->rec_empty[r], 2);
+      }
+      mbar_init(&bars->done, 1);
+      bars->abort_flag = given_up != 0 ? 1 : 0;
+      mbar_fence_init();
+      if (p.prefix_keys > 0) {
+        tma_prefetch_desc(&p.map_pk);
+        tma_prefetch_desc(&p.map_pv);
+      }
+      if (p.own_keys > 0) {
+        for (int i = 0; i < 2; ++i) {
+          tma_prefetch_desc(&p.map_k[i]);
+          tma_prefetch_desc(&p.map_v[i]);
+        }
+      }
+    }
+    __syncwarp();
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
+    tc_fence_before();
   }
-  tc_fence_before();
+  make_plan(p, bars);
   __syncthreads();
   tc_fence_after();
+  // no work for this CTA; shares of whole units may also come out empty
+  if ((int)blockIdx.x >= bars->ctas || bars->a0 + bars->s[0] == bars->a1 + bars->s[2]) {
+    if (warp == W_K) tmem_dealloc(bars->tmem_base, 512);
+    return;
+  }
   const uint32_t tmem = bars->tmem_base;
-
-  // One segment of this CTA's share: false when the rounding to whole key tiles leaves nothing of the item.
-  auto segment = [&](int item, PrefixSegment& g) {
-    g.hkv = item / work.pairs;
-    g.pair = item % work.pairs;
-    g.t0 = work.first_tile(item, x0);
-    g.t1 = work.first_tile(item, x1);
-    return g.t0 < g.t1;
-  };
+  const int n_pairs = bars->a1 - bars->a0, n_singles = bars->s[2] - bars->s[0], n_steps = n_pairs + n_singles;
 
   if (warp >= W_K) {
     // 384 x 168 registers at launch = 256 x 216 + 128 x 72
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == W_K || warp == W_V) {
-      // =============================== K and V producers ========================================
-      const bool is_v = warp == W_V;
-      const CUtensorMap* map = is_v ? &p.map_v : &p.map_k;
-      uint64_t* full = is_v ? bars->v_full : bars->k_full;
-      uint64_t* empty = is_v ? bars->v_empty : bars->k_empty;
-      uint8_t* ring = smem + (is_v ? SM::kV : SM::kK);
-      if (lane == 0) tma_prefetch_desc(map);
+    if (warp == W_PLAN) {
+      // =============================== planner ==================================================
       bool ok = !*abort_flag;
-      int n = 0;  // tiles requested so far
-      PrefixSegment g;
-      for (int item = item0; item <= item1 && ok; ++item) {
-        if (!segment(item, g)) continue;
-        for (int t = g.t0; t < g.t1 && ok; ++t, ++n) {
-          const int s = n % STAGES;
-          if (n >= STAGES) ok = mbar_wait(&empty[s], (n / STAGES - 1) & 1, abort_flag);
-          if (!ok) break;
-          uint8_t* dst = ring + s * SM::kTile;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&full[s], SM::kTile);
-            if (p.page_table) {
-              const int page_shift = 31 - __clz(p.page_size), row_shift = min(page_shift, 7);
-              for (int r = 0; r < PN; r += 1 << row_shift) {
-                const int n0 = t * PN + r;
-                int page = -1;  // outside the pool: TMA fills zeros
-                if (n0 < keys) {
-                  page = p.page_table[n0 >> page_shift];
-                  if (page < 0 || page >= p.num_pages) {
-                    page = -1;
-                    atomicExch(p.status, 3);
-                  }
-                }
-                for (int d = 0; d < HD; d += 64)
-                  tma_load_4d(dst + (d / 64) * (PN * 128) + r * 128, map, &full[s], d, g.hkv, n0 & (p.page_size - 1), page);
-              }
+      const int q = lane & 1;  // (of the singles; batches begin with a single of the first stream once the pairs are through)
+      int b = bars->b_at[q], cum = bars->cum_at[q];  // this stream's place among the own keys: sequence, tiles in front of it
+      int m0 = 0;
+      for (int batch = 0; m0 < n_steps && ok; ++batch) {
+        // a batch: steps m0 .. m0 + count - 1, pairs or singles, in lanes 0 .. count - 1
+        const bool pair = m0 < n_pairs;
+        const int count = min(BATCH, (pair ? n_pairs : n_steps) - m0), m = m0 + lane;
+        StepRecord r;
+        int item = 0, id = 0, keys_all = 0, tiles_all = 0, t = 0, left = 0;  // left: units of the item that are this CTA's from here on
+        bool own = false, first = false;
+        if (lane < count) {
+          r.info = 0;
+          if (pair) {
+            const int pos = bars->a0 + m, tiles = bars->tiles;
+            item = pos / tiles;
+            t = pos - item * tiles;
+            r.h = item / p.pairs;
+            r.b = 2 * (item - r.h * p.pairs);
+            id = blockIdx.x;
+            r.row0 = (item + id) * (2 * PM);
+            keys_all = bars->keys;
+            tiles_all = tiles;
+            left = min(tiles - t, bars->a1 - pos);
+            first = m == 0;
+          } else {
+            const int pos = bars->s[q] + ((m - n_pairs) >> 1), end = bars->s[q + 1];
+            const int y = pos - bars->singles_prefix;
+            id = 2 * (int)blockIdx.x + q;
+            own = y >= 0;
+            if (!own) {
+              tiles_all = bars->tiles;
+              item = r.h = pos / tiles_all;
+              t = pos - item * tiles_all;
+              r.b = p.q_tiles - 1;
+              r.row0 = (int)p.single_rows + (item + id) * PM;
+              keys_all = bars->keys;
+              item += p.Hkv * p.pairs;
             } else {
-              for (int d = 0; d < HD; d += 64) tma_load_4d(dst + (d / 64) * (PN * 128), map, &full[s], d, g.hkv, t * PN, 0);
+              int u;
+              for (;;) {
+                keys_all = own_keys(p, b);
+                u = tiles_of(keys_all);
+                if (y < (cum + u) * p.items_b) break;
+                cum += u;
+                ++b;
+              }
+              const int at = y - cum * p.items_b, i = at / u;
+              t = at - i * u;
+              r.h = i / p.head_tiles;
+              r.info = STEP_OWN | (uint32_t)(i - r.h * p.head_tiles) << 16;
+              r.b = b;
+              item = b * p.items_b + i;
+              r.row0 = (int)p.own_rows + (item + id) * p.item_rows;
+              tiles_all = u;
+              item += p.Hkv * (p.pairs + 1);
             }
+            left = min(tiles_all - t, end - pos);
+            first = m - n_pairs < 2;
           }
-          __syncwarp();
-          if (is_v && (t + 1) * PN > keys) {
-            // Keys behind the end carry probability 0, but what lies in their V rows may be anything, and 0 * NaN is NaN.
-            ok = mbar_wait(&full[s], (n / STAGES) & 1, abort_flag);
-            if (!ok) break;
-            const int r0 = keys - t * PN;
-            constexpr int CPR = HD / 8;
-            for (int i = lane; i < (PN - r0) * CPR; i += 32) {
-              const int r = r0 + i / CPR, c = i % CPR;
-              *reinterpret_cast<uint4*>(dst + (c >> 3) * (PN * 128) + sw128_offset(r, c & 7)) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->v_fixed);
+          first = first || t == 0;
+          // which pieces of the item there are, for the merge; a CTA with a single unit has no second stream
+          if (t == 0) p.plan_ws[2 * item] = id;
+          if (t == tiles_all - 1) p.plan_ws[2 * item + 1] = id;
+          r.gap = !pair && n_singles == 1 && t < tiles_all - 1 ? (own ? p.item_rows : PM) : 0;
+          const int keys = min(PN, keys_all - t * PN);
+          r.n = left;
+          r.keys = keys_all - t * PN;
+          r.n0 = t * PN;
+          r.info |= (first ? STEP_FIRST : 0u) | (left == 1 ? STEP_LAST : 0u) | ((uint32_t)keys << 8);
+          const int* table = own ? p.page_table : p.prefix_table;
+          if (table) {
+            const int size = own ? p.page_size : p.prefix_page_size, box = min(size, PN), shift = 31 - __clz(size), pages = own ? p.num_pages : p.prefix_pages;
+            if (own) table += (long long)b * p.max_pages;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.page[i] = i * box < keys ? table[(r.n0 + i * box) >> shift] : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (r.page[i] < 0 || r.page[i] >= pages) {  // outside the pool: -1, for which TMA fills zeros
+                r.page[i] = -1;
+                atomicExch(p.status, 3);
+              }
           }
         }
+        // the streams' places for the next batch are those of their last lanes
+        const int last = pair ? q : max((count - 1) - ((count - 1 - q) & 1), q);
+        b = __shfl_sync(0xffffffffu, b, last);
+        cum = __shfl_sync(0xffffffffu, cum, last);
+        if (batch >= 2) ok = mbar_wait(&bars->rec_empty[batch & 1], ((batch >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+        if (lane < count) bars->rec[(batch & 1) * BATCH + lane] = r;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->rec_full[batch & 1]);
+        m0 += count;
       }
-      // no copy is in flight when the CTA ends, whatever ended the loop
-      for (int i = max(0, n - STAGES); i < n; ++i) wait_out(&full[i % STAGES], (i / STAGES) & 1);
+    } else if (warp == W_K || warp == W_V) {
+      // =============================== requests of K and V ======================================
+      // With the first key tile of a segment come the query rows, and word for the groups of what they are about to walk.
+      if (lane == 0 && !*abort_flag) {
+        const bool is_v = warp == W_V;
+        uint64_t* const full = is_v ? bars->v_full : bars->k_full;
+        uint64_t* const empty = is_v ? bars->v_empty : bars->k_empty;
+        uint8_t* const ring = smem + (is_v ? SM::kV : SM::kK);
+        const CUtensorMap* const own_map = is_v ? p.map_v : p.map_k;
+        const CUtensorMap* const prefix_map = is_v ? &p.map_pv : &p.map_pk;
+        const int own_shift = p.page_table ? min(31 - __clz(p.page_size | 1), 7) : 7;  // rows of a box, of a tile at most
+        const int prefix_shift = p.prefix_table ? min(31 - __clz(p.prefix_page_size | 1), 7) : 7;
+        const int q_bytes = p.q_box * (HD / 64), pq_bytes = p.pq_box * (HD / 64);
+        bool ok = true;
+        int n = 0;                                // tiles requested so far
+        int n_seg[2] = {0, 0}, q_used[2] = {-1, -1};  // q_used: the last step whose scores read the group's rows
+        auto wait_for_rows = [&](int q) {  // until the last scores with the group's rows are there
+          if (q_used[q] >= 0) ok = ok && mbar_wait(&bars->k_empty[q_used[q] % STAGES], (q_used[q] / STAGES) & 1, abort_flag);
+        };
+        auto tell = [&](int q, const GroupSegment& x) {
+          // (The scores of all that was told before are there. Those of the last segment were issued behind the product of the one
+          // before it, and that behind the group's reading of this slot.)
+          const int slot = n_seg[q]++ & 1;
+          bars->seg[q][slot] = x;
+          mbar_arrive(&bars->seg_full[q][slot]);
+        };
+        auto request_q = [&](int q, bool own, int shift, int head, int b, int h, uint64_t* bar) {
+          uint8_t* dst = smem + SM::kQ + q * SM::kTile + shift * 128;
+#pragma unroll
+          for (int d = 0; d < HD; d += 64) tma_load_4d(dst + (d / 64) * (PM * 128), own ? &p.map_q : &p.map_pq, bar, d, head, b, h);
+        };
+        // Rows of a query tile that exist, and where they begin.
+        auto rows_of = [&](bool own, int q_tile, int heads_from, int& head, int& b) {
+          head = own ? heads_from : 0;
+          b = own ? q_tile : q_tile * p.tile_seqs;
+          if (own || p.G > PM) {
+            if (!own) {
+              b = q_tile / p.head_tiles;
+              head = (q_tile - b * p.head_tiles) * PM;
+            }
+            return min(PM, p.G - head);
+          }
+          return min(p.tile_seqs, p.B - b) * p.G;
+        };
+        for (int batch = 0; n < n_steps && ok; ++batch) {
+          const int count = min(BATCH, (n < n_pairs ? n_pairs : n_steps) - n);
+          ok = mbar_wait(&bars->rec_full[batch & 1], (batch >> 1) & 1, abort_flag);
+          if (!ok) break;
+          for (int i = 0; i < count; ++i, ++n) {
+            const int s = n % STAGES;
+            if (n >= STAGES) ok = mbar_wait(&empty[s], (n / STAGES - 1) & 1, abort_flag);
+            if (!ok) break;
+            const StepRecord& r = bars->rec[(batch & 1) * BATCH + i];
+            const uint32_t info = r.info;
+            const int keys = (int)(info >> 8) & 255, h = r.h, n0 = r.n0, b = r.b;
+            const bool own = info & STEP_OWN;
+            const int shift = own ? own_shift : prefix_shift;
+            // whole boxes, except at the end of a sequence's own keys: boxes of OWN_BOX rows
+            const int unit = own ? OWN_BOX : 1 << shift;
+            const uint32_t bytes = (uint32_t)((keys + unit - 1) & ~(unit - 1)) * (HD * 2);
+            if (is_v) {
+              bars->v_info[s] = info;
+              mbar_arrive_expect_tx(&full[s], bytes);
+            } else {
+              const bool pair = n < n_pairs;
+              const int q = pair ? 0 : (n - n_pairs) & 1;
+              if (info & STEP_FIRST) {
+                wait_for_rows(q);
+                if (pair) wait_for_rows(1);
+                if (!ok) break;
+                mbar_arrive_expect_tx(&full[s], bytes + (own ? q_bytes : (pair ? 2 * pq_bytes : pq_bytes)));
+                GroupSegment x;
+                x.n = r.n;
+                x.keys = r.keys;
+                x.row0 = r.row0;
+                x.gap = r.gap;
+                // own rows sit in other lanes of the second group, so that the two groups' warps with rows are on different schedulers
+                x.shift = own && p.item_rows <= 64 ? q * 64 : 0;
+                int head, first_b;
+                x.rows = rows_of(own, b, (int)(info >> 16) * PM, head, first_b);
+                tell(q, x);
+                request_q(q, own, x.shift, head, first_b, h, &full[s]);
+                if (pair) {
+                  x.rows = rows_of(false, b + 1, 0, head, first_b);
+                  x.row0 += PM;
+                  tell(1, x);
+                  request_q(1, false, 0, head, first_b, h, &full[s]);
+                }
+              } else {
+                mbar_arrive_expect_tx(&full[s], bytes);
+              }
+              if (pair || q == 0) q_used[0] = n;
+              if (pair || q == 1) q_used[1] = n;
+            }
+            uint8_t* const dst = ring + s * SM::kTile;
+            const bool paged = (own ? p.page_table : p.prefix_table) != nullptr;
+            const int mask = (own ? p.page_size : p.prefix_page_size) - 1;
+            for (int at = 0; at < keys;) {
+              const bool whole = !own || keys - at > (1 << shift) - OWN_BOX;
+              const int row = paged ? (n0 + at) & mask : n0 + at, last = paged ? r.page[at >> shift] : (own ? b : 0);
+              const CUtensorMap* map = own ? (whole ? own_map : own_map + 1) : prefix_map;
+#pragma unroll
+              for (int d = 0; d < HD; d += 64) tma_load_4d(dst + (d / 64) * (PN * 128) + at * 128, map, &full[s], d, h, row, last);
+              at += whole ? 1 << shift : OWN_BOX;
+            }
+          }
+          if (ok) mbar_arrive(&bars->rec_empty[batch & 1]);
+        }
+        if (!is_v)
+          for (int q = 0; q < 2 && ok; ++q) {
+            GroupSegment none;
+            none.n = 0;
+            wait_for_rows(q);
+            if (ok) tell(q, none);
+          }
+        // no copy is in flight when the CTA ends, whatever ended the loop
+        for (int i = max(0, n - STAGES); i < n; ++i) wait_out(&full[i % STAGES], (i / STAGES) & 1);
+      }
+      __syncwarp();
     } else if (warp == W_ISSUE) {
       // =============================== MMA issuer ===============================================
       constexpr uint32_t idesc_s = umma_idesc_f16(PM, PN, IS_BF16, false, false);
@@ -220,91 +453,86 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
       const uint32_t dq = umma_desc_lo(smem_u32(smem + SM::kQ), 16), dk = umma_desc_lo(smem_u32(smem + SM::kK), 16);
       const uint32_t dv = umma_desc_lo(smem_u32(smem + SM::kV), PN * 128);
       bool ok = !*abort_flag;
-      int nk = 0, nv = 0, n_fixed = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
-      auto wait_k = [&]() { return mbar_wait(&bars->k_full[nk % STAGES], (nk / STAGES) & 1, abort_flag); };
-      auto issue_s = [&](int q) {
-        const uint32_t a = dq + ((q * SM::kTile) >> 4), b = dk + (((nk % STAGES) * SM::kTile) >> 4);
+      int nk = 0, nv = 0, n_p[2] = {0, 0};
+      // The scores of group q with the next key tile; a pair's tile serves both groups before it is given back.
+      auto issue_s = [&](int q, bool fetch, bool release) {
+        const int s = nk % STAGES;
+        if (fetch) ok = mbar_wait(&bars->k_full[s], (nk / STAGES) & 1, abort_flag);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t a = dq + ((q * SM::kTile) >> 4), b = dk + ((s * SM::kTile) >> 4);
 #pragma unroll
         for (int kk = 0; kk < KK_QK; ++kk) {
           const uint32_t off = (kk >> 2) * (PN * 128) + (kk & 3) * 32;
           umma_ss_lead(lead, tmem + TMEM_S + q * 128, umma_desc_at(a, off), umma_desc_at(b, off), idesc_s, kk > 0);
         }
         umma_commit_lead(lead, &bars->s_full[q]);
+        if (release) {
+          umma_commit_lead(lead, &bars->k_empty[s]);
+          ++nk;
+        }
       };
-      auto release_k = [&]() {
-        umma_commit_lead(lead, &bars->k_empty[nk % STAGES]);
-        ++nk;
+      uint32_t info = 0;
+      auto wait_v = [&]() {
+        const int s = nv % STAGES;
+        ok = mbar_wait(&bars->v_full[s], (nv / STAGES) & 1, abort_flag);
+        if (!ok) return;
+        info = *reinterpret_cast<volatile uint32_t*>(&bars->v_info[s]);
+        const int r0 = (int)(info >> 8) & 255;
+        if (r0 < PN) {
+          // keys behind the end carry probability 0, but what lies in their V rows may be anything, and 0 * NaN is NaN
+          uint8_t* vt = smem + SM::kV + s * SM::kTile;
+          constexpr int CPR = HD / 8;
+          for (int i = lane; i < (PN - r0) * CPR; i += 32) {
+            const int r = r0 + i / CPR, c = i % CPR;
+            *reinterpret_cast<uint4*>(vt + (c >> 3) * (PN * 128) + sw128_offset(r, c & 7)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
       };
-      auto issue_pv = [&](int q, bool first) {
+      auto issue_pv = [&](int q) {
+        ok = mbar_wait(&bars->p_full[q], n_p[q]++ & 1, abort_flag);
+        if (!ok) return;
+        tc_fence_after();
         const uint32_t b = dv + (((nv % STAGES) * SM::kTile) >> 4);
 #pragma unroll
         for (int kk = 0; kk < KK_PV; ++kk)
           umma_ts_lead(lead, tmem + TMEM_O + q * 128, tmem + TMEM_S + q * 128 + kk * 8, umma_desc_at(b, kk * 2048), idesc_o,
-                       (kk > 0 || !first) ? 1u : 0u);
+                       (kk > 0 || !(info & STEP_FIRST)) ? 1u : 0u);
+        if (info & STEP_LAST) umma_commit_lead(lead, &bars->o_final[q]);
       };
-      auto wait_q = [&](int q) { return mbar_wait(&bars->q_full[q], n_q[q]++ & 1, abort_flag); };
-      auto wait_p = [&](int q) { return mbar_wait(&bars->p_full[q], n_p[q]++ & 1, abort_flag); };
-      PrefixSegment g;
-      for (int item = item0; item <= item1 && ok; ++item) {
-        if (!segment(item, g)) continue;
-        const int n = g.t1 - g.t0;
-        const bool two = work.weight(g.pair) == 2;
-        // the first score tile of each group
-        if (two) {
-          ok = wait_k() && wait_q(0) && wait_q(1);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(0);
-          issue_s(1);
-          release_k();
+      auto release_v = [&]() {
+        umma_commit_lead(lead, &bars->v_empty[nv % STAGES]);
+        ++nv;
+      };
+      if (ok) {
+        if (n_pairs > 0) {
+          issue_s(0, true, false);
+          if (ok) issue_s(1, false, true);
         } else {
-          for (int q = 0; q < min(n, 2) && ok; ++q) {
-            ok = wait_k() && wait_q(q);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(q);
-            release_k();
-          }
+          issue_s(0, true, true);
+          if (ok && n_singles > 1) issue_s(1, true, true);
         }
-        for (int i = 0; i < n && ok; ++i) {
-          ok = mbar_wait(&bars->v_full[nv % STAGES], (nv / STAGES) & 1, abort_flag);
-          if (ok && (g.t0 + i + 1) * PN > keys) ok = mbar_wait(&bars->v_fixed, n_fixed++ & 1, abort_flag);
+      }
+      for (int i = 0; i < n_pairs && ok; ++i) {
+        wait_v();
+        for (int q = 0; q < 2 && ok; ++q) {
+          issue_pv(q);
           if (!ok) break;
-          if (two) {
-            const bool more = i + 1 < n;
-            if (more) ok = wait_k();
-            for (int q = 0; q < 2 && ok; ++q) {
-              ok = wait_p(q);
-              if (!ok) break;
-              tc_fence_after();
-              issue_pv(q, i == 0);
-              if (more)
-                issue_s(q);
-              else
-                umma_commit_lead(lead, &bars->o_final[q]);
-            }
-            if (!ok) break;
-            umma_commit_lead(lead, &bars->v_empty[nv % STAGES]);
-            if (more) release_k();
-          } else {
-            const int q = i & 1;
-            ok = wait_p(q);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(q, i < 2);
-            umma_commit_lead(lead, &bars->v_empty[nv % STAGES]);
-            if (i + 2 < n) {
-              ok = wait_k();
-              if (!ok) break;
-              tc_fence_after();
-              issue_s(q);
-              release_k();
-            } else {
-              umma_commit_lead(lead, &bars->o_final[q]);
-            }
-          }
-          ++nv;
+          if (i + 1 < n_pairs)
+            issue_s(q, q == 0, q == 1);
+          else if (q < n_singles)
+            issue_s(q, true, true);
         }
+        if (ok) release_v();
+      }
+      for (int k = 0; k < n_singles && ok; ++k) {
+        wait_v();
+        if (ok) issue_pv(k & 1);
+        if (!ok) break;
+        release_v();
+        if (k + 2 < n_singles) issue_s(k & 1, true, true);
       }
       umma_commit_lead(lead, &bars->done);
       wait_out(&bars->done, 0);
@@ -312,41 +540,23 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
   } else {
     // =============================== softmax groups =============================================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int q = warp >> 2, wq = warp & 3, row = wq * 32 + lane;
+    const int q = warp >> 2, wq = warp & 3;
     const uint32_t lane_addr = uint32_t(wq * 32) << 16;
     const uint32_t tS = tmem + lane_addr + TMEM_S + q * 128, tO = tmem + lane_addr + TMEM_O + q * 128;
     const float c = p.scale_log2;
     bool ok = !*abort_flag;
-    int n_s = 0, n_o = 0;
-    PrefixSegment g;
-    for (int item = item0; item <= item1 && ok; ++item) {
-      if (!segment(item, g)) continue;
-      const bool two = work.weight(g.pair) == 2;
-      const int first = two ? g.t0 : g.t0 + q, step = two ? 1 : 2;
-      if (first >= g.t1) continue;  // a segment of one key tile has nothing for the second group
-      // ---- the group's query tile: rows (sequence, head of the group) -> shared memory, 128-byte swizzle ----
-      // (all score tiles of the segment before have been waited for, so no MMA reads the old one)
-      const int r = (2 * g.pair + (two ? q : 0)) * PM + row;
-      const bool live = r < p.rows;
-      const int b = live ? r / p.G : 0, head = g.hkv * p.G + (live ? r - b * p.G : 0);
-      {
-        const T* src = reinterpret_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)head * p.q_sh;
-        uint8_t* dst = smem + SM::kQ + q * SM::kTile;
-        uint4 v[HD / 8];
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i)
-          v[i] = live && i * 8 < p.D ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i)
-          *reinterpret_cast<uint4*>(dst + (i >> 3) * (PM * 128) + sw128_offset(row, i & 7)) = v[i];
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->q_full[q]);
-      }
-      const bool idle = !__any_sync(0xffffffffu, live);  // no row of this warp exists: what it leaves in P is never read out
+    int n_s = 0, n_seg = 0;
+    while (ok) {
+      ok = mbar_wait(&bars->seg_full[q][n_seg & 1], (n_seg >> 1) & 1, abort_flag);
+      if (!ok) break;
+      const GroupSegment g = bars->seg[q][n_seg & 1];
+      if (g.n == 0) break;
+      const int row = ((wq * 32 - g.shift) & 127) + lane;  // of the query tile
+      const bool live = row < g.rows;
+      const bool idle = row - lane >= g.rows;              // no row of this warp exists: what it leaves in P is never read out
       float m_ref = -INFINITY;  // what the exponentials are relative to; it moves when the maximum has grown by 2^8
       float l = 0.f;            // their sum
-      for (int t = first; t < g.t1; t += step) {
+      for (int t = 0; t < g.n; ++t) {
         ok = mbar_wait(&bars->s_full[q], n_s++ & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
@@ -355,8 +565,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
 #pragma unroll
           for (int ch = 0; ch < PN / 32; ++ch) tmem_ld32(tS + ch * 32, &sr[ch * 32]);
           tmem_ld_wait();
-          if ((t + 1) * PN > keys) {
-            const int n_live = keys - t * PN;
+          const int n_live = g.keys - t * PN;
+          if (n_live < PN) {
 #pragma unroll
             for (int i = 0; i < PN; ++i)
               if (i >= n_live) sr[i] = 0xff800000u;
@@ -379,7 +589,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
             l *= scale;
           }
           // (this tile's scores were issued behind the P V product before them, so O is at rest)
-          if (t != first && __any_sync(0xffffffffu, need)) {
+          if (t > 0 && __any_sync(0xffffffffu, need)) {
             constexpr int RC = HD == 64 ? 16 : 32;
 #pragma unroll 1
             for (int ch = 0; ch < HD / RC; ++ch) {
@@ -427,31 +637,54 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
       }
       if (!ok) break;
       // ---- the segment's partial result ----
-      ok = mbar_wait(&bars->o_final[q], n_o++ & 1, abort_flag);
+      ok = mbar_wait(&bars->o_final[q], n_seg++ & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
       if (!idle) {
-        const int piece = (int)blockIdx.x - work.cta_at(work.item_start(item));
-        const long long slot = 2 * piece + (two ? 0 : q);
-        const bool dead = l == 0.f || l != l;
-        const float inv = dead ? 1.f : 1.f / l;
-        float* dst = p.out_partial + slot * p.op_ss + ((long long)b * p.Hq + head) * p.D;
-#pragma unroll
-        for (int ch = 0; ch < HD / 32; ++ch) {
+        const float inv = l == 0.f ? 1.f : 1.f / l;
+        const long long at = (long long)g.row0 + row;
+        if (live) {
+          p.lse_partial[at] = l == 0.f ? -INFINITY : m_ref * c + log2f(l);
+          if (g.gap) p.lse_partial[at + g.gap] = -INFINITY;
+        }
+        // 32 columns at a time. The loop stays rolled: a CTA comes here a few times only, and each time the instructions have to be fetched
+        // (unrolled, the first segment's results took 7000 cycles on their way out, rolled X).
+        uint8_t* stage = smem + SM::kOut + warp * 4096;
+        const bool few = g.rows <= 8;
+        const int n_rows = g.rows - (row - lane), c4 = lane & 7;
+        float* const mine = p.out_partial + at * p.D;                      // this lane's row
+        float* const quad = p.out_partial + (at - lane + (lane >> 3)) * p.D + c4 * 4;  // row lane / 8 of the warp, four of the columns
+#pragma unroll 1
+        for (int c0 = 0; c0 < p.D; c0 += 32) {
           uint32_t o[32];
-          tmem_ld32(tO + ch * 32, o);
+          tmem_ld32(tO + c0, o);
           tmem_ld_wait();
-          if (live) {
+          float4 v[8];
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              if (ch * 32 + i < p.D)
-                *reinterpret_cast<float4*>(dst + ch * 32 + i) =
-                    make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv, __uint_as_float(o[i + 2]) * inv,
-                                __uint_as_float(o[i + 3]) * inv);
+          for (int i = 0; i < 8; ++i)
+            v[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv, __uint_as_float(o[4 * i + 2]) * inv,
+                               __uint_as_float(o[4 * i + 3]) * inv);
+          if (few) {  // a group's few heads: each lane writes its row
+            if (live) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (c0 + i * 4 < p.D) *reinterpret_cast<float4*>(mine + c0 + i * 4) = v[i];
+            }
+          } else {    // through shared memory, so that eight lanes write 128 bytes of a row
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = v[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = (lane >> 3) + i * 4;
+              v[i] = *reinterpret_cast<const float4*>(stage + r * 128 + ((c4 ^ (r & 7)) << 4));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if ((lane >> 3) + i * 4 < n_rows && c0 + c4 * 4 < p.D) *reinterpret_cast<float4*>(quad + i * 4 * p.D + c0) = v[i];
+            __syncwarp();
           }
         }
-        // (a row with NaN among its scores has l = NaN and is NaN as a whole)
-        if (live) p.lse_partial[slot * p.lp_ss + (long long)head * p.B + b] = l == 0.f ? -INFINITY : m_ref * c + log2f(l);
       }
       tc_fence_before();
     }
@@ -466,79 +699,69 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
   }
 }
 
-// One warp joins the partial results of a (sequence, query head): the pieces of its item over the prefix - which shares of the work
-// they are follows from the same arithmetic - and the splits over the sequence's own keys. Weights 2^(lse - max); 32 at a time.
+// One warp joins the partial results of a (sequence, query head): the pieces of its item over the prefix and of its own keys' item, from
+// the first to the last that the kernel in front noted. Weights 2^(lse - max), 32 pieces at a time, four rows under way.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixParams p) {
   after_previous();
   const int lane = threadIdx.x & 31;
-  const long long at = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (at >= (long long)p.B * p.Hq || *reinterpret_cast<volatile int*>(p.status) != 0) return;
-  const int b = (int)(at / p.Hq), head = (int)(at - (long long)b * p.Hq);
-  const int hkv = head / p.G, r = b * p.G + head - hkv * p.G;
-  const PrefixWork work(p);
-  const int item = hkv * work.pairs + r / (2 * PM);
-  const bool two = work.weight(item % work.pairs) == 2;
-  int c_first = 0, pieces = 0;
-  if (work.total > 0) {
-    const long long start = work.item_start(item);
-    c_first = work.cta_at(start);
-    pieces = work.cta_at(start + (long long)work.weight(item % work.pairs) * work.tiles - 1) - c_first + 1;
-  }
-  const int slots = 2 * pieces, count = slots + p.splits;
-  const float* lp = p.lse_partial + (long long)head * p.B + b;
-  const float* op = p.out_partial + at * p.D;
-  // slot i of the prefix is written when its piece has key tiles for that group
-  auto lse_of = [&](int i) {
-    if (i >= count) return -INFINITY;
-    if (i >= slots) return __ldcg(lp + (long long)(p.slots + i - slots) * p.lp_ss);
-    const int cta = c_first + (i >> 1);
-    const int t0 = work.first_tile(item, work.share_start(cta)), t1 = work.first_tile(item, work.share_start(cta + 1));
-    if ((i & 1) ? (two || t1 - t0 < 2) : t1 <= t0) return -INFINITY;
-    return __ldcg(lp + (long long)i * p.lp_ss);
-  };
+  const int at = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (at >= p.B * p.Hq) return;
+  const int b = at / p.Hq, head = at - b * p.Hq, h = head / p.G, gi = head - h * p.G, gt = gi / PM;
+  // pieces first .. last of the two items: all that is needed to find them is asked for at once
+  const int q_tile = p.G > PM ? b * p.head_tiles + gt : b / p.tile_seqs, r = p.G > PM ? gi - gt * PM : (b - q_tile * p.tile_seqs) * p.G + gi;
+  const bool pair = q_tile < 2 * p.pairs;
+  const int pre = pair ? h * p.pairs + q_tile / 2 : h, own = b * p.items_b + h * p.head_tiles + gt;
+  const int2 pre_at = p.prefix_keys > 0 ? __ldcg(reinterpret_cast<const int2*>(p.plan_ws) + (pair ? pre : pre + p.Hkv * p.pairs)) : make_int2(0, -1);
+  const int2 own_at = p.own_keys > 0 ? __ldcg(reinterpret_cast<const int2*>(p.plan_ws) + own + p.Hkv * (p.pairs + 1)) : make_int2(0, -1);
+  const bool skip = *reinterpret_cast<volatile int*>(p.status) != 0;
+  const int n_pre = min(p.prefix_used ? *p.prefix_used : p.prefix_keys, p.prefix_keys) > 0 ? pre_at.y - pre_at.x + 1 : 0;
+  const int n_own = own_keys(p, b) > 0 ? own_at.y - own_at.x + 1 : 0;
+  if (skip) return;
+  const int pre_pitch = pair ? 2 * PM : PM, pre_row = (pair ? 0 : (int)p.single_rows) + (pre + pre_at.x) * pre_pitch + r + (pair ? (q_tile & 1) * PM : 0);
+  const int own_row = (int)p.own_rows + (own + own_at.x) * p.item_rows + gi - gt * PM;
+  const int count = n_pre + n_own;
   float top = -INFINITY, sum = 0.f, acc[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
   const int d0 = lane * VEC;
   const bool active = d0 < p.D;
+  using Row = typename std::conditional<VEC == 4, float4, float2>::type;
   for (int s0 = 0; s0 < count; s0 += 32) {
-    const float lse = lse_of(s0 + lane);
+    const int i = s0 + lane, cnt = min(32, count - s0);
+    const int mine = i < n_pre ? pre_row + i * pre_pitch : own_row + (i - n_pre) * p.item_rows;
+    const float lse = i < count ? __ldcg(p.lse_partial + mine) : -INFINITY;
+    Row v[4];
+    auto load4 = [&](int first) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = __shfl_sync(0xffffffffu, mine, (first + j) & 31);
+        if (first + j < cnt && active) v[j] = __ldcg(reinterpret_cast<const Row*>(p.out_partial + (long long)row * p.D + d0));
+      }
+    };
+    load4(0);
     float m = lse;
-    unsigned used = __ballot_sync(0xffffffffu, lse != -INFINITY);  // NaN counts
-    const bool nan = __any_sync(0xffffffffu, lse != lse);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     m = fmaxf(m, top);
-    if (nan) m = __int_as_float(0x7fffffff);
-    if (m == -INFINITY) continue;
-    const float old = top == -INFINITY ? 0.f : exp2f(top - m);
-    const float w = lse == -INFINITY ? 0.f : exp2f(lse - m);
+    if (__any_sync(0xffffffffu, lse != lse)) m = __int_as_float(0x7fffffff);
+    const float old = top == -INFINITY ? 0.f : exp2f(top - m), w = lse == -INFINITY ? 0.f : exp2f(lse - m);
     float ws = w;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
     sum = sum * old + ws;
     top = m;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] *= old;
-    while (used) {
-      const int j = __ffs(used) - 1;
-      used &= used - 1;
-      const int i = s0 + j;
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      const float* src = op + (long long)(i < slots ? i : p.slots + i - slots) * p.op_ss + d0;
-      if (active) {
-        if constexpr (VEC == 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-          acc[0] += wj * v.x;
-          acc[1] += wj * v.y;
-          acc[2] += wj * v.z;
-          acc[3] += wj * v.w;
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-          acc[0] += wj * v.x;
-          acc[1] += wj * v.y;
-        }
+    for (int k = 0; k < VEC; ++k) acc[k] *= old;
+    for (int first = 0; first < cnt; first += 4) {
+      if (first > 0) load4(first);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float wj = __shfl_sync(0xffffffffu, w, (first + j) & 31);
+        if (first + j >= cnt || wj == 0.f) continue;  // a piece without weight adds nothing, whatever its row holds
+        const float* e = reinterpret_cast<const float*>(&v[j]);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += wj * e[k];
       }
     }
   }
@@ -558,13 +781,36 @@ cudaError_t launch_one(const PrefixParams& p, cudaStream_t stream) {
   constexpr int smem = PrefixSmem<HD>::kTotal;
   static std::atomic<unsigned long long> opted_in{0};
   if (cudaError_t e = smem_opt_in(kern, smem, opted_in); e != cudaSuccess) return e;
-  if (p.ctas > 0)  // a prefix without positions leaves no pieces
+  if (p.ctas > 0)  // otherwise there is no place for a key
     if (cudaError_t e = launch_early(kern, (unsigned)p.ctas, P_THREADS, smem, stream, 1, p); e != cudaSuccess) return e;
-  const unsigned grid = (unsigned)(((long long)p.B * p.Hq + 7) / 8);
-  return launch_early(prefix_merge_kernel<T, HD / 32>, grid, 256, 0, stream, 1, p);
+  return launch_early(prefix_merge_kernel<T, HD / 32>, (unsigned)(((long long)p.B * p.Hq + 7) / 8), 256, 0, stream, 1, p);
 }
 
 }  // namespace
+
+// Shares of the work: one CTA an SM, and no more than there can be units.
+bool prefix_shape(PrefixParams* p) {
+  p->head_tiles = (p->G + PM - 1) / PM;
+  p->tile_seqs = p->G <= PM ? PM / p->G : 1;
+  p->q_tiles = p->G <= PM ? (p->B + p->tile_seqs - 1) / p->tile_seqs : p->B * p->head_tiles;
+  p->pairs = p->q_tiles / 2;
+  p->items_b = p->Hkv * p->head_tiles;
+  p->item_rows = p->G < PM ? p->G : PM;
+  p->q_box = 64 * p->item_rows * 2;
+  p->pq_box = p->q_box * p->tile_seqs;
+  auto tiles = [](long long keys) { return (keys + PN - 1) / PN; };
+  const long long units = (long long)p->Hkv * (p->pairs + (p->q_tiles & 1)) * tiles(p->prefix_keys) + (long long)p->B * p->items_b * tiles(p->own_keys);
+  if (units >= (1ll << 30)) return false;  // units are counted in 32 bits
+  const int sms = device_sm_count();
+  p->ctas = units < sms ? (int)units : sms;
+  p->single_rows = p->prefix_keys > 0 ? ((long long)p->Hkv * p->pairs + p->ctas) * (2 * PM) : 0;
+  if (p->pairs == 0) p->single_rows = 0;
+  p->own_rows = p->single_rows + ((p->q_tiles & 1) && p->prefix_keys > 0 ? ((long long)p->Hkv + 2 * p->ctas) * PM : 0);
+  p->partial_rows = p->own_rows + (p->own_keys > 0 ? ((long long)p->B * p->items_b + 2 * p->ctas) * p->item_rows : 0);
+  if (p->partial_rows >= (1ll << 31)) return false;
+  p->plan_ints = 2 * ((long long)p->Hkv * (p->pairs + 1) + (long long)p->B * p->items_b);
+  return true;
+}
 
 cudaError_t launch_prefix(const PrefixParams& p, int dtype, int head_dim, cudaStream_t stream) {
   if (head_dim == 64) return dtype == DT_BF16 ? launch_one<64, __nv_bfloat16>(p, stream) : launch_one<64, __half>(p, stream);

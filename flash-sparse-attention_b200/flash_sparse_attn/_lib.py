@@ -408,23 +408,53 @@ class FsaKvAppendRotaryArgs(ctypes.Structure):
 
 class FsaSharedPrefixArgs(ctypes.Structure):
     _fields_ = [
-        ("decode", c_void_p),
+        ("q", c_void_p),
         ("k", c_void_p),
         ("v", c_void_p),
-        ("seqused", c_void_p),
+        ("prefix_k", c_void_p),
+        ("prefix_v", c_void_p),
+        ("out", c_void_p),
+        ("lse", c_void_p),
+        ("seqused_k", c_void_p),
         ("page_table", c_void_p),
+        ("prefix_seqused", c_void_p),
+        ("prefix_page_table", c_void_p),
         ("out_partial", c_void_p),
         ("lse_partial", c_void_p),
-        ("k_stride_p", c_int64),
+        ("plan_ws", c_void_p),
+        ("status", c_void_p),
+        ("q_stride_b", c_int64),
+        ("q_stride_h", c_int64),
+        ("o_stride_b", c_int64),
+        ("o_stride_h", c_int64),
+        ("lse_stride_b", c_int64),
+        ("lse_stride_h", c_int64),
+        ("k_stride_b", c_int64),
         ("k_stride_s", c_int64),
         ("k_stride_h", c_int64),
-        ("v_stride_p", c_int64),
+        ("v_stride_b", c_int64),
         ("v_stride_s", c_int64),
         ("v_stride_h", c_int64),
-        ("seqlen", c_int32),
+        ("prefix_k_stride_p", c_int64),
+        ("prefix_k_stride_s", c_int64),
+        ("prefix_k_stride_h", c_int64),
+        ("prefix_v_stride_p", c_int64),
+        ("prefix_v_stride_s", c_int64),
+        ("prefix_v_stride_h", c_int64),
+        ("batch", c_int32),
+        ("heads_q", c_int32),
+        ("heads_kv", c_int32),
+        ("head_dim", c_int32),
+        ("seqlen_k", c_int32),
         ("num_pages", c_int32),
         ("page_size", c_int32),
         ("max_pages", c_int32),
+        ("prefix_seqlen", c_int32),
+        ("prefix_num_pages", c_int32),
+        ("prefix_page_size", c_int32),
+        ("prefix_max_pages", c_int32),
+        ("dtype", c_int32),
+        ("softmax_scale", c_float),
     ]
 
 
@@ -432,6 +462,7 @@ class FsaSharedPrefixWorkspace(ctypes.Structure):
     _fields_ = [
         ("out_partial", c_size_t),
         ("lse_partial", c_size_t),
+        ("plan_ws", c_size_t),
     ]
 
 
@@ -562,6 +593,8 @@ def _load_host(lib):
             raise ImportError(f"built for {built_for}, not for {here} (ABI version, torch)")
         host.init(ctypes.cast(lib.fsa_decode, c_void_p).value, ctypes.cast(lib.fsa_fwd, c_void_p).value,
                   ctypes.cast(lib.fsa_topk_indices, c_void_p).value, ctypes.cast(lib.fsa_pack_scales, c_void_p).value)
+        host.init_cache(*(ctypes.cast(f, c_void_p).value for f in (lib.fsa_rotary, lib.fsa_kv_append_rotary,
+                                                                   lib.fsa_shared_prefix_workspace_bytes, lib.fsa_decode_shared_prefix)))
     except (ImportError, AttributeError, TypeError) as e:  # TypeError: a launcher that takes other addresses
         _host = None
         warnings.warn("flash_sparse_attn/_host.so is missing or does not load; calls go through the slower Python launchers until "

@@ -1,5 +1,4 @@
-"""Host launcher of the decode over a shared prefix: one argument block for the prefix beside the decode's own, workspaces, one call
-into the library. Shapes alone decide the launch (no device data is read on the host, nothing synchronises)."""
+"""Host launcher of the decode over a shared prefix: checks, workspaces, one call into the library. Shapes alone decide the launch (no device data is read on the host, nothing synchronises)."""
 
 import ctypes
 from typing import Optional
@@ -7,15 +6,14 @@ from typing import Optional
 import torch
 
 from flash_sparse_attn import _lib
-from flash_sparse_attn.ops.triton import assert_inputs, utils
-from flash_sparse_attn.ops.triton.flash_dec import decode_num_splits
+from flash_sparse_attn.ops.triton import assert_inputs
 
 
 def _rows_ok(t):
-    """Rows that the kernels can fetch in pieces of 16 bytes."""
+    """Rows that TMA can fetch: on 16-byte boundaries, none on top of another."""
     if t.numel() == 0:
         return True
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
 
 
 def _check(query, key, value, prefix_key, prefix_value, softmax_scale, page_table, seqused_k, prefix_page_table, prefix_seqused, out, lse):
@@ -26,7 +24,6 @@ def _check(query, key, value, prefix_key, prefix_value, softmax_scale, page_tabl
     heads_kv = key.shape[2]
     assert_inputs._check_qkv(query, key, value, None, None, None, heads_q, heads_kv, head_dim, False, device)
     assert key.shape[3] == head_dim, "query, key and value must have one head_dim"
-    assert key.stride() == value.stride(), "key and value must share one memory layout"
     if page_table is None:
         assert key.shape[0] == batch, "key and value must have one row per sequence"
     else:
@@ -42,7 +39,7 @@ def _check(query, key, value, prefix_key, prefix_value, softmax_scale, page_tabl
         assert prefix_page_table.ndim == 1 and prefix_page_table.is_contiguous(), "prefix_page_table must be a contiguous int32 tensor [max_pages]"
     assert prefix_key.shape[-2:] == key.shape[-2:], "the prefix must have the heads and head_dim of key"
     for t in (query, key, value, prefix_key, prefix_value):
-        assert _rows_ok(t), "rows must be contiguous along head_dim and lie on 16-byte boundaries"
+        assert _rows_ok(t), "rows must be contiguous along head_dim, lie on 16-byte boundaries and not be expanded"
     assert_inputs._same_device(device, prefix_key, prefix_value, page_table, seqused_k, prefix_page_table, prefix_seqused, out, lse)
     assert_inputs._int32(page_table, prefix_page_table, what="page_table and prefix_page_table")
     assert_inputs._int32(seqused_k, prefix_seqused, what="seqused_k and prefix_seqused")
@@ -52,65 +49,64 @@ def _check(query, key, value, prefix_key, prefix_value, softmax_scale, page_tabl
     assert_inputs.check_out_buffers(out, lse, query.shape, query.dtype, query.shape[:2])
 
 
-def attn_decode_shared_prefix(query, key, value, prefix_key, prefix_value, softmax_scale: Optional[float] = None, num_splits=None,
-                              page_table=None, seqused_k=None, prefix_page_table=None, prefix_seqused=None, out=None, lse=None,
-                              skip_checks=False):
+def attn_decode_shared_prefix(query, key, value, prefix_key, prefix_value, softmax_scale: Optional[float] = None, page_table=None,
+                              seqused_k=None, prefix_page_table=None, prefix_seqused=None, out=None, lse=None, skip_checks=False):
     """Returns ``(out, lse)``."""
     if not query.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
+    host = _lib.native()
+    if host is not None:
+        res = host.shared_prefix(query, key, value, prefix_key, prefix_value, softmax_scale, page_table, seqused_k, prefix_page_table,
+                                 prefix_seqused, out, lse)
+        if res is not None:
+            if type(res) is int:
+                _lib.check(res, "fsa_decode_shared_prefix")
+            return res
     if not skip_checks:
         _check(query, key, value, prefix_key, prefix_value, softmax_scale, page_table, seqused_k, prefix_page_table, prefix_seqused,
                out, lse)
     device = query.device
     batch, heads_q, head_dim = query.shape
-    heads_kv = key.shape[2]
     if out is None:
         out = torch.empty((batch, heads_q, head_dim), dtype=query.dtype, device=device)
     if lse is None:
         lse = torch.empty((batch, heads_q), dtype=torch.float32, device=device)
     if batch == 0:
         return out, lse
-    d = _lib.FsaDecArgs()
-    d.q, d.k, d.v, d.out, d.lse = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr(), lse.data_ptr()
-    d.seqused_k, d.page_table = _lib.ptr(seqused_k), None
-    d.status = _lib.status_word(device).data_ptr()
-    d.q_stride_b, d.q_stride_h = query.stride(0), query.stride(1)
-    d.k_stride_b, d.k_stride_s, d.k_stride_h = key.stride(0), key.stride(1), key.stride(2)
-    d.o_stride_b, d.o_stride_h = out.stride(0), out.stride(1)
-    d.lse_stride_b, d.lse_stride_h = lse.stride(0), lse.stride(1)
-    d.batch, d.heads_q, d.heads_kv, d.head_dim = batch, heads_q, heads_kv, head_dim
-    if page_table is not None:
-        # the kernel takes the row's pitch for the number of its pages
-        page_table = page_table.contiguous()
-        d.page_table, d.page_table_stride = page_table.data_ptr(), page_table.shape[1]
-        d.num_pages, d.page_size = key.shape[0], key.shape[1]
-        d.seqlen_k = page_table.shape[1] * key.shape[1]
-    else:
-        d.seqlen_k = key.shape[1]
-    d.num_splits = int(num_splits) if num_splits is not None else decode_num_splits(batch, heads_kv, d.seqlen_k, utils.device_num_sms(device))
-    d.num_splits = max(1, d.num_splits)
-    d.kind, d.dtype = _lib.KIND_DENSE, _lib.dtype_code(query.dtype)
-    d.softmax_scale = float(softmax_scale) if softmax_scale is not None else head_dim**-0.5
     a = _lib.FsaSharedPrefixArgs()
-    a.decode = ctypes.cast(ctypes.pointer(d), ctypes.c_void_p)
-    a.k, a.v = prefix_key.data_ptr(), prefix_value.data_ptr()
-    a.seqused, a.page_table = _lib.ptr(prefix_seqused), None
-    a.k_stride_s, a.k_stride_h = prefix_key.stride(-3), prefix_key.stride(-2)
-    a.v_stride_s, a.v_stride_h = prefix_value.stride(-3), prefix_value.stride(-2)
-    if prefix_page_table is not None:
-        a.k_stride_p, a.v_stride_p = prefix_key.stride(0), prefix_value.stride(0)
-        a.num_pages, a.page_size = prefix_key.shape[:2]
-        a.max_pages = prefix_page_table.numel()
-        # an empty table holds no pages: the same as a prefix of no keys
-        a.page_table = prefix_page_table.data_ptr() if a.max_pages else None
+    a.q, a.k, a.v, a.prefix_k, a.prefix_v = (t.data_ptr() for t in (query, key, value, prefix_key, prefix_value))
+    a.out, a.lse, a.status = out.data_ptr(), lse.data_ptr(), _lib.status_word(device).data_ptr()
+    a.seqused_k, a.prefix_seqused = _lib.ptr(seqused_k), _lib.ptr(prefix_seqused)
+    a.q_stride_b, a.q_stride_h = query.stride(0), query.stride(1)
+    a.o_stride_b, a.o_stride_h = out.stride(0), out.stride(1)
+    a.lse_stride_b, a.lse_stride_h = lse.stride(0), lse.stride(1)
+    a.k_stride_b, a.k_stride_s, a.k_stride_h = key.stride()[:3]
+    a.v_stride_b, a.v_stride_s, a.v_stride_h = value.stride()[:3]
+    a.prefix_k_stride_s, a.prefix_k_stride_h = prefix_key.stride()[-3:-1]
+    a.prefix_v_stride_s, a.prefix_v_stride_h = prefix_value.stride()[-3:-1]
+    a.batch, a.heads_q, a.heads_kv, a.head_dim = batch, heads_q, key.shape[2], head_dim
+    if page_table is None:
+        a.seqlen_k = key.shape[1]
     else:
-        a.seqlen = prefix_key.shape[0]
+        page_table = page_table.contiguous()
+        a.page_table, a.max_pages = page_table.data_ptr(), page_table.shape[1]
+        a.num_pages, a.page_size = key.shape[:2]
+    if prefix_page_table is None:
+        a.prefix_seqlen = prefix_key.shape[0]
+    elif prefix_page_table.numel():  # an empty table: a prefix of no keys
+        a.prefix_page_table, a.prefix_max_pages = prefix_page_table.data_ptr(), prefix_page_table.numel()
+        a.prefix_num_pages, a.prefix_page_size = prefix_key.shape[:2]
+        a.prefix_k_stride_p, a.prefix_v_stride_p = prefix_key.stride(0), prefix_value.stride(0)
+    a.dtype = _lib.dtype_code(query.dtype)
+    a.softmax_scale = float(softmax_scale) if softmax_scale is not None else head_dim**-0.5
     lib = _lib.load()
     ws = _lib.FsaSharedPrefixWorkspace()
     with torch.cuda.device(device):
         _lib.check(lib.fsa_shared_prefix_workspace_bytes(ctypes.byref(a), ctypes.byref(ws)), "fsa_shared_prefix_workspace_bytes")
-        partial = torch.empty((ws.out_partial + ws.lse_partial) // 4 + 1, dtype=torch.float32, device=device)
-        a.out_partial, a.lse_partial = partial.data_ptr(), partial.data_ptr() + ws.out_partial
+        room = torch.empty((ws.out_partial + ws.lse_partial + ws.plan_ws) // 4, dtype=torch.float32, device=device)
+        a.out_partial = room.data_ptr()
+        a.lse_partial = a.out_partial + ws.out_partial
+        a.plan_ws = a.lse_partial + ws.lse_partial
         rc = lib.fsa_decode_shared_prefix(ctypes.byref(a), _lib.current_stream_ptr(device))
     _lib.check(rc, "fsa_decode_shared_prefix")
     return out, lse

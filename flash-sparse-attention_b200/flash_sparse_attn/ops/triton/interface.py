@@ -515,7 +515,6 @@ def flash_dense_attn_with_shared_prefix_func(
     prefix_key: torch.Tensor,
     prefix_value: torch.Tensor,
     softmax_scale: Optional[float] = None,
-    num_splits: Optional[int] = None,
     page_table: Optional[torch.Tensor] = None,
     seqused_k: Optional[torch.Tensor] = None,
     prefix_page_table: Optional[torch.Tensor] = None,
@@ -532,10 +531,10 @@ def flash_dense_attn_with_shared_prefix_func(
 
     Paged caches: own keys as pages ``[num_pages, page, Hkv, D]`` + ``page_table [B, max_pages]``, the prefix as pages (of the same pool or
     another) + ``prefix_page_table [prefix_pages]``; ``prefix_seqused`` (int32, one element) says how many of the prefix's positions
-    count. bf16 / fp16, ``head_dim`` a multiple of 16 up to 128. ``num_splits`` concerns the own keys. A row without any key is 0 with
+    count. bf16 / fp16, ``head_dim`` a multiple of 16 up to 128. A row without any key is 0 with
     log-sum-exp ``-inf``. Returns ``out [B, Hq, D]`` or ``(out, lse [B, Hq])``; the reference has no such operator."""
     out, lse = attn_decode_shared_prefix(
-        query, key, value, prefix_key, prefix_value, softmax_scale=softmax_scale, num_splits=num_splits, page_table=page_table,
+        query, key, value, prefix_key, prefix_value, softmax_scale=softmax_scale, page_table=page_table,
         seqused_k=seqused_k, prefix_page_table=prefix_page_table, prefix_seqused=prefix_seqused, out=out, lse=lse, skip_checks=skip_checks)
     return (out, lse) if return_lse else out
 

@@ -114,27 +114,40 @@ def _launch(query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, inte
 
 
 class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, interleaved):
-        ctx.save_for_backward(cos, sin, position_ids, cu_seqlens, seqlen_offsets if isinstance(seqlen_offsets, torch.Tensor) else None)
-        ctx.offset = None if isinstance(seqlen_offsets, torch.Tensor) else seqlen_offsets
-        ctx.interleaved = interleaved
-        ctx.set_materialize_grads(False)
-        return _launch(query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, interleaved, False)
+    """The rotation with its gradient: the transposed rotation of the gradients, which is a rotation again and has a gradient too."""
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    def forward(ctx, query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, interleaved, transposed):
+        ctx.save_for_backward(cos, sin, position_ids, cu_seqlens, seqlen_offsets if isinstance(seqlen_offsets, torch.Tensor) else None)
+        ctx.offset = None if isinstance(seqlen_offsets, torch.Tensor) else seqlen_offsets
+        ctx.interleaved, ctx.transposed = interleaved, transposed
+        ctx.set_materialize_grads(False)
+        return _launch(query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, interleaved, transposed)
+
+    @staticmethod
     def backward(ctx, dq, dk):
         cos, sin, position_ids, cu_seqlens, offsets = ctx.saved_tensors
-        grads = [dq if ctx.needs_input_grad[0] else None, dk if ctx.needs_input_grad[1] else None]
-        if grads[0] is None:  # the launch's first tensor is the one that is there
-            if grads[1] is not None:
-                grads[1] = _launch(grads[1], None, cos, sin, offsets if offsets is not None else ctx.offset, position_ids,
-                                   cu_seqlens, ctx.interleaved, True)[0]
-        else:
-            grads = _launch(grads[0], grads[1], cos, sin, offsets if offsets is not None else ctx.offset, position_ids,
-                            cu_seqlens, ctx.interleaved, True)
-        return grads[0], grads[1], None, None, None, None, None, None
+        dq, dk = (g if needed else None for g, needed in zip((dq, dk), ctx.needs_input_grad))
+        how = (cos, sin, ctx.offset if offsets is None else offsets, position_ids, cu_seqlens, ctx.interleaved, not ctx.transposed)
+        if dq is not None:
+            dq, dk = _turn(dq, dk, *how)
+        elif dk is not None:  # a launch's first tensor is the one that is there
+            dk = _turn(dk, None, *how)[0]
+        return (dq, dk) + (None,) * 7
+
+
+def _turn(query, key, *how):
+    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+        return _Rotary.apply(query, key, *how)
+    return _launch(query, key, *how)
+
+
+def _native():
+    """The native launcher, where no transform, dual number, trace or compiler wants to see what runs."""
+    if (torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0
+            or torch._C._get_tracing_state() is not None):
+        return None
+    return _lib.native()
 
 
 def apply_rotary_func(
@@ -160,10 +173,12 @@ def apply_rotary_func(
     Results are computed in fp32 and rounded once; no host synchronisation."""
     if not query.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
+    host = _native()
+    if host is not None:
+        res = host.rotary(query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, interleaved)
+        if res is not None:
+            return res
     if not skip_checks:
         _check(query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens)
-    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
-        q_out, k_out = _Rotary.apply(query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, interleaved)
-    else:
-        q_out, k_out = _launch(query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, interleaved, False)
+    q_out, k_out = _turn(query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, interleaved, False)
     return q_out if key is None else (q_out, k_out)

@@ -131,6 +131,14 @@ def append_kv_rotary(query: Optional[torch.Tensor], key_new: torch.Tensor, value
     ``advance=False`` it stays, for layers that share the lengths: all but the last. No host synchronisation; no gradients."""
     if not key_new.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
+    host = _lib.native()
+    if host is not None:
+        res = host.append(query, key_new, value_new, key_cache, value_cache, seqused_k, cos, sin, page_table, free_pages, free_count,
+                          cu_seqlens_new, seqlen_offsets, interleaved, query_scale, key_scale, value_scale, advance, out)
+        if res is not None:
+            if type(res) is int:
+                _lib.check(res, "fsa_kv_append_rotary")
+            return None if res is True else res
     if not skip_checks:
         _check_append(query, key_new, value_new, key_cache, value_cache, seqused_k, cos, sin, page_table, free_pages, free_count,
                       cu_seqlens_new, query_scale, key_scale, value_scale, out)

@@ -332,32 +332,45 @@ int fsa_combine(const float* out_partial, const float* lse_partial, void* out, f
                 int64_t lse_partial_stride, void* stream);
 
 /*
- * Decode for a batch whose sequences share a prefix: every query attends to the prefix and to its sequence's own keys; the
- * prefix's keys are read once for the whole batch (tensor-core products of all queries of a KV head with them), the own keys by
- * fsa_decode, and the partial results are merged. The reference has no such operator.
- *   decode   query, own keys (contiguous, packed or paged, with seqused_k / cu_seqlens_k as for fsa_decode), out, lse, sizes,
- *            softmax_scale (> 0), num_splits, status. Dense kind, bf16 / fp16, head_dim a multiple of 8 up to 128, no windows, gathered
- *            positions or peers; out_partial, lse_partial and partial_only are ignored. seqlen_k may be 0: no own keys.
- *   k, v     prefix [seqlen, heads_kv, head_dim], or pages [num_pages, page_size, heads_kv, head_dim] with page_table [max_pages]
- *            (page_size 32, 64, 128 or 256; a page outside the pool that holds keys sets the status word to 3)
- *   seqused  optional, device: keys of the prefix that count (at most the capacity)
- *   out_partial, lse_partial   workspaces of fsa_shared_prefix_workspace_bytes()
- * A row without any key: out 0, lse -inf.
+ * Decode for a batch whose sequences share a prefix: every query attends to the prefix and to its sequence's own keys. The prefix is
+ * read once for the whole batch: tensor-core products of all queries of a KV head with it. The reference has no such operator.
+ *   q, out, lse   [batch, heads_q, head_dim], alike, [batch, heads_q]; bf16 / fp16, head_dim a multiple of 8 up to 128
+ *   k, v          own keys [batch, seqlen_k, heads_kv, head_dim], or pages [num_pages, page_size, heads_kv, head_dim] with page_table
+ *                 [batch, max_pages] (contiguous); seqused_k optional [batch]. seqlen_k or max_pages 0: no own keys.
+ *   prefix_k, _v  [prefix_seqlen, heads_kv, head_dim], or pages with prefix_page_table [prefix_max_pages]; prefix_seqused optional [1]
+ * Lengths are read on the device and count up to the capacity; page sizes are 32, 64, 128 or 256; a page outside its pool that holds keys
+ * sets the status word to 3. Rows of q, k, v lie on 16-byte boundaries, those of out on 4-byte boundaries. softmax_scale > 0.
+ * A row without any key: out 0, lse -inf. Workspaces of fsa_shared_prefix_workspace_bytes(), 16-byte aligned.
  */
 typedef struct FsaSharedPrefixArgs {
-  const FsaDecArgs* decode;
+  const void* q;
   const void* k;
   const void* v;
-  const int32_t* seqused;
+  const void* prefix_k;
+  const void* prefix_v;
+  void* out;
+  float* lse;
+  const int32_t* seqused_k;
   const int32_t* page_table;
+  const int32_t* prefix_seqused;
+  const int32_t* prefix_page_table;
   float* out_partial;
   float* lse_partial;
-  int64_t k_stride_p, k_stride_s, k_stride_h; /* paged: _p = page stride */
-  int64_t v_stride_p, v_stride_s, v_stride_h;
-  int32_t seqlen, num_pages, page_size, max_pages;
+  int32_t* plan_ws;
+  int32_t* status;
+  int64_t q_stride_b, q_stride_h, o_stride_b, o_stride_h, lse_stride_b, lse_stride_h;
+  int64_t k_stride_b, k_stride_s, k_stride_h; /* paged: _b = page stride */
+  int64_t v_stride_b, v_stride_s, v_stride_h;
+  int64_t prefix_k_stride_p, prefix_k_stride_s, prefix_k_stride_h; /* paged: _p = page stride */
+  int64_t prefix_v_stride_p, prefix_v_stride_s, prefix_v_stride_h;
+  int32_t batch, heads_q, heads_kv, head_dim;
+  int32_t seqlen_k, num_pages, page_size, max_pages;
+  int32_t prefix_seqlen, prefix_num_pages, prefix_page_size, prefix_max_pages;
+  int32_t dtype;
+  float softmax_scale;
 } FsaSharedPrefixArgs;
 typedef struct FsaSharedPrefixWorkspace {
-  size_t out_partial, lse_partial;
+  size_t out_partial, lse_partial, plan_ws;
 } FsaSharedPrefixWorkspace;
 int fsa_shared_prefix_workspace_bytes(const FsaSharedPrefixArgs* args, FsaSharedPrefixWorkspace* sizes);
 int fsa_decode_shared_prefix(const FsaSharedPrefixArgs* args, void* stream);

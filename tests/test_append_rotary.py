@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from test_rotary import check, done, normal, tables, turn
+from test_rotary import check, done, launcher, normal, tables, turn  # noqa: F401
 
 DEV = "cuda"
 FP8_TOP = {torch.float8_e4m3fn: 448.0, torch.float8_e5m2: 57344.0}

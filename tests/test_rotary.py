@@ -9,6 +9,18 @@ import torch
 DEV = "cuda"
 
 
+@pytest.fixture(params=["native", "python"], autouse=True)
+def launcher(request, monkeypatch):
+    """Every test runs through the native launcher and through the Python one."""
+    from flash_sparse_attn import _lib
+
+    _lib.load()
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_host", None)
+    else:
+        assert _lib.native() is not None
+
+
 def tables(rows, half, dtype=torch.float32, device=DEV):
     freq = 10000.0 ** (-torch.arange(half, dtype=torch.float64) / max(half, 1))
     angle = torch.arange(rows, dtype=torch.float64)[:, None] * freq
@@ -184,6 +196,22 @@ def test_only_what_is_asked_for():
     x[..., 3], x[..., 5] = float("inf"), float("nan")
     y = fsa.apply_rotary_func(x, None, cos, sin, seqlen_offsets=2)
     assert torch.isfinite(y).sum() == 28 and torch.isnan(y[..., [5, 21]]).all() and torch.isinf(y[..., [3, 19]]).all()
+
+
+@pytest.mark.gpu
+def test_gradients_of_gradients():
+    import flash_sparse_attn as fsa
+
+    cos, sin = tables(9, 16)
+    q, k, g = normal(1, 1, 9, 2, 32).requires_grad_(), normal(2, 1, 9, 1, 32).requires_grad_(), normal(3, 1, 9, 2, 32).requires_grad_()
+    oq, ok = fsa.apply_rotary_func(q, k, cos, sin)
+    (dq,) = torch.autograd.grad(oq, q, g, create_graph=True)
+    assert torch.autograd.grad(ok, q, torch.ones_like(ok), allow_unused=True, retain_graph=True) == (None,)
+    h = normal(4, *q.shape)
+    (dg,) = torch.autograd.grad(dq, g, h)
+    done()
+    check(dq.detach(), *turn(g.detach(), cos, sin, False, -1))
+    check(dg, *turn(h, cos, sin, False))
 
 
 @pytest.mark.gpu

@@ -6,6 +6,8 @@ import ctypes
 import pytest
 import torch
 
+from test_rotary import launcher  # noqa: F401
+
 DEV = "cuda"
 
 
@@ -54,7 +56,7 @@ def check(out, lse, want, q, pk, keys, scale=None):
     assert ((lse.double() - ref_lse).abs()[~dead] <= (f + 2.0**-22 * ref_lse.abs())[~dead]).all()
 
 
-def run(batch, prefix, lens, hq, hkv, d, dtype=torch.bfloat16, page=0, prefix_page=0, room=0, scale=None, spread=1.0, num_splits=None,
+def run(batch, prefix, lens, hq, hkv, d, dtype=torch.bfloat16, page=0, prefix_page=0, room=0, scale=None, spread=1.0,
         foreign=None, capacity=None, seed=0):
     """`room`: positions behind the prefix's end that exist but do not count; `foreign`: what lies in places that no key is in."""
     import flash_sparse_attn as fsa
@@ -64,7 +66,7 @@ def run(batch, prefix, lens, hq, hkv, d, dtype=torch.bfloat16, page=0, prefix_pa
     q = normal(g, batch, hq, d, dtype=dtype) * spread
     pk, pv = (normal(g, prefix, hkv, d, dtype=dtype) for _ in range(2))
     keys, values = ([normal(g, n, hkv, d, dtype=dtype) for n in lens] for _ in range(2))
-    kw = dict(seqused_k=torch.tensor(lens, dtype=torch.int32, device=DEV), softmax_scale=scale, num_splits=num_splits)
+    kw = dict(seqused_k=torch.tensor(lens, dtype=torch.int32, device=DEV), softmax_scale=scale)
     fill = 0.0 if foreign is None else foreign
     longest = max(lens) if capacity is None else capacity
     if page:
@@ -121,7 +123,7 @@ def test_lengths_of_the_prefix(prefix):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("batch,hq,hkv", [(1, 1, 1), (1, 8, 8), (127, 1, 1), (128, 1, 1), (129, 1, 1), (43, 6, 2), (43, 9, 3), (52, 5, 1),
-                                          (64, 32, 8), (300, 4, 4), (17, 96, 1), (3, 300, 1), (2, 14, 2)])
+                                          (64, 32, 8), (300, 4, 4), (17, 96, 1), (9, 65, 1), (7, 128, 2), (3, 300, 1), (2, 14, 2)])
 def test_rows_and_groups(batch, hq, hkv):
     """One row to several query tiles, even and odd numbers of them, groups that end inside a tile."""
     run(batch, 901, [i % 7 for i in range(batch)], hq, hkv, 64)
@@ -171,11 +173,9 @@ def test_concentrated_rows(spread):
 
 
 @pytest.mark.gpu
-def test_scale_and_splits():
+def test_scales():
     for scale in (1e-6, 0.3, 1.0):
         run(5, 400, [0, 1, 17, 64, 500], 8, 2, 64, scale=scale)
-    for splits in (1, 2, 7):
-        run(5, 400, [0, 1, 17, 64, 5000], 8, 2, 64, num_splits=splits)
 
 
 @pytest.mark.gpu
@@ -348,7 +348,7 @@ def test_refusals():
     for bad in (dict(query=q[0]), dict(query=q.half()), dict(query=q[:, :7]), dict(query=q[:2]), dict(query=q[..., :32]), dict(value=k[:, :31]),
                 dict(query=q.float(), key=k.float(), value=k.float(), prefix_key=pk.float(), prefix_value=pk.float()),
                 dict(prefix_value=pk[:8]), dict(prefix_key=pk.half(), prefix_value=pk.half()), dict(prefix_key=pk[None], prefix_value=pk[None]),
-                dict(prefix_key=pk[:, :1], prefix_value=pk[:, :1]), dict(value=k.transpose(1, 2).contiguous().transpose(1, 2)),
+                dict(prefix_key=pk[:, :1], prefix_value=pk[:, :1]), dict(value=k[..., None, :, 0]),
                 dict(prefix_page_table=table[0]), dict(prefix_key=pages[:, :20], prefix_value=pages[:, :20], prefix_page_table=table[0]),
                 dict(prefix_key=pages, prefix_value=pages, prefix_page_table=table), dict(page_table=table[:2], key=pages, value=pages),
                 dict(prefix_key=pages, prefix_value=pages, prefix_page_table=table[0].long()), dict(key=pages, value=pages, page_table=table.long()),
@@ -363,26 +363,27 @@ def test_refusals():
         flash_dense_attn_with_shared_prefix_func(q, k, k, pk, pk)
     lib = _lib.load()
 
-    def call(dec=None, **kw):
-        d, a = _lib.FsaDecArgs(), _lib.FsaSharedPrefixArgs()
-        d.q = d.k = d.v = d.out = d.lse = d.status = 256
-        d.batch, d.heads_q, d.heads_kv, d.head_dim, d.seqlen_k, d.num_splits, d.softmax_scale = 2, 4, 1, 64, 10, 1, 1.0
-        d.dtype, d.kind = _lib.DT_BF16, _lib.KIND_DENSE
-        a.decode, a.out_partial, a.lse_partial, a.k, a.v, a.seqlen = ctypes.addressof(d), 256, 256, 256, 256, 10
-        a.k_stride_s = a.k_stride_h = a.v_stride_s = a.v_stride_h = 64
-        for n, v in (dec or {}).items():
-            setattr(d, n, v)
+    def call(**kw):
+        a = _lib.FsaSharedPrefixArgs()
+        for n in ("q", "k", "v", "prefix_k", "prefix_v", "out", "lse", "status", "out_partial", "lse_partial", "plan_ws"):
+            setattr(a, n, 256)
+        a.batch, a.heads_q, a.heads_kv, a.head_dim, a.seqlen_k, a.prefix_seqlen, a.softmax_scale = 2, 4, 1, 64, 10, 10, 1.0
+        a.k_stride_s = a.v_stride_s = a.prefix_k_stride_s = a.prefix_v_stride_s = 64
+        a.k_stride_b = a.v_stride_b = 640
+        a.dtype = _lib.DT_BF16
         for n, v in kw.items():
             setattr(a, n, v)
         return lib.fsa_decode_shared_prefix(ctypes.byref(a), None)
 
-    for kw in (dict(decode=None), dict(out_partial=None), dict(k=None), dict(seqlen=-1), dict(dec=dict(q=None)), dict(dec=dict(out=None)),
-               dict(dec=dict(batch=0)), dict(dec=dict(heads_kv=3)), dict(dec=dict(head_dim=136)), dict(dec=dict(softmax_scale=0.0)),
-               dict(dec=dict(softmax_scale=float("nan"))), dict(dec=dict(out=257)), dict(dec=dict(q=264)), dict(dec=dict(q_stride_b=4)),
-               dict(page_table=256, page_size=48, max_pages=1, num_pages=1), dict(page_table=256, page_size=64, max_pages=1, num_pages=0)):
+    pages = dict(page_table=256, page_size=64, max_pages=1, num_pages=1)
+    common = dict(prefix_page_table=256, prefix_page_size=64, prefix_max_pages=1, prefix_num_pages=1)
+    for kw in (dict(q=None), dict(out=None), dict(lse=None), dict(status=None), dict(plan_ws=None), dict(out_partial=None), dict(out_partial=260), dict(plan_ws=260),
+               dict(k=None), dict(prefix_v=None), dict(seqlen_k=-1), dict(prefix_seqlen=-1), dict(batch=0), dict(heads_kv=3), dict(head_dim=136),
+               dict(head_dim=60), dict(softmax_scale=0.0), dict(softmax_scale=float("nan")), dict(softmax_scale=float("inf")), dict(out=257),
+               dict(out=258), dict(o_stride_b=3), dict(q=264), dict(q_stride_b=4), dict(q_stride_h=4), dict(pages, page_size=48),
+               dict(pages, max_pages=-1), dict(common, prefix_page_size=16), dict(common, prefix_num_pages=-1), dict(pages, max_pages=1 << 25)):
         assert call(**kw) == -1, kw
-    for kw in (dict(kind=_lib.KIND_SPARSE), dict(dtype=_lib.DT_E4M3), dict(flags=_lib.F_LOCAL), dict(gather_kv_indices=256), dict(qkv_scale=256)):
-        assert call(dec=kw) == -2, kw
+    assert call(dtype=_lib.DT_E4M3) == -2 and call(batch=1 << 29, heads_q=4, heads_kv=1) == -2
 
 
 def test_argument_blocks_match_the_header():
