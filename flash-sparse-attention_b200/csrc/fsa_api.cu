@@ -933,13 +933,13 @@ int fsa_shared_prefix_workspace_bytes(const FsaSharedPrefixArgs* a, FsaSharedPre
   const int rc = prefix_geometry(a, &p);
   if (rc != FSA_OK) return rc;
   w->out_partial = sizeof(float) * (size_t)p.partial_rows * (size_t)p.D;
-  w->lse_partial = sizeof(float) * (((size_t)p.partial_rows + 3) & ~(size_t)3);
+  w->sum_partial = sizeof(float) * 2 * (((size_t)p.partial_rows + 1) & ~(size_t)1);
   w->plan_ws = sizeof(int32_t) * (size_t)p.plan_ints;
   return FSA_OK;
 }
 
 int fsa_decode_shared_prefix(const FsaSharedPrefixArgs* a, void* stream_) {
-  if (!a || !a->q || !a->out || !a->lse || !a->status || !a->out_partial || !a->lse_partial || !a->plan_ws) return FSA_ERR_INVALID_ARG;
+  if (!a || !a->q || !a->out || !a->lse || !a->status || !a->out_partial || !a->sum_partial || !a->plan_ws) return FSA_ERR_INVALID_ARG;
   if (a->dtype != FSA_DT_BF16 && a->dtype != FSA_DT_FP16) return FSA_ERR_UNSUPPORTED;
   if (!(a->softmax_scale > 0.f) || a->softmax_scale > 3.4e38f) return FSA_ERR_INVALID_ARG;
   fsa::PrefixParams p;
@@ -950,7 +950,7 @@ int fsa_decode_shared_prefix(const FsaSharedPrefixArgs* a, void* stream_) {
     return FSA_ERR_INVALID_ARG;  // rows are written in pieces of 4 bytes
   if ((reinterpret_cast<uintptr_t>(a->q) & 15) || (a->batch > 1 && a->q_stride_b % 8) || (a->heads_q > 1 && a->q_stride_h % 8))
     return FSA_ERR_INVALID_ARG;  // and copied by TMA
-  if ((reinterpret_cast<uintptr_t>(a->out_partial) & 15) || (reinterpret_cast<uintptr_t>(a->lse_partial) & 3) ||
+  if ((reinterpret_cast<uintptr_t>(a->out_partial) & 15) || (reinterpret_cast<uintptr_t>(a->sum_partial) & 7) ||
       (reinterpret_cast<uintptr_t>(a->plan_ws) & 7))
     return FSA_ERR_INVALID_ARG;
   if ((p.own_keys > 0 && (!a->k || !a->v)) || (p.prefix_keys > 0 && (!a->prefix_k || !a->prefix_v))) return FSA_ERR_INVALID_ARG;
@@ -985,7 +985,7 @@ int fsa_decode_shared_prefix(const FsaSharedPrefixArgs* a, void* stream_) {
   p.out = a->out;
   p.lse = a->lse;
   p.out_partial = a->out_partial;
-  p.lse_partial = a->lse_partial;
+  p.ml_partial = reinterpret_cast<float2*>(a->sum_partial);
   p.plan_ws = a->plan_ws;
   p.status = a->status;
   p.o_sb = a->o_stride_b;

@@ -116,7 +116,7 @@ struct alignas(64) PrefixParams {
   void* out;                   // [B, Hq, D]
   float* lse;                  // [B, Hq]
   float* out_partial;          // [partial_rows, D]: pieces of the pairs of query tiles, of single ones, of own keys
-  float* lse_partial;          // [partial_rows] base 2
+  float2* ml_partial;          // [partial_rows]: reference maximum in base 2, sum
   int* plan_ws;                // [plan_ints]: first and last piece of every item
   int* status;
   long long o_sb, o_sh, l_sb, l_sh;

@@ -839,10 +839,10 @@ PyObject* shared_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int rc = g_prefix_bytes(&x, &w);
     Tensor room;
     if (rc == FSA_OK) {
-      room = at::empty({(int64_t)((w.out_partial + w.lse_partial + w.plan_ws) / 4)}, q.options().dtype(at::kFloat));
+      room = at::empty({(int64_t)((w.out_partial + w.sum_partial + w.plan_ws) / 4)}, q.options().dtype(at::kFloat));
       x.out_partial = ptr<float>(room);
-      x.lse_partial = x.out_partial + w.out_partial / 4;
-      x.plan_ws = reinterpret_cast<int32_t*>(x.lse_partial + w.lse_partial / 4);
+      x.sum_partial = x.out_partial + w.out_partial / 4;
+      x.plan_ws = reinterpret_cast<int32_t*>(x.sum_partial + w.sum_partial / 4);
       rc = g_prefix(&x, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
     }
     no_gil.reset();

@@ -12,7 +12,7 @@
 //             fit 128, or 128 heads of one)
 //   singles   prefix tile x the last query tile, where their number is odd; own tile x the G rows of its sequence
 // It is cut into shares of equal cost, one per CTA (one CTA an SM), at any unit: a share may end inside an item (the units of the same rows and
-// KV head) and begin the next, and every piece of an item leaves a partial result - normalised, with a base-2 log-sum-exp -
+// KV head) and begin the next, and every piece of an item leaves a partial result - its O, reference maximum and sum -
 // that prefix_merge_kernel joins. Lengths live on the device: every CTA works its share out from them.
 //
 // In a CTA two softmax warpgroups, each with a score tile and an accumulator in TMEM, alternate on the tensor pipe. They share the
@@ -36,8 +36,9 @@ constexpr int OWN_BOX = 32;     // rows of the copies at the end of a sequence's
 constexpr int P_THREADS = 384;  // two softmax warpgroups, and one warp each that requests K, issues the MMAs, requests V, plans
 constexpr int W_K = 8, W_ISSUE = 9, W_V = 10, W_PLAN = 11;
 constexpr int BATCH = 16;       // steps that the planner works out at a time, one a lane; it is two batches ahead at most
-// What a unit costs, in parts of an SM's time: a pair of the tensor-bound case against a single one bound by its bytes.
-constexpr int COST_PAIR = 4, COST_SINGLE = 3;
+// What an SM's time goes to, in units of 500 cycles: a pair of query tiles on a key tile (4000, tensor-bound), a single one (2500 to 2800, its
+// bytes), and what an item of own keys adds (query rows, results on their way out: 256 x 128 keys 3450 a unit, 64 x 1024 2760).
+constexpr int COST_PAIR = 9, COST_SINGLE = 5, COST_ITEM = 1;
 
 // What a softmax group has to know about the units of one item that it walks.
 struct GroupSegment {
@@ -66,6 +67,7 @@ struct PrefixBars {
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t seg_full[2][2], s_full[2], p_full[2], o_final[2];
   GroupSegment seg[2][2];
+  uint64_t v_tail[4];    // V tiles with rows behind the last key: when those are cleared, v_full is told
   uint64_t done;         // everything the tensor pipe was given
   uint32_t v_info[4];
   uint32_t tmem_base;
@@ -74,7 +76,6 @@ struct PrefixBars {
   // begins among the own keys and the tiles in front of it
   int a0, a1, s[3], b_at[2], cum_at[2];
   int ctas, tiles, keys, singles_prefix;
-  int warp_sum[16];
 };
 template <int HD>
 struct PrefixSmem {
@@ -97,52 +98,59 @@ __device__ __forceinline__ int own_keys(const PrefixParams& p, int b) { return p
 __device__ __forceinline__ int tiles_of(int keys) { return (keys + PN - 1) / PN; }
 
 // This CTA's share of the work, by all threads.
-__device__ __forceinline__ void make_plan(const PrefixParams& p, PrefixBars* s) {
+__device__ __forceinline__ void make_plan(const PrefixParams& p, PrefixBars* s, int2* warp_sum) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int prefix_keys = tid == 0 && p.prefix_used ? *p.prefix_used : p.prefix_keys;
   const int chunk = (p.B + P_THREADS - 1) / P_THREADS, b0 = tid * chunk, b1 = min(p.B, b0 + chunk);
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of(own_keys(p, b));
+  int mine = 0, some = 0;  // tiles, and sequences that have any
+  for (int b = b0; b < b1; ++b) {
+    const int u = tiles_of(own_keys(p, b));
+    mine += u;
+    some += u > 0;
+  }
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) s->warp_sum[warp] = incl;
+  some = __reduce_add_sync(0xffffffffu, some);
+  if (lane == 31) warp_sum[warp] = make_int2(incl, some);
   __syncthreads();
-  int cum = incl - mine, total_own = 0;
+  int cum = incl - mine, total_own = 0, sequences = 0;
 #pragma unroll
   for (int w = 0; w < P_THREADS / 32; ++w) {
-    const int v = s->warp_sum[w];
-    if (w < warp) cum += v;
-    total_own += v;
+    const int2 v = warp_sum[w];
+    if (w < warp) cum += v.x;
+    total_own += v.x;
+    sequences += v.y;
   }
   if (tid == 0) {
     const int keys = max(0, min(prefix_keys, p.prefix_keys)), tiles = tiles_of(keys);
     const int pairs = p.Hkv * p.pairs * tiles, odd = (p.q_tiles & 1) ? p.Hkv * tiles : 0, singles = odd + total_own * p.items_b;
-    const long long cost = (long long)COST_PAIR * pairs + (long long)COST_SINGLE * singles;
-    // shares of at least a pair's cost: every share between two that hold units of a kind then holds one of it, too
-    const int ctas = (int)min((long long)p.ctas, max(cost / COST_PAIR, min(cost, 1ll))), cta = blockIdx.x;
+    // Equal shares of the cost, in which own items' share is spread over all singles. Every CTA works the same bounds out, so they need not be
+    // exact; a share is more than any unit's cost, so that every share between two that hold units of a kind holds one, too.
+    const float pair_cost = (float)COST_PAIR * pairs, single_cost = (float)COST_SINGLE * singles + (float)COST_ITEM * sequences * p.items_b;
+    const float cost = pair_cost + single_cost;
+    const int ctas = (int)fminf((float)p.ctas, fmaxf(cost * (1.f / (COST_PAIR + 1)), fminf(cost, 1.f))), cta = blockIdx.x;
     s->ctas = ctas;
     s->tiles = tiles;
     s->keys = keys;
     s->singles_prefix = odd;
     s->b_at[0] = s->b_at[1] = 0;  // (a stream that begins in front of the own keys begins them with the first sequence)
     s->cum_at[0] = s->cum_at[1] = 0;
-    auto bounds = [&](int at_cta, int& a, int& x) {
-      // the quotient of numbers below 2^41 in 64-bit floating point, rounded down: exact, since it is 1 / 256 from the next integer
-      const long long at = (long long)((double)cost * (double)at_cta / (double)ctas), behind = at - (long long)COST_PAIR * pairs;
-      a = behind >= 0 ? pairs : (int)((unsigned)(at + COST_PAIR - 1) / COST_PAIR);
-      x = behind <= 0 ? 0 : (int)((unsigned)(behind + COST_SINGLE - 1) / COST_SINGLE);
-    };
     if (cta < ctas) {
+      const float share = __fdividef(cost, (float)ctas), per_cost = single_cost > 0.f ? __fdividef((float)singles, single_cost) : 0.f;
+      auto bounds = [&](int c, int& a, int& x) {
+        const float at = share * c, behind = at - pair_cost;
+        a = c == ctas ? pairs : min(pairs, (int)ceilf(at * (1.f / COST_PAIR)));
+        x = c == ctas ? singles : (behind <= 0.f ? 0 : min(singles, (int)ceilf(behind * per_cost)));
+      };
       int x0, x1;
       bounds(cta, s->a0, x0);
       bounds(cta + 1, s->a1, x1);
-      const int mid = x0 + (x1 - x0 + 1) / 2;
       s->s[0] = x0;
-      s->s[1] = mid;
+      s->s[1] = x0 + (x1 - x0 + 1) / 2;
       s->s[2] = x1;
     }
   }
@@ -150,12 +158,11 @@ __device__ __forceinline__ void make_plan(const PrefixParams& p, PrefixBars* s) 
   if ((int)blockIdx.x < s->ctas && total_own > 0) {
     // the sequences in which the streams begin
     const int at0 = s->s[0] - s->singles_prefix, at1 = s->s[1] - s->singles_prefix;
-    const int c0 = at0 >= 0 ? at0 / p.items_b : -1, c1 = at1 >= 0 ? at1 / p.items_b : -1;
     int c = cum;
     for (int b = b0; b < b1; ++b) {
-      const int u = tiles_of(own_keys(p, b));
-      if (c0 >= c && c0 < c + u) s->b_at[0] = b, s->cum_at[0] = c;
-      if (c1 >= c && c1 < c + u) s->b_at[1] = b, s->cum_at[1] = c;
+      const int u = tiles_of(own_keys(p, b)), from = c * p.items_b, to = (c + u) * p.items_b;
+      if (at0 >= from && at0 < to) s->b_at[0] = b, s->cum_at[0] = c;
+      if (at1 >= from && at1 < to) s->b_at[1] = b, s->cum_at[1] = c;
       c += u;
     }
   }
@@ -175,46 +182,46 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &bars->abort_flag;
 
+  // what has to be there before the roles begin, each by a warp of its own: the waits add up otherwise
   if (warp == W_K) {
-    if (lane == 0) {
-      const int given_up = *reinterpret_cast<volatile int*>(p.status);
-      for (int s = 0; s < STAGES; ++s) {
-        mbar_init(&bars->k_full[s], 1);
-        mbar_init(&bars->k_empty[s], 1);
-        mbar_init(&bars->v_full[s], 1);
-        mbar_init(&bars->v_empty[s], 1);
-      }
-      for (int q = 0; q < 2; ++q) {
-        mbar_init(&bars->seg_full[q][0], 1);
-        mbar_init(&bars->seg_full[q][1], 1);
-        mbar_init(&bars->s_full[q], 1);
-        mbar_init(&bars->p_full[q], 4);
-        mbar_init(&bars->o_final[q], 1);
-      }
-      for (int r = 0; r < 2; ++r) {
-        mbar_init(&bars->rec_full[r], 1);
-        mbar_init(&bars->rec_empty[r], 2);
-      }
-      mbar_init(&bars->done, 1);
-      bars->abort_flag = given_up != 0 ? 1 : 0;
-      mbar_fence_init();
-      if (p.prefix_keys > 0) {
-        tma_prefetch_desc(&p.map_pk);
-        tma_prefetch_desc(&p.map_pv);
-      }
-      if (p.own_keys > 0) {
-        for (int i = 0; i < 2; ++i) {
-          tma_prefetch_desc(&p.map_k[i]);
-          tma_prefetch_desc(&p.map_v[i]);
-        }
-      }
-    }
-    __syncwarp();
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
     tc_fence_before();
+  } else if (warp == W_ISSUE && lane == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&bars->k_full[s], 1);
+      mbar_init(&bars->k_empty[s], 1);
+      mbar_init(&bars->v_full[s], 1);
+      mbar_init(&bars->v_empty[s], 1);
+      mbar_init(&bars->v_tail[s], 1);
+    }
+    for (int q = 0; q < 2; ++q) {
+      mbar_init(&bars->seg_full[q][0], 1);
+      mbar_init(&bars->seg_full[q][1], 1);
+      mbar_init(&bars->s_full[q], 1);
+      mbar_init(&bars->p_full[q], 4);
+      mbar_init(&bars->o_final[q], 1);
+      mbar_init(&bars->rec_full[q], 1);
+      mbar_init(&bars->rec_empty[q], 2);
+    }
+    mbar_init(&bars->done, 1);
+    mbar_fence_init();
+  } else if (warp == W_V && lane == 0) {
+    bars->abort_flag = *reinterpret_cast<volatile int*>(p.status) != 0 ? 1 : 0;
+    tma_prefetch_desc(&p.map_q);
+    tma_prefetch_desc(&p.map_pq);
+    if (p.prefix_keys > 0) {
+      tma_prefetch_desc(&p.map_pk);
+      tma_prefetch_desc(&p.map_pv);
+    }
+    if (p.own_keys > 0) {
+      for (int i = 0; i < 2; ++i) {
+        tma_prefetch_desc(&p.map_k[i]);
+        tma_prefetch_desc(&p.map_v[i]);
+      }
+    }
   }
-  make_plan(p, bars);
+  make_plan(p, bars, reinterpret_cast<int2*>(smem + SM::kOut));
   __syncthreads();
   tc_fence_after();
   // no work for this CTA; shares of whole units may also come out empty
@@ -234,8 +241,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
       const int q = lane & 1;  // (of the singles; batches begin with a single of the first stream once the pairs are through)
       int b = bars->b_at[q], cum = bars->cum_at[q];  // this stream's place among the own keys: sequence, tiles in front of it
       int m0 = 0;
-      for (int batch = 0; m0 < n_steps && ok; ++batch) {
-        // a batch: steps m0 .. m0 + count - 1, pairs or singles, in lanes 0 .. count - 1
+      // A batch: steps m0 .. m0 + count - 1, pairs or singles, in lanes 0 .. count - 1.
+      auto publish = [&](int batch) {
         const bool pair = m0 < n_pairs;
         const int count = min(BATCH, (pair ? n_pairs : n_steps) - m0), m = m0 + lane;
         StepRecord r;
@@ -319,11 +326,36 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
         b = __shfl_sync(0xffffffffu, b, last);
         cum = __shfl_sync(0xffffffffu, cum, last);
         if (batch >= 2) ok = mbar_wait(&bars->rec_empty[batch & 1], ((batch >> 1) - 1) & 1, abort_flag);
-        if (!ok) break;
+        if (!ok) return;
         if (lane < count) bars->rec[(batch & 1) * BATCH + lane] = r;
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->rec_full[batch & 1]);
         m0 += count;
+      };
+      publish(0);
+      if (ok && m0 < n_steps) publish(1);
+      uint32_t n_tail = 0;  // parity of the tiles that were cleared, per place in the ring
+      for (int batch = 0, n = 0; n < n_steps && ok; ++batch) {
+        // Keys behind the end carry probability 0, but what lies in their V rows may be anything, and 0 * NaN is NaN: they are cleared here,
+        // when the tile has come (by the warp that issues the MMAs that took 600 to 900 cycles in which nothing was issued).
+        const int count = min(BATCH, (n < n_pairs ? n_pairs : n_steps) - n);
+        for (int i = 0; i < count && ok; ++i, ++n) {
+          const int r0 = (int)(bars->rec[(batch & 1) * BATCH + i].info >> 8) & 255, s = n % STAGES;
+          if (r0 == PN) continue;
+          ok = mbar_wait(&bars->v_tail[s], (n_tail >> s) & 1, abort_flag);
+          if (!ok) break;
+          n_tail ^= 1u << s;
+          uint8_t* vt = smem + SM::kV + s * SM::kTile;
+          constexpr int CPR = HD / 8;
+          for (int k = lane; k < (PN - r0) * CPR; k += 32) {
+            const int r = r0 + k / CPR, c = k % CPR;
+            *reinterpret_cast<uint4*>(vt + (c >> 3) * (PN * 128) + sw128_offset(r, c & 7)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->v_full[s]);
+        }
+        if (ok && m0 < n_steps) publish(batch + 2);
       }
     } else if (warp == W_K || warp == W_V) {
       // =============================== requests of K and V ======================================
@@ -385,9 +417,11 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
             // whole boxes, except at the end of a sequence's own keys: boxes of OWN_BOX rows
             const int unit = own ? OWN_BOX : 1 << shift;
             const uint32_t bytes = (uint32_t)((keys + unit - 1) & ~(unit - 1)) * (HD * 2);
+            uint64_t* bar = &full[s];
             if (is_v) {
               bars->v_info[s] = info;
-              mbar_arrive_expect_tx(&full[s], bytes);
+              if (keys < PN) bar = &bars->v_tail[s];
+              mbar_arrive_expect_tx(bar, bytes);
             } else {
               const bool pair = n < n_pairs;
               const int q = pair ? 0 : (n - n_pairs) & 1;
@@ -427,7 +461,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
               const int row = paged ? (n0 + at) & mask : n0 + at, last = paged ? r.page[at >> shift] : (own ? b : 0);
               const CUtensorMap* map = own ? (whole ? own_map : own_map + 1) : prefix_map;
 #pragma unroll
-              for (int d = 0; d < HD; d += 64) tma_load_4d(dst + (d / 64) * (PN * 128) + at * 128, map, &full[s], d, h, row, last);
+              for (int d = 0; d < HD; d += 64) tma_load_4d(dst + (d / 64) * (PN * 128) + at * 128, map, bar, d, h, row, last);
               at += whole ? 1 << shift : OWN_BOX;
             }
           }
@@ -478,18 +512,6 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
         ok = mbar_wait(&bars->v_full[s], (nv / STAGES) & 1, abort_flag);
         if (!ok) return;
         info = *reinterpret_cast<volatile uint32_t*>(&bars->v_info[s]);
-        const int r0 = (int)(info >> 8) & 255;
-        if (r0 < PN) {
-          // keys behind the end carry probability 0, but what lies in their V rows may be anything, and 0 * NaN is NaN
-          uint8_t* vt = smem + SM::kV + s * SM::kTile;
-          constexpr int CPR = HD / 8;
-          for (int i = lane; i < (PN - r0) * CPR; i += 32) {
-            const int r = r0 + i / CPR, c = i % CPR;
-            *reinterpret_cast<uint4*>(vt + (c >> 3) * (PN * 128) + sw128_offset(r, c & 7)) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
       };
       auto issue_pv = [&](int q) {
         ok = mbar_wait(&bars->p_full[q], n_p[q]++ & 1, abort_flag);
@@ -641,47 +663,47 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
       if (!ok) break;
       tc_fence_after();
       if (!idle) {
-        const float inv = l == 0.f ? 1.f : 1.f / l;
+        // as it is: the merge divides by the sum of all pieces
         const long long at = (long long)g.row0 + row;
         if (live) {
-          p.lse_partial[at] = l == 0.f ? -INFINITY : m_ref * c + log2f(l);
-          if (g.gap) p.lse_partial[at + g.gap] = -INFINITY;
+          p.ml_partial[at] = make_float2(l == 0.f ? -INFINITY : m_ref * c, l);
+          if (g.gap) p.ml_partial[at + g.gap] = make_float2(-INFINITY, 0.f);
         }
-        // 32 columns at a time. The loop stays rolled: a CTA comes here a few times only, and each time the instructions have to be fetched
-        // (unrolled, the first segment's results took 7000 cycles on their way out, rolled X).
-        uint8_t* stage = smem + SM::kOut + warp * 4096;
-        const bool few = g.rows <= 8;
-        const int n_rows = g.rows - (row - lane), c4 = lane & 7;
-        float* const mine = p.out_partial + at * p.D;                      // this lane's row
-        float* const quad = p.out_partial + (at - lane + (lane >> 3)) * p.D + c4 * 4;  // row lane / 8 of the warp, four of the columns
-#pragma unroll 1
-        for (int c0 = 0; c0 < p.D; c0 += 32) {
-          uint32_t o[32];
-          tmem_ld32(tO + c0, o);
+        float* const mine = p.out_partial + at * p.D;  // this lane's row
+        if (g.rows <= 8) {  // a group's few heads: each lane writes its row
+          uint32_t o[HD];
+#pragma unroll
+          for (int ch = 0; ch < HD / 32; ++ch) tmem_ld32(tO + ch * 32, &o[ch * 32]);
           tmem_ld_wait();
-          float4 v[8];
+          if (live) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            v[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv, __uint_as_float(o[4 * i + 2]) * inv,
-                               __uint_as_float(o[4 * i + 3]) * inv);
-          if (few) {  // a group's few heads: each lane writes its row
-            if (live) {
+            for (int i = 0; i < HD; i += 4)
+              if (i < p.D) *reinterpret_cast<uint4*>(mine + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        } else {
+          // 32 columns at a time through shared memory, so that eight lanes write 128 bytes of a row. The loop stays rolled: a CTA comes here once or
+          // twice, and unrolled its instructions took 7000 cycles to arrive, rolled 5000.
+          uint8_t* stage = smem + SM::kOut + warp * 4096;
+          const int n_rows = g.rows - (row - lane), c4 = lane & 7;
+          float* const quad = mine + ((lane >> 3) - lane) * p.D + c4 * 4;  // row lane / 8 of the warp, four of the columns
+#pragma unroll 1
+          for (int c0 = 0; c0 < p.D; c0 += 32) {
+            uint32_t o[32];
+            tmem_ld32(tO + c0, o);
+            tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (c0 + i * 4 < p.D) *reinterpret_cast<float4*>(mine + c0 + i * 4) = v[i];
-            }
-          } else {    // through shared memory, so that eight lanes write 128 bytes of a row
-#pragma unroll
-            for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = v[i];
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             __syncwarp();
+            uint4 v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int r = (lane >> 3) + i * 4;
-              v[i] = *reinterpret_cast<const float4*>(stage + r * 128 + ((c4 ^ (r & 7)) << 4));
+              v[i] = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c4 ^ (r & 7)) << 4));
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              if ((lane >> 3) + i * 4 < n_rows && c0 + c4 * 4 < p.D) *reinterpret_cast<float4*>(quad + i * 4 * p.D + c0) = v[i];
+              if ((lane >> 3) + i * 4 < n_rows && c0 + c4 * 4 < p.D) *reinterpret_cast<uint4*>(quad + i * 4 * p.D + c0) = v[i];
             __syncwarp();
           }
         }
@@ -699,14 +721,14 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
   }
 }
 
-// One warp joins the partial results of a (sequence, query head): the pieces of its item over the prefix and of its own keys' item, from
-// the first to the last that the kernel in front noted. Weights 2^(lse - max), 32 pieces at a time, four rows under way.
-template <typename T, int VEC>
+// WPR warps join the partial results of a (sequence, query head): the pieces of its item over the prefix and of its own keys' item, from
+// the first to the last that the kernel in front noted. A piece has its
+// reference maximum m, its sum l and its O, so o = sum 2^(m - max) O / sum 2^(m - max) l. 32 pieces a warp at a time, four rows under way.
+template <typename T, int VEC, int WPR>
 __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixParams p) {
   after_previous();
-  const int lane = threadIdx.x & 31;
-  const int at = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (at >= p.B * p.Hq) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPR;
+  const int spare = blockIdx.x * (8 / WPR) + warp / WPR, at = min(spare, p.B * p.Hq - 1);  // (spare warps: the last row again)
   const int b = at / p.Hq, head = at - b * p.Hq, h = head / p.G, gi = head - h * p.G, gt = gi / PM;
   // pieces first .. last of the two items: all that is needed to find them is asked for at once
   const int q_tile = p.G > PM ? b * p.head_tiles + gt : b / p.tile_seqs, r = p.G > PM ? gi - gt * PM : (b - q_tile * p.tile_seqs) * p.G + gi;
@@ -717,20 +739,21 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixParams p)
   const bool skip = *reinterpret_cast<volatile int*>(p.status) != 0;
   const int n_pre = min(p.prefix_used ? *p.prefix_used : p.prefix_keys, p.prefix_keys) > 0 ? pre_at.y - pre_at.x + 1 : 0;
   const int n_own = own_keys(p, b) > 0 ? own_at.y - own_at.x + 1 : 0;
-  if (skip) return;
+  if (WPR == 1 && skip) return;
   const int pre_pitch = pair ? 2 * PM : PM, pre_row = (pair ? 0 : (int)p.single_rows) + (pre + pre_at.x) * pre_pitch + r + (pair ? (q_tile & 1) * PM : 0);
   const int own_row = (int)p.own_rows + (own + own_at.x) * p.item_rows + gi - gt * PM;
-  const int count = n_pre + n_own;
+  const int count = skip ? 0 : n_pre + n_own;
   float top = -INFINITY, sum = 0.f, acc[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
   const int d0 = lane * VEC;
   const bool active = d0 < p.D;
   using Row = typename std::conditional<VEC == 4, float4, float2>::type;
-  for (int s0 = 0; s0 < count; s0 += 32) {
-    const int i = s0 + lane, cnt = min(32, count - s0);
+  // this warp's pieces: part, part + WPR, ...
+  for (int s0 = 0; s0 < count; s0 += 32 * WPR) {
+    const int i = s0 + lane * WPR + part, cnt = min(32, (count - s0 - part + WPR - 1) / WPR);
     const int mine = i < n_pre ? pre_row + i * pre_pitch : own_row + (i - n_pre) * p.item_rows;
-    const float lse = i < count ? __ldcg(p.lse_partial + mine) : -INFINITY;
+    const float2 ml = i < count ? __ldcg(p.ml_partial + mine) : make_float2(-INFINITY, 0.f);
     Row v[4];
     auto load4 = [&](int first) {
 #pragma unroll
@@ -740,13 +763,12 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixParams p)
       }
     };
     load4(0);
-    float m = lse;
+    float m = ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     m = fmaxf(m, top);
-    if (__any_sync(0xffffffffu, lse != lse)) m = __int_as_float(0x7fffffff);
-    const float old = top == -INFINITY ? 0.f : exp2f(top - m), w = lse == -INFINITY ? 0.f : exp2f(lse - m);
-    float ws = w;
+    const float old = top == -INFINITY ? 0.f : exp2f(top - m), w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+    float ws = w * ml.y;  // (NaN among a piece's scores: its sum is NaN, and so is the row)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
     sum = sum * old + ws;
@@ -764,6 +786,33 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixParams p)
         for (int k = 0; k < VEC; ++k) acc[k] += wj * e[k];
       }
     }
+  }
+  if constexpr (WPR > 1) {  // the warps' sums, relative to the row's maximum
+    __shared__ float parts[8][32 * VEC + 2];
+    if (lane == 0) {
+      parts[warp][32 * VEC] = top;
+      parts[warp][32 * VEC + 1] = sum;
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) parts[warp][k * 32 + lane] = acc[k];
+    __syncthreads();
+    if (part != 0 || skip) return;
+    float m = top, total = 0.f;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) m = fmaxf(m, parts[warp + w][32 * VEC]);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) {
+      const float tw = parts[warp + w][32 * VEC];
+      if (tw == -INFINITY) continue;
+      const float f = exp2f(tw - m);
+      total += parts[warp + w][32 * VEC + 1] * f;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += parts[warp + w][k * 32 + lane] * f;
+    }
+    top = m;
+    sum = total;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (active) {
@@ -783,7 +832,10 @@ cudaError_t launch_one(const PrefixParams& p, cudaStream_t stream) {
   if (cudaError_t e = smem_opt_in(kern, smem, opted_in); e != cudaSuccess) return e;
   if (p.ctas > 0)  // otherwise there is no place for a key
     if (cudaError_t e = launch_early(kern, (unsigned)p.ctas, P_THREADS, smem, stream, 1, p); e != cudaSuccess) return e;
-  return launch_early(prefix_merge_kernel<T, HD / 32>, (unsigned)(((long long)p.B * p.Hq + 7) / 8), 256, 0, stream, 1, p);
+  // Few rows have many pieces: four warps a row where that still is one wave of blocks (6 sequences x 64 heads, 37 pieces: X us, so Y).
+  const long long rows = (long long)p.B * p.Hq;
+  if (rows <= 2ll * 4 * device_sm_count()) return launch_early(prefix_merge_kernel<T, HD / 32, 4>, (unsigned)((rows + 1) / 2), 256, 0, stream, 1, p);
+  return launch_early(prefix_merge_kernel<T, HD / 32, 1>, (unsigned)((rows + 7) / 8), 256, 0, stream, 1, p);
 }
 
 }  // namespace

@@ -420,7 +420,7 @@ class FsaSharedPrefixArgs(ctypes.Structure):
         ("prefix_seqused", c_void_p),
         ("prefix_page_table", c_void_p),
         ("out_partial", c_void_p),
-        ("lse_partial", c_void_p),
+        ("sum_partial", c_void_p),
         ("plan_ws", c_void_p),
         ("status", c_void_p),
         ("q_stride_b", c_int64),
@@ -461,7 +461,7 @@ class FsaSharedPrefixArgs(ctypes.Structure):
 class FsaSharedPrefixWorkspace(ctypes.Structure):
     _fields_ = [
         ("out_partial", c_size_t),
-        ("lse_partial", c_size_t),
+        ("sum_partial", c_size_t),
         ("plan_ws", c_size_t),
     ]
 

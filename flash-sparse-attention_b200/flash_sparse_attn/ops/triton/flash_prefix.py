@@ -103,10 +103,10 @@ def attn_decode_shared_prefix(query, key, value, prefix_key, prefix_value, softm
     ws = _lib.FsaSharedPrefixWorkspace()
     with torch.cuda.device(device):
         _lib.check(lib.fsa_shared_prefix_workspace_bytes(ctypes.byref(a), ctypes.byref(ws)), "fsa_shared_prefix_workspace_bytes")
-        room = torch.empty((ws.out_partial + ws.lse_partial + ws.plan_ws) // 4, dtype=torch.float32, device=device)
+        room = torch.empty((ws.out_partial + ws.sum_partial + ws.plan_ws) // 4, dtype=torch.float32, device=device)
         a.out_partial = room.data_ptr()
-        a.lse_partial = a.out_partial + ws.out_partial
-        a.plan_ws = a.lse_partial + ws.lse_partial
+        a.sum_partial = a.out_partial + ws.out_partial
+        a.plan_ws = a.sum_partial + ws.sum_partial
         rc = lib.fsa_decode_shared_prefix(ctypes.byref(a), _lib.current_stream_ptr(device))
     _lib.check(rc, "fsa_decode_shared_prefix")
     return out, lse

@@ -355,7 +355,7 @@ typedef struct FsaSharedPrefixArgs {
   const int32_t* prefix_seqused;
   const int32_t* prefix_page_table;
   float* out_partial;
-  float* lse_partial;
+  float* sum_partial;
   int32_t* plan_ws;
   int32_t* status;
   int64_t q_stride_b, q_stride_h, o_stride_b, o_stride_h, lse_stride_b, lse_stride_h;
@@ -370,7 +370,7 @@ typedef struct FsaSharedPrefixArgs {
   float softmax_scale;
 } FsaSharedPrefixArgs;
 typedef struct FsaSharedPrefixWorkspace {
-  size_t out_partial, lse_partial, plan_ws;
+  size_t out_partial, sum_partial, plan_ws;
 } FsaSharedPrefixWorkspace;
 int fsa_shared_prefix_workspace_bytes(const FsaSharedPrefixArgs* args, FsaSharedPrefixWorkspace* sizes);
 int fsa_decode_shared_prefix(const FsaSharedPrefixArgs* args, void* stream);

@@ -365,7 +365,7 @@ def test_refusals():
 
     def call(**kw):
         a = _lib.FsaSharedPrefixArgs()
-        for n in ("q", "k", "v", "prefix_k", "prefix_v", "out", "lse", "status", "out_partial", "lse_partial", "plan_ws"):
+        for n in ("q", "k", "v", "prefix_k", "prefix_v", "out", "lse", "status", "out_partial", "sum_partial", "plan_ws"):
             setattr(a, n, 256)
         a.batch, a.heads_q, a.heads_kv, a.head_dim, a.seqlen_k, a.prefix_seqlen, a.softmax_scale = 2, 4, 1, 64, 10, 10, 1.0
         a.k_stride_s = a.v_stride_s = a.prefix_k_stride_s = a.prefix_v_stride_s = 64
