@@ -28,6 +28,7 @@ decltype(&fsa_fwd) g_fwd = nullptr;
 decltype(&fsa_topk_indices) g_topk = nullptr;
 decltype(&fsa_pack_scales) g_pack = nullptr;
 decltype(&fsa_rotary) g_rotary = nullptr;
+decltype(&fsa_kv_append_rotary_workspace_ints) g_append_ints = nullptr;
 decltype(&fsa_kv_append_rotary) g_append = nullptr;
 decltype(&fsa_shared_prefix_workspace_bytes) g_prefix_bytes = nullptr;
 decltype(&fsa_decode_shared_prefix) g_prefix = nullptr;
@@ -665,7 +666,6 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (out.defined() && (!q.defined() || out.sizes() != q.sizes() || out.scalar_type() != out_type || !flat(out))) return none();
     std::optional<NoGil> no_gil(std::in_place);
     if (q.defined() && !out.defined()) out = at::empty(q.sizes(), q.options().dtype(out_type));
-    const Tensor place = at::empty({2 * batch}, used.options());
     FsaKvAppendRotaryArgs x = {};
     auto put = [](const Tensor& t, int64_t* sb, int64_t* ss, int64_t* sh) {
       *sb = t.dim() == 3 ? 0 : t.stride(0);
@@ -700,7 +700,6 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       x.k_scale = ptr<float>(ks);
       x.v_scale = ptr<float>(vs);
     }
-    x.place_ws = ptr<int32_t>(place);
     x.status = ptr<int32_t>(*g_status[dev.index()]);
     x.table_stride = cos.stride(0);
     x.table_rows = (int)cos.size(0);
@@ -726,6 +725,10 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     x.cache_dtype = cache_code;
     x.interleaved = a[13] == Py_True;
     x.advance = a[17] == Py_True;
+    const int64_t ints = g_append_ints(&x);
+    Tensor place;
+    if (ints > 0) place = at::empty({ints}, used.options());
+    x.place_ws = ptr<int32_t>(place);
     const int rc = g_append(&x, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
     no_gil.reset();
     if (rc != FSA_OK) return PyLong_FromLong(rc);
@@ -857,19 +860,21 @@ PyObject* shared_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// init_cache(addresses of fsa_rotary, fsa_kv_append_rotary, fsa_shared_prefix_workspace_bytes, fsa_decode_shared_prefix)
+// init_cache(addresses of fsa_rotary, fsa_kv_append_rotary_workspace_ints, fsa_kv_append_rotary, fsa_shared_prefix_workspace_bytes,
+//            fsa_decode_shared_prefix)
 PyObject* init_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 4) {
-    PyErr_SetString(PyExc_TypeError, "init_cache takes four addresses");
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "init_cache takes five addresses");
     return nullptr;
   }
-  void* at[4] = {};
+  void* at[5] = {};
   for (Py_ssize_t i = 0; i < n && !PyErr_Occurred(); ++i) at[i] = PyLong_AsVoidPtr(a[i]);
   if (PyErr_Occurred()) return nullptr;
   g_rotary = reinterpret_cast<decltype(g_rotary)>(at[0]);
-  g_append = reinterpret_cast<decltype(g_append)>(at[1]);
-  g_prefix_bytes = reinterpret_cast<decltype(g_prefix_bytes)>(at[2]);
-  g_prefix = reinterpret_cast<decltype(g_prefix)>(at[3]);
+  g_append_ints = reinterpret_cast<decltype(g_append_ints)>(at[1]);
+  g_append = reinterpret_cast<decltype(g_append)>(at[2]);
+  g_prefix_bytes = reinterpret_cast<decltype(g_prefix_bytes)>(at[3]);
+  g_prefix = reinterpret_cast<decltype(g_prefix)>(at[4]);
   return none();
 }
 

@@ -5,10 +5,13 @@
 //     y1 = x1 cos[p, i] - x2 sin[p, i]      y2 = x2 cos[p, i] + x1 sin[p, i]
 //   gradient: the transposed rotation, i.e. the same kernel with -sin.
 //
-// Both are bound by memory: every element is read once and written once, for three operations. A thread takes two chunks of V
-// elements of a head that hold V whole pairs (halves: chunk u and chunk u + rotary_dim / 2V; interleaved: chunks 2u and 2u + 1),
-// so that it needs V angles, and does that for HPT heads of the same token, so that it loads the angles once. V is the widest of
-// 8, 4, 2, 1 elements that sizes, strides and addresses allow. Angles, products and sums are fp32 and rounded once.
+// Both are bound by memory: every element is read once and written once, for three operations. A thread takes two chunks of V elements of a
+// head that hold V whole pairs (chunk u and chunk u + rotary_dim / 2V, which hold the partners of each other's pairs where those are
+// halves apart), so that it needs V angles, and does that for HPT heads of the same token, so that it loads the angles once. V is the
+// widest of 8, 4, 2, 1 elements that sizes, strides and addresses allow. Angles, products and sums are fp32 and rounded once.
+// Measured (copy of as many bytes: 6538 GB/s): 4 x 4096 tokens, 40 heads of 128, both directions 115 us = 5870 GB/s; appending 16 chunks of up to
+// 4000 tokens to a paged cache, 48 heads, 178 us = 5790 GB/s; blocks of 128 threads, of 256 118 and 181; append with six blocks an SM, as many as
+// its registers would leave it (four) 218, eight 208.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -23,6 +26,7 @@ namespace fsa {
 
 namespace {
 
+constexpr int THREADS = 128;
 constexpr int STATUS_NO_ROOM = 3;    // new rows found no page, or lie behind the end of the cache
 constexpr int STATUS_NO_ANGLES = 5;  // a position outside the tables
 
@@ -33,7 +37,6 @@ struct RotaryShape {
   long long table_stride;
   int table_rows, table_dtype;
   int units, turned;  // threads a head; the first `turned` of them hold pairs
-  int second;         // halves: chunks between the two of a pair
   int chunks;         // head_dim / V
 };
 
@@ -57,50 +60,67 @@ union Chunk {
   __device__ Chunk() {}
 };
 
-template <int V>
-__device__ __forceinline__ void load_angles(const RotaryShape& r, long long row, int first, float* c, float* s) {
+// N angles from `first` on.
+template <int N>
+__device__ __forceinline__ void load_some(const RotaryShape& r, long long row, int first, float* c, float* s) {
   const long long at = row * r.table_stride + first;
   if (r.table_dtype == FSA_DT_F32) {
     const float* pc = reinterpret_cast<const float*>(r.cos) + at;
     const float* ps = reinterpret_cast<const float*>(r.sin) + at;
-    if constexpr (V >= 4) {
+    if constexpr (N >= 4) {
 #pragma unroll
-      for (int i = 0; i < V; i += 4) {
+      for (int i = 0; i < N; i += 4) {
         const float4 a = *reinterpret_cast<const float4*>(pc + i), b = *reinterpret_cast<const float4*>(ps + i);
         c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
         s[i] = b.x; s[i + 1] = b.y; s[i + 2] = b.z; s[i + 3] = b.w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
+      for (int i = 0; i < N; ++i) {
         c[i] = pc[i];
         s[i] = ps[i];
       }
     }
   } else if (r.table_dtype == FSA_DT_BF16) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < N; ++i) {
       c[i] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(r.cos)[at + i]);
       s[i] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(r.sin)[at + i]);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < N; ++i) {
       c[i] = __half2float(reinterpret_cast<const __half*>(r.cos)[at + i]);
       s[i] = __half2float(reinterpret_cast<const __half*>(r.sin)[at + i]);
     }
   }
 }
 
+// The V angles of a thread's two chunks at elements a and b.
+template <int V, bool IL>
+__device__ __forceinline__ void load_angles(const RotaryShape& r, long long row, int a, int b, float* c, float* s) {
+  if constexpr (IL && V > 1) {
+    load_some<V / 2>(r, row, a / 2, c, s);
+    load_some<V / 2>(r, row, b / 2, c + V / 2, s + V / 2);
+  } else {
+    load_some<V>(r, row, IL ? a / 2 : a, c, s);
+  }
+}
+
 // Element offsets of a thread's two chunks; the second may lie behind the last column (an odd number of columns to copy).
 template <int V, bool IL>
 __device__ __forceinline__ void chunk_columns(const RotaryShape& r, int u, int& a, int& b, bool& has_b) {
-  if (u < r.turned) {
-    a = IL ? 2 * u : u;
-    b = IL ? 2 * u + 1 : u + r.second;
-  } else {
-    a = 2 * u;  // behind the 2 * turned rotated chunks
+  // neighbouring threads take neighbouring chunks: with both chunks of a thread side by side a warp's requests were full of holes
+  // (packed tokens of 64 columns, neighbouring pairs, both directions: 46.8 us, so 41.4)
+  if (IL && V == 1) {  // a pair is two chunks
+    a = 2 * u;
     b = a + 1;
+  } else if (u < r.turned) {
+    a = u;
+    b = u + r.turned;
+  } else {
+    a = u + r.turned;  // 2 * turned chunks are rotated
+    b = a + r.units - r.turned;
   }
   has_b = b < r.chunks;
   a *= V;
@@ -183,7 +203,7 @@ struct RotaryParams {
 };
 
 template <typename T, int V, bool IL, int HPT>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryParams p) {
   after_previous();
   const unsigned per_token = (unsigned)(p.slots * p.r.units);
   const unsigned idx = blockIdx.x * blockDim.x + threadIdx.x;
@@ -235,7 +255,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   const bool turns = u < p.r.turned;
   float c[V], s[V];
   if (live && turns) {
-    load_angles<V>(p.r, pos, u * V, c, s);
+    load_angles<V, IL>(p.r, pos, a, b, c, s);
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] *= p.sign;
   }
@@ -295,7 +315,7 @@ __device__ __forceinline__ int new_rows(const AppendParams& p, int b) {
 }
 
 // Rows of sequence b that have a slot and angles, by its length alone; what is missing is reported.
-__device__ __forceinline__ int rows_in_reach(const AppendParams& p, int b, int first, int rows) {
+__device__ __forceinline__ int rows_in_reach(const AppendParams& p, int b, int first, int rows, bool report) {
   const long long cap = p.page_table ? (long long)p.max_pages * p.page_size : p.capacity;
   long long n = min((long long)rows, cap - first);
   int why = n < rows ? STATUS_NO_ROOM : 0;
@@ -306,7 +326,7 @@ __device__ __forceinline__ int rows_in_reach(const AppendParams& p, int b, int f
   }
   if (first < 0 || n < 0) n = 0;
   if (first < 0) why = STATUS_NO_ROOM;
-  if (why && rows > 0) atomicExch(p.status, why);
+  if (why && rows > 0 && report) atomicExch(p.status, why);
   return (int)n;
 }
 
@@ -328,7 +348,7 @@ __global__ void __launch_bounds__(1024) append_place_kernel(const AppendParams p
     if (b < p.batch) {
       first = p.used[b];
       const int rows = new_rows(p, b);
-      n = rows > 0 ? rows_in_reach(p, b, first, rows) : 0;
+      n = rows > 0 ? rows_in_reach(p, b, first, rows, sub == 0) : 0;
       if (p.page_table && n > 0) {
         lo = first / p.page_size;
         hi = (first + n - 1) / p.page_size;
@@ -474,7 +494,7 @@ __device__ __forceinline__ void cache_rows(const AppendParams& p, int b, int slo
 }
 
 template <typename T, int V, bool IL, int HPT>
-__global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(THREADS, 6) append_rows_kernel(const AppendParams p) {
   after_previous();
   const unsigned per_token = (unsigned)(p.slots * p.r.units);
   const unsigned idx = blockIdx.x * blockDim.x + threadIdx.x;
@@ -512,13 +532,61 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendParams p) 
     if (live) {
       cache_rows(p, seq, place.x + row, k_row, v_row);
       if (turns)
-        load_angles<V>(p.r, (long long)place.x + row + p.offset + (p.offsets ? p.offsets[seq] : 0), u * V, c, s);
+        load_angles<V, IL>(p.r, (long long)place.x + row + p.offset + (p.offsets ? p.offsets[seq] : 0), a, b, c, s);
     }
   }
 #pragma unroll
   for (int i = 0; i < HPT; ++i)
     if (slot + i * p.slots < heads)
       append_store<T, V, IL>(p, bi, si, slot + i * p.slots, a, b, has_b, turns, live, k_row, v_row, c, s, xa[i], xb[i]);
+}
+
+// Few tokens, pages assigned: a block per sequence finds its slots, stores its rows and advances its length by itself. One launch, where the
+// two kernels above wait for one another (one token each of 64 sequences, 80 heads of 128: 6.1 us, so
+// 4.4; one sequence 5.1 and 3.1).
+constexpr int STEP_PAGES = 4;  // that the new rows of a sequence may touch
+
+template <typename T, int V, bool IL>
+__global__ void __launch_bounds__(1024) append_step_kernel(const AppendParams p) {
+  after_previous();
+  const int b = blockIdx.x, heads = p.heads_q + 2 * p.heads_kv, items = p.new_tokens * heads * p.r.units;
+  const int first = p.used[b];
+  int n = rows_in_reach(p, b, first, p.new_tokens, threadIdx.x == 0);
+  if (p.page_table && n > 0) {
+    const int lo = first / p.page_size, hi = (first + n - 1) / p.page_size;
+    int page[STEP_PAGES];
+#pragma unroll
+    for (int i = 0; i < STEP_PAGES; ++i) page[i] = lo + i <= hi ? p.page_table[b * p.pt_stride + lo + i] : 0;
+    int bad = hi + 1;
+#pragma unroll
+    for (int i = STEP_PAGES - 1; i >= 0; --i)
+      if (lo + i <= hi && (page[i] < 0 || page[i] >= p.num_pages)) bad = lo + i;
+    if (bad <= hi) {
+      n = max(0, bad * p.page_size - first);
+      if (threadIdx.x == 0) atomicExch(p.status, STATUS_NO_ROOM);
+    }
+  }
+  const int at = first + p.offset + (p.offsets ? p.offsets[b] : 0);
+  if (p.advance) {
+    __syncthreads();  // every thread has read the length
+    if (threadIdx.x == 0 && n > 0) p.used[b] = first + n;
+  }
+  for (int k = threadIdx.x; k < items; k += blockDim.x) {
+    const int row = k / (heads * p.r.units), rest = k - row * (heads * p.r.units), h = rest / p.r.units, u = rest - h * p.r.units;
+    int ca, cb;
+    bool has_b;
+    chunk_columns<V, IL>(p.r, u, ca, cb, has_b);
+    Chunk<T, V> xa, xb;
+    append_load<T, V>(p, b, row, h, ca, cb, has_b, xa, xb);
+    const bool live = row < n, turns = u < p.r.turned;
+    float c[V], s[V];
+    long long k_row = 0, v_row = 0;
+    if (live) {
+      cache_rows(p, b, first + row, k_row, v_row);
+      if (turns && h < p.heads_q + p.heads_kv) load_angles<V, IL>(p.r, at + row, ca, cb, c, s);
+    }
+    append_store<T, V, IL>(p, b, row, h, ca, cb, has_b, turns, live, k_row, v_row, c, s, xa, xb);
+  }
 }
 
 // ----------------------------------------------------------------------------------------------
@@ -549,7 +617,6 @@ int make_shape(RotaryShape* r, Width w, const void* cos, const void* sin, long l
   r->table_rows = table_rows;
   r->table_dtype = table_dtype;
   r->turned = rotary_dim / (2 * v);
-  r->second = rotary_dim / (2 * v);
   r->chunks = head_dim / v;
   r->units = r->turned + (r->chunks - 2 * r->turned + 1) / 2;
   return v;
@@ -581,6 +648,13 @@ cudaError_t for_each_form(int dtype, int v, bool interleaved, bool many, F&& f) 
 }
 
 constexpr int HEADS_PER_THREAD = 4;
+
+// Whether append_step_kernel takes the call: rows of equal number, few enough that a block per sequence is no longer at them than the
+// kernels are at being launched (4096 rows of a head, ten microseconds' worth of one block), and nothing to be taken off a stack.
+bool append_in_one_step(const FsaKvAppendRotaryArgs* a) {
+  if (a->cu_seqlens_new || a->free_pages || (long long)a->new_tokens * (a->heads_q + 2ll * a->heads_kv) > 512) return false;
+  return !a->page_table || (a->new_tokens - 1) / a->page_size + 2 <= STEP_PAGES;
+}
 
 }  // namespace
 
@@ -635,18 +709,23 @@ extern "C" int fsa_rotary(const FsaRotaryArgs* a, void* stream_) {
   p.sign = a->transposed ? -1.f : 1.f;
   const bool many = total * p.heads * p.r.units >= 148ll * 2048;
   p.slots = many ? (p.heads + HEADS_PER_THREAD - 1) / HEADS_PER_THREAD : p.heads;
-  const long long blocks = (total * p.slots * p.r.units + 255) / 256;
-  if (blocks * 256 > 0xffffffffll) return FSA_ERR_UNSUPPORTED;  // threads are counted in 32 bits
+  const long long blocks = (total * p.slots * p.r.units + THREADS - 1) / THREADS;
+  if (blocks * THREADS > 0xffffffffll) return FSA_ERR_UNSUPPORTED;  // threads are counted in 32 bits
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const cudaError_t e = for_each_form(a->dtype, v, a->interleaved, many, [&](auto t, auto vv, auto il, auto hpt) {
-    return launch_early(rotary_kernel<decltype(t), vv(), il(), hpt()>, (unsigned)blocks, 256, 0, stream, 1, p);
+    return launch_early(rotary_kernel<decltype(t), vv(), il(), hpt()>, (unsigned)blocks, THREADS, 0, stream, 1, p);
   });
   return e == cudaSuccess ? FSA_OK : FSA_ERR_LAUNCH;
 }
 
+extern "C" int64_t fsa_kv_append_rotary_workspace_ints(const FsaKvAppendRotaryArgs* a) {
+  if (!a || a->batch <= 0 || (a->page_table && a->page_size <= 0)) return 0;
+  return fsa::append_in_one_step(a) ? 0 : 2 * (int64_t)a->batch;
+}
+
 extern "C" int fsa_kv_append_rotary(const FsaKvAppendRotaryArgs* a, void* stream_) {
   using namespace fsa;
-  if (!a || !a->status || !a->k_new || !a->v_new || !a->k_cache || !a->v_cache || !a->seqused_k || !a->place_ws ||
+  if (!a || !a->status || !a->k_new || !a->v_new || !a->k_cache || !a->v_cache || !a->seqused_k ||
       (a->heads_q > 0 && (!a->q || !a->q_out)))
     return FSA_ERR_INVALID_ARG;
   if (a->batch <= 0 || a->heads_q < 0 || a->heads_kv <= 0 || a->head_dim <= 0) return FSA_ERR_INVALID_ARG;
@@ -657,6 +736,7 @@ extern "C" int fsa_kv_append_rotary(const FsaKvAppendRotaryArgs* a, void* stream
   if (!table_ok(a->cos, a->sin, a->table_rows, a->table_dtype, a->head_dim, a->rotary_dim)) return FSA_ERR_INVALID_ARG;
   if (a->page_table ? (a->page_size <= 0 || a->max_pages <= 0 || a->num_pages <= 0) : a->capacity <= 0) return FSA_ERR_INVALID_ARG;
   if ((a->free_pages != nullptr) != (a->free_count != nullptr) || (a->free_pages && !a->page_table)) return FSA_ERR_INVALID_ARG;
+  if (fsa_kv_append_rotary_workspace_ints(a) > 0 && !a->place_ws) return FSA_ERR_INVALID_ARG;
   const long long total = a->cu_seqlens_new ? (long long)a->total : (long long)a->batch * a->new_tokens;
   if (total < 0 || total > 0x7fffffffll) return FSA_ERR_INVALID_ARG;
   if (total == 0) return FSA_OK;
@@ -712,17 +792,25 @@ extern "C" int fsa_kv_append_rotary(const FsaKvAppendRotaryArgs* a, void* stream
   p.advance = a->advance;
   p.cache_dtype = a->cache_dtype;
   const int heads = a->heads_q + 2 * a->heads_kv;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  if (append_in_one_step(a)) {
+    const long long items = (long long)a->new_tokens * heads * p.r.units;
+    const int threads = items >= 1024 ? 1024 : (int)((items + 31) & ~31ll);
+    const cudaError_t e = for_each_form(a->dtype, v, a->interleaved, false, [&](auto t, auto vv, auto il, auto) {
+      return launch_early(append_step_kernel<decltype(t), vv(), il()>, (unsigned)a->batch, threads, 0, stream, 1, p);
+    });
+    return e == cudaSuccess ? FSA_OK : FSA_ERR_LAUNCH;
+  }
   const bool many = total * heads * p.r.units >= 148ll * 2048;
   p.slots = many ? (heads + HEADS_PER_THREAD - 1) / HEADS_PER_THREAD : heads;
-  const long long blocks = (total * p.slots * p.r.units + 255) / 256;
-  if (blocks * 256 > 0xffffffffll) return FSA_ERR_UNSUPPORTED;  // threads are counted in 32 bits
-  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  const long long blocks = (total * p.slots * p.r.units + THREADS - 1) / THREADS;
+  if (blocks * THREADS > 0xffffffffll) return FSA_ERR_UNSUPPORTED;  // threads are counted in 32 bits
   // a warp looks at a sequence's slots where it may have many
   const int lanes = a->page_table && total / a->page_size > 2ll * a->batch ? 32 : 1;
   cudaError_t e = launch_early(append_place_kernel, 1u, 1024, 0, stream, 1, p, lanes);
   if (e != cudaSuccess) return FSA_ERR_LAUNCH;
   e = for_each_form(a->dtype, v, a->interleaved, many, [&](auto t, auto vv, auto il, auto hpt) {
-    return launch_early(append_rows_kernel<decltype(t), vv(), il(), hpt()>, (unsigned)blocks, 256, 0, stream, 1, p);
+    return launch_early(append_rows_kernel<decltype(t), vv(), il(), hpt()>, (unsigned)blocks, THREADS, 0, stream, 1, p);
   });
   return e == cudaSuccess ? FSA_OK : FSA_ERR_LAUNCH;
 }

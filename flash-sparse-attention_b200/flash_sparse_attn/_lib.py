@@ -542,6 +542,8 @@ def load():
     lib.fsa_decode_shared_prefix.argtypes = [POINTER(FsaSharedPrefixArgs), c_void_p]
     lib.fsa_rotary.restype = c_int
     lib.fsa_rotary.argtypes = [POINTER(FsaRotaryArgs), c_void_p]
+    lib.fsa_kv_append_rotary_workspace_ints.restype = c_int64
+    lib.fsa_kv_append_rotary_workspace_ints.argtypes = [POINTER(FsaKvAppendRotaryArgs)]
     lib.fsa_kv_append_rotary.restype = c_int
     lib.fsa_kv_append_rotary.argtypes = [POINTER(FsaKvAppendRotaryArgs), c_void_p]
     lib.fsa_localize_indices.restype = c_int
@@ -593,8 +595,9 @@ def _load_host(lib):
             raise ImportError(f"built for {built_for}, not for {here} (ABI version, torch)")
         host.init(ctypes.cast(lib.fsa_decode, c_void_p).value, ctypes.cast(lib.fsa_fwd, c_void_p).value,
                   ctypes.cast(lib.fsa_topk_indices, c_void_p).value, ctypes.cast(lib.fsa_pack_scales, c_void_p).value)
-        host.init_cache(*(ctypes.cast(f, c_void_p).value for f in (lib.fsa_rotary, lib.fsa_kv_append_rotary,
-                                                                   lib.fsa_shared_prefix_workspace_bytes, lib.fsa_decode_shared_prefix)))
+        host.init_cache(*(ctypes.cast(f, c_void_p).value for f in (
+            lib.fsa_rotary, lib.fsa_kv_append_rotary_workspace_ints, lib.fsa_kv_append_rotary, lib.fsa_shared_prefix_workspace_bytes,
+            lib.fsa_decode_shared_prefix)))
     except (ImportError, AttributeError, TypeError) as e:  # TypeError: a launcher that takes other addresses
         _host = None
         warnings.warn("flash_sparse_attn/_host.so is missing or does not load; calls go through the slower Python launchers until "

@@ -172,8 +172,7 @@ def append_kv_rotary(query: Optional[torch.Tensor], key_new: torch.Tensor, value
     a.seqlen_offsets = _lib.ptr(offsets)
     if fp8:
         a.q_scale, a.k_scale, a.v_scale = _lib.ptr(query_scale), key_scale.data_ptr(), value_scale.data_ptr()
-    place_ws = torch.empty(2 * batch, dtype=torch.int32, device=device)
-    a.place_ws, a.status = place_ws.data_ptr(), _lib.status_word(device).data_ptr()
+    a.status = _lib.status_word(device).data_ptr()
     a.batch, a.heads_kv, a.head_dim = batch, key_new.shape[-2], key_new.shape[-1]
     if cu_seqlens_new is not None:
         a.total = key_new.shape[0]
@@ -186,6 +185,9 @@ def append_kv_rotary(query: Optional[torch.Tensor], key_new: torch.Tensor, value
         a.capacity = key_cache.shape[1]
     a.dtype, a.cache_dtype, a.table_dtype = (_lib.dtype_code(t.dtype) for t in (key_new, key_cache, cos))
     a.interleaved, a.advance = int(interleaved), int(advance)
+    ints = _lib.load().fsa_kv_append_rotary_workspace_ints(ctypes.byref(a))
+    place_ws = torch.empty(ints, dtype=torch.int32, device=device) if ints else None
+    a.place_ws = _lib.ptr(place_ws)
     with torch.cuda.device(device):
         rc = _lib.load().fsa_kv_append_rotary(ctypes.byref(a), _lib.current_stream_ptr(device))
     _lib.check(rc, "fsa_kv_append_rotary")

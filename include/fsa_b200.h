@@ -580,7 +580,7 @@ int fsa_rotary(const FsaRotaryArgs* args, void* stream);
  * Rows without room - no page left, a page number outside [0, num_pages), the end of the table or of the cache - are not stored
  * and set the status word to 3, rows whose position is outside the tables to 5; a sequence keeps the rows in front of the first
  * such one, and the q_out rows of those that are not stored are zeros. With `advance` seqused_k[b] grows by the rows that were
- * stored; without, the lengths stay (layers that share them advance once). place_ws: 2 * batch int32, written by this call.
+ * stored; without, the lengths stay (layers that share them advance once). place_ws: workspace of fsa_kv_append_rotary_workspace_ints() int32.
  */
 typedef struct FsaKvAppendRotaryArgs {
   const void* q;
@@ -617,6 +617,7 @@ typedef struct FsaKvAppendRotaryArgs {
   int32_t dtype, cache_dtype, table_dtype;
   int32_t interleaved, advance;
 } FsaKvAppendRotaryArgs;
+int64_t fsa_kv_append_rotary_workspace_ints(const FsaKvAppendRotaryArgs* args); /* 0: none is needed */
 int fsa_kv_append_rotary(const FsaKvAppendRotaryArgs* args, void* stream);
 
 /* ---- Peer exchange of decode partials (context-parallel decode over the GPUs of one node) -------------------

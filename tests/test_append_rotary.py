@@ -373,7 +373,7 @@ def test_refusals():
             setattr(a, n, v)
         return lib.fsa_kv_append_rotary(ctypes.byref(a), None)
 
-    for kw in (dict(k_new=None), dict(v_cache=None), dict(place_ws=None), dict(heads_q=4), dict(k_new=257), dict(k_cache=257), dict(capacity=0),
+    for kw in (dict(k_new=None), dict(v_cache=None), dict(place_ws=None, free_pages=256, free_count=256, page_table=256, page_size=32, max_pages=1, num_pages=1), dict(heads_q=4), dict(k_new=257), dict(k_cache=257), dict(capacity=0),
                dict(page_table=256, page_size=0, max_pages=1, num_pages=1), dict(page_table=256, page_size=32, max_pages=0, num_pages=1),
                dict(page_table=256, page_size=32, max_pages=1, num_pages=0), dict(free_pages=256, free_count=256),
                dict(page_table=256, page_size=32, max_pages=1, num_pages=1, free_pages=256), dict(cache_dtype=_lib.DT_E4M3),
