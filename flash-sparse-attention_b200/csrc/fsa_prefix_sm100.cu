@@ -36,9 +36,10 @@ constexpr int OWN_BOX = 32;     // rows of the copies at the end of a sequence's
 constexpr int P_THREADS = 384;  // two softmax warpgroups, and one warp each that requests K, issues the MMAs, requests V, plans
 constexpr int W_K = 8, W_ISSUE = 9, W_V = 10, W_PLAN = 11;
 constexpr int BATCH = 16;       // steps that the planner works out at a time, one a lane; it is two batches ahead at most
-// What an SM's time goes to, in units of 500 cycles: a pair of query tiles on a key tile (4000, tensor-bound), a single one (2500 to 2800, its
-// bytes), and what an item of own keys adds (query rows, results on their way out: 256 x 128 keys 3450 a unit, 64 x 1024 2760).
-constexpr int COST_PAIR = 9, COST_SINGLE = 5, COST_ITEM = 1;
+// What an SM's time goes to, in units of about 450 cycles: a pair of query tiles on a key tile (3900 where there are many, tensor-bound; 4800 in
+// short runs), a single one (2400 to 2800, its bytes), and what an item of own keys adds (results on their way out). 256 sequences over 32 768 +
+// up to 256 keys 173 us with 9 / 5 / 2, 178 with 9 / 5 / 1, 177 with 8 / 5 / 2; 64 over 8192 + up to 1024 keys 49.6, 49.5, 51.7.
+constexpr int COST_PAIR = 9, COST_SINGLE = 5, COST_ITEM = 2;
 
 // What a softmax group has to know about the units of one item that it walks.
 struct GroupSegment {

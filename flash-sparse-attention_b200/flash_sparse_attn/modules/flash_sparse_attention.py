@@ -7,15 +7,16 @@ across unchanged. One difference in how the gate inputs are produced: the kernel
 transpose-and-copy of the ``[batch, positions, heads]`` projections (ops/triton/interface.py:646-648).
 Here the two small projections are computed as ``W x^T`` and land in that layout directly; the operator is
 handed a transposed view, for which its own ``.contiguous()`` is a no-op, and autograd routes the gradients
-back through the same views.
+back through the same views. Beyond the reference's layer, ``forward`` takes the tables of rotary positions.
 """
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
 
 from flash_sparse_attn.ops.triton.interface import flash_gated_attn_func
+from flash_sparse_attn.ops.triton.rotary import apply_rotary_func
 
 
 class FlashSparseAttentionConfig:
@@ -65,11 +66,17 @@ class FlashSparseAttention(nn.Module):
         """``[heads, hidden] x [batch, positions, hidden] -> [batch, heads, positions]`` (positions contiguous)."""
         return torch.matmul(weight, hidden_states.transpose(1, 2))
 
-    def forward(self, hidden_states: torch.Tensor, **kwargs):
+    def forward(self, hidden_states: torch.Tensor, rotary: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                position_ids: Optional[torch.Tensor] = None, rotary_interleaved: bool = False, **kwargs):
+        """``rotary``: the tables ``(cos, sin)`` of ``apply_rotary_func``; queries and keys are then turned by their positions (or by
+        ``position_ids``), and the keys that are returned are the turned ones."""
         bsz, seq_len, _ = hidden_states.size()
         query_states = self.q_proj(hidden_states).view(bsz, seq_len, self.num_attention_heads, self.head_dim)
         key_states = self.k_proj(hidden_states).view(bsz, seq_len, self.num_key_value_heads, self.head_dim)
         value_states = self.v_proj(hidden_states).view(bsz, seq_len, self.num_key_value_heads, self.head_dim)
+        if rotary is not None:
+            query_states, key_states = apply_rotary_func(query_states, key_states, *rotary, position_ids=position_ids,
+                                                         interleaved=rotary_interleaved)
         # [B, H, S] buffers, passed as the [B, S, H] views the operator's signature asks for
         alpha_states = self._gate_rows(self.a_proj.weight, hidden_states).transpose(1, 2)
         delta_states = self._gate_rows(self.d_proj.weight, hidden_states).transpose(1, 2)
