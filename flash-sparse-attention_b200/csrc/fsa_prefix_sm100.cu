@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
         if (lane == 0) mbar_arrive(&bars->rec_full[batch & 1]);
         m0 += count;
       };
-      publish(0);
+      if (ok) publish(0);
       if (ok && m0 < n_steps) publish(1);
       uint32_t n_tail = 0;  // parity of the tiles that were cleared, per place in the ring
       for (int batch = 0, n = 0; n < n_steps && ok; ++batch) {
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
           }
           const float m_cand = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m_ref);
           const bool none = m_cand == -INFINITY;  // every score so far is -inf: no reference yet, the exponentials are zeros
-          const bool need = !none && !((m_cand - m_ref) * c <= 8.0f);
+          const bool need = live && !none && !((m_cand - m_ref) * c <= 8.0f);  // (rows that do not exist hold what lay there)
           float scale = 1.0f;
           if (need) {
             scale = ex2_approx((m_ref - m_cand) * c);

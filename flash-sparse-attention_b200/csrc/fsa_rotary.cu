@@ -311,7 +311,7 @@ struct AppendParams {
 };
 
 __device__ __forceinline__ int new_rows(const AppendParams& p, int b) {
-  return p.cu ? p.cu[b + 1] - p.cu[b] : p.new_tokens;
+  return p.cu ? min(p.cu[b + 1], p.total) - p.cu[b] : p.new_tokens;
 }
 
 // Rows of sequence b that have a slot and angles, by its length alone; what is missing is reported.
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(THREADS, 6) append_rows_kernel(const AppendPar
   const bool turns = u < p.r.turned;
   if (live) {
     const int2 place = p.place[seq];
-    live = row < place.y;
+    live = row >= 0 && row < place.y;
     if (live) {
       cache_rows(p, seq, place.x + row, k_row, v_row);
       if (turns)

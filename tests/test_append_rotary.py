@@ -248,6 +248,29 @@ def test_rows_far_into_a_large_cache():
 
 
 @pytest.mark.gpu
+def test_tokens_outside_every_sequence():
+    """Packed bounds that begin behind the first token and end behind the last: nothing is stored that is not there."""
+    from flash_sparse_attn.utils.kvcache import append_kv_rotary
+
+    cos, sin = tables(40, 16)
+    q, k, v = normal(1, 9, 2, 32), normal(2, 9, 1, 32), normal(3, 9, 1, 32)
+    kc = torch.zeros(3, 20, 1, 32, dtype=torch.bfloat16, device=DEV)
+    vc, used = torch.zeros_like(kc), torch.tensor([0, 5, 19], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([2, 4, 4, 30], dtype=torch.int32, device=DEV)
+    out = append_kv_rotary(q, k, v, kc, vc, used, cos, sin, cu_seqlens_new=cu)
+    torch.cuda.synchronize()
+    assert used.tolist() == [2, 5, 20]  # two rows, none, and the one of five that there is room for
+    assert not out[:2].any() and not out[5:].any() and torch.equal(vc[0, :2], v[2:4]) and torch.equal(vc[2, 19], v[4])
+    assert not vc[0, 2:].any() and not vc[1].any() and not vc[2, :19].any()
+    check(out[2:4], *turn(q[2:4], cos[:2], sin[:2], False))
+    check(out[4:5], *turn(q[4:5], cos[19:20], sin[19:20], False))
+    import flash_sparse_attn as fsa
+
+    with pytest.raises(RuntimeError, match="device status 3"):
+        fsa.check_status()
+
+
+@pytest.mark.gpu
 def test_strided_rows_and_result_buffer():
     from flash_sparse_attn.utils.kvcache import append_kv_rotary
 
