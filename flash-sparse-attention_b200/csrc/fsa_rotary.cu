@@ -542,8 +542,8 @@ __global__ void __launch_bounds__(THREADS, 6) append_rows_kernel(const AppendPar
 }
 
 // Few tokens, pages assigned: a block per sequence finds its slots, stores its rows and advances its length by itself. One launch, where the
-// two kernels above wait for one another (one token each of 64 sequences, 80 heads of 128: 6.1 us, so
-// 4.4; one sequence 5.1 and 3.1).
+// two kernels above wait for one another (one token each of 64 sequences, 80 heads of 128: 6.1 us, so 4.4;
+// one sequence 5.1 and 3.1).
 constexpr int STEP_PAGES = 4;  // that the new rows of a sequence may touch
 
 template <typename T, int V, bool IL>
@@ -649,10 +649,13 @@ cudaError_t for_each_form(int dtype, int v, bool interleaved, bool many, F&& f) 
 
 constexpr int HEADS_PER_THREAD = 4;
 
-// Whether append_step_kernel takes the call: rows of equal number, few enough that a block per sequence is no longer at them than the
-// kernels are at being launched (4096 rows of a head, ten microseconds' worth of one block), and nothing to be taken off a stack.
+// Whether append_step_kernel takes the call: rows of equal number, few enough that a block per sequence is no longer at them than a second
+// launch takes, and nothing to be taken off a stack. Rows of 128 columns (query, key and value heads times tokens) of a sequence, one launch
+// and two: 16 sequences 48 rows 2.4 and 4.3 us, 192 rows 4.5 and 4.4, 384 rows 6.4 and 4.6; 256 sequences 3.1 and 4.9, 8.5 and 7.3, 12.4 and
+// 10.9. At 192 rows the host still gains a launch.
+constexpr long long STEP_ELEMENTS = 192 * 128;
 bool append_in_one_step(const FsaKvAppendRotaryArgs* a) {
-  if (a->cu_seqlens_new || a->free_pages || (long long)a->new_tokens * (a->heads_q + 2ll * a->heads_kv) > 512) return false;
+  if (a->cu_seqlens_new || a->free_pages || (long long)a->new_tokens * (a->heads_q + 2ll * a->heads_kv) * a->head_dim > STEP_ELEMENTS) return false;
   return !a->page_table || (a->new_tokens - 1) / a->page_size + 2 <= STEP_PAGES;
 }
 
