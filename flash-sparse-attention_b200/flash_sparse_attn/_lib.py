@@ -661,14 +661,15 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 
 def check_status(device=None):
-    """Synchronise and raise if any kernel launched so far gave up on a bounded wait."""
+    """Synchronise and raise if any kernel launched so far gave up: on a bounded wait, for want of room in a cache or of a position's angles."""
     for key, t in list(_status_words.items()):
         if device is not None and torch.device(device).type != key[0]:
             continue
         v = int(t.item())
         if v != 0:
             t.zero_()
-            raise RuntimeError(f"fsa kernel reported device status {v} (a pipeline wait expired)")
+            why = {3: "no room in the cache, or a page outside the pool", 5: "a position outside the rotary tables"}.get(v, "a pipeline wait expired")
+            raise RuntimeError(f"fsa kernel reported device status {v} ({why})")
 
 
 _profile = {"before": None, "after": None}
