@@ -806,8 +806,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixParams p)
 #pragma unroll
     for (int w = 0; w < WPR; ++w) {
       const float tw = parts[warp + w][32 * VEC];
-      if (tw == -INFINITY) continue;
-      const float f = exp2f(tw - m);
+      const float f = tw == -INFINITY ? 0.f : exp2f(tw - m);  // (without weight, but its sum may be a NaN: 0 * NaN is one)
       total += parts[warp + w][32 * VEC + 1] * f;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[k] += parts[warp + w][k * 32 + lane] * f;

@@ -199,6 +199,30 @@ def test_scores_of_minus_infinity():
 
 
 @pytest.mark.gpu
+def test_nan_stays_with_its_rows():
+    """A NaN in a query, or in a key that counts, makes the rows that meet it NaN and no other, however the pieces are merged."""
+    import flash_sparse_attn as fsa
+
+    g = torch.Generator().manual_seed(2)
+    for batch, prefix in ((3, 600), (3, 40_000), (80, 600), (500, 600)):
+        q = normal(g, batch, 4, 64)
+        pk, pv = normal(g, prefix, 2, 64), normal(g, prefix, 2, 64)
+        k, v = normal(g, batch, 9, 2, 64), normal(g, batch, 9, 2, 64)
+        clean, clean_lse = fsa.flash_dense_attn_with_shared_prefix_func(q, k, v, pk, pv, return_lse=True)
+        for where in ("query", "own key", "prefix key"):
+            q1, k1, pk1, hit = q.clone(), k.clone(), pk.clone(), torch.zeros(batch, 4, dtype=torch.bool, device=DEV)
+            if where == "query":
+                q1[1, 2, 5], hit[1, 2] = torch.nan, True
+            elif where == "own key":
+                k1[2, 8, 1, 3], hit[2, 2:] = torch.nan, True
+            else:
+                pk1[prefix - 1, 0, 63], hit[:, :2] = torch.nan, True
+            out, lse = fsa.flash_dense_attn_with_shared_prefix_func(q1, k1, v, pk1, pv, return_lse=True)
+            assert out[hit].isnan().all() and lse[hit].isnan().all(), where
+            assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit]), where
+
+
+@pytest.mark.gpu
 def test_strides_buffers_streams_and_graphs():
     import flash_sparse_attn as fsa
 
