@@ -570,7 +570,9 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
     return {q_out, k_out};
   }
   static torch::autograd::variable_list turn(const Tensor& q, const Tensor& k, const RotaryCall& c) {
-    const bool records = at::GradMode::is_enabled() && ((q.defined() && q.requires_grad()) || (k.defined() && k.requires_grad()));
+    // (a tangent is seen by the Function, which says that it has none for its results)
+    auto seen = [](const Tensor& t) { return t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined()); };
+    const bool records = seen(q) || seen(k);
     auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     return records ? apply(maybe(q), maybe(k), c) : launch(q, k, c);
   }

@@ -137,17 +137,15 @@ class _Rotary(torch.autograd.Function):
 
 
 def _turn(query, key, *how):
-    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+    if not _unseen() or (torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))):
         return _Rotary.apply(query, key, *how)
     return _launch(query, key, *how)
 
 
-def _native():
-    """The native launcher, where no transform, dual number, trace or compiler wants to see what runs."""
-    if (torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0
-            or torch._C._get_tracing_state() is not None):
-        return None
-    return _lib.native()
+def _unseen() -> bool:
+    """Whether no transform, dual number, trace or compiler wants to see what runs. Those see the Function, which has no tangents and says so."""
+    return not (torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active()
+                or torch.autograd.forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None)
 
 
 def apply_rotary_func(
@@ -173,7 +171,7 @@ def apply_rotary_func(
     Results are computed in fp32 and rounded once; no host synchronisation."""
     if not query.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
-    host = _native()
+    host = _lib.native() if _unseen() else None
     if host is not None:
         res = host.rotary(query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, interleaved)
         if res is not None:

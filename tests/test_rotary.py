@@ -215,6 +215,25 @@ def test_gradients_of_gradients():
 
 
 @pytest.mark.gpu
+def test_tangents_are_refused():
+    """Forward mode has no rule here: it has to be told so, not to lose its tangents. Also in a gradient of gradients."""
+    import torch.autograd.forward_ad as fw
+
+    import flash_sparse_attn as fsa
+
+    cos, sin = tables(9, 16)
+    x, y = normal(1, 1, 9, 2, 32), normal(2, 1, 9, 2, 32).requires_grad_()
+    out = fsa.apply_rotary_func(y, None, cos, sin)
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for q, k in ((dual, None), (x, dual)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                fsa.apply_rotary_func(q, k, cos, sin)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.autograd.grad(out, y, dual)
+
+
+@pytest.mark.gpu
 def test_positions_outside_the_tables_are_reported():
     import flash_sparse_attn as fsa
 
