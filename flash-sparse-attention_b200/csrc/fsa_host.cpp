@@ -639,6 +639,10 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t hkv = k.size(-2), d = k.size(-1), batch = used.numel();
     auto flat = [d](const Tensor& t) { return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1; };
     if (hkv <= 0 || d <= 0 || batch <= 0 || k.numel() == 0 || !flat(k) || !flat(v)) return none();
+    for (const Tensor* t : {&kc, &vc, &used, &table, &free, &out})
+      if (t->defined())
+        for (int64_t i = 0; i < t->dim(); ++i)
+          if (t->size(i) > 1 && t->stride(i) <= 0) return none();
     if (q.defined()) {
       if (q.dim() != dims || q.scalar_type() != type || q.size(-1) != d || q.size(-2) <= 0 || q.size(-2) % hkv || !flat(q)) return none();
       for (int64_t i = 0; i < dims - 2; ++i)

@@ -52,6 +52,9 @@ def _check(query, key, value, prefix_key, prefix_value, softmax_scale, page_tabl
 def attn_decode_shared_prefix(query, key, value, prefix_key, prefix_value, softmax_scale: Optional[float] = None, page_table=None,
                               seqused_k=None, prefix_page_table=None, prefix_seqused=None, out=None, lse=None, skip_checks=False):
     """Returns ``(out, lse)``."""
+    if torch.compiler.is_compiling():  # a launch is not for the compiler to trace: its graph is cut here
+        return torch.compiler.disable(attn_decode_shared_prefix)(query, key, value, prefix_key, prefix_value, softmax_scale, page_table, seqused_k,
+                                                                 prefix_page_table, prefix_seqused, out, lse, skip_checks)
     if not query.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
     host = _lib.native()

@@ -143,9 +143,9 @@ def _turn(query, key, *how):
 
 
 def _unseen() -> bool:
-    """Whether no transform, dual number, trace or compiler wants to see what runs. Those see the Function, which has no tangents and says so."""
-    return not (torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active()
-                or torch.autograd.forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None)
+    """Whether no transform, dual number or trace wants to see what runs. Those see the Function, which has no tangents and says so."""
+    return not (torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0
+                or torch._C._get_tracing_state() is not None)
 
 
 def apply_rotary_func(
@@ -169,6 +169,8 @@ def apply_rotary_func(
 
     Returns new tensors ``(query, key)``, or ``query`` alone with ``key=None``; gradients flow to both, not to the tables.
     Results are computed in fp32 and rounded once; no host synchronisation."""
+    if torch.compiler.is_compiling():  # a launch is not for the compiler to trace: its graph is cut here
+        return torch.compiler.disable(apply_rotary_func)(query, key, cos, sin, seqlen_offsets, position_ids, cu_seqlens, interleaved, skip_checks)
     if not query.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
     host = _lib.native() if _unseen() else None

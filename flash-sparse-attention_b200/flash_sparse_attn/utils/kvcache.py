@@ -63,6 +63,8 @@ def _check_append(query, key_new, value_new, key_cache, value_cache, seqused_k, 
         assert t is None or t.device == device, "All inputs must be on the same device"
     assert key_new.ndim == ndim and key_new.shape == value_new.shape, (
         "key_new and value_new must be [batch, new_tokens, heads, head_dim], or packed [tokens, heads, head_dim] with cu_seqlens_new")
+    for t in (key_cache, value_cache, seqused_k, page_table, free_pages, out):
+        assert t is None or all(n == 1 or s > 0 for n, s in zip(t.shape, t.stride())), "what is written, and page_table, must not be expanded"
     heads_kv, head_dim = key_new.shape[-2:]
     assert key_new.dtype in _F16 and value_new.dtype == key_new.dtype, "new rows must be float16 or bfloat16, of one dtype"
     if query is not None:
@@ -129,6 +131,10 @@ def append_kv_rotary(query: Optional[torch.Tensor], key_new: torch.Tensor, value
     not stored, nor are the rows behind them in their sequence, and their query rows come out as zeros;
     ``flash_sparse_attn.check_status()`` reports it. ``seqused_k`` (int32 [B]) grows by the rows stored, in place; with
     ``advance=False`` it stays, for layers that share the lengths: all but the last. No host synchronisation; no gradients."""
+    if torch.compiler.is_compiling():  # a launch is not for the compiler to trace: its graph is cut here
+        return torch.compiler.disable(append_kv_rotary)(
+            query, key_new, value_new, key_cache, value_cache, seqused_k, cos, sin, page_table, free_pages, free_count, cu_seqlens_new,
+            seqlen_offsets, interleaved, query_scale, key_scale, value_scale, advance, out, skip_checks)
     if not key_new.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
     host = _lib.native()

@@ -378,6 +378,8 @@ def test_refusals():
                 dict(page_table=table.long()), dict(free_pages=table[0]), dict(page_table=table, free_pages=table[0]),
                 dict(cu_seqlens_new=torch.zeros(3, dtype=i32)), dict(cos=cos[:, :16]), dict(out=good["query"][:, :2]),
                 dict(out=good["query"].half()), dict(query=None, out=good["query"]), dict(key_new=good["key_new"].transpose(2, 3).contiguous().transpose(2, 3)),
+                dict(key_cache=good["key_cache"][:, :1].expand(b, 9, hkv, d)), dict(value_cache=good["value_cache"][:1].expand(b, 9, hkv, d)),
+                dict(out=good["query"][:1].expand(b, t, hq, d)), dict(page_table=table[:1].expand(b, 2)),
                 dict(page_table=torch.zeros(2, b, dtype=i32).T[:, :2] if b != 2 else torch.zeros(b, 4, dtype=i32)[:, ::2])):
         with pytest.raises(AssertionError):
             kvcache._check_append(**dict(good, **bad))

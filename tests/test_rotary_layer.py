@@ -67,3 +67,37 @@ def test_layer_calls_the_operator(monkeypatch):
     seen.clear()
     layer(x)
     assert "tables" not in seen and not seen["q"].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore")
+def test_a_compiled_step_is_the_same():
+    """The compiler cuts its graph at the three operators of a step."""
+    import flash_sparse_attn as fsa
+    from flash_sparse_attn.utils.kvcache import append_kv_rotary
+
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(3, 1, h, 64, generator=g).to(torch.bfloat16).to(DEV) for h in (4, 2, 2))
+    pk, pv = (torch.randn(40, 2, 64, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    cos, sin = (torch.randn(60, 32, generator=g).to(DEV) for _ in range(2))
+    weight = torch.randn(3, 1, 4, 64, generator=g).to(torch.bfloat16).to(DEV)
+
+    def step(q, k, v, kc, vc, used):
+        turned = append_kv_rotary(q + 1, k, v, kc, vc, used, cos, sin, seqlen_offsets=40)
+        return fsa.flash_dense_attn_with_shared_prefix_func(turned[:, 0], kc, vc, pk, pv, seqused_k=used) * 2
+
+    def loss(q):
+        return (fsa.apply_rotary_func(q + 1, None, cos, sin) * weight).sum()
+
+    results = []
+    for run in (step, torch.compile(step, backend="eager")):
+        kc, vc = (torch.zeros(3, 8, 2, 64, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        used = torch.tensor([0, 3, 7], dtype=torch.int32, device=DEV)
+        results.append((run(q, k, v, kc, vc, used), kc, vc, used))
+    for run in (loss, torch.compile(loss, backend="eager")):
+        x = q.clone().requires_grad_()
+        results.append((torch.autograd.grad(run(x), x)[0],))
+    torch.cuda.synchronize()
+    fsa.check_status()
+    for a, b in (results[:2], results[2:]):
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
