@@ -37,9 +37,11 @@ constexpr int P_THREADS = 384;  // two softmax warpgroups, and one warp each tha
 constexpr int W_K = 8, W_ISSUE = 9, W_V = 10, W_PLAN = 11;
 constexpr int BATCH = 16;       // steps that the planner works out at a time, one a lane; it is two batches ahead at most
 // What an SM's time goes to, in units of about 450 cycles: a pair of query tiles on a key tile (3900 where there are many, tensor-bound; 4800 in
-// short runs), a single one (2400 to 2800, its bytes), and what an item of own keys adds (results on their way out). 256 sequences over 32 768 +
-// up to 256 keys 173 us with 9 / 5 / 2, 178 with 9 / 5 / 1, 177 with 8 / 5 / 2; 64 over 8192 + up to 1024 keys 49.6, 49.5, 51.7.
-constexpr int COST_PAIR = 9, COST_SINGLE = 5, COST_ITEM = 2;
+// short runs), a single one (2400 to 2800, its bytes), and what an item adds (results on their way out, and the next item's first scores): of own
+// keys, and of a pair, whose 128 KB take 4500 cycles to be written. 256 sequences over 32 768 + up to 256 keys 173 us with 9 / 5 / 2, 178 with
+// 9 / 5 / 1, 177 with 8 / 5 / 2; 64 over 8192 + up to 1024 keys 49.6, 49.5, 51.7. A pair's item at 16 and at 0: 235 sequences over 2 + 645 keys
+// 26.3 and 41.8 us, 148 over 7 + 16 20.1 and 26.0, the two long ones alike.
+constexpr int COST_PAIR = 9, COST_SINGLE = 5, COST_ITEM = 2, COST_PAIR_ITEM = 16;
 
 // What a softmax group has to know about the units of one item that it walks.
 struct GroupSegment {
@@ -129,11 +131,13 @@ __device__ __forceinline__ void make_plan(const PrefixParams& p, PrefixBars* s, 
   if (tid == 0) {
     const int keys = max(0, min(prefix_keys, p.prefix_keys)), tiles = tiles_of(keys);
     const int pairs = p.Hkv * p.pairs * tiles, odd = (p.q_tiles & 1) ? p.Hkv * tiles : 0, singles = odd + total_own * p.items_b;
-    // Equal shares of the cost, in which own items' share is spread over all singles. Every CTA works the same bounds out, so they need not be
+    // Equal shares of the cost, in which items' share is spread over the units of their kind. Every CTA works the same bounds out, so they need not be
     // exact; a share is more than any unit's cost, so that every share between two that hold units of a kind holds one, too.
-    const float pair_cost = (float)COST_PAIR * pairs, single_cost = (float)COST_SINGLE * singles + (float)COST_ITEM * sequences * p.items_b;
-    const float cost = pair_cost + single_cost;
-    const int ctas = (int)fminf((float)p.ctas, fmaxf(cost * (1.f / (COST_PAIR + 1)), fminf(cost, 1.f))), cta = blockIdx.x;
+    const float pair_cost = pairs > 0 ? (float)COST_PAIR * pairs + (float)COST_PAIR_ITEM * p.Hkv * p.pairs : 0.f;
+    const float single_cost = (float)COST_SINGLE * singles + (float)COST_ITEM * sequences * p.items_b, cost = pair_cost + single_cost;
+    const float pairs_per = pairs > 0 ? __fdividef((float)pairs, pair_cost) : 1.f, singles_per = singles > 0 ? __fdividef((float)singles, single_cost) : 1.f;
+    const float most = fmaxf(cost * fminf(pairs_per, singles_per) * 0.95f, 1.f);
+    const int ctas = cost > 0.f ? (int)fminf((float)p.ctas, most) : 0, cta = blockIdx.x;
     s->ctas = ctas;
     s->tiles = tiles;
     s->keys = keys;
@@ -141,11 +145,11 @@ __device__ __forceinline__ void make_plan(const PrefixParams& p, PrefixBars* s, 
     s->b_at[0] = s->b_at[1] = 0;  // (a stream that begins in front of the own keys begins them with the first sequence)
     s->cum_at[0] = s->cum_at[1] = 0;
     if (cta < ctas) {
-      const float share = __fdividef(cost, (float)ctas), per_cost = single_cost > 0.f ? __fdividef((float)singles, single_cost) : 0.f;
+      const float share = __fdividef(cost, (float)ctas);
       auto bounds = [&](int c, int& a, int& x) {
         const float at = share * c, behind = at - pair_cost;
-        a = c == ctas ? pairs : min(pairs, (int)ceilf(at * (1.f / COST_PAIR)));
-        x = c == ctas ? singles : (behind <= 0.f ? 0 : min(singles, (int)ceilf(behind * per_cost)));
+        a = c == ctas ? pairs : min(pairs, (int)ceilf(at * pairs_per));
+        x = c == ctas ? singles : (behind <= 0.f ? 0 : min(singles, (int)ceilf(behind * singles_per)));
       };
       int x0, x1;
       bounds(cta, s->a0, x0);
