@@ -38,8 +38,8 @@ CUtensorMapDataType tma_dtype(int dt) {
 }
 int dtype_bytes(int dt) { return (dt == FSA_DT_BF16 || dt == FSA_DT_FP16) ? 2 : (dt == FSA_DT_F32 ? 4 : 1); }
 
-// 3-D map over the fp32 dQ accumulator [heads, rows, head_dim] with 32 x 32 boxes (one warp's share).
-int make_map_dq(CUtensorMap* map, const float* base, uint64_t head_dim, uint64_t rows, uint64_t heads) {
+// 3-D map over fp32 rows [heads, rows, head_dim] (dQ accumulator; partial results) with 32 x 32 boxes (one warp's share).
+int make_map_rows(CUtensorMap* map, const float* base, uint64_t head_dim, uint64_t rows, uint64_t heads) {
   EncodeTiledFn enc = get_encode();
   if (!enc) return FSA_ERR_NO_DRIVER;
   if (reinterpret_cast<uintptr_t>(base) & 15) return FSA_ERR_INVALID_ARG;
@@ -545,7 +545,7 @@ int fsa_bwd(const FsaBwdArgs* a, void* stream_) {
                    varlen_k ? a->v_stride_s * (int64_t)a->total_k : a->v_stride_b, 64, 1, 128);
     if (rc != FSA_OK) return rc;
   }
-  rc = make_map_dq(&p.map_dq, a->dq_accum, hdk, R, a->heads_q);
+  rc = make_map_rows(&p.map_dq, a->dq_accum, hdk, R, a->heads_q);
   if (rc != FSA_OK) return rc;
   p.lse2_ws = a->lse2_ws;
   p.dpsum_ws = a->dpsum_ws;
@@ -978,6 +978,7 @@ int fsa_decode_shared_prefix(const FsaSharedPrefixArgs* a, void* stream_) {
     if ((rc = make_map4(i ? &p.map_pq : &p.map_q, a->dtype, a->q, p.D, p.G, sh, p.B, sb, p.Hkv, sg, 64, p.item_rows, i ? p.tile_seqs : 1)) != FSA_OK)
       return rc;
   }
+  if (p.partial_rows > 0 && (rc = make_map_rows(&p.map_o, a->out_partial, p.D, p.partial_rows, 1)) != FSA_OK) return rc;
   p.used = a->seqused_k;
   p.page_table = a->page_table;
   p.prefix_used = a->prefix_seqused;

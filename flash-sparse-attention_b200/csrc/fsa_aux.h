@@ -109,6 +109,7 @@ struct alignas(64) PrefixParams {
   CUtensorMap map_q, map_pq;   // the query's rows of one sequence and KV head (at most 128), of the sequences of a tile
   CUtensorMap map_pk, map_pv;  // prefix
   CUtensorMap map_k[2], map_v[2];  // own keys: boxes of a page (at most 128 rows), and of 32 rows
+  CUtensorMap map_o;               // out_partial in boxes of 32 x 32
   const int* used;             // optional [B]: own keys
   const int* page_table;       // optional [B, max_pages]
   const int* prefix_used;      // optional [1]
@@ -124,6 +125,7 @@ struct alignas(64) PrefixParams {
   int B, Hq, Hkv, G, D;
   int tile_seqs, q_tiles, pairs;        // over the prefix: sequences of a query tile, tiles of a KV head, pairs of them
   int head_tiles, items_b, item_rows;   // own keys: tiles of the group's heads, items of a sequence, rows of an item
+  int own_pitch;                        // and of a piece of it in the workspaces
   int q_box, pq_box;                    // bytes of 64 columns of the query rows
   int own_keys, prefix_keys;            // capacities
   int page_size, max_pages, num_pages, prefix_page_size, prefix_pages;

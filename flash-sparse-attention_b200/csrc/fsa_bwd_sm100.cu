@@ -164,9 +164,6 @@ __device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* map, const 
                "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // WHOLE_DQ: the dQ warps take a whole 128-wide tile out of TMEM at once (launch_bwd says where).
 template <int HD, typename T, int KIND, bool WHOLE_DQ>

@@ -33,6 +33,7 @@ namespace {
 constexpr int PM = 128;         // rows of a query tile
 constexpr int PN = 128;         // keys of a key tile
 constexpr int OWN_BOX = 32;     // rows of the copies at the end of a sequence's own keys: no more than that is read in vain behind it
+constexpr int DIRECT_ROWS = 8;  // of results that lanes write themselves; pieces of more have whole boxes of 32 rows
 constexpr int P_THREADS = 384;  // two softmax warpgroups, and one warp each that requests K, issues the MMAs, requests V, plans
 constexpr int W_K = 8, W_ISSUE = 9, W_V = 10, W_PLAN = 11;
 constexpr int BATCH = 16;       // steps that the planner works out at a time, one a lane; it is two batches ahead at most
@@ -295,7 +296,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
               r.info = STEP_OWN | (uint32_t)(i - r.h * p.head_tiles) << 16;
               r.b = b;
               item = b * p.items_b + i;
-              r.row0 = (int)p.own_rows + (item + id) * p.item_rows;
+              r.row0 = (int)p.own_rows + (item + id) * p.own_pitch;
               tiles_all = u;
               item += p.Hkv * (p.pairs + 1);
             }
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
           // which pieces of the item there are, for the merge; a CTA with a single unit has no second stream
           if (t == 0) p.plan_ws[2 * item] = id;
           if (t == tiles_all - 1) p.plan_ws[2 * item + 1] = id;
-          r.gap = !pair && n_singles == 1 && t < tiles_all - 1 ? (own ? p.item_rows : PM) : 0;
+          r.gap = !pair && n_singles == 1 && t < tiles_all - 1 ? (own ? p.own_pitch : PM) : 0;
           const int keys = min(PN, keys_all - t * PN);
           r.n = left;
           r.keys = keys_all - t * PN;
@@ -675,7 +676,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
           if (g.gap) p.ml_partial[at + g.gap] = make_float2(-INFINITY, 0.f);
         }
         float* const mine = p.out_partial + at * p.D;  // this lane's row
-        if (g.rows <= 8) {  // a group's few heads: each lane writes its row
+        if (g.rows <= DIRECT_ROWS) {  // a group's few heads: each lane writes its row
           uint32_t o[HD];
 #pragma unroll
           for (int ch = 0; ch < HD / 32; ++ch) tmem_ld32(tO + ch * 32, &o[ch * 32]);
@@ -686,35 +687,31 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
               if (i < p.D) *reinterpret_cast<uint4*>(mine + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         } else {
-          // 32 columns at a time through shared memory, so that eight lanes write 128 bytes of a row. The loop stays rolled: a CTA comes here once or
-          // twice, and unrolled its instructions took 7000 cycles to arrive, rolled 5000.
+          // 32 columns at a time through shared memory and TMA; the rows of the warp that do not exist belong to the piece, too. (Written by the lanes,
+          // the rows went through L1 three times.) The loop stays rolled: a CTA comes here once or twice, and its instructions have to arrive.
           uint8_t* stage = smem + SM::kOut + warp * 4096;
-          const int n_rows = g.rows - (row - lane), c4 = lane & 7;
-          float* const quad = mine + ((lane >> 3) - lane) * p.D + c4 * 4;  // row lane / 8 of the warp, four of the columns
 #pragma unroll 1
           for (int c0 = 0; c0 < p.D; c0 += 32) {
             uint32_t o[32];
             tmem_ld32(tO + c0, o);
             tmem_ld_wait();
+            if (lane == 0) bulk_wait_read0();
+            __syncwarp();
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            fence_proxy_async_smem();
             __syncwarp();
-            uint4 v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = (lane >> 3) + i * 4;
-              v[i] = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c4 ^ (r & 7)) << 4));
+            if (lane == 0) {
+              tma_store_3d(&p.map_o, stage, c0, g.row0 + row, 0);
+              bulk_commit();
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if ((lane >> 3) + i * 4 < n_rows && c0 + c4 * 4 < p.D) *reinterpret_cast<uint4*>(quad + i * 4 * p.D + c0) = v[i];
-            __syncwarp();
           }
         }
       }
       tc_fence_before();
     }
+    if (lane == 0) bulk_wait0();
   }
 
   tc_fence_before();
@@ -746,7 +743,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixParams p)
   const int n_own = own_keys(p, b) > 0 ? own_at.y - own_at.x + 1 : 0;
   if (WPR == 1 && skip) return;
   const int pre_pitch = pair ? 2 * PM : PM, pre_row = (pair ? 0 : (int)p.single_rows) + (pre + pre_at.x) * pre_pitch + r + (pair ? (q_tile & 1) * PM : 0);
-  const int own_row = (int)p.own_rows + (own + own_at.x) * p.item_rows + gi - gt * PM;
+  const int own_row = (int)p.own_rows + (own + own_at.x) * p.own_pitch + gi - gt * PM;
   const int count = skip ? 0 : n_pre + n_own;
   float top = -INFINITY, sum = 0.f, acc[VEC];
 #pragma unroll
@@ -757,7 +754,7 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixParams p)
   // this warp's pieces: part, part + WPR, ...
   for (int s0 = 0; s0 < count; s0 += 32 * WPR) {
     const int i = s0 + lane * WPR + part, cnt = min(32, (count - s0 - part + WPR - 1) / WPR);
-    const int mine = i < n_pre ? pre_row + i * pre_pitch : own_row + (i - n_pre) * p.item_rows;
+    const int mine = i < n_pre ? pre_row + i * pre_pitch : own_row + (i - n_pre) * p.own_pitch;
     const float2 ml = i < count ? __ldcg(p.ml_partial + mine) : make_float2(-INFINITY, 0.f);
     Row v[4];
     auto load4 = [&](int first) {
@@ -853,6 +850,7 @@ bool prefix_shape(PrefixParams* p) {
   p->pairs = p->q_tiles / 2;
   p->items_b = p->Hkv * p->head_tiles;
   p->item_rows = p->G < PM ? p->G : PM;
+  p->own_pitch = p->item_rows <= DIRECT_ROWS ? p->item_rows : (p->item_rows + 31) & ~31;
   p->q_box = 64 * p->item_rows * 2;
   p->pq_box = p->q_box * p->tile_seqs;
   auto tiles = [](long long keys) { return (keys + PN - 1) / PN; };
@@ -863,7 +861,7 @@ bool prefix_shape(PrefixParams* p) {
   p->single_rows = p->prefix_keys > 0 ? ((long long)p->Hkv * p->pairs + p->ctas) * (2 * PM) : 0;
   if (p->pairs == 0) p->single_rows = 0;
   p->own_rows = p->single_rows + ((p->q_tiles & 1) && p->prefix_keys > 0 ? ((long long)p->Hkv + 2 * p->ctas) * PM : 0);
-  p->partial_rows = p->own_rows + (p->own_keys > 0 ? ((long long)p->B * p->items_b + 2 * p->ctas) * p->item_rows : 0);
+  p->partial_rows = p->own_rows + (p->own_keys > 0 ? ((long long)p->B * p->items_b + 2 * p->ctas) * p->own_pitch : 0);
   if (p->partial_rows >= (1ll << 31)) return false;
   p->plan_ints = 2 * ((long long)p->Hkv * (p->pairs + 1) + (long long)p->B * p->items_b);
   return true;
