@@ -39,9 +39,9 @@ constexpr int W_K = 8, W_ISSUE = 9, W_V = 10, W_PLAN = 11;
 constexpr int BATCH = 16;       // steps that the planner works out at a time, one a lane; it is two batches ahead at most
 // What an SM's time goes to, in units of about 450 cycles: a pair of query tiles on a key tile (3900 where there are many, tensor-bound; 4800 in
 // short runs), a single one (2400 to 2800, its bytes), and what an item adds (results on their way out, and the next item's first scores): of own
-// keys, and of a pair, whose 128 KB take 4500 cycles to be written. 256 sequences over 32 768 + up to 256 keys 173 us with 9 / 5 / 2, 178 with
-// 9 / 5 / 1, 177 with 8 / 5 / 2; 64 over 8192 + up to 1024 keys 49.6, 49.5, 51.7. A pair's item at 16 and at 0: 235 sequences over 2 + 645 keys
-// 26.3 and 41.8 us, 148 over 7 + 16 20.1 and 26.0, the two long ones alike.
+// keys, and of a pair, whose 128 KB take 2000 to 2700 cycles to be written. 256 sequences over 32 768 + up to 256 keys 173 us with 9 / 5 / 2, 178 with
+// 9 / 5 / 1, 177 with 8 / 5 / 2; 64 over 8192 + up to 1024 keys 49.6, 49.5, 51.7. A pair's item at 16 and at 8: 235 sequences over 2 + 645 keys
+// 25.6 and 30.6 us (41.8 at 0, with slower stores), 148 over 7 + 16 19.5 and 20.1, 64 over 500 + 200 24.2 and 21.2, the two long ones alike.
 constexpr int COST_PAIR = 9, COST_SINGLE = 5, COST_ITEM = 2, COST_PAIR_ITEM = 16;
 
 // What a softmax group has to know about the units of one item that it walks.
