@@ -5,7 +5,7 @@
 // Over the prefix, the rows r = (sequence, query head of the group) of one KV head meet the same keys: with them on the M side of tcgen05 the
 // prefix is read once for all sequences, where a decode of each would read it `batch` times. Over a sequence's own keys only the G heads
 // of the group share them; those tiles run through the same pipeline with G of 128 rows filled: a key tile's 64 KB take an SM's share of
-// HBM about 2900 cycles, its two products and one warp's softmax fewer.
+// HBM about 2900 cycles where all SMs ask for them, its two products and one warp's softmax fewer.
 //
 // The work is a list of units of one key tile each (128 keys of one KV head):
 //   pairs     prefix tile x two query tiles, for every KV head and pair of query tiles (a tile: the rows of as many sequences as
@@ -37,12 +37,13 @@ constexpr int DIRECT_ROWS = 8;  // of results that lanes write themselves; piece
 constexpr int P_THREADS = 384;  // two softmax warpgroups, and one warp each that requests K, issues the MMAs, requests V, plans
 constexpr int W_K = 8, W_ISSUE = 9, W_V = 10, W_PLAN = 11;
 constexpr int BATCH = 16;       // steps that the planner works out at a time, one a lane; it is two batches ahead at most
-// What an SM's time goes to, in units of about 450 cycles: a pair of query tiles on a key tile (3900 where there are many, tensor-bound; 4800 in
-// short runs), a single one (2400 to 2800, its bytes), and what an item adds (results on their way out, and the next item's first scores): of own
-// keys, and of a pair, whose 128 KB take 2000 to 2700 cycles to be written. 256 sequences over 32 768 + up to 256 keys 173 us with 9 / 5 / 2, 178 with
-// 9 / 5 / 1, 177 with 8 / 5 / 2; 64 over 8192 + up to 1024 keys 49.6, 49.5, 51.7. A pair's item at 16 and at 8: 235 sequences over 2 + 645 keys
-// 25.6 and 30.6 us (41.8 at 0, with slower stores), 148 over 7 + 16 19.5 and 20.1, 64 over 500 + 200 24.2 and 21.2, the two long ones alike.
-constexpr int COST_PAIR = 9, COST_SINGLE = 5, COST_ITEM = 2, COST_PAIR_ITEM = 16;
+// What an SM's time goes to, in units of about 220 cycles: a pair of query tiles on a key tile (3900), a single one (1950 while others work on pairs
+// and leave HBM to it: own keys alone come at 6.0 TB/s on 96 SMs, 1950 cycles a tile, at 3.6 on 48, 1640, and at 6.3 on 148), and what an item adds (results on
+// their way out, and the next item's first scores): of own keys, and of a pair, whose 128 KB take 2000 to 2700 cycles to be written.
+// With 18 / 9 / 4 / 32, 18 / 10 / 4 / 32, 18 / 8 / 4 / 32 and 18 / 9 / 8 / 32: 64 sequences over 8192 + up to 1024 keys 46.5, 46.3, 46.4, 46.1 us;
+// 256 over 1000 + 100 45.5, 46.7, 44.7, 50.3; 100 over 20 000 + 1000 57.8, 61.2, 61.3, 60.4; 256 over 32 768 + up to 256 173, 172, 180, 176. A pair's
+// item at half as much: 235 over 2 + up to 645 keys 30 us instead of 25, at none 42.
+constexpr int COST_PAIR = 18, COST_SINGLE = 9, COST_ITEM = 4, COST_PAIR_ITEM = 32;
 
 // What a softmax group has to know about the units of one item that it walks.
 struct GroupSegment {
