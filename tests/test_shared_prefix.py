@@ -131,6 +131,15 @@ def test_rows_and_groups(batch, hq, hkv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("group", [8, 9, 12, 16, 31, 32, 33, 48, 63, 64, 65, 127, 129, 136])
+def test_results_in_boxes_of_rows(group):
+    """Pieces of a group's rows are written 32 rows and 32 columns at a time where there are more than eight: neighbours stay as they are."""
+    run(23, 300, [(37 * i) % 400 for i in range(23)], 2 * group, 2, 80)
+    run(90, 0, [1 + i % 3 for i in range(90)], 2 * group, 2, 48, torch.float16)
+    run(3, 3000, [130, 0, 700], 2 * group, 2, 128)
+
+
+@pytest.mark.gpu
 def test_many_items_with_few_tiles():
     """More items than CTAs, one key tile each: shares that hold several items."""
     run(600, 100, 1, 32, 32, 64)
