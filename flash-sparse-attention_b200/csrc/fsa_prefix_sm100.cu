@@ -11,9 +11,10 @@
 //   pairs     prefix tile x two query tiles, for every KV head and pair of query tiles (a tile: the rows of as many sequences as
 //             fit 128, or 128 heads of one)
 //   singles   prefix tile x the last query tile, where their number is odd; own tile x the G rows of its sequence
-// It is cut into shares of equal cost, one per CTA (one CTA an SM), at any unit: a share may end inside an item (the units of the same rows and
-// KV head) and begin the next, and every piece of an item leaves a partial result - its O, reference maximum and sum -
-// that prefix_merge_kernel joins. Lengths live on the device: every CTA works its share out from them.
+// It is cut into shares of equal cost, one per CTA (one CTA an SM): items of pairs (an item: the units of the same rows and KV head)
+// in equal pieces where that comes out, otherwise at any unit, so that a share may end inside an item and begin the next. Every piece
+// of an item leaves a partial result - its O, reference maximum and sum - that prefix_merge_kernel joins. Lengths live on the device:
+// every CTA works its share out from them.
 //
 // In a CTA two softmax warpgroups, each with a score tile and an accumulator in TMEM, alternate on the tensor pipe. They share the
 // key tile of a pair; of the singles each walks its own half of the share ("stream"), tile by tile in turn.
@@ -81,6 +82,7 @@ struct PrefixBars {
   // begins among the own keys and the tiles in front of it
   int a0, a1, s[3], b_at[2], cum_at[2];
   int ctas, tiles, keys, singles_prefix;
+  int pair_id;  // number of this CTA's piece of pairs: those of an item follow one another
 };
 template <int HD>
 struct PrefixSmem {
@@ -105,7 +107,7 @@ __device__ __forceinline__ int tiles_of(int keys) { return (keys + PN - 1) / PN;
 // This CTA's share of the work, by all threads.
 __device__ __forceinline__ void make_plan(const PrefixParams& p, PrefixBars* s, int2* warp_sum) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int prefix_keys = tid == 0 && p.prefix_used ? *p.prefix_used : p.prefix_keys;
+  const int prefix_keys = warp == 0 && p.prefix_used ? *p.prefix_used : p.prefix_keys;
   const int chunk = (p.B + P_THREADS - 1) / P_THREADS, b0 = tid * chunk, b1 = min(p.B, b0 + chunk);
   int mine = 0, some = 0;  // tiles, and sequences that have any
   for (int b = b0; b < b1; ++b) {
@@ -130,7 +132,7 @@ __device__ __forceinline__ void make_plan(const PrefixParams& p, PrefixBars* s, 
     total_own += v.x;
     sequences += v.y;
   }
-  if (tid == 0) {
+  if (warp == 0) {
     const int keys = max(0, min(prefix_keys, p.prefix_keys)), tiles = tiles_of(keys);
     const int pairs = p.Hkv * p.pairs * tiles, odd = (p.q_tiles & 1) ? p.Hkv * tiles : 0, singles = odd + total_own * p.items_b;
     // Equal shares of the cost, in which items' share is spread over the units of their kind. Every CTA works the same bounds out, so they need not be
@@ -139,25 +141,65 @@ __device__ __forceinline__ void make_plan(const PrefixParams& p, PrefixBars* s, 
     const float single_cost = (float)COST_SINGLE * singles + (float)COST_ITEM * sequences * p.items_b, cost = pair_cost + single_cost;
     const float pairs_per = pairs > 0 ? __fdividef((float)pairs, pair_cost) : 1.f, singles_per = singles > 0 ? __fdividef((float)singles, single_cost) : 1.f;
     const float most = fmaxf(cost * fminf(pairs_per, singles_per) * 0.95f, 1.f);
-    const int ctas = cost > 0.f ? (int)fminf((float)p.ctas, most) : 0, cta = blockIdx.x;
-    s->ctas = ctas;
-    s->tiles = tiles;
-    s->keys = keys;
-    s->singles_prefix = odd;
-    s->b_at[0] = s->b_at[1] = 0;  // (a stream that begins in front of the own keys begins them with the first sequence)
-    s->cum_at[0] = s->cum_at[1] = 0;
-    if (cta < ctas) {
-      const float share = __fdividef(cost, (float)ctas);
-      auto bounds = [&](int c, int& a, int& x) {
-        const float at = share * c, behind = at - pair_cost;
-        a = c == ctas ? pairs : min(pairs, (int)ceilf(at * pairs_per));
-        x = c == ctas ? singles : (behind <= 0.f ? 0 : min(singles, (int)ceilf(behind * singles_per)));
-      };
-      int x0, x1;
-      bounds(cta, s->a0, x0);
-      bounds(cta + 1, s->a1, x1);
-      s->s[0] = x0;
-      s->s[1] = x0 + (x1 - x0 + 1) / 2;
+    int ctas = cost > 0.f ? (int)fminf((float)p.ctas, most) : 0;
+    const int cta = blockIdx.x, items = p.Hkv * p.pairs;
+    float share = ctas > 0 ? __fdividef(cost, (float)ctas) : 0.f;
+    // Where there are no more items of pairs than CTAs, each is cut into `cuts` equal pieces, one a CTA, and the pieces of a KV head over the same keys go to
+    // neighbours, that read them at the same time. What their shares have left is singles, if it is some for each; if not, the other CTAs take
+    // those. It is not done where the pieces come out too uneven. 256 sequences over 32 768 + up to 256 keys 172 us where pieces lie anywhere, so 159;
+    // 256 over 16 000 + 64 103 and 96, 64 over 8192 + up to 1024 46.3 and 45.6; small calls gain or lose up to 8 % (40 over 4000 + 200 19.4 and 21.0,
+    // 64 over 500 + 200 24.0 and 21.1).
+    int cuts = 0, own_from = 0;  // own_from: CTAs that have no singles
+    float cut_tiles = 0.f;
+    if (pairs > 0 && items <= ctas && cost < 16777216.f) {  // (sums of costs are exact)
+      cuts = min(min((int)ceilf(__fdividef((float)(COST_PAIR * tiles), fmaxf(share - 0.5f * COST_PAIR_ITEM, 1.f))), tiles), (int)__fdividef((float)ctas + 0.5f, (float)items));
+      cut_tiles = tiles == cuts ? 1.f : __fdividef((float)tiles, (float)cuts);  // (more than one by more than its error)
+      const float piece = COST_PAIR * ceilf(cut_tiles) + COST_PAIR_ITEM, even = __fdividef(cost + (float)COST_PAIR_ITEM * items * (cuts - 1), (float)ctas);
+      const int rest = min(ctas - cuts * items, max(singles - (singles + 15) / 16, min(singles, 1)));  // CTAs for singles alone: more than one each
+      const float alone = singles > 0 ? (rest > 0 ? __fdividef(single_cost, (float)rest) : cost) : 0.f, limit = even + 0.5f * COST_PAIR_ITEM;
+      if ((even - piece) * singles_per >= 4.f) {
+        share = even;
+      } else if (fmaxf(piece, alone) <= limit) {
+        own_from = cuts * items;
+        ctas = own_from + rest;
+        share = alone;
+      } else {
+        cuts = 0;
+      }
+    }
+    // lane 0: this CTA's bounds, lane 1: the next one's
+    const int c = cta + (lane & 1);
+    int a = 0, x, id = cta;
+    float behind = share * c - pair_cost;  // of the cost, what is singles'
+    if (cuts == 0) {
+      a = c == ctas ? pairs : min(pairs, (int)ceilf(share * c * pairs_per));
+    } else {
+      auto start = [&](int cut) { return cut == cuts ? tiles : (int)(cut * cut_tiles); };  // first tile of a piece
+      const int n = min(c, cuts * items), group = p.pairs * cuts, h = (int)__fdividef(n + 0.5f, (float)group), left = n - h * group;
+      const int cut = (int)__fdividef(left + 0.5f, (float)p.pairs), pair = left - cut * p.pairs, item = h * p.pairs + pair, from = start(cut);
+      // pairs of the CTAs in front; the piece itself, as units of its item (lane 1 has its end)
+      const int before = (h * tiles + from) * p.pairs + (n < cuts * items ? pair * (start(cut + 1) - from) : 0);
+      behind = own_from > 0 ? share * (c - own_from) : share * c - (float)COST_PAIR * before - (float)COST_PAIR_ITEM * n;
+      id = item * cuts + cut;
+      a = item * tiles + from;
+      const int end = item * tiles + start(cut + 1), end0 = __shfl_sync(0xffffffffu, end, 0);
+      if (lane & 1) a = end0;
+      if (cta >= cuts * items) a = 0;
+    }
+    x = c == ctas ? singles : (behind <= 0.f ? 0 : min(singles, (int)ceilf(behind * singles_per)));
+    const int a1 = __shfl_sync(0xffffffffu, a, 1), x1 = __shfl_sync(0xffffffffu, x, 1);
+    if (lane == 0) {
+      s->ctas = ctas;
+      s->tiles = tiles;
+      s->keys = keys;
+      s->singles_prefix = odd;
+      s->b_at[0] = s->b_at[1] = 0;  // (a stream that begins in front of the own keys begins them with the first sequence)
+      s->cum_at[0] = s->cum_at[1] = 0;
+      s->a0 = a;
+      s->a1 = a1;
+      s->pair_id = id;
+      s->s[0] = x;
+      s->s[1] = x + (x1 - x + 1) / 2;
       s->s[2] = x1;
     }
   }
@@ -263,7 +305,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
             t = pos - item * tiles;
             r.h = item / p.pairs;
             r.b = 2 * (item - r.h * p.pairs);
-            id = blockIdx.x;
+            id = bars->pair_id;
             r.row0 = (item + id) * (2 * PM);
             keys_all = bars->keys;
             tiles_all = tiles;
