@@ -147,6 +147,14 @@ def test_many_items_with_few_tiles():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,prefix,own,hq,hkv", [(256, 4000, 4, 8, 2), (520, 20000, 1, 1, 1), (200, 2500, 199, 4, 1), (520, 3000, 300, 1, 1),
+                                                     (600, 100, 1, 32, 32), (128, 700, 3000, 4, 2), (64, 1500, 3000, 8, 2), (130, 9000, 3, 16, 16)])
+def test_shares(batch, prefix, own, hq, hkv):
+    """Pairs of query tiles in equal pieces, one a CTA, with the own keys on the other CTAs, behind the pieces, and cut anywhere."""
+    run(batch, prefix, [(97 * i) % (own + 1) for i in range(batch)], hq, hkv, 64)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("page,prefix_page", [(0, 32), (32, 0), (32, 32), (64, 128), (128, 64), (256, 256)])
 @pytest.mark.parametrize("prefix", [1, 31, 256, 1111])
 def test_pages(page, prefix_page, prefix):
