@@ -171,7 +171,8 @@ __device__ __forceinline__ void store8(void* base, long long at, const float* y,
   *reinterpret_cast<typename Raw<V>::type*>(reinterpret_cast<uint8_t*>(base) + at) = o.raw;
 }
 
-// The sequence that packed token t belongs to (cu[b] <= t < cu[b + 1]), or `batch` behind the last one.
+// The sequence that packed token t belongs to (cu[b] <= t < cu[b + 1]), or `batch` behind the last one. In front of the first one: 0, in
+// which it has a negative place.
 __device__ __forceinline__ int sequence_of(const int* cu, int batch, int t) {
   if (t >= cu[batch]) return batch;
   int lo = 0, hi = batch;  // cu[lo] <= t < cu[hi]
@@ -244,6 +245,7 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryParams p) {
       seq = sequence_of(p.cu, p.batch, (int)t);
       live = seq < p.batch;
       if (live) pos -= p.cu[seq];
+      live = live && pos >= 0;
     }
     pos += p.offset;
     if (p.offsets && live) pos += p.offsets[seq];
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryParams p) {
       store16<T, V>(dst, a, ya);
       store16<T, V>(dst, b, yb);
     } else {
-      if (!live) {  // tokens behind the last sequence, or without angles: zeros
+      if (!live) {  // tokens outside every sequence, or without angles: zeros
         xa[i].raw = {};
         xb[i].raw = {};
       }

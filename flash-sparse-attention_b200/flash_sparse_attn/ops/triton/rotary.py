@@ -164,7 +164,7 @@ def apply_rotary_func(
     head: pairs ``(i, i + R / 2)``, or neighbours ``(2i, 2i + 1)`` with ``interleaved``; the other columns are copied.
 
     A token's position is its place in its sequence plus ``seqlen_offsets`` (an int, or int32 ``[B]``), or its entry of
-    ``position_ids`` (int32 / int64, ``[B, S]``, ``[1, S]`` or ``[T]``). Tokens behind the last packed sequence come out as zeros,
+    ``position_ids`` (int32 / int64, ``[B, S]``, ``[1, S]`` or ``[T]``). Packed tokens outside every sequence come out as zeros,
     and so do tokens whose position is outside the tables, which ``flash_sparse_attn.check_status()`` reports (status 5).
 
     Returns new tensors ``(query, key)``, or ``query`` alone with ``key=None``; gradients flow to both, not to the tables.

@@ -543,7 +543,7 @@ int fsa_kv_append(const FsaKvAppendArgs* args, void* stream);
  *   tables    cos, sin [table_rows, rotary_dim / 2], rows table_stride apart, fp32 or 16 bits (table_dtype)
  *   position  place in the sequence + offset + seqlen_offsets[sequence] (optional), or position_ids (optional, int32 or
  *             int64) as they are
- * Tokens behind the last sequence come out as zeros; so do tokens whose position is outside the tables, which also set the
+ * Packed tokens outside every sequence come out as zeros; so do tokens whose position is outside the tables, which also set the
  * status word to 5. q_out may be q and k_out may be k (same strides).
  */
 typedef struct FsaRotaryArgs {

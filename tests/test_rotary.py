@@ -315,3 +315,24 @@ def test_refusals():
                dict(rotary_dim=0), dict(table_rows=0), dict(batch=0), dict(heads_q=0), dict(heads_k=1), dict(seqlen=-1), dict(table_dtype=2)):
         assert call(**kw) == -1, kw
     assert call(dtype=_lib.DT_F32) == -2 and call(seqlen=0) == 0 and call(batch=1 << 20, seqlen=2047, heads_q=1 << 9) == -2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [0, 5, "tensor"])
+def test_packed_tokens_outside_every_sequence(offset):
+    """Bounds that begin behind the first token and end in front of the last: those tokens are in no sequence and have no position,
+    whatever is added to it. They come out as zeros, and so do their gradients."""
+    import flash_sparse_attn as fsa
+
+    cos, sin = tables(12, 16)
+    q, k = normal(1, 11, 4, 32).requires_grad_(), normal(2, 11, 2, 32)
+    cu = torch.tensor([3, 3, 5, 5, 9], dtype=torch.int32, device=DEV)
+    more = [5, 3, 1, 7] if offset == "tensor" else [offset] * 4
+    kw = dict(seqlen_offsets=torch.tensor(more, dtype=torch.int32, device=DEV) if offset == "tensor" else offset)
+    oq, ok = fsa.apply_rotary_func(q, k, cos, sin, cu_seqlens=cu, **kw)
+    (dq,) = torch.autograd.grad(oq, q, torch.ones_like(oq))
+    done()
+    at = torch.tensor([more[1], more[1] + 1, *range(more[3], more[3] + 4)])
+    for got, x, sign in ((oq.detach(), q.detach(), 1), (ok, k, 1), (dq, torch.ones_like(q), -1)):
+        assert not got[:3].any() and not got[9:].any()
+        check(got[3:9], *turn(x[3:9], cos[at], sin[at], False, sign))
