@@ -615,6 +615,11 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// What a kernel wrote in place: a graph that kept it for its gradient has to notice (tensors of inference mode are in no graph).
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // append(q, k_new, v_new, k_cache, v_cache, seqused_k, cos, sin, page_table, free_pages, free_count, cu_seqlens_new, seqlen_offsets,
 //        interleaved, q_scale, k_scale, v_scale, advance, out) -> the turned queries (True without queries), an error code, or None
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -736,6 +741,10 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (ints > 0) place = at::empty({ints}, used.options());
     x.place_ws = ptr<int32_t>(place);
     const int rc = g_append(&x, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+    if (rc == FSA_OK) {
+      if (x.advance) written(used);
+      if (a[18] != Py_None) written(out);
+    }
     no_gil.reset();
     if (rc != FSA_OK) return PyLong_FromLong(rc);
     if (!q.defined()) Py_RETURN_TRUE;

@@ -13,6 +13,12 @@ from flash_sparse_attn import _lib
 from flash_sparse_attn.ops.triton.rotary import check_tables, split_offsets
 
 
+def _written(t):
+    """What a kernel wrote in place: a graph that kept it for its gradient has to notice (tensors of inference mode are in no graph)."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def append_kv(key_new: torch.Tensor, value_new: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
               seqused_k: torch.Tensor, page_table: Optional[torch.Tensor] = None,
               free_pages: Optional[torch.Tensor] = None, free_count: Optional[torch.Tensor] = None,
@@ -49,6 +55,7 @@ def append_kv(key_new: torch.Tensor, value_new: torch.Tensor, key_cache: torch.T
     with torch.cuda.device(device):
         rc = _lib.load().fsa_kv_append(ctypes.byref(a), _lib.current_stream_ptr(device))
     _lib.check(rc, "fsa_kv_append")
+    _written(seqused_k)
     return seqused_k
 
 
@@ -150,7 +157,8 @@ def append_kv_rotary(query: Optional[torch.Tensor], key_new: torch.Tensor, value
                       cu_seqlens_new, query_scale, key_scale, value_scale, out)
     device, fp8 = key_new.device, key_cache.dtype in _FP8
     batch = seqused_k.numel()
-    if query is not None and out is None:
+    own_buffer = out is None
+    if query is not None and own_buffer:
         out = torch.empty(query.shape, dtype=key_cache.dtype if fp8 else query.dtype, device=device)
     if key_new.numel() == 0:
         return out
@@ -197,6 +205,10 @@ def append_kv_rotary(query: Optional[torch.Tensor], key_new: torch.Tensor, value
     with torch.cuda.device(device):
         rc = _lib.load().fsa_kv_append_rotary(ctypes.byref(a), _lib.current_stream_ptr(device))
     _lib.check(rc, "fsa_kv_append_rotary")
+    if advance:
+        _written(seqused_k)
+    if not own_buffer:
+        _written(out)
     return out
 
 

@@ -418,3 +418,51 @@ def test_argument_blocks_match_the_header():
         body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1), flags=re.S)
         fields = [re.findall(r"[A-Za-z_]\w*", part)[-1] for stmt in body.split(";") if stmt.strip() for part in stmt.split(",")]
         assert fields == [f[0] for f in getattr(_lib, name)._fields_]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", [False, True])
+def test_a_gradient_notices_lengths_that_were_advanced(rotary):
+    """A rotation keeps its offsets for the gradient: when an append has advanced them in place that gradient would be another one's.
+    Autograd has to say so. Lengths that stay may be used."""
+    import flash_sparse_attn as fsa
+    from flash_sparse_attn.utils.kvcache import append_kv, append_kv_rotary
+
+    cos, sin = tables(20, 16)
+    x, k = normal(1, 2, 1, 2, 32).requires_grad_(), normal(2, 2, 1, 2, 32)
+    kc = torch.zeros(2, 9, 2, 32, dtype=torch.bfloat16, device=DEV)
+    vc, used = torch.zeros_like(kc), torch.tensor([3, 5], dtype=torch.int32, device=DEV)
+    want = turn(torch.ones_like(k), cos[used.long()][:, None], sin[used.long()][:, None], False, -1)
+    y = fsa.apply_rotary_func(x, None, cos, sin, seqlen_offsets=used)
+    append_kv_rotary(None, k, k, kc, vc, used, cos, sin, advance=False)
+    (d,) = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+    check(d, *want)
+    if rotary:
+        append_kv_rotary(None, k, k, kc, vc, used, cos, sin)
+    else:
+        append_kv(k, k, kc, vc, used)
+    done()
+    assert used.tolist() == [4, 6]
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, x, torch.ones_like(y))
+    with torch.inference_mode():  # lengths that autograd does not follow at all
+        more = torch.tensor([3, 5], dtype=torch.int32, device=DEV)
+    (append_kv_rotary(None, k, k, kc, vc, more, cos, sin) if rotary else append_kv(k, k, kc, vc, more))
+    done()
+    assert more.tolist() == [4, 6]
+
+
+@pytest.mark.gpu
+def test_a_gradient_notices_a_result_buffer_that_was_written():
+    from flash_sparse_attn.utils.kvcache import append_kv_rotary
+
+    cos, sin = tables(20, 16)
+    q, k = normal(1, 1, 1, 2, 32), normal(2, 1, 1, 1, 32)
+    kc = torch.zeros(1, 9, 1, 32, dtype=torch.bfloat16, device=DEV)
+    vc, used, out = torch.zeros_like(kc), torch.zeros(1, dtype=torch.int32, device=DEV), torch.ones_like(q)
+    w = torch.ones_like(q).requires_grad_()
+    y = (w * out).sum()
+    append_kv_rotary(q, k, k, kc, vc, used, cos, sin, out=out)
+    done()
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
