@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(256) combine_kernel(CombineParams p) {
         asm volatile("ld.acquire.sys.global.u64 %0, [%1];" : "=l"(seen) : "l"(f) : "memory");
         if (seen >= want) break;
         if (clock64() - t0 > FSA_WAIT_CYCLES) {
-          atomicExch(p.status, 4);
+          report_status(p.status, 4);
           break;
         }
         __nanosleep(100);

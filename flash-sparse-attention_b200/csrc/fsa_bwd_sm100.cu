@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) bwd_kernel(const __grid_constant_
   const int sk = (p.flags & F_USED_K) ? p.used_k[b] : ((p.flags & F_VARLEN_K) ? p.cu_k[b + 1] - off_k : p.sk);
   if (n_block * TN >= sk) return;  // nothing of this key tile exists (before any allocation)
   if (smem_u32(smem) & 1023u) {    // the tile buffers need a 1024-byte aligned base
-    if (tid == 0) atomicExch(p.status, 2);
+    if (tid == 0) report_status(p.status, 2);
     return;
   }
   const long long pad_off = (p.flags & F_VARLEN_Q) ? (long long)((off_q + b * 128) / 128) * 128
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) bwd_kernel(const __grid_constant_
     mbar_init(&bars->dd_sync, 12);
     mbar_init(&bars->stg_full, 4);
     mbar_init(&bars->stg_free, 1);
-    bars->abort_flag = (*reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
+    bars->abort_flag = *reinterpret_cast<volatile int*>(p.status);
     mbar_fence_init();
   }
   if (warp == W_MMA) {
@@ -1262,7 +1262,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) bwd_kernel(const __grid_constant_
   // ---- teardown ------------------------------------------------------------------------------------
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort_flag) atomicExch(p.status, 1);
+  if (tid == 0 && *abort_flag) report_status(p.status, *abort_flag);  // the reason it was launched with, or 1
   if (warp == W_PROD) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);

@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(FwdRoles<HD, KIND>::NTHREADS, 1) fwd_kernel(co
       mbar_init(&bars->d_full[q], 1);
       mbar_init(&bars->d_empty[q], 2 * RO::GW);
     }
-    bars->abort_flag = (*reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
+    bars->abort_flag = *reinterpret_cast<volatile int*>(p.status);
     mbar_fence_init();
   }
   if (warp == RO::W_PROD) {
@@ -1373,7 +1373,7 @@ __global__ void __launch_bounds__(FwdRoles<HD, KIND>::NTHREADS, 1) fwd_kernel(co
   // ---- teardown ------------------------------------------------------------------------------------
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort_flag) atomicExch(p.status, 1);
+  if (tid == 0 && *abort_flag) report_status(p.status, *abort_flag);  // the reason it was launched with, or 1
   if (warp == RO::W_PROD) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);

@@ -34,13 +34,13 @@ __global__ void kv_reserve_kernel(const FsaKvAppendArgs a) {
       int32_t* slot = a.page_table + (long long)b * a.page_table_stride + pi;
       if (*slot >= 0) continue;
       if (!a.free_pages || !a.free_count) {
-        atomicExch(a.status, 3);
+        report_status(a.status, 3);
         continue;
       }
       const int idx = atomicSub(a.free_count, 1) - 1;
       if (idx < 0) {
         atomicAdd(a.free_count, 1);
-        atomicExch(a.status, 3);
+        report_status(a.status, 3);
         continue;
       }
       *slot = a.free_pages[idx];

@@ -223,6 +223,9 @@ __device__ __forceinline__ void after_previous() {
   wait_for_previous();
   let_next_be_set_up();
 }
+
+// Sets the status word, if nobody has: the first reason stands, and what follows from it does not hide it.
+__device__ __forceinline__ void report_status(int* status, int why) { atomicCAS(status, 0, why); }
 #endif
 
 // Multiprocessor count of the current device (148 on B200), cached per device ordinal.

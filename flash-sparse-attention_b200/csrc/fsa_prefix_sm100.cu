@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
     mbar_init(&bars->done, 1);
     mbar_fence_init();
   } else if (warp == W_V && lane == 0) {
-    bars->abort_flag = *reinterpret_cast<volatile int*>(p.status) != 0 ? 1 : 0;
+    bars->abort_flag = *reinterpret_cast<volatile int*>(p.status);
     tma_prefetch_desc(&p.map_q);
     tma_prefetch_desc(&p.map_pq);
     if (p.prefix_keys > 0) {
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
             for (int i = 0; i < 4; ++i)
               if (r.page[i] < 0 || r.page[i] >= pages) {  // outside the pool: -1, for which TMA fills zeros
                 r.page[i] = -1;
-                atomicExch(p.status, 3);
+                report_status(p.status, 3);
               }
           }
         }
@@ -759,7 +759,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
 
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort_flag) atomicExch(p.status, 1);
+  if (tid == 0 && *abort_flag) report_status(p.status, *abort_flag);  // the reason it was launched with, or 1
   if (warp == W_K) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

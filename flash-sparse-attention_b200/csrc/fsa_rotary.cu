@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryParams p) {
   }
   if (live && (pos < 0 || pos >= p.r.table_rows)) {
     live = false;
-    atomicExch(p.status, STATUS_NO_ANGLES);
+    report_status(p.status, STATUS_NO_ANGLES);
   }
   const bool turns = u < p.r.turned;
   float c[V], s[V];
@@ -328,7 +328,7 @@ __device__ __forceinline__ int rows_in_reach(const AppendParams& p, int b, int f
   }
   if (first < 0 || n < 0) n = 0;
   if (first < 0) why = STATUS_NO_ROOM;
-  if (why && rows > 0 && report) atomicExch(p.status, why);
+  if (why && rows > 0 && report) report_status(p.status, why);
   return (int)n;
 }
 
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(1024) append_place_kernel(const AppendParams p
         if (lanes == 32) bad = __reduce_min_sync(0xffffffffu, bad);
         if (bad <= hi) {
           n = max(0, bad * p.page_size - first);
-          if (sub == 0) atomicExch(p.status, STATUS_NO_ROOM);
+          if (sub == 0) report_status(p.status, STATUS_NO_ROOM);
         }
       }
       if (sub == 0) {
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(1024) append_step_kernel(const AppendParams p)
       if (lo + i <= hi && (page[i] < 0 || page[i] >= p.num_pages)) bad = lo + i;
     if (bad <= hi) {
       n = max(0, bad * p.page_size - first);
-      if (threadIdx.x == 0) atomicExch(p.status, STATUS_NO_ROOM);
+      if (threadIdx.x == 0) report_status(p.status, STATUS_NO_ROOM);
     }
   }
   const int at = first + p.offset + (p.offsets ? p.offsets[b] : 0);

@@ -11,9 +11,10 @@
  * (fsa_status_string() names it); nothing throws or aborts.
  *
  * Device-side trouble: every kernel wait is bounded; a kernel that gives up sets the caller's `status` word
- * (non-zero) and drains. The word is STICKY: kernels launched while it is non-zero return at once without
- * writing their outputs, so a caller must read it (after synchronising) before trusting results, and zero it to
- * go on.
+ * (non-zero) and drains. The word is STICKY: forward, backward and shared-prefix kernels launched while it is non-zero
+ * return at once without writing their outputs, so a caller must read it (after synchronising) before trusting results,
+ * and zero it to go on. The first reason stands: 1 a wait expired, 2 a kernel's shared memory was not aligned, 3 no room in a
+ * cache or a page outside its pool, 4 another GPU's partials did not arrive, 5 a position outside the rotary tables.
  *
  * ev_before / ev_after (optional, may be null): cudaEvent_t handles recorded on the launch stream right before
  * and right after the call's MAIN kernel, so that a benchmark can time that kernel inside a full step without a
