@@ -286,7 +286,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == W_PLAN) {
       // =============================== planner ==================================================
-      bool ok = !*abort_flag;
+      // (A warp that goes on together waits together: were some lanes to see the phase and others the abort, those that go on would wait
+      // in their next vote or TMEM access for lanes that never come.)
+      bool ok = !__any_sync(0xffffffffu, *abort_flag);
       const int q = lane & 1;  // (of the singles; batches begin with a single of the first stream once the pairs are through)
       int b = bars->b_at[q], cum = bars->cum_at[q];  // this stream's place among the own keys: sequence, tiles in front of it
       int m0 = 0;
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
         const int last = pair ? q : max((count - 1) - ((count - 1 - q) & 1), q);
         b = __shfl_sync(0xffffffffu, b, last);
         cum = __shfl_sync(0xffffffffu, cum, last);
-        if (batch >= 2) ok = mbar_wait(&bars->rec_empty[batch & 1], ((batch >> 1) - 1) & 1, abort_flag);
+        if (batch >= 2) ok = mbar_wait_uniform(&bars->rec_empty[batch & 1], ((batch >> 1) - 1) & 1, abort_flag);
         if (!ok) return;
         if (lane < count) bars->rec[(batch & 1) * BATCH + lane] = r;
         __syncwarp();
@@ -391,7 +393,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
         for (int i = 0; i < count && ok; ++i, ++n) {
           const int r0 = (int)(bars->rec[(batch & 1) * BATCH + i].info >> 8) & 255, s = n % STAGES;
           if (r0 == PN) continue;
-          ok = mbar_wait(&bars->v_tail[s], (n_tail >> s) & 1, abort_flag);
+          ok = mbar_wait_uniform(&bars->v_tail[s], (n_tail >> s) & 1, abort_flag);
           if (!ok) break;
           n_tail ^= 1u << s;
           uint8_t* vt = smem + SM::kV + s * SM::kTile;
@@ -615,10 +617,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
     const uint32_t lane_addr = uint32_t(wq * 32) << 16;
     const uint32_t tS = tmem + lane_addr + TMEM_S + q * 128, tO = tmem + lane_addr + TMEM_O + q * 128;
     const float c = p.scale_log2;
-    bool ok = !*abort_flag;
+    bool ok = !__any_sync(0xffffffffu, *abort_flag);  // (waits are the warp's: see the planner)
     int n_s = 0, n_seg = 0;
     while (ok) {
-      ok = mbar_wait(&bars->seg_full[q][n_seg & 1], (n_seg >> 1) & 1, abort_flag);
+      ok = mbar_wait_uniform(&bars->seg_full[q][n_seg & 1], (n_seg >> 1) & 1, abort_flag);
       if (!ok) break;
       const GroupSegment g = bars->seg[q][n_seg & 1];
       if (g.n == 0) break;
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
       float m_ref = -INFINITY;  // what the exponentials are relative to; it moves when the maximum has grown by 2^8
       float l = 0.f;            // their sum
       for (int t = 0; t < g.n; ++t) {
-        ok = mbar_wait(&bars->s_full[q], n_s++ & 1, abort_flag);
+        ok = mbar_wait_uniform(&bars->s_full[q], n_s++ & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
         if (!idle) {
@@ -708,7 +710,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
       }
       if (!ok) break;
       // ---- the segment's partial result ----
-      ok = mbar_wait(&bars->o_final[q], n_seg++ & 1, abort_flag);
+      ok = mbar_wait_uniform(&bars->o_final[q], n_seg++ & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
       if (!idle) {

@@ -50,3 +50,15 @@ def test_backward_producer_waits_for_tiles_that_nobody_uses():
     producer = _rest_of_block(text, text.index("mbar_arrive_expect_tx(&bars->kv_full"))
     first_walk = producer[producer.index("bool more = walk_next("):producer.index("for (int it = 0")]
     assert re.search(r"if \(!more\)\s*mbar_wait\(&bars->kv_full, 0, abort_flag\);", first_walk)
+
+
+def test_warps_of_the_shared_prefix_leave_together():
+    # when a wait is given up, every lane of a warp that goes on with warp-wide operations has to learn of it: lanes that saw the
+    # phase would wait in the next vote or TMEM access for those that saw the abort, and the kernel would not end
+    text = _code("fsa_prefix_sm100.cu")
+    planner = _rest_of_block(text, text.index("warp == W_PLAN) {") + len("warp == W_PLAN) {"))
+    softmax = _rest_of_block(text, text.index("setmaxnreg.inc"))
+    assert "__shfl_sync" in planner and "tmem_ld" in softmax
+    for role in (planner, softmax):
+        assert re.search(r"bool ok = !__any_sync\(0xffffffffu, \*abort_flag\);", role)
+        assert "mbar_wait_uniform(" in role and not re.search(r"\bmbar_wait\(|ok = !\*abort_flag", role)
