@@ -784,8 +784,11 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixParams p)
   const int2 pre_at = p.prefix_keys > 0 ? __ldcg(reinterpret_cast<const int2*>(p.plan_ws) + (pair ? pre : pre + p.Hkv * p.pairs)) : make_int2(0, -1);
   const int2 own_at = p.own_keys > 0 ? __ldcg(reinterpret_cast<const int2*>(p.plan_ws) + own + p.Hkv * (p.pairs + 1)) : make_int2(0, -1);
   const bool skip = *reinterpret_cast<volatile int*>(p.status) != 0;
-  const int n_pre = min(p.prefix_used ? *p.prefix_used : p.prefix_keys, p.prefix_keys) > 0 ? pre_at.y - pre_at.x + 1 : 0;
-  const int n_own = own_keys(p, b) > 0 ? own_at.y - own_at.x + 1 : 0;
+  // Numbers of pieces that there can be, and no others: where the kernel in front left because of the status word, what it has not noted is
+  // whatever lay there, and the word may have been cleared since.
+  auto pieces = [](int2 at, int limit) { return at.x >= 0 && at.y < limit ? max(at.y - at.x + 1, 0) : 0; };
+  const int n_pre = min(p.prefix_used ? *p.prefix_used : p.prefix_keys, p.prefix_keys) > 0 ? pieces(pre_at, pair ? p.ctas : 2 * p.ctas) : 0;
+  const int n_own = own_keys(p, b) > 0 ? pieces(own_at, 2 * p.ctas) : 0;
   if (WPR == 1 && skip) return;
   const int pre_pitch = pair ? 2 * PM : PM, pre_row = (pair ? 0 : (int)p.single_rows) + (pre + pre_at.x) * pre_pitch + r + (pair ? (q_tile & 1) * PM : 0);
   const int own_row = (int)p.own_rows + (own + own_at.x) * p.own_pitch + gi - gt * PM;

@@ -107,3 +107,37 @@ def test_a_page_outside_the_pool_is_reported_as_that():
     for _ in range(20):
         shared_prefix(bad_page=20)
         raised(3)
+
+
+def test_the_word_is_set_and_cleared_while_calls_are_under_way():
+    """A call of two kernels may find the word set in the first and cleared in the second, which then meets what the first has not
+    written: it must not take that for places to read from."""
+    import flash_sparse_attn as fsa
+    from flash_sparse_attn import _lib
+
+    word = _lib.status_word(torch.device(DEV, torch.cuda.current_device()))
+    good = shared_prefix()
+    torch.cuda.synchronize()
+    q, k = normal(2, 40, 8, 64), normal(3, 40, 200, 2, 64)
+    pool, pages = normal(4, 20, 64, 2, 64), torch.arange(20, dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    seen = 0
+    for i in range(200):
+        with torch.cuda.stream(side):
+            torch.full((1 << 20,), -1.0, device=DEV)  # what a workspace is then made of: not places
+            for _ in range(4):
+                fsa.flash_dense_attn_with_shared_prefix_func(q, k, k, pool, pool, prefix_page_table=pages)
+        word.fill_(7)
+        for _ in range(i % 4):
+            word.zero_()
+            word.fill_(7)
+        try:
+            fsa.check_status()
+        except RuntimeError as e:
+            seen += "device status 7 " in str(e)
+    torch.cuda.synchronize()
+    word.zero_()
+    assert seen > 0
+    assert torch.equal(shared_prefix(), good)
+    raised_nothing()
