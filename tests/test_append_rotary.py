@@ -466,3 +466,12 @@ def test_a_gradient_notices_a_result_buffer_that_was_written():
     done()
     with pytest.raises(RuntimeError, match="inplace"):
         y.backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", [None, torch.float8_e4m3fn, torch.float8_e5m2])
+@pytest.mark.parametrize("form", [dict(d=128, half=32), dict(d=40, half=10, interleaved=True)], ids=["128", "40"])
+def test_many_rows_in_packed_chunks(form, cache):
+    """Enough elements for threads that take several heads of a row each, of 6 query, 2 key and 2 value heads; pages off the stack."""
+    run(dict(form, new=[1300, 0, 1, 1700, 900], used=[5, 9, 63, 64, 0], page=64, slots=28, packed=True, behind=2, hq=6, hkv=2, rows=1800, cache=cache))
+    done()

@@ -336,3 +336,33 @@ def test_packed_tokens_outside_every_sequence(offset):
     for got, x, sign in ((oq.detach(), q.detach(), 1), (ok, k, 1), (dq, torch.ones_like(q), -1)):
         assert not got[:3].any() and not got[9:].any()
         check(got[3:9], *turn(x[3:9], cos[at], sin[at], False, sign))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("head_dim,rotary_dim,threads", [(128, 64, 8), (24, 24, 3), (40, 20, 10), (7, 4, 4)])
+def test_many_tokens(head_dim, rotary_dim, threads, dtype, packed, interleaved):
+    """Enough elements for threads that take several heads of a token each, and heads that do not come out even: 7 and 3."""
+    import flash_sparse_attn as fsa
+
+    total = 148 * 2048 // (10 * threads) + 53
+    lens = [0, total // 3, 1, 0, total // 2, 17]
+    lens.append(total - sum(lens) - 9)  # and nine tokens behind the last sequence
+    if packed:
+        lead, kw = (total,), dict(cu_seqlens=torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()], dtype=torch.int32, device=DEV))
+        at = torch.cat([torch.arange(n) for n in lens] + [torch.zeros(9, dtype=torch.long)]) + 2
+    else:
+        lead, kw, at = (2, (total + 1) // 2), {}, torch.arange((total + 1) // 2) + 2
+    cos, sin = tables(int(at.max()) + 1, rotary_dim // 2)
+    q, k = normal(1, *lead, 7, head_dim, dtype=dtype).requires_grad_(), normal(2, *lead, 3, head_dim, dtype=dtype).requires_grad_()
+    gq, gk = normal(3, *q.shape, dtype=dtype), normal(4, *k.shape, dtype=dtype)
+    oq, ok = fsa.apply_rotary_func(q, k, cos, sin, seqlen_offsets=2, interleaved=interleaved, **kw)
+    dq, dk = torch.autograd.grad((oq, ok), (q, k), (gq, gk))
+    done()
+    for got, x, sign in ((oq, q, 1), (ok, k, 1), (dq, gq, -1), (dk, gk, -1)):
+        want, size = turn(x.detach(), cos.cpu()[at], sin.cpu()[at], interleaved, sign)
+        if packed:
+            want[-9:] = 0
+        check(got.detach(), want, size)
