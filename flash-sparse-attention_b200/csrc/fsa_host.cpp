@@ -797,6 +797,10 @@ PyObject* shared_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (lse.defined() && (lse.dim() != 2 || lse.size(0) != batch || lse.size(1) != hq || lse.scalar_type() != at::kFloat || lse.device() != dev ||
                           lse.stride(1) != 1))
       return none();
+    for (const Tensor* t : {&out, &lse})
+      if (t->defined())
+        for (int64_t i = 0; i < t->dim(); ++i)
+          if (t->size(i) > 1 && t->stride(i) <= 0) return none();
     double scale;
     if (!opt_double(a[5], 1.0 / std::sqrt((double)d), &scale) || !(scale > 0.0) || std::isinf(scale)) return none();
     std::optional<NoGil> no_gil(std::in_place);

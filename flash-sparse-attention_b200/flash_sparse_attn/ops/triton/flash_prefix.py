@@ -47,6 +47,8 @@ def _check(query, key, value, prefix_key, prefix_value, softmax_scale, page_tabl
     assert prefix_seqused is None or prefix_seqused.numel() == 1, "prefix_seqused must have one element"
     assert softmax_scale is None or 0.0 < softmax_scale < float("inf"), "softmax_scale must be positive and finite"
     assert_inputs.check_out_buffers(out, lse, query.shape, query.dtype, query.shape[:2])
+    for t in (out, lse):
+        assert t is None or all(n == 1 or st > 0 for n, st in zip(t.shape, t.stride())), "out and lse must not be expanded"
 
 
 def attn_decode_shared_prefix(query, key, value, prefix_key, prefix_value, softmax_scale: Optional[float] = None, page_table=None,

@@ -438,3 +438,29 @@ def test_argument_blocks_match_the_header():
         body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1), flags=re.S)
         fields = [re.findall(r"[A-Za-z_]\w*", part)[-1] for stmt in body.split(";") if stmt.strip() for part in stmt.split(",")]
         assert fields == [f[0] for f in getattr(_lib, name)._fields_]
+
+
+def test_expanded_result_buffers_are_refused():
+    """Rows on top of one another: which of them stays would be chance."""
+    from flash_sparse_attn.ops.triton import flash_prefix
+
+    q, k, pk = (torch.zeros(*s, dtype=torch.bfloat16) for s in ((3, 8, 64), (3, 32, 2, 64), (9, 2, 64)))
+    good = dict(query=q, key=k, value=k, prefix_key=pk, prefix_value=pk, softmax_scale=None, page_table=None, seqused_k=None,
+                prefix_page_table=None, prefix_seqused=None, out=None, lse=None)
+    flash_prefix._check(**dict(good, out=torch.zeros(3, 16, 64, dtype=torch.bfloat16)[:, ::2], lse=torch.zeros(3, 20)[:, :8]))
+    flash_prefix._check(**dict(good, query=q[:1], key=k[:1], value=k[:1], out=q[:1].expand(1, 8, 64)))
+    for bad in (dict(out=q[:1].expand(3, 8, 64)), dict(out=q[:, :1].expand(3, 8, 64)), dict(lse=torch.zeros(1, 8).expand(3, 8))):
+        with pytest.raises(AssertionError):
+            flash_prefix._check(**dict(good, **bad))
+
+
+@pytest.mark.gpu
+def test_expanded_result_buffers_are_refused_by_the_call():
+    import flash_sparse_attn as fsa
+
+    g = torch.Generator().manual_seed(7)
+    q, k, pk = normal(g, 3, 8, 64), normal(g, 3, 32, 2, 64), normal(g, 9, 2, 64)
+    for bad in (dict(out=q[:1].clone().expand(3, 8, 64)), dict(out=q[:, :1].clone().expand(3, 8, 64)),
+                dict(lse=torch.zeros(1, 8, device=DEV).expand(3, 8))):
+        with pytest.raises(AssertionError):
+            fsa.flash_dense_attn_with_shared_prefix_func(q, k, k, pk, pk, **bad)
