@@ -40,10 +40,16 @@ constexpr int W_K = 8, W_ISSUE = 9, W_V = 10, W_PLAN = 11;
 constexpr int BATCH = 16;       // steps that the planner works out at a time, one a lane; it is two batches ahead at most
 // What an SM's time goes to, in units of about 220 cycles: a pair of query tiles on a key tile (3900), a single one (1950 while others work on pairs
 // and leave HBM to it: own keys alone come at 6.0 TB/s on 96 SMs, 1950 cycles a tile, at 3.6 on 48, 1640, and at 6.3 on 148), and what an item adds (results on
-// their way out, and the next item's first scores): of own keys, and of a pair, whose 128 KB take 2000 to 2700 cycles to be written.
-// With 18 / 9 / 4 / 32, 18 / 10 / 4 / 32, 18 / 8 / 4 / 32 and 18 / 9 / 8 / 32: 64 sequences over 8192 + up to 1024 keys 46.5, 46.3, 46.4, 46.1 us;
-// 256 over 1000 + 100 45.5, 46.7, 44.7, 50.3; 100 over 20 000 + 1000 57.8, 61.2, 61.3, 60.4; 256 over 32 768 + up to 256 173, 172, 180, 176. A pair's
-// item at half as much: 235 over 2 + up to 645 keys 30 us instead of 25, at none 42.
+// their way out, and the next item's first scores): of own keys, and of a pair, whose 128 KB take 2000 to 2700 cycles to be written. In a call where 100 SMs
+// work on own keys beside 48 on pairs a single takes 1.47 us with its share of items, where these make 1.2.
+// Replayed calls of 32 query heads over 8 KV heads of 128, pages of 64, us, for 18 / 9 / 4 / 32, a single at 10, at 8, an item at 8, a pair's item at 16 and at 0:
+//   64 sequences over 8192 + up to 1024 keys   45.6   45.8   49.8   45.9   45.6   45.8
+//   256 over 1000 + up to 100                  43.1   43.3   43.4   47.0   47.9   46.1
+//   100 over 20 000 + up to 1000               83.3   80.7   88.3   80.4   82.1   81.9
+//   256 over 32 768 + up to 256                159    158    170    158    158    156
+//   40 over 4000 + up to 200                   28.5   26.2   28.6   25.9   27.0   27.2
+//   64 over 500 + up to 200                    20.8   20.8   20.8   20.5   20.8   25.8
+//   235 over 2 + up to 645                     73.4   73.4   73.1   73.4   73.6   74.8
 constexpr int COST_PAIR = 18, COST_SINGLE = 9, COST_ITEM = 4, COST_PAIR_ITEM = 32;
 
 // What a softmax group has to know about the units of one item that it walks.
@@ -146,9 +152,10 @@ __device__ __forceinline__ void make_plan(const PrefixParams& p, PrefixBars* s, 
     float share = ctas > 0 ? __fdividef(cost, (float)ctas) : 0.f;
     // Where there are no more items of pairs than CTAs, each is cut into `cuts` equal pieces, one a CTA, and the pieces of a KV head over the same keys go to
     // neighbours, that read them at the same time. What their shares have left is singles, if it is some for each; if not, the other CTAs take
-    // those. It is not done where the pieces come out too uneven. 256 sequences over 32 768 + up to 256 keys 172 us where pieces lie anywhere, so 159;
-    // 256 over 16 000 + 64 103 and 96, 64 over 8192 + up to 1024 46.3 and 45.6; small calls gain or lose up to 8 % (40 over 4000 + 200 19.4 and 21.0,
-    // 64 over 500 + 200 24.0 and 21.1).
+    // those. It is not done where the pieces come out too uneven. 256 sequences over 32 768 + up to 256 keys 171 us where pieces lie anywhere, so 159;
+    // 256 over 16 000 + up to 64 107 and 98, 64 over 8192 + up to 1024 46.4 and 45.6, 256 over 1000 + up to 100 46.2 and 43.1, 64 over 500 + up to 200 24.0
+    // and 20.8. One of the calls above loses, 40 over 4000 + up to 200, 27.0 and 28.5; no condition was found that leaves it out. (Pieces' bounds go
+    // through an approximate quotient, which may give a piece a tile of its neighbour's.)
     int cuts = 0, own_from = 0;  // own_from: CTAs that have no singles
     float cut_tiles = 0.f;
     if (pairs > 0 && items <= ctas && cost < 16777216.f) {  // (sums of costs are exact)
@@ -282,7 +289,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
   const int n_pairs = bars->a1 - bars->a0, n_singles = bars->s[2] - bars->s[0], n_steps = n_pairs + n_singles;
 
   if (warp >= W_K) {
-    // 384 x 168 registers at launch = 256 x 216 + 128 x 72
+    // 384 x 168 registers at launch = 256 x 216 + 128 x 72. (With 72 the issuer's and the copy warps' code spills: at head size 128 116 bytes are
+    // stored and 188 read back, at 64 52 and 708. What that costs has not been measured.)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == W_PLAN) {
       // =============================== planner ==================================================

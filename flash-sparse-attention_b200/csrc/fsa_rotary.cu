@@ -544,8 +544,7 @@ __global__ void __launch_bounds__(THREADS, 6) append_rows_kernel(const AppendPar
 }
 
 // Few tokens, pages assigned: a block per sequence finds its slots, stores its rows and advances its length by itself. One launch, where the
-// two kernels above wait for one another (one token each of 64 sequences, 80 heads of 128: 6.1 us, so 4.4;
-// one sequence 5.1 and 3.1).
+// two kernels above wait for one another (one token each of 64 sequences, 48 heads of 128: 5.3 us, so 3.3; one sequence 4.9 and 3.0).
 constexpr int STEP_PAGES = 4;  // that the new rows of a sequence may touch
 
 template <typename T, int V, bool IL>
@@ -652,9 +651,15 @@ cudaError_t for_each_form(int dtype, int v, bool interleaved, bool many, F&& f) 
 constexpr int HEADS_PER_THREAD = 4;
 
 // Whether append_step_kernel takes the call: rows of equal number, few enough that a block per sequence is no longer at them than a second
-// launch takes, and nothing to be taken off a stack. Rows of 128 columns (query, key and value heads times tokens) of a sequence, one launch
-// and two: 16 sequences 48 rows 2.4 and 4.3 us, 192 rows 4.5 and 4.4, 384 rows 6.4 and 4.6; 256 sequences 3.1 and 4.9, 8.5 and 7.3, 12.4 and
-// 10.9. At 192 rows the host still gains a launch.
+// launch takes, and nothing to be taken off a stack. Replayed calls, us in one launch and in two, by sequences and rows of 128 columns (query, key
+// and value heads times tokens) of each:
+//          48 rows        96             192            384
+//     1    3.0  4.9       3.7  4.9       5.0  4.9       7.3  5.3
+//    16    3.1  5.2       3.8  5.3       5.3  5.3       7.4  5.6
+//    64    3.3  5.3       4.0  5.6       5.3  5.8       7.6  7.8
+//   128    3.2  5.3       4.3  6.0       5.5  7.7       7.8  8.4
+//   256    4.0  5.8       7.2  8.2      10.6  9.2      14.8 13.8
+// The bound is one for all numbers of sequences: at 192 rows one launch loses with 256 of them and wins with 64 and 128.
 constexpr long long STEP_ELEMENTS = 192 * 128;
 bool append_in_one_step(const FsaKvAppendRotaryArgs* a) {
   if (a->cu_seqlens_new || a->free_pages || (long long)a->new_tokens * (a->heads_q + 2ll * a->heads_kv) * a->head_dim > STEP_ELEMENTS) return false;

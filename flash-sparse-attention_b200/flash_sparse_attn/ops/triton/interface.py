@@ -532,7 +532,11 @@ def flash_dense_attn_with_shared_prefix_func(
     Paged caches: own keys as pages ``[num_pages, page, Hkv, D]`` + ``page_table [B, max_pages]``, the prefix as pages (of the same pool or
     another) + ``prefix_page_table [prefix_pages]``; ``prefix_seqused`` (int32, one element) says how many of the prefix's positions
     count. bf16 / fp16, ``head_dim`` a multiple of 16 up to 128. A row without any key is 0 with
-    log-sum-exp ``-inf``. Returns ``out [B, Hq, D]`` or ``(out, lse [B, Hq])``; the reference has no such operator."""
+    log-sum-exp ``-inf``. Returns ``out [B, Hq, D]`` or ``(out, lse [B, Hq])``, without gradients; the reference has no such operator.
+
+    Results of the whole batch are left unwritten when a page that holds keys is outside its pool (status 3), and when the status word
+    was set before the call: by an append in front of it, for one, that had no room for one of the sequences. Ask
+    ``flash_sparse_attn.check_status()``, which raises and clears it, before they are trusted."""
     out, lse = attn_decode_shared_prefix(
         query, key, value, prefix_key, prefix_value, softmax_scale=softmax_scale, page_table=page_table,
         seqused_k=seqused_k, prefix_page_table=prefix_page_table, prefix_seqused=prefix_seqused, out=out, lse=lse, skip_checks=skip_checks)

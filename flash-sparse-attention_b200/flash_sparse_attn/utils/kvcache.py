@@ -136,7 +136,7 @@ def append_kv_rotary(query: Optional[torch.Tensor], key_new: torch.Tensor, value
     Missing pages (page-table entries < 0) come off the top of the stack ``free_pages`` (int32) of height ``free_count`` (int32
     [1], in place), in the order of sequences and slots. Rows without room (status 3) or without a row in the tables (status 5) are
     not stored, nor are the rows behind them in their sequence, and their query rows come out as zeros;
-    ``flash_sparse_attn.check_status()`` reports it. ``seqused_k`` (int32 [B]) grows by the rows stored, in place; with
+    ``flash_sparse_attn.check_status()`` reports it, and until it has been asked forward, backward and shared-prefix calls write no results. ``seqused_k`` (int32 [B]) grows by the rows stored, in place; with
     ``advance=False`` it stays, for layers that share the lengths: all but the last. No host synchronisation; no gradients."""
     if torch.compiler.is_compiling():  # a launch is not for the compiler to trace: its graph is cut here
         return torch.compiler.disable(append_kv_rotary)(
