@@ -335,16 +335,18 @@ __global__ void __launch_bounds__(P_THREADS, 1) prefix_kernel(const __grid_const
               keys_all = bars->keys;
               item += p.Hkv * p.pairs;
             } else {
+              // (The share was worked out from the lengths as they were. Were another stream to change them meanwhile, against the rules, the search
+              // could pass the last sequence: it ends there, with a place that exists, and the call with a wait that expires.)
               int u;
               for (;;) {
                 keys_all = own_keys(p, b);
                 u = tiles_of(keys_all);
-                if (y < (cum + u) * p.items_b) break;
+                if (y < (cum + u) * p.items_b || b + 1 >= p.B) break;
                 cum += u;
                 ++b;
               }
-              const int at = y - cum * p.items_b, i = at / u;
-              t = at - i * u;
+              const int per = max(u, 1), at = min(y - cum * p.items_b, per * p.items_b - 1), i = at / per;
+              t = at - i * per;
               r.h = i / p.head_tiles;
               r.info = STEP_OWN | (uint32_t)(i - r.h * p.head_tiles) << 16;
               r.b = b;

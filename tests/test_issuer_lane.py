@@ -62,3 +62,13 @@ def test_warps_of_the_shared_prefix_leave_together():
     for role in (planner, softmax):
         assert re.search(r"bool ok = !__any_sync\(0xffffffffu, \*abort_flag\);", role)
         assert "mbar_wait_uniform(" in role and not re.search(r"\bmbar_wait\(|ok = !\*abort_flag", role)
+
+
+def test_search_of_the_shared_prefix_ends_at_the_last_sequence():
+    # shares are worked out from the lengths, which the planner reads again: it must not look for a sequence behind the last one, nor
+    # divide by the tiles of one that has none, whatever another stream has made of the lengths meanwhile
+    text = _code("fsa_prefix_sm100.cu")
+    planner = _rest_of_block(text, text.index("warp == W_PLAN) {") + len("warp == W_PLAN) {"))
+    assert re.search(r"if \(y < \(cum \+ u\) \* p\.items_b \|\| b \+ 1 >= p\.B\) break;", planner)
+    assert re.search(r"per = max\(u, 1\), at = min\(y - cum \* p\.items_b, per \* p\.items_b - 1\), i = at / per;", planner)
+    assert "/ u" not in planner
