@@ -30,6 +30,9 @@ SOURCES = [
     "fsa_topk.cu",
     "fsa_kvcache.cu",
     "fsa_rotary.cu",
+    "fsa_axes.cu",
+    "fsa_quant_cache.cu",
+    "fsa_quant_dec_sm100.cu",
     "fsa_peer.cu",
 ]
 

@@ -11,6 +11,7 @@ from flash_sparse_attn.ops.triton.interface import (  # noqa: F401
     flash_dense_attn_varlen_func,
     flash_dense_attn_varlen_with_kvcache_func,
     flash_dense_attn_with_kvcache_func,
+    flash_dense_attn_with_quantized_kvcache_func,
     flash_dense_attn_with_shared_prefix_func,
     flash_gated_attn_func,
     flash_gated_attn_varlen_func,
@@ -23,4 +24,5 @@ from flash_sparse_attn.ops.triton.interface import (  # noqa: F401
 )
 from flash_sparse_attn._lib import check_status  # noqa: F401
 from flash_sparse_attn.ops.triton.rotary import apply_rotary_func  # noqa: F401
+from flash_sparse_attn.ops.triton.rotary_axes import apply_rotary_axes_func  # noqa: F401
 from flash_sparse_attn.ops.triton.utils import deterministic_enabled, set_deterministic  # noqa: F401

@@ -466,6 +466,64 @@ class FsaSharedPrefixWorkspace(ctypes.Structure):
     ]
 
 
+def _fields(text):
+    """ctypes fields from lines `type: names`."""
+    kinds = {"p": c_void_p, "q": c_int64, "i": c_int32, "f": c_float}
+    return [(name, kinds[line.split(":")[0].strip()]) for line in text.strip().splitlines() for name in line.split(":")[1].split()]
+
+
+class FsaRotaryAxesArgs(ctypes.Structure):
+    _fields_ = _fields("""
+        p: q k q_out k_out cos sin position_ids status
+        q: q_stride_b q_stride_s q_stride_h k_stride_b k_stride_s k_stride_h
+        q: q_out_stride_b q_out_stride_s q_out_stride_h k_out_stride_b k_out_stride_s k_out_stride_h
+        q: position_stride_a position_stride_b position_stride_s table_stride
+    """) + [("axis_bits", ctypes.c_uint32 * 8)] + _fields("""
+        i: batch seqlen heads_q heads_k head_dim rotary_dim table_rows axes dtype table_dtype
+        i: position_ids_int64 interleaved transposed
+    """)
+
+
+QC_INT8, QC_E4M3, QC_INT4 = 0, 1, 2
+MAX_AXES = 4
+
+
+class FsaQuantCache(ctypes.Structure):
+    _fields_ = _fields("""
+        p: k v k_scales v_scales page_table
+        q: k_stride_b k_stride_s k_stride_h v_stride_b v_stride_s v_stride_h
+        q: ks_stride_b ks_stride_s ks_stride_h vs_stride_b vs_stride_s vs_stride_h page_table_stride
+        i: capacity page_size max_pages num_pages heads_kv head_dim format group
+    """)
+
+
+class FsaKvAppendQuantArgs(ctypes.Structure):
+    _fields_ = [("cache", FsaQuantCache)] + _fields("""
+        p: q k_new v_new q_out cos sin seqused_k free_pages free_count cu_seqlens_new seqlen_offsets position_ids place_ws status
+        q: q_stride_b q_stride_s q_stride_h k_stride_b k_stride_s k_stride_h v_stride_b v_stride_s v_stride_h
+        q: q_out_stride_b q_out_stride_s q_out_stride_h position_stride_a position_stride_b position_stride_s table_stride
+    """) + [("axis_bits", ctypes.c_uint32 * 8)] + _fields("""
+        i: batch new_tokens total heads_q rotary_dim table_rows offset axes dtype table_dtype position_ids_int64 interleaved advance
+    """)
+
+
+class FsaKvReadQuantArgs(ctypes.Structure):
+    _fields_ = [("cache", FsaQuantCache)] + _fields("""
+        p: k_out v_out seqused_k cu_seqlens status
+        q: k_out_stride_b k_out_stride_s k_out_stride_h v_out_stride_b v_out_stride_s v_out_stride_h
+        i: batch seqlen total dtype
+    """)
+
+
+class FsaQuantDecodeArgs(ctypes.Structure):
+    _fields_ = [("cache", FsaQuantCache)] + _fields("""
+        p: q out lse seqused_k gather_kv_indices ws status
+        q: q_stride_b q_stride_h o_stride_b o_stride_h lse_stride_b lse_stride_h gather_stride
+        i: batch heads_q topk dtype
+        f: softmax_scale
+    """)
+
+
 PEER_MAX_RANKS = 16
 
 
@@ -546,6 +604,14 @@ def load():
     lib.fsa_kv_append_rotary_workspace_ints.argtypes = [POINTER(FsaKvAppendRotaryArgs)]
     lib.fsa_kv_append_rotary.restype = c_int
     lib.fsa_kv_append_rotary.argtypes = [POINTER(FsaKvAppendRotaryArgs), c_void_p]
+    for name, args in (("fsa_rotary_axes", FsaRotaryAxesArgs), ("fsa_kv_append_quantized", FsaKvAppendQuantArgs),
+                       ("fsa_kv_read_quantized", FsaKvReadQuantArgs), ("fsa_decode_quantized", FsaQuantDecodeArgs)):
+        getattr(lib, name).restype = c_int
+        getattr(lib, name).argtypes = [POINTER(args), c_void_p]
+    for name, args in (("fsa_kv_append_quantized_workspace_ints", FsaKvAppendQuantArgs),
+                       ("fsa_decode_quantized_workspace_bytes", FsaQuantDecodeArgs)):
+        getattr(lib, name).restype = c_int64
+        getattr(lib, name).argtypes = [POINTER(args)]
     lib.fsa_localize_indices.restype = c_int
     lib.fsa_localize_indices.argtypes = [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p]
     lib.fsa_peer_region_bytes.restype = c_int
@@ -694,6 +760,12 @@ def workspace(nbytes: int, device, dtype=torch.float32):
     if nbytes == 0:
         return None
     return torch.empty(nbytes // dtype.itemsize, dtype=dtype, device=device)
+
+
+def written(t):
+    """What a kernel wrote in place: a graph that kept it for its gradient has to notice (tensors of inference mode are in no graph)."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
 
 
 def current_stream_ptr(device) -> int:

@@ -19,6 +19,7 @@ from flash_sparse_attn.ops.triton.flash_bwd import attn_backward
 from flash_sparse_attn.ops.triton.flash_dec import attn_decode
 from flash_sparse_attn.ops.triton.flash_fwd import attn_forward
 from flash_sparse_attn.ops.triton.flash_prefix import attn_decode_shared_prefix
+from flash_sparse_attn.ops.triton.flash_quant_dec import attn_decode_quantized
 from flash_sparse_attn.ops.triton.utils import ensure_contiguous
 
 _Out = Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]
@@ -540,6 +541,37 @@ def flash_dense_attn_with_shared_prefix_func(
     out, lse = attn_decode_shared_prefix(
         query, key, value, prefix_key, prefix_value, softmax_scale=softmax_scale, page_table=page_table,
         seqused_k=seqused_k, prefix_page_table=prefix_page_table, prefix_seqused=prefix_seqused, out=out, lse=lse, skip_checks=skip_checks)
+    return (out, lse) if return_lse else out
+
+
+def flash_dense_attn_with_quantized_kvcache_func(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    softmax_scale: Optional[float] = None,
+    page_table: Optional[torch.Tensor] = None,
+    gather_kv_indices: Optional[torch.Tensor] = None,
+    seqused_k: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+    skip_checks: bool = False,
+    return_lse: bool = False,
+) -> _Out:
+    """Dense decode over a cache whose rows carry their own scales, as ``flash_sparse_attn.utils.kvcache.append_kv_quantized`` writes
+    it (int8, e4m3 or 4 bits): ``query [B, Hq, D]`` (bf16 / fp16) attends to the ``seqused_k [B]`` first positions of its sequence, or to
+    those of them that ``gather_kv_indices [B, topk]`` names (negative = masked). ``key / value`` are the codes ``[B, Sk, Hkv, ..]``, or
+    pages ``[num_pages, page, Hkv, ..]`` + ``page_table [B, max_pages]``, ``key_scales / value_scales`` their scales. The result is that of
+    the values that codes and scales stand for, none of which is rounded on its way; the work is cut evenly over the GPU whatever
+    the lengths. ``head_dim`` a multiple of 16 up to 128.
+
+    A row without any key is 0 with log-sum-exp ``-inf``. Keys on a page outside the pool are left out and reported by
+    ``flash_sparse_attn.check_status()`` (status 3). Returns ``out [B, Hq, D]`` or ``(out, lse [B, Hq])``, without gradients; the
+    reference has no such operator."""
+    out, lse = attn_decode_quantized(
+        query, key, value, key_scales, value_scales, softmax_scale=softmax_scale, page_table=page_table,
+        gather_kv_indices=gather_kv_indices, seqused_k=seqused_k, out=out, lse=lse, skip_checks=skip_checks)
     return (out, lse) if return_lse else out
 
 

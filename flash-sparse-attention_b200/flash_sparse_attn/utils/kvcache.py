@@ -11,12 +11,7 @@ import torch
 
 from flash_sparse_attn import _lib
 from flash_sparse_attn.ops.triton.rotary import check_tables, split_offsets
-
-
-def _written(t):
-    """What a kernel wrote in place: a graph that kept it for its gradient has to notice (tensors of inference mode are in no graph)."""
-    if not t.is_inference():
-        torch.autograd.graph.increment_version(t)
+from flash_sparse_attn.utils.quantized_kvcache import append_kv_quantized, empty_kv_quantized, read_kv_quantized  # noqa: F401
 
 
 def append_kv(key_new: torch.Tensor, value_new: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -55,7 +50,7 @@ def append_kv(key_new: torch.Tensor, value_new: torch.Tensor, key_cache: torch.T
     with torch.cuda.device(device):
         rc = _lib.load().fsa_kv_append(ctypes.byref(a), _lib.current_stream_ptr(device))
     _lib.check(rc, "fsa_kv_append")
-    _written(seqused_k)
+    _lib.written(seqused_k)
     return seqused_k
 
 
@@ -206,9 +201,9 @@ def append_kv_rotary(query: Optional[torch.Tensor], key_new: torch.Tensor, value
         rc = _lib.load().fsa_kv_append_rotary(ctypes.byref(a), _lib.current_stream_ptr(device))
     _lib.check(rc, "fsa_kv_append_rotary")
     if advance:
-        _written(seqused_k)
+        _lib.written(seqused_k)
     if not own_buffer:
-        _written(out)
+        _lib.written(out)
     return out
 
 

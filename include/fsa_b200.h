@@ -621,6 +621,152 @@ typedef struct FsaKvAppendRotaryArgs {
 int64_t fsa_kv_append_rotary_workspace_ints(const FsaKvAppendRotaryArgs* args); /* 0: none is needed */
 int fsa_kv_append_rotary(const FsaKvAppendRotaryArgs* args, void* stream);
 
+/*
+ * Rotary positions with several axes (tokens of images and video have a time, a row and a column): fsa_rotary with the angle of
+ * pair i taken at the position that the token has on the pair's axis, cos / sin[position_ids[axis(i)][token], i]. axis_bits holds two
+ * bits a pair, pair i in bits 2 (i mod 16) of word i / 16. Tensors as in fsa_rotary, padded [batch, seqlen, heads, head_dim] or, with batch
+ * 1, packed; position_ids int32 or int64, position_stride_a elements between axes. A token with a position outside the tables on any axis
+ * comes out as zeros and sets the status word to 5. head_dim up to 256.
+ */
+#define FSA_MAX_AXES 4
+typedef struct FsaRotaryAxesArgs {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const void* cos;
+  const void* sin;
+  const void* position_ids;
+  int32_t* status;
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  int64_t q_out_stride_b, q_out_stride_s, q_out_stride_h;
+  int64_t k_out_stride_b, k_out_stride_s, k_out_stride_h;
+  int64_t position_stride_a, position_stride_b, position_stride_s;
+  int64_t table_stride;
+  uint32_t axis_bits[8];
+  int32_t batch, seqlen;
+  int32_t heads_q, heads_k, head_dim, rotary_dim;
+  int32_t table_rows, axes;
+  int32_t dtype, table_dtype;
+  int32_t position_ids_int64, interleaved, transposed;
+} FsaRotaryAxesArgs;
+int fsa_rotary_axes(const FsaRotaryAxesArgs* args, void* stream);
+
+/*
+ * A key-value cache whose rows (one token of one KV head) carry scales of their own, written by fsa_kv_append_quantized. No
+ * counterpart in the reference, whose quantisation is per tensor (flash_sparse_attn/ops/triton/quant.py:42-64).
+ *   FSA_QC_INT8  head_dim int8 codes and one fp32 scale s: value = code * s, s = max|x| / 127, code = rne(x * (1 / s))
+ *   FSA_QC_E4M3  the same with e4m3 codes and s = max|x| / 448
+ *   FSA_QC_INT4  two codes a byte (column 2i in the low four bits) and, for each group of `group` = 32 or 64 columns, a bf16 pair (s, z):
+ *                value = z + (code - 8) s, s = bf16((max - min) / 15), z = bf16(min + 8 s), code = clamp(rne((x - z) * (1 / s)) + 8, 0, 15)
+ * all in fp32. A row (of INT4: a group) with an infinity or a NaN in it reads back as NaN; one whose s would be below 2^-126 has s = 0.
+ *   codes   [blocks, slots, heads_kv, bytes of a row], strides in bytes, a row contiguous; scales [blocks, slots, heads_kv, words of a
+ *           row], strides in 32-bit words, a row contiguous. With page_table [batch, max_pages] a block is one of num_pages pages of
+ *           page_size slots, else the sequence and has `capacity` slots. Codes and their strides are multiples of 16 bytes.
+ *   sizes   head_dim a multiple of 16 (INT4: of group) up to 128
+ */
+enum { FSA_QC_INT8 = 0, FSA_QC_E4M3 = 1, FSA_QC_INT4 = 2 };
+typedef struct FsaQuantCache {
+  void* k;
+  void* v;
+  void* k_scales;
+  void* v_scales;
+  int32_t* page_table; /* [batch, max_pages] or null */
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  int64_t v_stride_b, v_stride_s, v_stride_h;
+  int64_t ks_stride_b, ks_stride_s, ks_stride_h;
+  int64_t vs_stride_b, vs_stride_s, vs_stride_h;
+  int64_t page_table_stride;
+  int32_t capacity, page_size, max_pages, num_pages;
+  int32_t heads_kv, head_dim, format, group;
+} FsaQuantCache;
+
+/*
+ * fsa_kv_append_rotary into such a cache: keys turned by their position (rotary_dim 0: as they are), values as they are, both quantised
+ * row by row; queries turned alike into q_out (heads_q may be 0). Positions are those of the slots (slot + offset + seqlen_offsets[b]) or,
+ * with position_ids, given for every new token on `axes` axes as in fsa_rotary_axes. Places, pages, room (status 3) and `advance` as
+ * in fsa_kv_append_rotary; a new token whose position_ids lie outside the tables is stored with a key of zeros (and status 5), one whose
+ * slot has no angles is not stored. head_dim and rotary_dim multiples of 16, new rows and q_out on 16-byte boundaries.
+ */
+typedef struct FsaKvAppendQuantArgs {
+  FsaQuantCache cache;
+  const void* q;
+  const void* k_new;
+  const void* v_new;
+  void* q_out;
+  const void* cos;
+  const void* sin;
+  int32_t* seqused_k;
+  const int32_t* free_pages;
+  int32_t* free_count;
+  const int32_t* cu_seqlens_new; /* [batch + 1] or null */
+  const int32_t* seqlen_offsets; /* [batch] or null */
+  const void* position_ids;      /* or null */
+  int32_t* place_ws;
+  int32_t* status;
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  int64_t v_stride_b, v_stride_s, v_stride_h;
+  int64_t q_out_stride_b, q_out_stride_s, q_out_stride_h;
+  int64_t position_stride_a, position_stride_b, position_stride_s;
+  int64_t table_stride;
+  uint32_t axis_bits[8];
+  int32_t batch, new_tokens, total;
+  int32_t heads_q, rotary_dim, table_rows, offset, axes;
+  int32_t dtype, table_dtype;
+  int32_t position_ids_int64, interleaved, advance;
+} FsaKvAppendQuantArgs;
+int64_t fsa_kv_append_quantized_workspace_ints(const FsaKvAppendQuantArgs* args); /* 0: none is needed */
+int fsa_kv_append_quantized(const FsaKvAppendQuantArgs* args, void* stream);
+
+/*
+ * The values of such a cache in 16 bits, computed in fp32 and rounded once: the first seqused_k[b] slots of every sequence (null: all) as
+ * rows [batch, seqlen, heads_kv, head_dim], zeros behind them, or packed [total, heads_kv, head_dim] where cu_seqlens says; packed rows
+ * outside every sequence and behind its last slot are zeros. Slots on a page outside the pool read as zeros and set the status word to 3.
+ * Results on 16-byte boundaries.
+ */
+typedef struct FsaKvReadQuantArgs {
+  FsaQuantCache cache;
+  void* k_out;
+  void* v_out;
+  const int32_t* seqused_k;  /* [batch] or null */
+  const int32_t* cu_seqlens; /* [batch + 1] or null */
+  int32_t* status;
+  int64_t k_out_stride_b, k_out_stride_s, k_out_stride_h;
+  int64_t v_out_stride_b, v_out_stride_s, v_out_stride_h;
+  int32_t batch, seqlen, total;
+  int32_t dtype;
+} FsaKvReadQuantArgs;
+int fsa_kv_read_quantized(const FsaKvReadQuantArgs* args, void* stream);
+
+/*
+ * Decode attention over such a cache: q [batch, heads_q, head_dim] (bf16 / fp16) against the first seqused_k[b] slots of its sequence (null:
+ * all), or against the slots that gather_kv_indices [batch, topk] names (entries outside [0, seqused_k[b]) are left out). Scores, the
+ * statistics and sums are fp32; a sequence without keys gets zeros and a log-sum-exp of -inf. Keys on a page outside the pool are left
+ * out and set the status word to 3. The work is cut evenly over the GPU whatever the lengths; pieces meet in `ws`, of
+ * fsa_decode_quantized_workspace_bytes bytes, one per call under way. Rows of q and out on 16-byte boundaries.
+ */
+typedef struct FsaQuantDecodeArgs {
+  FsaQuantCache cache;
+  const void* q;
+  void* out;
+  float* lse; /* [batch, heads_q] */
+  const int32_t* seqused_k;
+  const int32_t* gather_kv_indices;
+  void* ws;
+  int32_t* status;
+  int64_t q_stride_b, q_stride_h;
+  int64_t o_stride_b, o_stride_h;
+  int64_t lse_stride_b, lse_stride_h;
+  int64_t gather_stride;
+  int32_t batch, heads_q, topk;
+  int32_t dtype;
+  float softmax_scale;
+} FsaQuantDecodeArgs;
+int64_t fsa_decode_quantized_workspace_bytes(const FsaQuantDecodeArgs* args); /* negative: a FSA_ERR_* code */
+int fsa_decode_quantized(const FsaQuantDecodeArgs* args, void* stream);
+
 /* ---- Peer exchange of decode partials (context-parallel decode over the GPUs of one node) -------------------
  * No counterpart in the reference (it has no multi-GPU code). Every rank owns one region (fsa_peer_alloc: cudaMalloc,
  * so that it can be exported), opens the regions of the others (fsa_peer_open on their handles) and then, per step:
