@@ -91,6 +91,28 @@ void mark(void* ev, cudaStream_t s) {
 
 }  // namespace
 
+namespace fsa {
+
+int make_byte_map(CUtensorMap* map, const void* base, uint64_t bytes, uint64_t d1, int64_t s1, uint64_t d2, int64_t s2, uint64_t d3, int64_t s3,
+                  uint32_t box_bytes, uint32_t rows) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return FSA_ERR_NO_DRIVER;
+  if (d1 == 0 || d2 == 0 || d3 == 0) return FSA_ERR_INVALID_ARG;
+  if (d1 == 1) s1 = 16;  // (a dimension of one has no stride that matters: one that TMA takes)
+  if (d2 == 1) s2 = 16;
+  if (d3 == 1) s3 = 16;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || ((s1 | s2 | s3) & 15)) return FSA_ERR_INVALID_ARG;
+  const cuuint64_t dims[4] = {bytes, d1, d2, d3}, strides[3] = {(cuuint64_t)s1, (cuuint64_t)s2, (cuuint64_t)s3};
+  const cuuint32_t box[4] = {box_bytes, 1, rows, 1}, estr[4] = {1, 1, 1, 1};
+  const CUtensorMapSwizzle swizzle =
+      box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FSA_OK : FSA_ERR_LAUNCH;
+}
+
+}  // namespace fsa
+
 extern "C" {
 
 int fsa_abi_version(void) { return FSA_ABI_VERSION; }

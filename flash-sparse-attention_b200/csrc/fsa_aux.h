@@ -132,6 +132,10 @@ struct alignas(64) PrefixParams {
   int ctas;
   float scale_log2;
 };
+// Map over rows of bytes [d3, d2, d1, bytes] in boxes of `rows` x 1 x `box_bytes` (32, 64 or 128, which is also the swizzle). Strides in bytes, of
+// dimensions of one any. FSA_OK or a FSA_ERR_* code.
+int make_byte_map(CUtensorMap* map, const void* base, uint64_t bytes, uint64_t d1, int64_t s1, uint64_t d2, int64_t s2, uint64_t d3, int64_t s3,
+                  uint32_t box_bytes, uint32_t rows);
 bool prefix_shape(PrefixParams* p);  // fills in what follows from sizes and capacities; false: too many units of work
 cudaError_t launch_prefix(const PrefixParams& p, int dtype, int head_dim, cudaStream_t stream);
 cudaError_t launch_gate_ext(const GateExtParams& p, int dtype, cudaStream_t stream);

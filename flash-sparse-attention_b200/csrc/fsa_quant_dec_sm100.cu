@@ -9,19 +9,21 @@
 // element to [1, 2) (exact but for elements 2^-14 below it, whose lost bits are below the fp32 sum's own), probabilities as fp16 (2^-12) times b_j times a power
 // of two that keeps them in range. Running maxima, sums and outputs are fp32.
 //
-// Bound by memory: a key is read once, at 2 * 8 * (heads per KV head) operations a byte. What a warp does with a tile of sixteen keys has to fit
+// Bound by memory: a key is read once, at 2 * 8 * (heads per KV head) operations a byte. What a warp does with a tile of 32 keys has to fit
 // into the time that its bytes take, so: products run transposed (keys or value columns on the M = 16 side of mma.m16n8k16, up to eight query
 // heads on the N = 8 side); columns are dealt to lanes so that a lane's codes are neighbours in memory (the sum over columns has no order), and
 // value columns so that the two keys of a register pair are two words of one lane; codes become fp16 by inserting them into the bits of 1024.
 //
-// The work is one list of tiles (sequence, KV head and block of query heads, sixteen keys), cut into equal pieces for all warps of the grid whatever the
-// lengths are. A warp streams its piece through a ring of its own in shared memory (cp.async; no barrier but the warp's), a piece that is a whole item
-// is written out, the others meet inside the CTA and then, for items that several CTAs share, in quant_merge_kernel.
+// The work is one list of tiles (sequence, KV head and block of query heads, 32 keys), cut into equal pieces for all warps of the grid whatever the
+// lengths are. A warp streams its piece through a ring of its own in shared memory: TMA brings a tile's codes (cp.async, where positions are
+// chosen one by one), the warp's own mbarriers say when, and no barrier of the CTA is in the loop. A piece that is a whole item is written out, the
+// others meet inside the CTA and then, for items that several CTAs share, in quant_merge_kernel.
 #include <math_constants.h>
 
 #include <atomic>
 #include <type_traits>
 
+#include "fsa_aux.h"
 #include "fsa_params.h"
 #include "fsa_ptx.cuh"
 #include "fsa_quant_cache.h"
@@ -30,12 +32,14 @@ namespace fsa {
 
 namespace {
 
-constexpr int TILE = 16;             // keys
-constexpr int STATUS_BAD_PAGE = 3;
+constexpr int TILE = 32;             // keys
+constexpr uint32_t ALL = 0xffffffffu;
+constexpr int STATUS_WAIT = 1, STATUS_BAD_PAGE = 3;
 constexpr float LAG = 6.f;           // how far (base 2) a score may be above the reference maximum before that moves
 constexpr float MOST_SCALE = 512.f;  // and a value scale above 1: 2^6 * 2^9 is within fp16
 
-struct QuantDecParams {
+struct alignas(64) QuantDecParams {
+  CUtensorMap map_k, map_v;  // codes: bytes of a row, heads, slots, blocks
   FsaQuantCache c;
   const void* q;
   void* out;
@@ -50,13 +54,14 @@ struct QuantDecParams {
   int blocks, items;                // of query heads a KV head, and of a sequence
   int topk, keys;                   // keys: slots of a sequence
   int chunks, words;                // of a row: 16-byte pieces, scales
-  int ctas, bf16;
+  int ctas;
   float scale_log2;
 };
 
-template <int HD_, int FMT_, int GROUPS_, int NT_>
+template <int HD_, int FMT_, int GROUPS_, int NT_, bool HALF_>
 struct Shape {
   static constexpr int HD = HD_, FMT = FMT_, GROUPS = GROUPS_, NT = NT_;  // NT: blocks of eight query heads
+  static constexpr bool HALF = HALF_;              // queries and results are fp16, not bf16
   static constexpr bool INT4 = FMT == FSA_QC_INT4;
   static constexpr int GS = HD / GROUPS;           // columns of a group
   static constexpr int RB = INT4 ? HD / 2 : HD;    // bytes of a row
@@ -64,14 +69,16 @@ struct Shape {
   static constexpr int KSTEPS = HD / 16, MTILES = HD / 16;
   static constexpr int HEADS = 8 * NT;
   static constexpr int TILE_BYTES = TILE * RB, SCALE_BYTES = TILE * GROUPS * 4;
-  static constexpr int STAGE = 2 * TILE_BYTES + 2 * SCALE_BYTES + 16;  // keys, values, their scales, what the tile is
+  // a stage: keys and values, and elsewhere (swizzled tiles begin where their pattern does) their scales and what the tile is
+  static constexpr int CODES = 2 * TILE_BYTES, EXTRA = 2 * SCALE_BYTES + 16;
   static constexpr int WARPS = NT == 1 ? 12 : 8, THREADS = 32 * WARPS;
-  static constexpr int ROOM = 220 * 1024 / WARPS;
-  static constexpr int STAGES = ROOM / STAGE > 8 ? 8 : ROOM / STAGE;
+  static constexpr int ALIGN = 8 * RB;             // the swizzle's pattern
+  static constexpr int ROOM = 222 * 1024 / WARPS / ALIGN * ALIGN;
+  static constexpr int STAGES = ROOM / (CODES + EXTRA) > 6 ? 6 : ROOM / (CODES + EXTRA);
   static constexpr int PIECE = HEADS * (HD + 2);   // floats: outputs, maxima, sums
-  static constexpr int RING = STAGES * STAGE;
-  static constexpr int SMEM = WARPS * RING;
-  static_assert(STAGES >= 3 && RING >= PIECE * 4 && RING % 16 == 0, "ring");
+  static constexpr int RING = (STAGES * (CODES + EXTRA) + ALIGN - 1) / ALIGN * ALIGN;
+  static constexpr int SMEM = WARPS * RING + 1024;
+  static_assert(STAGES >= 2 && RING >= PIECE * 4 && SMEM <= 225 * 1024, "ring");
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
@@ -80,39 +87,18 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t r;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a) : "memory");
-  return r;
-}
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-  uint16_t r;
-  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(r) : "r"(a) : "memory");
-  return r;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 r;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
-  return r;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 r;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
-  return r;
+// The barrier counts this lane in when its copies so far have landed.
+__device__ __forceinline__ void arrive_with_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -131,8 +117,7 @@ __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
   return r;
 }
 
-// Four codes of eight bits as two pairs: bytes (0, 1) and (2, 3); of e4m3 bytes (0, 2) and (1, 3), times 2^-8 (its bits, moved, are an fp16
-// with an exponent eight lower; a byte that is no number of the format comes out as a finite one).
+// Four codes of eight bits as two pairs, bytes (0, 1) and (2, 3).
 template <int FMT>
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t* lo, uint32_t* hi) {
   if constexpr (FMT == FSA_QC_INT8) {
@@ -140,9 +125,7 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t* lo, uint32_t* hi) {
     *lo = sub2(__byte_perm(w, 0x64646464u, 0x4140), 0x64806480u);  // 1024 + code + 128, less 1152
     *hi = sub2(__byte_perm(w, 0x64646464u, 0x4342), 0x64806480u);
   } else {
-    const uint32_t e = w << 8;
-    *lo = (e & 0x80008000u) | ((e >> 1) & 0x3f803f80u);
-    *hi = (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u);
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(*lo), "=r"(*hi) : "r"(w));
   }
 }
 // Eight codes of four bits, less 8, as pairs (0, 4), (1, 5), (2, 6), (3, 7).
@@ -154,22 +137,14 @@ __device__ __forceinline__ void widen8(uint32_t w, uint32_t* out) {
   out[3] = fma2((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
 }
 
-// Where a 16-byte piece lies in the shared memory of a tile: so that the lanes that read together meet no bank twice. Keys are read by rows of
-// lane / 4 (and eight more), pieces of lane % 4; values by rows 2 (lane % 4) and so on, which lie side by side (value_row).
+// Where a 16-byte piece of a row lies in a tile's shared memory: TMA's swizzle for rows of that many bytes. Lanes read keys by rows of lane / 4,
+// pieces 2 (lane % 4) and the next (of 128 bytes), values by rows 2 (lane % 4) and so on, pieces of lane / 4: neither meets a bank twice at 128
+// bytes a row; narrower rows of values twice.
 template <typename S>
-__device__ __forceinline__ int key_at(int row, int ch) {
-  if constexpr (S::RB == 128) ch ^= (row & 1) << 2;
-  else if constexpr (S::RB == 64 && S::GROUPS < 4) ch ^= (row >> 1 & 1) << 1;
+__device__ __forceinline__ int place_of(int row, int ch) {
+  if constexpr (S::RB == 128) ch ^= row & 7;
   else if constexpr (S::RB == 64) ch ^= row >> 1 & 3;
-  else if constexpr (S::GROUPS == 2) ch ^= row >> 2 & 1;
-  return row * S::RB + ch * 16;
-}
-__device__ __forceinline__ int value_row(int key) { return (key >> 1) + 8 * (key & 1); }
-template <typename S>
-__device__ __forceinline__ int value_at(int row, int ch) {
-  if constexpr (S::RB == 128) ch ^= 2 * (row & 3);
-  else if constexpr (S::RB == 64 && S::GROUPS < 4) ch ^= (row >> 1 & 1) << 1;
-  else if constexpr (S::RB == 64) ch ^= row >> 1 & 3;
+  else ch ^= row >> 2 & 1;
   return row * S::RB + ch * 16;
 }
 
@@ -195,7 +170,7 @@ struct Walk {
 
 // The position that this lane's row of a tile is chosen to have (gather), or -1.
 __device__ __forceinline__ int chosen(const QuantDecParams& p, const Walk& w, int lane) {
-  const int at = w.t * TILE + (lane & 15);
+  const int at = w.t * TILE + lane;
   return w.b < p.batch && at < w.count ? p.gather[w.b * p.g_sb + at] : -1;
 }
 // The block that a position lies in.
@@ -215,46 +190,56 @@ __device__ __forceinline__ Place look_up(const QuantDecParams& p, const Walk& w,
   return at;
 }
 
-// Sends for a tile. Pages hold a multiple of sixteen slots, so that without gather the keys of a tile lie in one.
+// Sends for a tile. Pages hold a multiple of 32 slots, so that without gather the keys of a tile lie in one.
 template <typename S>
-__device__ __forceinline__ void fetch(const QuantDecParams& p, const Walk& w, const Place& at, uint32_t stage, int lane) {
+__device__ __forceinline__ void fetch(const QuantDecParams& p, const Walk& w, const Place& at, uint8_t* stage, uint8_t* extra, uint64_t* full, int lane) {
   const FsaQuantCache& c = p.c;
-  const int h = w.i / p.blocks;
+  const int h = p.blocks == 1 ? w.i : w.i / p.blocks;
   const bool known = at.position >= 0 && at.block >= 0 && (!c.page_table || at.block < c.num_pages);
   if (at.position >= 0 && !known) report_status(p.status, STATUS_BAD_PAGE);
   const int slot = known ? (c.page_table ? at.position % c.page_size : at.position) : 0;
   const int block = known ? at.block : 0;
-  const bool here = known && (p.gather || w.t * TILE + (lane & 15) < w.count);  // this lane's row
-  const uint32_t rows = __ballot_sync(0xffffffffu, here) & 0xffffu;
-  if (lane == 0) {
-    const uint32_t what = rows | (w.t + 1 == w.tiles ? 1u << 16 : 0u) | (w.t == 0 ? 1u << 17 : 0u);
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + S::STAGE - 16), "r"(what), "r"(w.b), "r"(w.i), "r"(0) : "memory");
+  const bool here = known && (p.gather || w.t * TILE + lane < w.count);  // this lane's row
+  const uint32_t rows = __ballot_sync(ALL, here);
+  if (lane == 0) *reinterpret_cast<int4*>(extra + 2 * S::SCALE_BYTES) = make_int4((int)rows, (w.t + 1 == w.tiles) | (w.t == 0) << 1, w.b, w.i);
+  const int row_slot = p.gather ? slot : slot + lane;
+  if (!p.gather) {
+    if (lane == 0) {
+      if (known) {
+        mbar_arrive_expect_tx(full, 2 * S::TILE_BYTES);
+        tma_load_4d(stage, &p.map_k, full, 0, h, slot, block);
+        tma_load_4d(stage + S::TILE_BYTES, &p.map_v, full, 0, h, slot, block);
+      } else {
+        mbar_arrive(full);
+      }
+    }
+  } else {
+    const long long k_row = (long long)block * c.k_stride_b + (long long)slot * c.k_stride_s + h * c.k_stride_h;
+    const long long v_row = (long long)block * c.v_stride_b + (long long)slot * c.v_stride_s + h * c.v_stride_h;
+    constexpr int ROWS = 32 / S::CH;  // that an instruction of the warp covers
+    const uint32_t k_at = smem_u32(stage), v_at = k_at + S::TILE_BYTES;
+    const int ch = lane % S::CH;
+#pragma unroll 4
+    for (int it = 0; it < TILE / ROWS; ++it) {
+      const int row = it * ROWS + lane / S::CH;
+      const long long k_from = __shfl_sync(ALL, k_row, row), v_from = __shfl_sync(ALL, v_row, row);
+      const bool take = (rows >> row & 1) && ch < p.chunks;
+      copy16(k_at + place_of<S>(row, ch), reinterpret_cast<const uint8_t*>(c.k) + (take ? k_from + ch * 16 : 0), take ? 16 : 0);
+      copy16(v_at + place_of<S>(row, ch), reinterpret_cast<const uint8_t*>(c.v) + (take ? v_from + ch * 16 : 0), take ? 16 : 0);
+    }
+    if (lane == 0) mbar_arrive(full);
   }
-  const uint8_t* kb = reinterpret_cast<const uint8_t*>(c.k) + h * c.k_stride_h;
-  const uint8_t* vb = reinterpret_cast<const uint8_t*>(c.v) + h * c.v_stride_h;
-  constexpr int ROWS = 32 / S::CH;  // that an instruction of the warp covers
+  // scales: a lane those of its own row
+  const long long ks_row = block * c.ks_stride_b + row_slot * c.ks_stride_s + h * c.ks_stride_h;
+  const long long vs_row = block * c.vs_stride_b + row_slot * c.vs_stride_s + h * c.vs_stride_h;
+  const uint32_t ks_at = smem_u32(extra) + lane * S::GROUPS * 4, vs_at = ks_at + S::SCALE_BYTES;
 #pragma unroll
-  for (int it = 0; it < TILE / ROWS; ++it) {
-    const int row = it * ROWS + lane / S::CH, ch = lane % S::CH;
-    const int bl = p.gather ? __shfl_sync(0xffffffffu, block, row) : block;
-    const int sl = p.gather ? __shfl_sync(0xffffffffu, slot, row) : slot + row;
-    const bool take = (rows >> row & 1) && ch < p.chunks;
-    const long long at_k = take ? (long long)bl * c.k_stride_b + (long long)sl * c.k_stride_s + ch * 16 : 0;
-    const long long at_v = take ? (long long)bl * c.v_stride_b + (long long)sl * c.v_stride_s + ch * 16 : 0;
-    copy16(stage + key_at<S>(row, ch), kb + at_k, take ? 16 : 0);
-    copy16(stage + S::TILE_BYTES + value_at<S>(value_row(row), ch), vb + at_v, take ? 16 : 0);
+  for (int g = 0; g < S::GROUPS; ++g) {
+    const bool take = here && g < p.words;
+    copy4(ks_at + 4 * g, reinterpret_cast<const uint32_t*>(c.k_scales) + (take ? ks_row + g : 0), take ? 4 : 0);
+    copy4(vs_at + 4 * g, reinterpret_cast<const uint32_t*>(c.v_scales) + (take ? vs_row + g : 0), take ? 4 : 0);
   }
-  const uint32_t* ks = reinterpret_cast<const uint32_t*>(c.k_scales) + h * c.ks_stride_h;
-  const uint32_t* vs = reinterpret_cast<const uint32_t*>(c.v_scales) + h * c.vs_stride_h;
-#pragma unroll
-  for (int it = 0; it < S::GROUPS; ++it) {  // sixteen rows of words of keys, then of values
-    const int word = it * 32 + lane, of_v = word / (TILE * S::GROUPS), row = word / S::GROUPS % TILE, g = word % S::GROUPS;
-    const int bl = p.gather ? __shfl_sync(0xffffffffu, block, row) : block;
-    const int sl = p.gather ? __shfl_sync(0xffffffffu, slot, row) : slot + row;
-    const bool take = (rows >> row & 1) && g < p.words;
-    const long long sb = of_v ? c.vs_stride_b : c.ks_stride_b, ss = of_v ? c.vs_stride_s : c.ks_stride_s;
-    copy4(stage + 2 * S::TILE_BYTES + word * 4, (of_v ? vs : ks) + (take ? bl * sb + sl * ss + g : 0), take ? 4 : 0);
-  }
+  arrive_with_copies(full);
 }
 
 // The queries of an item as B operands, with what scores are multiplied by; of 4 bits their sums by groups.
@@ -278,7 +263,8 @@ __device__ __forceinline__ void load_queries(const QuantDecParams& p, int b, int
 #pragma unroll
     for (int i = 0; i < S::KSTEPS / 2; ++i) {  // eight neighbouring columns
       constexpr int RUNS = S::INT4 ? S::GS / 32 : 2;  // of a group or a piece
-      const int col = S::INT4 ? i / RUNS * S::GS + c * (S::GS / 4) + 8 * (i % RUNS) : 16 * (4 * (i / 2) + c) + 8 * (i % 2);
+      const int col = S::INT4 ? i / RUNS * S::GS + c * (S::GS / 4) + 8 * (i % RUNS)
+                              : 16 * (S::RB == 128 ? 2 * c + i / 2 : c) + 8 * (i % 2);
       raw[i] = there && col < p.c.head_dim ? *reinterpret_cast<const uint4*>(row + col) : uint4{};
       const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
@@ -288,7 +274,7 @@ __device__ __forceinline__ void load_queries(const QuantDecParams& p, int b, int
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
     // bf16: the exponent of the largest element; rows of zeros, and with an infinity or a NaN, as they are
     int e = 0;
-    if (p.bf16) {
+    if constexpr (!S::HALF) {
       e = (int)(most >> 7) - 127;
       if (most < 0x80u || most >= 0x7f80u) e = 0;
       e = min(max(e, -100), 126);
@@ -302,7 +288,7 @@ __device__ __forceinline__ void load_queries(const QuantDecParams& p, int b, int
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[j] = w[j];
-        if (p.bf16) x[j] = pack2<__half>(__uint_as_float(w[j] << 16) * down, __uint_as_float(w[j] & 0xffff0000u) * down);
+        if constexpr (!S::HALF) x[j] = pack2<__half>(__uint_as_float(w[j] << 16) * down, __uint_as_float(w[j] & 0xffff0000u) * down);
         if constexpr (S::INT4) {
           const __half2 two = *reinterpret_cast<const __half2*>(&x[j]);
           sums[i / (S::GS / 32)] += __low2float(two) + __high2float(two);
@@ -310,17 +296,14 @@ __device__ __forceinline__ void load_queries(const QuantDecParams& p, int b, int
       }
       uint32_t* f0 = q.f[nt][2 * i];
       uint32_t* f1 = q.f[nt][2 * i + 1];
-      if constexpr (S::FMT == FSA_QC_INT8) {
+      if constexpr (!S::INT4) {
         f0[0] = x[0]; f0[1] = x[1]; f1[0] = x[2]; f1[1] = x[3];
-      } else if constexpr (S::FMT == FSA_QC_E4M3) {
-        f0[0] = __byte_perm(x[0], x[1], 0x5410); f0[1] = __byte_perm(x[0], x[1], 0x7632);
-        f1[0] = __byte_perm(x[2], x[3], 0x5410); f1[1] = __byte_perm(x[2], x[3], 0x7632);
       } else {
         f0[0] = __byte_perm(x[0], x[2], 0x5410); f0[1] = __byte_perm(x[0], x[2], 0x7632);
         f1[0] = __byte_perm(x[1], x[3], 0x5410); f1[1] = __byte_perm(x[1], x[3], 0x7632);
       }
     }
-    const float mine = up * p.scale_log2 * (S::FMT == FSA_QC_E4M3 ? 256.f : 1.f);
+    const float mine = up * p.scale_log2;
 #pragma unroll
     for (int x = 0; x < 2; ++x) q.scale[nt][x] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + x));
     if constexpr (S::INT4) {
@@ -367,7 +350,7 @@ __device__ __forceinline__ float centre_of(uint32_t word) { return __uint_as_flo
 
 // Moves the reference maxima to what the tile brings, and the power of two of the value scales.
 template <typename S>
-__device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[4], float most_scale) {
+__device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[S::NT][4], float most_scale) {
 #pragma unroll
   for (int d = 4; d < 32; d <<= 1) most_scale = fmaxf(most_scale, __shfl_xor_sync(0xffffffffu, most_scale, d));
   float ratio = 1.f;
@@ -382,7 +365,7 @@ __device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[4]
   for (int nt = 0; nt < S::NT; ++nt) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      float m = fmaxf(s[nt][x], s[nt][x + 2]);
+      float m = fmaxf(fmaxf(s[0][nt][x], s[0][nt][x + 2]), fmaxf(s[1][nt][x], s[1][nt][x + 2]));
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
       m = fmaxf(m, st.m[nt][x]);
@@ -400,194 +383,212 @@ __device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[4]
   }
 }
 
-// One tile.
+// One tile: its two halves of sixteen keys.
 template <typename S>
-__device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uint32_t stage, uint32_t rows, int lane) {
+__device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, const uint8_t* stage, const uint8_t* extra, uint32_t rows, int lane) {
   const int r = lane >> 2, c = lane & 3;
-  uint32_t a_words[2][S::GROUPS], b_words[2][S::GROUPS];
+  uint32_t a_words[4][S::GROUPS], b_words[4][S::GROUPS];  // scales of rows r, r + 8, ..
+  const uint32_t* scales = reinterpret_cast<const uint32_t*>(extra);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t at = stage + 2 * S::TILE_BYTES + (r + 8 * i) * S::GROUPS * 4;
-    if constexpr (S::GROUPS == 1) {
-      a_words[i][0] = lds32(at);
-      b_words[i][0] = lds32(at + S::SCALE_BYTES);
-    } else if constexpr (S::GROUPS == 2) {
-      const uint2 a = lds64(at), b = lds64(at + S::SCALE_BYTES);
-      a_words[i][0] = a.x; a_words[i][1] = a.y;
-      b_words[i][0] = b.x; b_words[i][1] = b.y;
-    } else {
-      const uint4 a = lds128(at), b = lds128(at + S::SCALE_BYTES);
-      a_words[i][0] = a.x; a_words[i][1] = a.y; a_words[i][2] = a.z; a_words[i][3] = a.w;
-      b_words[i][0] = b.x; b_words[i][1] = b.y; b_words[i][2] = b.z; b_words[i][3] = b.w;
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int g = 0; g < S::GROUPS; ++g) {
+      a_words[i][g] = scales[(r + 8 * i) * S::GROUPS + g];
+      b_words[i][g] = scales[(TILE + r + 8 * i) * S::GROUPS + g];
     }
-  }
-  // ---- scores: keys r and r + 8, heads 2 c and 2 c + 1 of each block -------------------------------------------------
-  float s[S::NT][4];
-#pragma unroll
-  for (int nt = 0; nt < S::NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+  // ---- scores: keys r and r + 8 of each half, heads 2 c and 2 c + 1 of each block --------------------------------------
+  float s[2][S::NT][4];
   constexpr int KWORDS = S::RB / 16 / S::GROUPS;  // of a group, of a lane
 #pragma unroll
-  for (int g = 0; g < S::GROUPS; ++g) {
-    uint32_t w[2][KWORDS];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = r + 8 * i;
-      if constexpr (!S::INT4) {
-#pragma unroll
-        for (int j = 0; j < KWORDS / 4; ++j) {
-          const uint4 x = lds128(stage + key_at<S>(row, 4 * j + c));
-          w[i][4 * j] = x.x; w[i][4 * j + 1] = x.y; w[i][4 * j + 2] = x.z; w[i][4 * j + 3] = x.w;
-        }
-      } else if constexpr (KWORDS == 2) {
-        const uint2 x = lds64(stage + key_at<S>(row, 2 * g + (c >> 1)) + 8 * (c & 1));
-        w[i][0] = x.x; w[i][1] = x.y;
-      } else {
-        w[i][0] = lds32(stage + key_at<S>(row, g) + 4 * c);
-      }
-    }
-    float acc[S::NT][4];
+  for (int half = 0; half < 2; ++half) {
 #pragma unroll
     for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
+      for (int i = 0; i < 4; ++i) s[half][nt][i] = 0.f;
 #pragma unroll
-    for (int j = 0; j < KWORDS; ++j) {
-      if constexpr (!S::INT4) {
-        uint32_t lo0, hi0, lo1, hi1;
-        widen4<S::FMT>(w[0][j], &lo0, &hi0);
-        widen4<S::FMT>(w[1][j], &lo1, &hi1);
+    for (int g = 0; g < S::GROUPS; ++g) {
+      uint32_t w[2][KWORDS];
 #pragma unroll
-        for (int nt = 0; nt < S::NT; ++nt) mma(acc[nt], lo0, lo1, hi0, hi1, q.f[nt][j][0], q.f[nt][j][1]);
-      } else {
-        uint32_t x0[4], x1[4];
-        widen8(w[0][j], x0);
-        widen8(w[1][j], x1);
-        const int k = 2 * (g * KWORDS + j);
+      for (int i = 0; i < 2; ++i) {
+        const int row = 16 * half + r + 8 * i;
+        if constexpr (!S::INT4) {
 #pragma unroll
-        for (int nt = 0; nt < S::NT; ++nt) {
-          mma(acc[nt], x0[0], x1[0], x0[1], x1[1], q.f[nt][k][0], q.f[nt][k][1]);
-          mma(acc[nt], x0[2], x1[2], x0[3], x1[3], q.f[nt][k + 1][0], q.f[nt][k + 1][1]);
+          for (int j = 0; j < KWORDS / 4; ++j) {
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + place_of<S>(row, S::RB == 128 ? 2 * c + j : c));
+            w[i][4 * j] = x.x; w[i][4 * j + 1] = x.y; w[i][4 * j + 2] = x.z; w[i][4 * j + 3] = x.w;
+          }
+        } else if constexpr (KWORDS == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(stage + place_of<S>(row, 2 * g + (c >> 1)) + 8 * (c & 1));
+          w[i][0] = x.x; w[i][1] = x.y;
+        } else {
+          w[i][0] = *reinterpret_cast<const uint32_t*>(stage + place_of<S>(row, g) + 4 * c);
         }
       }
+      float acc[S::NT][4];
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KWORDS; ++j) {
+        if constexpr (!S::INT4) {
+          uint32_t lo0, hi0, lo1, hi1;
+          widen4<S::FMT>(w[0][j], &lo0, &hi0);
+          widen4<S::FMT>(w[1][j], &lo1, &hi1);
+#pragma unroll
+          for (int nt = 0; nt < S::NT; ++nt) mma(acc[nt], lo0, lo1, hi0, hi1, q.f[nt][j][0], q.f[nt][j][1]);
+        } else {
+          uint32_t x0[4], x1[4];
+          widen8(w[0][j], x0);
+          widen8(w[1][j], x1);
+          const int k = 2 * (g * KWORDS + j);
+#pragma unroll
+          for (int nt = 0; nt < S::NT; ++nt) {
+            mma(acc[nt], x0[0], x1[0], x0[1], x1[1], q.f[nt][k][0], q.f[nt][k][1]);
+            mma(acc[nt], x0[2], x1[2], x0[3], x1[3], q.f[nt][k + 1][0], q.f[nt][k + 1][1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t word = a_words[2 * half + (i >> 1)][g];
+          const float by = scale_of(word, S::INT4);
+          if constexpr (S::INT4)
+            s[half][nt][i] = fmaf(acc[nt][i], by, fmaf(q.sum[g][nt][i & 1], centre_of(word), s[half][nt][i]));
+          else
+            s[half][nt][i] = acc[nt][i] * by;
+        }
     }
 #pragma unroll
     for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t word = a_words[i >> 1][g];
-        const float by = scale_of(word, S::INT4);
-        if constexpr (S::INT4)
-          s[nt][i] = fmaf(acc[nt][i], by, fmaf(q.sum[g][nt][i & 1], centre_of(word), s[nt][i]));
-        else
-          s[nt][i] = acc[nt][i] * by;
-      }
+      for (int i = 0; i < 4; ++i) s[half][nt][i] *= q.scale[nt][i & 1];
+  }
+  if (rows != ALL) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(rows >> (16 * half + r + 8 * (i >> 1)) & 1)) s[half][nt][i] = -CUDART_INF_F;
   }
   bool move = false;
 #pragma unroll
   for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[nt][i] = rows >> (r + 8 * (i >> 1)) & 1 ? s[nt][i] * q.scale[nt][i & 1] : -CUDART_INF_F;
-      move = move || s[nt][i] > st.m[nt][i & 1] + LAG;
-    }
+    for (int x = 0; x < 2; ++x)
+      move = move || fmaxf(fmaxf(s[0][nt][x], s[0][nt][x + 2]), fmaxf(s[1][nt][x], s[1][nt][x + 2])) > st.m[nt][x] + LAG;
   float most_scale = 0.f;
 #pragma unroll
-  for (int g = 0; g < S::GROUPS; ++g) most_scale = fmaxf(most_scale, fmaxf(scale_of(b_words[0][g], S::INT4), scale_of(b_words[1][g], S::INT4)));
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int g = 0; g < S::GROUPS; ++g) most_scale = fmaxf(most_scale, scale_of(b_words[i][g], S::INT4));
   move = move || most_scale * st.v_inv > MOST_SCALE;
-  if (__any_sync(0xffffffffu, move)) move_reference<S>(st, s, most_scale);
+  if (__any_sync(ALL, move)) move_reference<S>(st, s, most_scale);
 
   // ---- probabilities -------------------------------------------------------------------------------------------------
 #pragma unroll
-  for (int nt = 0; nt < S::NT; ++nt) {
+  for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float m = st.m[nt][i & 1];
-      s[nt][i] = exp2_fast(s[nt][i] - (m == -CUDART_INF_F ? 0.f : m));
-      st.l[nt][i & 1] += s[nt][i];
-    }
-    if constexpr (S::INT4) {
+    for (int x = 0; x < 2; ++x) {
+      const float m = st.m[nt][x] == -CUDART_INF_F ? 0.f : st.m[nt][x];
 #pragma unroll
-      for (int g = 0; g < S::GROUPS; ++g)
+      for (int i = 0; i < 4; ++i) {
+        float& e = s[i >> 1][nt][x + 2 * (i & 1)];
+        e = exp2_fast(e - m);
+        st.l[nt][x] += e;
+        if constexpr (S::INT4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st.centre[g][nt][i & 1] = fmaf(s[nt][i], centre_of(b_words[i >> 1][g]), st.centre[g][nt][i & 1]);
-    }
-  }
-  // ---- outputs: value columns of lane / 4, keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 ----------------------------------------
-  const uint32_t values = stage + S::TILE_BYTES;
-  constexpr int GT = S::GS / 16;  // tiles of sixteen columns of a group
-#pragma unroll
-  for (int g = 0; g < S::GROUPS; ++g) {
-    uint32_t pb[S::NT][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float by = scale_of(b_words[i][g], S::INT4) * st.v_inv;
-#pragma unroll
-      for (int nt = 0; nt < S::NT; ++nt) pb[nt][i] = transposed(pack2<__half>(s[nt][2 * i] * by, s[nt][2 * i + 1] * by));
-    }
-    // columns g GS + r GS / 8 + i, i = 0 .. GS / 8: of tile t the two i = 2 t and 2 t + 1
-    constexpr int VWORDS = S::INT4 ? 1 : S::GS / 32;
-    uint32_t w[4][VWORDS];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int row = c + 4 * (k >> 1) + 8 * (k & 1);  // of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-      if constexpr (!S::INT4 && S::RB == 128) {
-        const uint4 x = lds128(values + value_at<S>(row, r));
-        w[k][0] = x.x; w[k][1] = x.y; w[k][2] = x.z; w[k][3] = x.w;
-      } else if constexpr (!S::INT4) {
-        const uint2 x = lds64(values + value_at<S>(row, r >> 1) + 8 * (r & 1));
-        w[k][0] = x.x; w[k][1] = x.y;
-      } else if constexpr (S::GS == 64) {
-        w[k][0] = lds32(values + value_at<S>(row, 2 * g + (r >> 2)) + 4 * (r & 3));
-      } else {
-        w[k][0] = lds16(values + value_at<S>(row, g) + 2 * r);
+          for (int g = 0; g < S::GROUPS; ++g) st.centre[g][nt][x] = fmaf(e, centre_of(b_words[i][g]), st.centre[g][nt][x]);
+        }
       }
     }
-    if constexpr (!S::INT4) {
+  // ---- outputs: value columns of lane / 4, keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 of each half -----------------------------
+  const uint8_t* values = stage + S::TILE_BYTES;
+  constexpr int GT = S::GS / 16;                        // tiles of sixteen columns of a group
+  constexpr int VWORDS = S::INT4 ? 1 : S::GS / 32;
 #pragma unroll
-      for (int x = 0; x < VWORDS; ++x) {
-        uint32_t f[2][4];  // keys 2 c and 2 c + 1, 2 c + 8 and 2 c + 9; columns 4 x ..
+  for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if constexpr (S::FMT == FSA_QC_INT8) {
-            widen4<S::FMT>(__byte_perm(w[2 * k][x], w[2 * k + 1][x], 0x5140), &f[k][0], &f[k][1]);
-            widen4<S::FMT>(__byte_perm(w[2 * k][x], w[2 * k + 1][x], 0x7362), &f[k][2], &f[k][3]);
-          } else {
-            widen4<S::FMT>(__byte_perm(w[2 * k][x], w[2 * k + 1][x], 0x5410), &f[k][0], &f[k][1]);
-            widen4<S::FMT>(__byte_perm(w[2 * k][x], w[2 * k + 1][x], 0x7632), &f[k][2], &f[k][3]);
+    for (int g = 0; g < S::GROUPS; ++g) {
+      // Probabilities times scales, of fp16 results with what the rounding to fp16 leaves (else it would be as large as the result's own).
+      uint32_t pb[S::NT][2], rest[S::HALF ? S::NT : 1][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float by = scale_of(b_words[2 * half + i][g], S::INT4) * st.v_inv;
+#pragma unroll
+        for (int nt = 0; nt < S::NT; ++nt) {
+          const float x = s[half][nt][2 * i] * by, y = s[half][nt][2 * i + 1] * by;
+          const uint32_t two = pack2<__half>(x, y);
+          pb[nt][i] = transposed(two);
+          if constexpr (S::HALF) {
+            const __half2 h = *reinterpret_cast<const __half2*>(&two);
+            rest[nt][i] = transposed(pack2<__half>(x - __low2float(h), y - __high2float(h)));
           }
         }
+      }
+      // columns g GS + r GS / 8 + i, i = 0 .. GS / 8: of tile t the two i = 2 t and 2 t + 1
+      uint32_t w[4][VWORDS];
 #pragma unroll
-        for (int nt = 0; nt < S::NT; ++nt) {
-          mma(st.o[2 * x][nt], f[0][0], f[0][1], f[1][0], f[1][1], pb[nt][0], pb[nt][1]);
-          mma(st.o[2 * x + 1][nt], f[0][2], f[0][3], f[1][2], f[1][3], pb[nt][0], pb[nt][1]);
+      for (int k = 0; k < 4; ++k) {
+        const int row = 16 * half + 2 * c + (k & 1) + 8 * (k >> 1);
+        if constexpr (!S::INT4 && S::RB == 128) {
+          const uint4 x = *reinterpret_cast<const uint4*>(values + place_of<S>(row, r));
+          w[k][0] = x.x; w[k][1] = x.y; w[k][2] = x.z; w[k][3] = x.w;
+        } else if constexpr (!S::INT4) {
+          const uint2 x = *reinterpret_cast<const uint2*>(values + place_of<S>(row, r >> 1) + 8 * (r & 1));
+          w[k][0] = x.x; w[k][1] = x.y;
+        } else if constexpr (S::GS == 64) {
+          w[k][0] = *reinterpret_cast<const uint32_t*>(values + place_of<S>(row, 2 * g + (r >> 2)) + 4 * (r & 3));
+        } else {
+          w[k][0] = *reinterpret_cast<const uint16_t*>(values + place_of<S>(row, g) + 2 * r);
+        }
+        if constexpr (S::FMT == FSA_QC_E4M3) {  // what lies in rows that are not there may be no number
+          if (rows != ALL && !(rows >> row & 1)) {
+#pragma unroll
+            for (int x = 0; x < VWORDS; ++x) w[k][x] = 0;
+          }
         }
       }
-    } else {
-#pragma unroll
-      for (int half = 0; half < S::GS / 32; ++half) {  // four columns
-        uint32_t f[2][4];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t y = __byte_perm(w[2 * k][0], w[2 * k + 1][0], half ? 0x7632 : 0x5410);
-          widen8(y, f[k]);  // columns 0, 1, 2, 3 of the two keys
-        }
-        const int t = g * GT + 2 * half;
+      auto add = [&](int t, const uint32_t* f0, const uint32_t* f1) {
 #pragma unroll
         for (int nt = 0; nt < S::NT; ++nt) {
-          mma(st.o[t][nt], f[0][0], f[0][1], f[1][0], f[1][1], pb[nt][0], pb[nt][1]);
-          mma(st.o[t + 1][nt], f[0][2], f[0][3], f[1][2], f[1][3], pb[nt][0], pb[nt][1]);
+          mma(st.o[t][nt], f0[0], f0[1], f1[0], f1[1], pb[nt][0], pb[nt][1]);
+          if constexpr (S::HALF) mma(st.o[t][nt], f0[0], f0[1], f1[0], f1[1], rest[nt][0], rest[nt][1]);
+        }
+      };
+      if constexpr (!S::INT4) {
+#pragma unroll
+        for (int x = 0; x < VWORDS; ++x) {
+          uint32_t f[2][4];  // keys 2 c and 2 c + 1, 2 c + 8 and 2 c + 9; columns 4 x ..
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            widen4<S::FMT>(__byte_perm(w[2 * k][x], w[2 * k + 1][x], 0x5140), &f[k][0], &f[k][1]);
+            widen4<S::FMT>(__byte_perm(w[2 * k][x], w[2 * k + 1][x], 0x7362), &f[k][2], &f[k][3]);
+          }
+          add(2 * x, f[0], f[1]);
+          add(2 * x + 1, f[0] + 2, f[1] + 2);
+        }
+      } else {
+#pragma unroll
+        for (int four = 0; four < S::GS / 32; ++four) {  // four columns
+          uint32_t f[2][4];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) widen8(__byte_perm(w[2 * k][0], w[2 * k + 1][0], four ? 0x7632 : 0x5410), f[k]);  // columns 0 .. 3 of the two keys
+          add(g * GT + 2 * four, f[0], f[1]);
+          add(g * GT + 2 * four + 1, f[0] + 2, f[1] + 2);
         }
       }
     }
-  }
 }
 
 // Sums over the lanes that share heads, and the outputs in the values' own units.
 template <typename S>
 __device__ __forceinline__ void settle(State<S>& st) {
-  const float by = (st.v_inv == 0.f ? 1.f : 1.f / st.v_inv) * (S::FMT == FSA_QC_E4M3 ? 256.f : 1.f);
+  const float by = st.v_inv == 0.f ? 1.f : 1.f / st.v_inv;
 #pragma unroll
   for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
@@ -616,8 +617,8 @@ __device__ __forceinline__ int column_of(int t, int r) {
   return t / GT * S::GS + r * (S::GS / 8) + 2 * (t % GT);
 }
 
-__device__ __forceinline__ void store_two(const QuantDecParams& p, uint16_t* row, int col, float a, float b) {
-  if (col < p.c.head_dim) *reinterpret_cast<uint32_t*>(row + col) = p.bf16 ? pack2<__nv_bfloat16>(a, b) : pack2<__half>(a, b);
+__device__ __forceinline__ void store_two(const QuantDecParams& p, bool half, uint16_t* row, int col, float a, float b) {
+  if (col < p.c.head_dim) *reinterpret_cast<uint32_t*>(row + col) = half ? pack2<__half>(a, b) : pack2<__nv_bfloat16>(a, b);
 }
 
 // A whole item.
@@ -634,7 +635,7 @@ __device__ __forceinline__ void write_out(const QuantDecParams& p, const State<S
       const long long hq = (long long)h * p.group_heads + head;
       uint16_t* row = reinterpret_cast<uint16_t*>(p.out) + b * p.o_sb + hq * p.o_sh;
 #pragma unroll
-      for (int t = 0; t < S::MTILES; ++t) store_two(p, row, column_of<S>(t, r), st.o[t][nt][x] * by, st.o[t][nt][x + 2] * by);
+      for (int t = 0; t < S::MTILES; ++t) store_two(p, S::HALF, row, column_of<S>(t, r), st.o[t][nt][x] * by, st.o[t][nt][x + 2] * by);
       if (r == 0) p.lse[b * p.l_sb + hq * p.l_sh] = l == 0.f ? -CUDART_INF_F : (st.m[nt][x] + log2f(l)) * CUDART_LN2_F;
     }
 }
@@ -680,21 +681,24 @@ __device__ __forceinline__ float4 join(int parts, int head, int col, F&& part, f
   return o;
 }
 
-__device__ __forceinline__ void finish(const QuantDecParams& p, int b, int item, int heads, int head, int col, float4 o, float m, float l) {
+__device__ __forceinline__ void finish(const QuantDecParams& p, bool half, int b, int item, int heads, int head, int col, float4 o, float m, float l) {
   const int h = item / p.blocks, at = (item - h * p.blocks) * heads + head;
   if (at >= p.group_heads) return;
   const float by = l == 0.f ? 0.f : 1.f / l;
   const long long hq = (long long)h * p.group_heads + at;
   uint16_t* row = reinterpret_cast<uint16_t*>(p.out) + b * p.o_sb + hq * p.o_sh;
-  store_two(p, row, col, o.x * by, o.y * by);
-  store_two(p, row, col + 2, o.z * by, o.w * by);
+  store_two(p, half, row, col, o.x * by, o.y * by);
+  store_two(p, half, row, col + 2, o.z * by, o.w * by);
   if (col == 0) p.lse[b * p.l_sb + hq * p.l_sh] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * CUDART_LN2_F;
 }
 
 template <typename S>
 __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __grid_constant__ QuantDecParams p) {
   after_previous();
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ uint64_t full_s[S::WARPS][S::STAGES];
+  __shared__ int abort_s;
   __shared__ long long sums[32];
   __shared__ long long total_s;
   __shared__ Walk begin_s[S::WARPS];
@@ -732,6 +736,10 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     scan(mine);
     if (tid == 0) total_s = sums[31] * p.items;
     if (tid < S::WARPS) begin_s[tid].b = -1;
+    // a stage is there when its scales are (each lane's copies) and its codes (lane 0, with TMA's bytes)
+    if (tid < S::WARPS * S::STAGES) mbar_init(&full_s[0][0] + tid, 33);
+    if (tid == 0) abort_s = 0;
+    mbar_fence_init();
     __syncthreads();
   }
   // The first `warps` warps of the grid have equal pieces, of at least a tile; the others none.
@@ -761,7 +769,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
 
   // ---- this warp's tiles -----------------------------------------------------------------------------------------------
   uint8_t* ring = smem + warp * S::RING;
-  const uint32_t ring_at = smem_u32(ring);
+  uint8_t* extras = ring + S::STAGES * S::CODES;
+  uint64_t* full = full_s[warp];
   float* own_pieces = p.pieces + (long long)blockIdx.x * 2 * S::PIECE;
   if (lane == 0) {
     part_s[warp][0] = part_s[warp][1] = nullptr;
@@ -782,7 +791,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     }
     auto send = [&]() {
       if (sent < mine) {
-        fetch<S>(p, walk, place, ring_at + sent % S::STAGES * S::STAGE, lane);
+        const int k = sent % S::STAGES;
+        fetch<S>(p, walk, place, ring + k * S::CODES, extras + k * S::EXTRA, full + k, lane);
         ++sent;
         walk.next(p);
         place = look_up(p, walk, chosen_next);
@@ -792,7 +802,6 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
           chosen_next = chosen(p, ahead, lane);
         }
       }
-      copies_close();
     };
     for (int i = 0; i < S::STAGES - 1; ++i) send();
     Queries<S> q;
@@ -800,19 +809,25 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     bool fresh = true, whole = begun;  // whole: the item began in this warp
     int2 item;
     for (int i = 0; i < mine; ++i) {
-      copies_wait<S::STAGES - 2>();
+      // all lanes see the tile, and are done with the one whose place the next copies take
+      if (!mbar_wait_uniform(full + i % S::STAGES, i / S::STAGES & 1, &abort_s)) {
+        report_status(p.status, STATUS_WAIT);
+        for (int j = i + 1; j < sent; ++j) mbar_wait_uniform(full + j % S::STAGES, j / S::STAGES & 1, &abort_s);
+        break;
+      }
       __syncwarp();
       send();
-      const uint32_t stage = ring_at + i % S::STAGES * S::STAGE;
-      const uint4 what = lds128(stage + S::STAGE - 16);
+      const uint8_t* stage = ring + i % S::STAGES * S::CODES;
+      const uint8_t* extra = extras + i % S::STAGES * S::EXTRA;
+      const int4 what = *reinterpret_cast<const int4*>(extra + 2 * S::SCALE_BYTES);
       if (fresh) {
-        item = make_int2((int)what.y, (int)what.z);
+        item = make_int2(what.z, what.w);
         load_queries<S>(p, item.x, item.y, lane, q);
         st.clear();
         fresh = false;
       }
-      take_tile<S>(st, q, stage, what.x & 0xffffu, lane);
-      const bool ends = what.x >> 16 & 1;
+      take_tile<S>(st, q, stage, extra, (uint32_t)what.x, lane);
+      const bool ends = what.y & 1;
       if (ends || i + 1 == mine) {
         settle<S>(st);
         if (whole && ends) {
@@ -820,10 +835,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
         } else {
           // the ring is free behind the last tile; a first piece that is done before goes through the workspace
           float* to = i + 1 == mine ? reinterpret_cast<float*>(ring) : p.pieces + ((long long)p.ctas * 2 + g_warp) * S::PIECE;
-          if (i + 1 == mine) {
-            copies_wait<0>();
-            __syncwarp();
-          }
+          __syncwarp();
           write_piece<S>(to, st, lane);
           if (lane == 0) {
             part_s[warp][whole] = to;
@@ -839,6 +851,10 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     }
   }
   __syncthreads();
+  if (abort_s) {  // a wait ran out: nothing to join
+    if (tid == 0) p.shared[blockIdx.x] = make_int2(0, -1);
+    return;
+  }
 
   // ---- items that several warps share ------------------------------------------------------------------------------------
   // Runs of pieces of one item, in the order of the warps.
@@ -855,7 +871,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
       float m, l;
       const float4 o = join<S::HD, S::HEADS>(last - w0 + 1, head, col, part, &m, &l);
       if (whole) {
-        finish(p, item.x, item.y, S::HEADS, head, col, o, m, l);
+        finish(p, S::HALF, item.x, item.y, S::HEADS, head, col, o, m, l);
       } else {
         *reinterpret_cast<float4*>(to + head * S::HD + col) = o;
         if (col == 0) {
@@ -890,7 +906,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
 // Items that several CTAs share: a block takes a quarter of the columns of the item that begins in its CTA, if it goes on in others.
 constexpr int MERGE_THREADS = 128, SLICES = 4;
 
-template <int HD, int HEADS>
+template <int HD, int HEADS, bool HALF>
 __global__ void __launch_bounds__(MERGE_THREADS) quant_merge_kernel(const __grid_constant__ QuantDecParams p) {
   after_previous();
   __shared__ int end_s;
@@ -913,7 +929,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) quant_merge_kernel(const __grid
     const int head = j / WIDE, col = 4 * (slice * WIDE + j % WIDE);
     float m, l;
     const float4 o = join<HD, HEADS>(last - cta + 1, head, col, part, &m, &l);
-    finish(p, item / p.items, item % p.items, HEADS, head, col, o, m, l);
+    finish(p, HALF, item / p.items, item % p.items, HEADS, head, col, o, m, l);
   }
 }
 
@@ -927,14 +943,15 @@ cudaError_t launch_both(const QuantDecParams& p, cudaStream_t stream) {
   if (cudaError_t e = smem_opt_in(kern, S::SMEM, opted_in); e != cudaSuccess) return e;
   cudaError_t e = launch_early(kern, (unsigned)p.ctas, S::THREADS, S::SMEM, stream, 1, p);
   if (e != cudaSuccess || p.ctas == 1) return e;
-  return launch_early(quant_merge_kernel<S::HD, S::HEADS>, (unsigned)(p.ctas * SLICES), MERGE_THREADS, 0, stream, 1, p);
+  return launch_early(quant_merge_kernel<S::HD, S::HEADS, S::HALF>, (unsigned)(p.ctas * SLICES), MERGE_THREADS, 0, stream, 1, p);
 }
 
 // Calls f with the shape that a cache and a number of query heads a KV head need.
 template <typename F>
-auto for_shape(const FsaQuantCache& c, int group_heads, F&& f) {
+auto for_shape(const FsaQuantCache& c, int dtype, int group_heads, F&& f) {
   auto with_heads = [&](auto hd, auto fmt, auto groups) {
-    return group_heads > 8 ? f(Shape<hd(), fmt(), groups(), 2>{}) : f(Shape<hd(), fmt(), groups(), 1>{});
+    if (dtype == FSA_DT_FP16) return group_heads > 8 ? f(Shape<hd(), fmt(), groups(), 2, true>{}) : f(Shape<hd(), fmt(), groups(), 1, true>{});
+    return group_heads > 8 ? f(Shape<hd(), fmt(), groups(), 2, false>{}) : f(Shape<hd(), fmt(), groups(), 1, false>{});
   };
   auto with_width = [&](auto hd) {
     using std::integral_constant;
@@ -961,7 +978,7 @@ int plan(const FsaQuantDecodeArgs* a, QuantDecParams* p, int* warps, int* piece)
   p->batch = a->batch;
   p->heads_q = a->heads_q;
   p->group_heads = a->heads_q / c.heads_kv;
-  const int heads = for_shape(c, p->group_heads, [&](auto s) {
+  const int heads = for_shape(c, a->dtype, p->group_heads, [&](auto s) {
     *warps = decltype(s)::WARPS;
     *piece = decltype(s)::PIECE;
     return (int)decltype(s)::HEADS;
@@ -1019,9 +1036,18 @@ extern "C" int fsa_decode_quantized(const FsaQuantDecodeArgs* a, void* stream_) 
   p.o_sb = a->o_stride_b; p.o_sh = a->o_stride_h;
   p.l_sb = a->lse_stride_b; p.l_sh = a->lse_stride_h;
   p.g_sb = a->gather_stride;
-  p.bf16 = a->dtype == FSA_DT_BF16;
+  {
+    const FsaQuantCache& c = p.c;
+    const int wide = c.head_dim > 64 ? 128 : 64, bytes = c.format == FSA_QC_INT4 ? wide / 2 : wide;
+    const uint64_t slots = c.page_table ? c.page_size : c.capacity, blocks = c.page_table ? c.num_pages : a->batch;
+    auto map = [&](CUtensorMap* m, const void* base, int64_t sb, int64_t ss, int64_t sh) {
+      return make_byte_map(m, base, quant_row_bytes(c), c.heads_kv, sh, slots, ss, blocks, sb, bytes, TILE);
+    };
+    if (const int e = map(&p.map_k, c.k, c.k_stride_b, c.k_stride_s, c.k_stride_h); e != FSA_OK) return e;
+    if (const int e = map(&p.map_v, c.v, c.v_stride_b, c.v_stride_s, c.v_stride_h); e != FSA_OK) return e;
+  }
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   const cudaError_t e =
-      for_shape(p.c, p.group_heads, [&](auto s) { return launch_both<decltype(s)>(p, reinterpret_cast<cudaStream_t>(stream_)); });
+      for_shape(p.c, a->dtype, p.group_heads, [&](auto s) { return launch_both<decltype(s)>(p, reinterpret_cast<cudaStream_t>(stream_)); });
   return e == cudaSuccess ? FSA_OK : FSA_ERR_LAUNCH;
 }
