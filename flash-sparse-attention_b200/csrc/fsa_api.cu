@@ -111,6 +111,20 @@ int make_byte_map(CUtensorMap* map, const void* base, uint64_t bytes, uint64_t d
   return r == CUDA_SUCCESS ? FSA_OK : FSA_ERR_LAUNCH;
 }
 
+int make_word_map(CUtensorMap* map, const void* base, uint64_t words, uint64_t d1, int64_t s1, uint64_t d2, int64_t s2, uint32_t box) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return FSA_ERR_NO_DRIVER;
+  if (words == 0 || d1 == 0 || d2 == 0) return FSA_ERR_INVALID_ARG;
+  if (d1 == 1) s1 = 4;
+  if (d2 == 1) s2 = 4;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || ((s1 | s2) & 3)) return FSA_ERR_INVALID_ARG;
+  const cuuint64_t dims[3] = {words, d1, d2}, strides[2] = {(cuuint64_t)s1 * 4, (cuuint64_t)s2 * 4};
+  const cuuint32_t boxes[3] = {box, 1, 1}, estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FSA_OK : FSA_ERR_LAUNCH;
+}
+
 }  // namespace fsa
 
 extern "C" {

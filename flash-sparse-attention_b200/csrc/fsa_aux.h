@@ -136,6 +136,8 @@ struct alignas(64) PrefixParams {
 // dimensions of one any. FSA_OK or a FSA_ERR_* code.
 int make_byte_map(CUtensorMap* map, const void* base, uint64_t bytes, uint64_t d1, int64_t s1, uint64_t d2, int64_t s2, uint64_t d3, int64_t s3,
                   uint32_t box_bytes, uint32_t rows);
+// The same over rows of 32-bit words [d2, d1, words] in boxes of one row's `box` words, strides in words, without swizzle.
+int make_word_map(CUtensorMap* map, const void* base, uint64_t words, uint64_t d1, int64_t s1, uint64_t d2, int64_t s2, uint32_t box);
 bool prefix_shape(PrefixParams* p);  // fills in what follows from sizes and capacities; false: too many units of work
 cudaError_t launch_prefix(const PrefixParams& p, int dtype, int head_dim, cudaStream_t stream);
 cudaError_t launch_gate_ext(const GateExtParams& p, int dtype, cudaStream_t stream);

@@ -39,7 +39,8 @@ constexpr float LAG = 6.f;           // how far (base 2) a score may be above th
 constexpr float MOST_SCALE = 512.f;  // and a value scale above 1: 2^6 * 2^9 is within fp16
 
 struct alignas(64) QuantDecParams {
-  CUtensorMap map_k, map_v;  // codes: bytes of a row, heads, slots, blocks
+  CUtensorMap map_k, map_v;    // codes: bytes of a row, heads, slots, blocks
+  CUtensorMap map_ks, map_vs;  // scales, where a head's lie side by side: words of its slots, heads, blocks
   FsaQuantCache c;
   const void* q;
   void* out;
@@ -54,7 +55,9 @@ struct alignas(64) QuantDecParams {
   int blocks, items;                // of query heads a KV head, and of a sequence
   int topk, keys;                   // keys: slots of a sequence
   int chunks, words;                // of a row: 16-byte pieces, scales
+  int page_shift;                   // log2 of the slots of a page
   int ctas;
+  bool scales_by_tma;
   float scale_log2;
 };
 
@@ -70,7 +73,7 @@ struct Shape {
   static constexpr int HEADS = 8 * NT;
   static constexpr int TILE_BYTES = TILE * RB, SCALE_BYTES = TILE * GROUPS * 4;
   // a stage: keys and values, and elsewhere (swizzled tiles begin where their pattern does) their scales and what the tile is
-  static constexpr int CODES = 2 * TILE_BYTES, EXTRA = 2 * SCALE_BYTES + 16;
+  static constexpr int CODES = 2 * TILE_BYTES, EXTRA = 2 * SCALE_BYTES + 128;
   static constexpr int WARPS = NT == 1 ? 12 : 8, THREADS = 32 * WARPS;
   static constexpr int ALIGN = 8 * RB;             // the swizzle's pattern
   static constexpr int ROOM = 222 * 1024 / WARPS / ALIGN * ALIGN;
@@ -175,7 +178,7 @@ __device__ __forceinline__ int chosen(const QuantDecParams& p, const Walk& w, in
 }
 // The block that a position lies in.
 __device__ __forceinline__ int block_of(const QuantDecParams& p, int b, int position) {
-  return p.c.page_table ? p.c.page_table[b * p.c.page_table_stride + position / p.c.page_size] : b;
+  return p.c.page_table ? p.c.page_table[b * p.c.page_table_stride + (position >> p.page_shift)] : b;
 }
 
 // What the copies of a tile need to know, fetched one tile ahead: of this lane's row (gather), or of the tile's first key.
@@ -197,7 +200,7 @@ __device__ __forceinline__ void fetch(const QuantDecParams& p, const Walk& w, co
   const int h = p.blocks == 1 ? w.i : w.i / p.blocks;
   const bool known = at.position >= 0 && at.block >= 0 && (!c.page_table || at.block < c.num_pages);
   if (at.position >= 0 && !known) report_status(p.status, STATUS_BAD_PAGE);
-  const int slot = known ? (c.page_table ? at.position % c.page_size : at.position) : 0;
+  const int slot = known ? (c.page_table ? at.position & (c.page_size - 1) : at.position) : 0;
   const int block = known ? at.block : 0;
   const bool here = known && (p.gather || w.t * TILE + lane < w.count);  // this lane's row
   const uint32_t rows = __ballot_sync(ALL, here);
@@ -206,13 +209,18 @@ __device__ __forceinline__ void fetch(const QuantDecParams& p, const Walk& w, co
   if (!p.gather) {
     if (lane == 0) {
       if (known) {
-        mbar_arrive_expect_tx(full, 2 * S::TILE_BYTES);
+        mbar_arrive_expect_tx(full, 2 * S::TILE_BYTES + (p.scales_by_tma ? 2 * S::SCALE_BYTES : 0));
         tma_load_4d(stage, &p.map_k, full, 0, h, slot, block);
         tma_load_4d(stage + S::TILE_BYTES, &p.map_v, full, 0, h, slot, block);
+        if (p.scales_by_tma) {
+          tma_load_3d(extra, &p.map_ks, full, slot * S::GROUPS, h, block);
+          tma_load_3d(extra + S::SCALE_BYTES, &p.map_vs, full, slot * S::GROUPS, h, block);
+        }
       } else {
         mbar_arrive(full);
       }
     }
+    if (p.scales_by_tma) return;
   } else {
     const long long k_row = (long long)block * c.k_stride_b + (long long)slot * c.k_stride_s + h * c.k_stride_h;
     const long long v_row = (long long)block * c.v_stride_b + (long long)slot * c.v_stride_s + h * c.v_stride_h;
@@ -474,6 +482,11 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, con
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (!(rows >> (16 * half + r + 8 * (i >> 1)) & 1)) s[half][nt][i] = -CUDART_INF_F;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int g = 0; g < S::GROUPS; ++g)
+        if (!(rows >> (r + 8 * i) & 1)) b_words[i][g] = 0;
   }
   bool move = false;
 #pragma unroll
@@ -699,87 +712,80 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ uint64_t full_s[S::WARPS][S::STAGES];
   __shared__ int abort_s;
-  __shared__ long long sums[32];
-  __shared__ long long total_s;
-  __shared__ Walk begin_s[S::WARPS];
   // what a warp's first piece (of an item that began before it) and its last one (of an item that goes on behind it) are
   __shared__ const float* part_s[S::WARPS][2];
   __shared__ int2 item_s[S::WARPS];  // of the last piece: sequence, item
   __shared__ int ends_s[S::WARPS];   // whether the first piece's item ends in this warp
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  // ---- where this CTA's warps begin ------------------------------------------------------------------------------------
-  auto scan = [&](long long x) {  // inclusive, over the CTA; the total goes to sums[31]
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, x, d);
-      if (lane >= d) x += o;
-    }
-    if (lane == 31) sums[warp] = x;
-    __syncthreads();
-    if (warp == 0) {
-      long long y = lane < S::WARPS ? sums[lane] : 0;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, y, d);
-        if (lane >= d) y += o;
-      }
-      sums[lane] = y;
-    }
-    __syncthreads();
-    return x + (warp ? sums[warp - 1] : 0);
-  };
-  auto tiles_at = [&](int b) { return b < p.batch ? tiles_of(p.gather ? p.topk : keys_of(p, b)) : 0; };
-  {
-    long long mine = 0;
-    for (int b = tid; b < p.batch; b += S::THREADS) mine += tiles_at(b);
-    scan(mine);
-    if (tid == 0) total_s = sums[31] * p.items;
-    if (tid < S::WARPS) begin_s[tid].b = -1;
-    // a stage is there when its scales are (each lane's copies) and its codes (lane 0, with TMA's bytes)
-    if (tid < S::WARPS * S::STAGES) mbar_init(&full_s[0][0] + tid, 33);
-    if (tid == 0) abort_s = 0;
-    mbar_fence_init();
-    __syncthreads();
-  }
-  // The first `warps` warps of the grid have equal pieces, of at least a tile; the others none.
-  const long long total = total_s, warps = min(total, (long long)p.ctas * S::WARPS);
-  auto cut = [&](long long w) { return w >= warps ? total : total * w / warps; };
-  {
-    long long before = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += S::THREADS) {
-      const int b = b0 + tid, tiles = tiles_at(b);
-      const long long upto = (before + scan(tiles)) * p.items, from = upto - (long long)tiles * p.items;
-      before += sums[31];
-      for (int w = 0; w < S::WARPS; ++w) {
-        const long long at = cut((long long)blockIdx.x * S::WARPS + w);
-        if (at >= from && at < upto && at < cut((long long)blockIdx.x * S::WARPS + w + 1)) {
-          Walk& x = begin_s[w];
-          x.b = b;
-          x.i = (int)((at - from) / tiles);
-          x.t = (int)((at - from) % tiles);
-        }
-      }
-      __syncthreads();  // sums are read
-    }
-  }
-  Walk walk = begin_s[warp];
-  const long long g_warp = (long long)blockIdx.x * S::WARPS + warp;
-  const int mine = walk.b < 0 ? 0 : (int)min(cut(g_warp + 1) - cut(g_warp), 0x7fffffffll);
-
-  // ---- this warp's tiles -----------------------------------------------------------------------------------------------
-  uint8_t* ring = smem + warp * S::RING;
-  uint8_t* extras = ring + S::STAGES * S::CODES;
   uint64_t* full = full_s[warp];
-  float* own_pieces = p.pieces + (long long)blockIdx.x * 2 * S::PIECE;
+  // a stage is there when its codes are (lane 0, with TMA's bytes) and its scales (the same, or each lane's copies)
+  if (lane < S::STAGES) mbar_init(full + lane, p.scales_by_tma ? 1 : 33);
+  if (tid == 0) abort_s = 0;  // (read by a wait that runs out, long after)
+  mbar_fence_init();
   if (lane == 0) {
     part_s[warp][0] = part_s[warp][1] = nullptr;
     ends_s[warp] = 0;
   }
+  __syncwarp();
+
+  // ---- where this warp begins ------------------------------------------------------------------------------------------
+  // The first `warps` warps of the grid have equal pieces of the list, of at least a tile; the others none. Every warp adds up the
+  // lengths by itself, a lane those of neighbouring sequences: no warp waits for another before it has its first tiles under way.
+  const long long g_warp = (long long)blockIdx.x * S::WARPS + warp;
+  Walk walk;
+  int mine = 0;
+  {
+    auto tiles_at = [&](int b) { return tiles_of(p.gather ? p.topk : keys_of(p, b)); };
+    const bool alike = p.gather || !p.used;
+    const int per = (p.batch + 31) / 32, b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
+    long long own = 0;
+    if (alike) own = (long long)(b1 - b0) * tiles_at(0);
+    else for (int b = b0; b < b1; ++b) own += tiles_at(b);
+    long long upto = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(ALL, upto, d);
+      if (lane >= d) upto += o;
+    }
+    const long long total = __shfl_sync(ALL, upto, 31) * p.items, warps = min(total, (long long)p.ctas * S::WARPS);
+    if (g_warp < warps) {
+      const long long at = total * g_warp / warps;
+      mine = (int)min(total * (g_warp + 1) / warps - at, 0x7fffffffll);
+      long long from = (upto - own) * p.items;
+      const bool have = at >= from && at < upto * p.items;
+      int where[3] = {0, 0, 0};
+      if (have) {
+        int b = b0, tiles = tiles_at(b);
+        if (alike) {
+          const long long skip = (at - from) / ((long long)tiles * p.items);
+          b += (int)skip;
+          from += skip * tiles * p.items;
+        } else {
+          while (at >= from + (long long)tiles * p.items) {
+            from += (long long)tiles * p.items;
+            tiles = tiles_at(++b);
+          }
+        }
+        where[0] = b;
+        where[1] = (int)((at - from) / tiles);
+        where[2] = (int)((at - from) % tiles);
+      }
+      const int src = __ffs(__ballot_sync(ALL, have)) - 1;
+      walk.b = __shfl_sync(ALL, where[0], src);
+      walk.i = __shfl_sync(ALL, where[1], src);
+      walk.t = __shfl_sync(ALL, where[2], src);
+    }
+  }
+
+  // ---- this warp's tiles -----------------------------------------------------------------------------------------------
+  uint8_t* ring = smem + warp * S::RING;
+  uint8_t* extras = ring + S::STAGES * S::CODES;
+  float* own_pieces = p.pieces + (long long)blockIdx.x * 2 * S::PIECE;
   if (mine > 0) {
     walk.sequence(p);
     const bool begun = walk.t == 0;
-    int sent = 0, chosen_next = -1;
+    int sent = 0, into = 0, chosen_next = -1;  // into: the stage that the next copies take
     Place place;
     {
       place = look_up(p, walk, p.gather ? chosen(p, walk, lane) : 0);
@@ -791,9 +797,9 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     }
     auto send = [&]() {
       if (sent < mine) {
-        const int k = sent % S::STAGES;
-        fetch<S>(p, walk, place, ring + k * S::CODES, extras + k * S::EXTRA, full + k, lane);
+        fetch<S>(p, walk, place, ring + into * S::CODES, extras + into * S::EXTRA, full + into, lane);
         ++sent;
+        into = into + 1 == S::STAGES ? 0 : into + 1;
         walk.next(p);
         place = look_up(p, walk, chosen_next);
         if (p.gather) {
@@ -803,22 +809,30 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
         }
       }
     };
+    int2 item = make_int2(walk.b, walk.i);
     for (int i = 0; i < S::STAGES - 1; ++i) send();
     Queries<S> q;
     State<S> st;
-    bool fresh = true, whole = begun;  // whole: the item began in this warp
-    int2 item;
+    load_queries<S>(p, item.x, item.y, lane, q);
+    st.clear();
+    bool fresh = false, whole = begun;  // whole: the item began in this warp
+    int at = 0;
+    uint32_t phase = 0;
     for (int i = 0; i < mine; ++i) {
       // all lanes see the tile, and are done with the one whose place the next copies take
-      if (!mbar_wait_uniform(full + i % S::STAGES, i / S::STAGES & 1, &abort_s)) {
+      if (!mbar_wait_uniform(full + at, phase, &abort_s)) {
         report_status(p.status, STATUS_WAIT);
         for (int j = i + 1; j < sent; ++j) mbar_wait_uniform(full + j % S::STAGES, j / S::STAGES & 1, &abort_s);
         break;
       }
       __syncwarp();
       send();
-      const uint8_t* stage = ring + i % S::STAGES * S::CODES;
-      const uint8_t* extra = extras + i % S::STAGES * S::EXTRA;
+      const uint8_t* stage = ring + at * S::CODES;
+      const uint8_t* extra = extras + at * S::EXTRA;
+      if (++at == S::STAGES) {
+        at = 0;
+        phase ^= 1;
+      }
       const int4 what = *reinterpret_cast<const int4*>(extra + 2 * S::SCALE_BYTES);
       if (fresh) {
         item = make_int2(what.z, what.w);
@@ -972,7 +986,9 @@ int plan(const FsaQuantDecodeArgs* a, QuantDecParams* p, int* warps, int* piece)
   const int rc = check_quant_cache(c);
   if (rc != FSA_OK) return rc;
   if (a->batch <= 0 || a->heads_q <= 0 || a->heads_q % c.heads_kv || a->topk < 0) return FSA_ERR_INVALID_ARG;
-  if (c.page_table && c.page_size % TILE) return FSA_ERR_UNSUPPORTED;  // the keys of a tile lie in one page
+  // the keys of a tile lie in one page
+  if (c.page_table && (c.page_size < TILE || (c.page_size & (c.page_size - 1)))) return FSA_ERR_UNSUPPORTED;
+  for (p->page_shift = 0; c.page_table && 1 << p->page_shift < c.page_size;) ++p->page_shift;
   const long long keys = c.page_table ? (long long)c.max_pages * c.page_size : c.capacity;
   p->keys = (int)(keys < 0x7fffff00ll ? keys : 0x7fffff00ll);
   p->batch = a->batch;
@@ -1045,6 +1061,19 @@ extern "C" int fsa_decode_quantized(const FsaQuantDecodeArgs* a, void* stream_) 
     };
     if (const int e = map(&p.map_k, c.k, c.k_stride_b, c.k_stride_s, c.k_stride_h); e != FSA_OK) return e;
     if (const int e = map(&p.map_v, c.v, c.v_stride_b, c.v_stride_s, c.v_stride_h); e != FSA_OK) return e;
+    // a tile's scales come by TMA too where they are one piece that it can fetch, else lane by lane
+    const int64_t groups = c.format == FSA_QC_INT4 ? wide / c.group : 1;
+    auto one_piece = [&](const void* base, int64_t sb, int64_t ss, int64_t sh) {
+      return ss == groups && p.words == groups && !((uintptr_t)base & 15) && (blocks == 1 || sb % 4 == 0) && (c.heads_kv == 1 || sh % 4 == 0) &&
+             slots * groups < (1ull << 31);
+    };
+    p.scales_by_tma = !p.gather && one_piece(c.k_scales, c.ks_stride_b, c.ks_stride_s, c.ks_stride_h) &&
+                      one_piece(c.v_scales, c.vs_stride_b, c.vs_stride_s, c.vs_stride_h);
+    if (p.scales_by_tma) {
+      const uint32_t box = (uint32_t)(TILE * groups);
+      if (const int e = make_word_map(&p.map_ks, c.k_scales, slots * groups, c.heads_kv, c.ks_stride_h, blocks, c.ks_stride_b, box); e != FSA_OK) return e;
+      if (const int e = make_word_map(&p.map_vs, c.v_scales, slots * groups, c.heads_kv, c.vs_stride_h, blocks, c.vs_stride_b, box); e != FSA_OK) return e;
+    }
   }
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   const cudaError_t e =
