@@ -56,6 +56,7 @@ struct alignas(64) QuantDecParams {
   int topk, keys;                   // keys: slots of a sequence
   int chunks, words;                // of a row: 16-byte pieces, scales
   int page_shift;                   // log2 of the slots of a page
+  int cache_blocks;                 // pages of the pool, or sequences
   int ctas;
   bool scales_by_tma;
   float scale_log2;
@@ -154,12 +155,16 @@ __device__ __forceinline__ int place_of(int row, int ch) {
 __device__ __forceinline__ int keys_of(const QuantDecParams& p, int b) { return p.used ? min(max(p.used[b], 0), p.keys) : p.keys; }
 __device__ __forceinline__ int tiles_of(int keys) { return keys > 0 ? (keys + TILE - 1) / TILE : 1; }  // (an empty sequence has its zeros written)
 
+// A value that is the same in all lanes, for the compiler to know: branches on it are the warp's, and TMA's operands need no detour.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(ALL, x, 0); }
+
 // Walk over the list: tile t of item (b, i); `keys` of the sequence, `count` of them (or of the chosen ones) to look at.
+template <bool GATHER>
 struct Walk {
   int b, i, t, tiles, keys, count;
   __device__ __forceinline__ void sequence(const QuantDecParams& p) {
-    keys = keys_of(p, b);
-    count = p.gather ? p.topk : keys;
+    keys = uniform(keys_of(p, b));
+    count = GATHER ? p.topk : keys;
     tiles = tiles_of(count);
   }
   __device__ __forceinline__ void next(const QuantDecParams& p) {
@@ -171,43 +176,48 @@ struct Walk {
   }
 };
 
-// The position that this lane's row of a tile is chosen to have (gather), or -1.
-__device__ __forceinline__ int chosen(const QuantDecParams& p, const Walk& w, int lane) {
+// The position that this lane's row of a tile is chosen to have, or -1.
+__device__ __forceinline__ int chosen(const QuantDecParams& p, const Walk<true>& w, int lane) {
   const int at = w.t * TILE + lane;
   return w.b < p.batch && at < w.count ? p.gather[w.b * p.g_sb + at] : -1;
 }
-// The block that a position lies in.
-__device__ __forceinline__ int block_of(const QuantDecParams& p, int b, int position) {
-  return p.c.page_table ? p.c.page_table[b * p.c.page_table_stride + (position >> p.page_shift)] : b;
-}
 
-// What the copies of a tile need to know, fetched one tile ahead: of this lane's row (gather), or of the tile's first key.
+// Where the rows of a tile lie, fetched one tile ahead: of this lane's row (gather), or of the tile's first key.
 struct Place {
   int position, block;
 };
-__device__ __forceinline__ Place look_up(const QuantDecParams& p, const Walk& w, int position) {
+template <bool GATHER>
+__device__ __forceinline__ Place look_up(const QuantDecParams& p, const Walk<GATHER>& w, int position) {
   Place at;
-  at.position = p.gather ? position : w.t * TILE;
+  at.position = GATHER ? position : w.t * TILE;
   if (w.b >= p.batch || at.position < 0 || at.position >= w.keys) at.position = -1;
-  at.block = at.position >= 0 ? block_of(p, w.b, at.position) : 0;
+  at.block = w.b;
+  if (p.c.page_table) at.block = at.position >= 0 ? p.c.page_table[w.b * p.c.page_table_stride + (at.position >> p.page_shift)] : -1;
   return at;
 }
 
 // Sends for a tile. Pages hold a multiple of 32 slots, so that without gather the keys of a tile lie in one.
-template <typename S>
-__device__ __forceinline__ void fetch(const QuantDecParams& p, const Walk& w, const Place& at, uint8_t* stage, uint8_t* extra, uint64_t* full, int lane) {
+template <typename S, bool GATHER>
+__device__ __forceinline__ void fetch(const QuantDecParams& p, const Walk<GATHER>& w, const Place& at, uint8_t* stage, uint8_t* extra, uint64_t* full,
+                                      int lane) {
   const FsaQuantCache& c = p.c;
   const int h = p.blocks == 1 ? w.i : w.i / p.blocks;
-  const bool known = at.position >= 0 && at.block >= 0 && (!c.page_table || at.block < c.num_pages);
-  if (at.position >= 0 && !known) report_status(p.status, STATUS_BAD_PAGE);
-  const int slot = known ? (c.page_table ? at.position & (c.page_size - 1) : at.position) : 0;
-  const int block = known ? at.block : 0;
-  const bool here = known && (p.gather || w.t * TILE + lane < w.count);  // this lane's row
-  const uint32_t rows = __ballot_sync(ALL, here);
-  if (lane == 0) *reinterpret_cast<int4*>(extra + 2 * S::SCALE_BYTES) = make_int4((int)rows, (w.t + 1 == w.tiles) | (w.t == 0) << 1, w.b, w.i);
-  const int row_slot = p.gather ? slot : slot + lane;
-  if (!p.gather) {
-    if (lane == 0) {
+  const int block = GATHER ? at.block : uniform(at.block);
+  const bool there = at.position >= 0, known = there && (unsigned)block < (unsigned)p.cache_blocks;
+  if (there && !known) report_status(p.status, STATUS_BAD_PAGE);
+  const int slot = c.page_table ? at.position & (c.page_size - 1) : at.position;
+  uint32_t rows;
+  if constexpr (GATHER) {
+    rows = __ballot_sync(ALL, known);
+  } else {
+    const int left = w.count - w.t * TILE;
+    rows = !known ? 0u : (left >= TILE ? ALL : (1u << left) - 1);
+  }
+  const bool lead = elect_one();
+  if (lead) *reinterpret_cast<int4*>(extra + 2 * S::SCALE_BYTES) = make_int4((int)rows, w.t + 1 == w.tiles, w.b, w.i);
+  const bool here = rows >> lane & 1;  // this lane's row
+  if constexpr (!GATHER) {
+    if (lead) {
       if (known) {
         mbar_arrive_expect_tx(full, 2 * S::TILE_BYTES + (p.scales_by_tma ? 2 * S::SCALE_BYTES : 0));
         tma_load_4d(stage, &p.map_k, full, 0, h, slot, block);
@@ -222,8 +232,8 @@ __device__ __forceinline__ void fetch(const QuantDecParams& p, const Walk& w, co
     }
     if (p.scales_by_tma) return;
   } else {
-    const long long k_row = (long long)block * c.k_stride_b + (long long)slot * c.k_stride_s + h * c.k_stride_h;
-    const long long v_row = (long long)block * c.v_stride_b + (long long)slot * c.v_stride_s + h * c.v_stride_h;
+    const long long k_row = here ? (long long)block * c.k_stride_b + (long long)slot * c.k_stride_s + h * c.k_stride_h : 0;
+    const long long v_row = here ? (long long)block * c.v_stride_b + (long long)slot * c.v_stride_s + h * c.v_stride_h : 0;
     constexpr int ROWS = 32 / S::CH;  // that an instruction of the warp covers
     const uint32_t k_at = smem_u32(stage), v_at = k_at + S::TILE_BYTES;
     const int ch = lane % S::CH;
@@ -235,9 +245,10 @@ __device__ __forceinline__ void fetch(const QuantDecParams& p, const Walk& w, co
       copy16(k_at + place_of<S>(row, ch), reinterpret_cast<const uint8_t*>(c.k) + (take ? k_from + ch * 16 : 0), take ? 16 : 0);
       copy16(v_at + place_of<S>(row, ch), reinterpret_cast<const uint8_t*>(c.v) + (take ? v_from + ch * 16 : 0), take ? 16 : 0);
     }
-    if (lane == 0) mbar_arrive(full);
+    if (lead) mbar_arrive(full);
   }
   // scales: a lane those of its own row
+  const int row_slot = GATHER ? slot : slot + lane;
   const long long ks_row = block * c.ks_stride_b + row_slot * c.ks_stride_s + h * c.ks_stride_h;
   const long long vs_row = block * c.vs_stride_b + row_slot * c.vs_stride_s + h * c.vs_stride_h;
   const uint32_t ks_at = smem_u32(extra) + lane * S::GROUPS * 4, vs_at = ks_at + S::SCALE_BYTES;
@@ -474,7 +485,8 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, con
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[half][nt][i] *= q.scale[nt][i & 1];
   }
-  if (rows != ALL) {
+  const bool partial = __any_sync(ALL, rows != ALL);
+  if (partial) {
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -560,7 +572,7 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, con
           w[k][0] = *reinterpret_cast<const uint16_t*>(values + place_of<S>(row, g) + 2 * r);
         }
         if constexpr (S::FMT == FSA_QC_E4M3) {  // what lies in rows that are not there may be no number
-          if (rows != ALL && !(rows >> row & 1)) {
+          if (partial && !(rows >> row & 1)) {
 #pragma unroll
             for (int x = 0; x < VWORDS; ++x) w[k][x] = 0;
           }
@@ -705,7 +717,7 @@ __device__ __forceinline__ void finish(const QuantDecParams& p, bool half, int b
   if (col == 0) p.lse[b * p.l_sb + hq * p.l_sh] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * CUDART_LN2_F;
 }
 
-template <typename S>
+template <typename S, bool GATHER>
 __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __grid_constant__ QuantDecParams p) {
   after_previous();
   extern __shared__ uint8_t smem_raw[];
@@ -716,28 +728,28 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
   __shared__ const float* part_s[S::WARPS][2];
   __shared__ int2 item_s[S::WARPS];  // of the last piece: sequence, item
   __shared__ int ends_s[S::WARPS];   // whether the first piece's item ends in this warp
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
   uint64_t* full = full_s[warp];
   // a stage is there when its codes are (lane 0, with TMA's bytes) and its scales (the same, or each lane's copies)
   if (lane < S::STAGES) mbar_init(full + lane, p.scales_by_tma ? 1 : 33);
-  if (tid == 0) abort_s = 0;  // (read by a wait that runs out, long after)
+  if (tid == 0) abort_s = 0;
   mbar_fence_init();
   if (lane == 0) {
     part_s[warp][0] = part_s[warp][1] = nullptr;
     ends_s[warp] = 0;
   }
-  __syncwarp();
+  __syncthreads();
 
   // ---- where this warp begins ------------------------------------------------------------------------------------------
   // The first `warps` warps of the grid have equal pieces of the list, of at least a tile; the others none. Every warp adds up the
   // lengths by itself, a lane those of neighbouring sequences: no warp waits for another before it has its first tiles under way.
   const long long g_warp = (long long)blockIdx.x * S::WARPS + warp;
-  Walk walk;
+  Walk<GATHER> walk;
   int mine = 0;
   {
-    auto tiles_at = [&](int b) { return tiles_of(p.gather ? p.topk : keys_of(p, b)); };
-    const bool alike = p.gather || !p.used;
+    auto tiles_at = [&](int b) { return tiles_of(GATHER ? p.topk : keys_of(p, b)); };
+    const bool alike = GATHER || !p.used;
     const int per = (p.batch + 31) / 32, b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
     long long own = 0;
     if (alike) own = (long long)(b1 - b0) * tiles_at(0);
@@ -787,23 +799,23 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     const bool begun = walk.t == 0;
     int sent = 0, into = 0, chosen_next = -1;  // into: the stage that the next copies take
     Place place;
-    {
-      place = look_up(p, walk, p.gather ? chosen(p, walk, lane) : 0);
-      if (p.gather) {
-        Walk ahead = walk;
-        ahead.next(p);
-        chosen_next = chosen(p, ahead, lane);
-      }
+    if constexpr (GATHER) {
+      place = look_up(p, walk, chosen(p, walk, lane));
+      Walk<GATHER> ahead = walk;
+      ahead.next(p);
+      chosen_next = chosen(p, ahead, lane);
+    } else {
+      place = look_up(p, walk, 0);
     }
     auto send = [&]() {
       if (sent < mine) {
-        fetch<S>(p, walk, place, ring + into * S::CODES, extras + into * S::EXTRA, full + into, lane);
+        fetch<S, GATHER>(p, walk, place, ring + into * S::CODES, extras + into * S::EXTRA, full + into, lane);
         ++sent;
         into = into + 1 == S::STAGES ? 0 : into + 1;
         walk.next(p);
         place = look_up(p, walk, chosen_next);
-        if (p.gather) {
-          Walk ahead = walk;
+        if constexpr (GATHER) {
+          Walk<GATHER> ahead = walk;
           if (ahead.b < p.batch) ahead.next(p);
           chosen_next = chosen(p, ahead, lane);
         }
@@ -841,7 +853,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
         fresh = false;
       }
       take_tile<S>(st, q, stage, extra, (uint32_t)what.x, lane);
-      const bool ends = what.y & 1;
+      const bool ends = __any_sync(ALL, what.y);
       if (ends || i + 1 == mine) {
         settle<S>(st);
         if (whole && ends) {
@@ -950,10 +962,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) quant_merge_kernel(const __grid
 // ----------------------------------------------------------------------------------------------
 // Launches
 // ----------------------------------------------------------------------------------------------
-template <typename S>
+template <typename S, bool GATHER>
 cudaError_t launch_both(const QuantDecParams& p, cudaStream_t stream) {
   static std::atomic<unsigned long long> opted_in{0};
-  auto kern = quant_decode_kernel<S>;
+  auto kern = quant_decode_kernel<S, GATHER>;
   if (cudaError_t e = smem_opt_in(kern, S::SMEM, opted_in); e != cudaSuccess) return e;
   cudaError_t e = launch_early(kern, (unsigned)p.ctas, S::THREADS, S::SMEM, stream, 1, p);
   if (e != cudaSuccess || p.ctas == 1) return e;
@@ -1056,6 +1068,7 @@ extern "C" int fsa_decode_quantized(const FsaQuantDecodeArgs* a, void* stream_) 
     const FsaQuantCache& c = p.c;
     const int wide = c.head_dim > 64 ? 128 : 64, bytes = c.format == FSA_QC_INT4 ? wide / 2 : wide;
     const uint64_t slots = c.page_table ? c.page_size : c.capacity, blocks = c.page_table ? c.num_pages : a->batch;
+    p.cache_blocks = (int)blocks;
     auto map = [&](CUtensorMap* m, const void* base, int64_t sb, int64_t ss, int64_t sh) {
       return make_byte_map(m, base, quant_row_bytes(c), c.heads_kv, sh, slots, ss, blocks, sb, bytes, TILE);
     };
@@ -1077,6 +1090,9 @@ extern "C" int fsa_decode_quantized(const FsaQuantDecodeArgs* a, void* stream_) 
   }
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   const cudaError_t e =
-      for_shape(p.c, a->dtype, p.group_heads, [&](auto s) { return launch_both<decltype(s)>(p, reinterpret_cast<cudaStream_t>(stream_)); });
+      for_shape(p.c, a->dtype, p.group_heads, [&](auto s) { 
+        const auto stream = reinterpret_cast<cudaStream_t>(stream_);
+        return p.gather ? launch_both<decltype(s), true>(p, stream) : launch_both<decltype(s), false>(p, stream);
+      });
   return e == cudaSuccess ? FSA_OK : FSA_ERR_LAUNCH;
 }
