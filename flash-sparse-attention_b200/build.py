@@ -33,6 +33,9 @@ SOURCES = [
     "fsa_axes.cu",
     "fsa_quant_cache.cu",
     "fsa_quant_dec_sm100.cu",
+    "fsa_quant_dec_int8_sm100.cu",
+    "fsa_quant_dec_e4m3_sm100.cu",
+    "fsa_quant_dec_int4_sm100.cu",
     "fsa_peer.cu",
 ]
 

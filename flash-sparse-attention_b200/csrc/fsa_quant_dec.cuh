@@ -1,0 +1,985 @@
+// Decode attention over a cache whose rows carry their own scales (fsa_quant_cache.cu): one query position per sequence.
+//
+// With codes k^, v^ and a row's scales a_j (keys), b_j (values)
+//   s_jh = c (q_h . k^_j) a_j            8 bits            c = softmax_scale log2(e)
+//   s_jh = c sum_g (q_hg . (k^_jg - 8)) a_jg + (sum q_hg) z_jg     4 bits, group by group
+//   o_h  = sum_j p_jh b_j v^_j / sum_j p_jh,  p_jh = 2^(s_jh - m_h)
+// so no value is ever rounded on its way: codes are exact in fp16, products and sums are those of the matrix instructions in fp32, scales are
+// applied to scores and to probabilities. The queries enter as fp16 too: a bf16 row is multiplied by a power of two that brings its largest
+// element to [1, 2) (exact but for elements 2^-14 below it, whose lost bits are below the fp32 sum's own), probabilities as fp16 (2^-12) times b_j times a power
+// of two that keeps them in range. Running maxima, sums and outputs are fp32.
+//
+// Bound by memory: a key is read once, at 2 * 8 * (heads per KV head) operations a byte. What a warp does with a tile of 32 keys has to fit
+// into the time that its bytes take, so: products run transposed (keys or value columns on the M = 16 side of mma.m16n8k16, up to eight query
+// heads on the N = 8 side); columns of keys are dealt to lanes so that a lane's codes are neighbours in memory (the sum over columns has no order),
+// values are transposed on their way out of shared memory (ldmatrix on bytes); and codes become fp16 numbers by being taken for the bits of one:
+// n below 1024 in the low bits is the subnormal n 2^-24, which the matrix instructions multiply exactly. Codes are made positive for that (+128, of 4
+// bits they are), and what this adds is taken off where it cannot grow: of scores, a sum over columns, in the first accumulator (-128 2^-24 sum q);
+// of outputs, whose sums over keys run on and on, by a product of the same probabilities with the constant, tile by tile.
+//
+// The work is one list of tiles (sequence, KV head and block of query heads, 32 keys), cut into equal pieces for all warps of the grid whatever the
+// lengths are. A warp streams its piece through a ring of its own in shared memory: TMA brings a tile's codes (cp.async, where positions are
+// chosen one by one), the warp's own mbarriers say when, and no barrier of the CTA is in the loop. A piece that is a whole item is written out, the
+// others meet inside the CTA and then, for items that several CTAs share, in quant_merge_kernel.
+#pragma once
+#include <math_constants.h>
+
+#include <atomic>
+
+#include "fsa_params.h"
+#include "fsa_ptx.cuh"
+#include "fsa_quant_dec.h"
+
+namespace fsa {
+
+constexpr int TILE = QUANT_TILE;
+constexpr uint32_t ALL = 0xffffffffu;
+constexpr int STATUS_WAIT = 1, STATUS_BAD_PAGE = 3;
+constexpr float LAG = 6.f;           // how far (base 2) a score may be above the reference maximum before that moves
+constexpr float MOST_SCALE = 512.f;  // and a value scale above 1: 2^6 * 2^9 is within fp16
+
+template <int HD_, int FMT_, int GROUPS_, int NT_, bool HALF_>
+struct Shape {
+  static constexpr int HD = HD_, FMT = FMT_, GROUPS = GROUPS_, NT = NT_;  // NT: blocks of eight query heads
+  static constexpr bool HALF = HALF_;              // queries and results are fp16, not bf16
+  static constexpr bool INT4 = FMT == FSA_QC_INT4;
+  static constexpr int GS = HD / GROUPS;           // columns of a group
+  static constexpr int RB = INT4 ? HD / 2 : HD;    // bytes of a row
+  static constexpr int CH = RB / 16;
+  static constexpr int KSTEPS = HD / 16, MTILES = HD / 16;
+  // One of a code's units, as it enters the products, and what was added to it. (Of 4 bits every other column enters 16 times as large: of
+  // keys the others' queries make up for it, of values the result is divided.)
+  static constexpr float UNIT = FMT == FSA_QC_E4M3 ? 1.f : 1.f / 16777216.f, K_UNIT = INT4 ? 16.f * UNIT : UNIT;
+  static constexpr float ADDED = FMT == FSA_QC_E4M3 ? 0.f : (FMT == FSA_QC_INT8 ? 128.f : 8.f);
+  static constexpr int HEADS = 8 * NT;
+  static constexpr int TILE_BYTES = TILE * RB, SCALE_BYTES = TILE * GROUPS * 4;
+  // a stage: keys and values, and elsewhere (swizzled tiles begin where their pattern does) their scales and what the tile is
+  static constexpr int CODES = 2 * TILE_BYTES, EXTRA = 2 * SCALE_BYTES + 128;
+  static constexpr int WARPS = NT == 1 ? 12 : 8, THREADS = 32 * WARPS;
+  static constexpr int ALIGN = 8 * RB;             // the swizzle's pattern
+  static constexpr int ROOM = 222 * 1024 / WARPS / ALIGN * ALIGN;
+  static constexpr int STAGES = ROOM / (CODES + EXTRA) > 6 ? 6 : ROOM / (CODES + EXTRA);
+  static constexpr int PIECE = HEADS * (HD + 2);   // floats: outputs, maxima, sums
+  static constexpr int RING = (STAGES * (CODES + EXTRA) + ALIGN - 1) / ALIGN * ALIGN;
+  static constexpr int SMEM = WARPS * RING + 1024;
+  static_assert(STAGES >= 2 && RING >= PIECE * 4 && SMEM <= 225 * 1024, "ring");
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// The barrier counts this lane in when its copies so far have landed.
+__device__ __forceinline__ void arrive_with_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Four codes of eight bits as two pairs of fp16: of int8 bytes (0, 2) and (1, 3) as (code + 128) 2^-24, of e4m3 (0, 1) and (2, 3).
+template <int FMT>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t* lo, uint32_t* hi) {
+  if constexpr (FMT == FSA_QC_INT8) {
+    w ^= 0x80808080u;
+    *lo = __byte_perm(w, 0, 0x4240);
+    *hi = __byte_perm(w, 0, 0x4341);
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(*lo), "=r"(*hi) : "r"(w));
+  }
+}
+// Eight codes of four bits as pairs (0, 4), (1, 5), (2, 6), (3, 7) of fp16: n 2^-24, the second and fourth 16 n 2^-24.
+__device__ __forceinline__ void widen8(uint32_t w, uint32_t* out) {
+  const uint32_t v = w >> 8;
+  out[0] = w & 0x000f000fu;
+  out[1] = w & 0x00f000f0u;
+  out[2] = v & 0x000f000fu;
+  out[3] = v & 0x00f000f0u;
+}
+// Two tiles of 16 rows x 16 bytes, transposed: lane's row address; registers 0, 1 hold bytes lane / 4 and that + 8 of rows 4 (lane % 4) .. + 3 of the
+// first tile, 2 and 3 of the second.
+__device__ __forceinline__ void load_transposed(uint32_t at, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+
+// Where a 16-byte piece of a row lies in a tile's shared memory: TMA's swizzle for rows of that many bytes. Lanes read keys by rows of lane / 4,
+// pieces 2 (lane % 4) and the next (of 128 bytes), values by rows 2 (lane % 4) and so on, pieces of lane / 4: neither meets a bank twice at 128
+// bytes a row; narrower rows of values twice.
+template <typename S>
+__device__ __forceinline__ int place_of(int row, int ch) {
+  if constexpr (S::RB == 128) ch ^= row & 7;
+  else if constexpr (S::RB == 64) ch ^= row >> 1 & 3;
+  else ch ^= row >> 2 & 1;
+  return row * S::RB + ch * 16;
+}
+
+__device__ __forceinline__ int keys_of(const QuantDecParams& p, int b) { return p.used ? min(max(p.used[b], 0), p.keys) : p.keys; }
+__device__ __forceinline__ int tiles_of(int keys) { return keys > 0 ? (keys + TILE - 1) / TILE : 1; }  // (an empty sequence has its zeros written)
+
+// A value that is the same in all lanes, for the compiler to know: branches on it are the warp's, and TMA's operands need no detour.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(ALL, x, 0); }
+
+// Walk over the list: tile t of item (b, i), `left` of the item with this one; `keys` of the sequence, `count` of them (or of the chosen ones) to
+// look at. Behind the last item b is the batch.
+template <bool GATHER>
+struct Walk {
+  int b, i, t, left, tiles, keys, count;
+  __device__ __forceinline__ void sequence(const QuantDecParams& p) {
+    keys = uniform(keys_of(p, b));
+    count = GATHER ? p.topk : keys;
+    tiles = tiles_of(count);
+  }
+  __device__ __forceinline__ void next(const QuantDecParams& p) {
+    ++t;
+    if (--left > 0) return;
+    t = 0;
+    if (++i == p.items) {
+      i = 0;
+      if (++b < p.batch) sequence(p);
+    }
+    left = tiles;
+  }
+};
+
+// The position that this lane's row of a tile is chosen to have, or -1.
+__device__ __forceinline__ int chosen(const QuantDecParams& p, const Walk<true>& w, int lane) {
+  const int at = w.t * TILE + lane;
+  return w.b < p.batch && at < w.count ? p.gather[w.b * p.g_sb + at] : -1;
+}
+
+// Where the rows of a tile lie, fetched one tile ahead: of this lane's row (gather), or of the tile's first key.
+struct Place {
+  int position, block;
+};
+template <bool GATHER>
+__device__ __forceinline__ Place look_up(const QuantDecParams& p, const Walk<GATHER>& w, int position) {
+  Place at;
+  at.position = GATHER ? position : w.t * TILE;
+  if (w.b >= p.batch || at.position < 0 || at.position >= w.keys) at.position = -1;
+  at.block = w.b;
+  if (p.c.page_table) at.block = at.position >= 0 ? p.c.page_table[w.b * p.c.page_table_stride + (at.position >> p.page_shift)] : -1;
+  return at;
+}
+
+// Sends for a tile. Pages hold a multiple of 32 slots, so that without gather the keys of a tile lie in one.
+template <typename S, bool GATHER>
+__device__ __forceinline__ void fetch(const QuantDecParams& p, const Walk<GATHER>& w, const Place& at, uint8_t* stage, uint8_t* extra, uint64_t* full,
+                                      int lane) {
+  const FsaQuantCache& c = p.c;
+  const int h = p.blocks == 1 ? w.i : w.i / p.blocks;
+  const int block = GATHER ? at.block : uniform(at.block);
+  const bool there = at.position >= 0, known = there && (unsigned)block < (unsigned)p.cache_blocks;
+  if (there && !known) report_status(p.status, STATUS_BAD_PAGE);
+  const int slot = c.page_table ? at.position & (c.page_size - 1) : at.position;
+  uint32_t rows;
+  if constexpr (GATHER) {
+    rows = __ballot_sync(ALL, known);
+  } else {
+    const int left = w.count - w.t * TILE;
+    rows = !known ? 0u : (left >= TILE ? ALL : (1u << left) - 1);
+  }
+  const bool lead = elect_one();
+  if (lead) *reinterpret_cast<int4*>(extra + 2 * S::SCALE_BYTES) = make_int4((int)rows, w.left, w.b, w.i);
+  const bool here = rows >> lane & 1;  // this lane's row
+  if constexpr (!GATHER) {
+    if (lead) {
+      if (known) {
+        mbar_arrive_expect_tx(full, 2 * S::TILE_BYTES + (p.scales_by_tma ? 2 * S::SCALE_BYTES : 0));
+        tma_load_4d(stage, &p.map_k, full, 0, h, slot, block);
+        tma_load_4d(stage + S::TILE_BYTES, &p.map_v, full, 0, h, slot, block);
+        if (p.scales_by_tma) {
+          tma_load_3d(extra, &p.map_ks, full, slot * S::GROUPS, h, block);
+          tma_load_3d(extra + S::SCALE_BYTES, &p.map_vs, full, slot * S::GROUPS, h, block);
+        }
+      } else {
+        mbar_arrive(full);
+      }
+    }
+    if (p.scales_by_tma) return;
+  } else {
+    const long long k_row = here ? (long long)block * c.k_stride_b + (long long)slot * c.k_stride_s + h * c.k_stride_h : 0;
+    const long long v_row = here ? (long long)block * c.v_stride_b + (long long)slot * c.v_stride_s + h * c.v_stride_h : 0;
+    constexpr int ROWS = 32 / S::CH;  // that an instruction of the warp covers
+    const uint32_t k_at = smem_u32(stage), v_at = k_at + S::TILE_BYTES;
+    const int ch = lane % S::CH;
+#pragma unroll 4
+    for (int it = 0; it < TILE / ROWS; ++it) {
+      const int row = it * ROWS + lane / S::CH;
+      const long long k_from = __shfl_sync(ALL, k_row, row), v_from = __shfl_sync(ALL, v_row, row);
+      const bool take = (rows >> row & 1) && ch < p.chunks;
+      copy16(k_at + place_of<S>(row, ch), reinterpret_cast<const uint8_t*>(c.k) + (take ? k_from + ch * 16 : 0), take ? 16 : 0);
+      copy16(v_at + place_of<S>(row, ch), reinterpret_cast<const uint8_t*>(c.v) + (take ? v_from + ch * 16 : 0), take ? 16 : 0);
+    }
+    if (lead) mbar_arrive(full);
+  }
+  // scales: a lane those of its own row
+  const int row_slot = GATHER ? slot : slot + lane;
+  const long long ks_row = block * c.ks_stride_b + row_slot * c.ks_stride_s + h * c.ks_stride_h;
+  const long long vs_row = block * c.vs_stride_b + row_slot * c.vs_stride_s + h * c.vs_stride_h;
+  const uint32_t ks_at = smem_u32(extra) + lane * S::GROUPS * 4, vs_at = ks_at + S::SCALE_BYTES;
+#pragma unroll
+  for (int g = 0; g < S::GROUPS; ++g) {
+    const bool take = here && g < p.words;
+    copy4(ks_at + 4 * g, reinterpret_cast<const uint32_t*>(c.k_scales) + (take ? ks_row + g : 0), take ? 4 : 0);
+    copy4(vs_at + 4 * g, reinterpret_cast<const uint32_t*>(c.v_scales) + (take ? vs_row + g : 0), take ? 4 : 0);
+  }
+  arrive_with_copies(full);
+}
+
+// The queries of an item as B operands, with what scores are multiplied by, and their sums (of 4 bits by groups) in units of the codes.
+template <typename S>
+struct Queries {
+  uint32_t f[S::NT][S::KSTEPS][2];
+  float scale[S::NT][2];
+  float sum[S::GROUPS][S::NT][2];
+};
+
+__device__ __forceinline__ uint32_t by16(uint32_t two) {
+  const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&two), __float2half2_rn(16.f));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+template <typename S>
+__device__ __forceinline__ void load_queries(const QuantDecParams& p, int b, int item, int lane, Queries<S>& q) {
+  const int r = lane >> 2, c = lane & 3, h = item / p.blocks, first = (item - h * p.blocks) * S::HEADS;
+#pragma unroll
+  for (int nt = 0; nt < S::NT; ++nt) {
+    const int head = first + nt * 8 + r;
+    const bool there = head < p.group_heads;
+    const uint16_t* row = reinterpret_cast<const uint16_t*>(p.q) + b * p.q_sb + (long long)(h * p.group_heads + (there ? head : 0)) * p.q_sh;
+    uint4 raw[S::KSTEPS / 2];
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < S::KSTEPS / 2; ++i) {  // eight neighbouring columns
+      constexpr int RUNS = S::INT4 ? S::GS / 32 : 2;  // of a group or a piece
+      const int col = S::INT4 ? i / RUNS * S::GS + c * (S::GS / 4) + 8 * (i % RUNS)
+                              : 16 * (S::RB == 128 ? 2 * c + i / 2 : c) + 8 * (i % 2);
+      raw[i] = there && col < p.c.head_dim ? *reinterpret_cast<const uint4*>(row + col) : uint4{};
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) most = max(most, max(w[j] & 0x7fffu, w[j] >> 16 & 0x7fffu));
+    }
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    // the largest element goes to [2^10, 2^11); rows of zeros, and with an infinity or a NaN, stay as they are
+    constexpr int MANTISSA = S::HALF ? 10 : 7, BIAS = S::HALF ? 15 : 127;
+    int e = max((int)(most >> MANTISSA), 1) - BIAS - 10;
+    if (most == 0 || most >= ((2u * BIAS + 1) << MANTISSA)) e = 0;
+    e = min(max(e, -100), 100);
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+    float sums[S::GROUPS] = {};
+#pragma unroll
+    for (int i = 0; i < S::KSTEPS / 2; ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      uint32_t x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __half2 in = *reinterpret_cast<const __half2*>(&w[j]);
+        const float a = S::HALF ? __low2float(in) : __uint_as_float(w[j] << 16), b = S::HALF ? __high2float(in) : __uint_as_float(w[j] & 0xffff0000u);
+        x[j] = pack2<__half>(a * down, b * down);
+        const __half2 two = *reinterpret_cast<const __half2*>(&x[j]);
+        sums[S::INT4 ? i / (S::GS / 32) : 0] += __low2float(two) + __high2float(two);
+      }
+      uint32_t* f0 = q.f[nt][2 * i];
+      uint32_t* f1 = q.f[nt][2 * i + 1];
+      if constexpr (S::FMT == FSA_QC_E4M3) {
+        f0[0] = x[0]; f0[1] = x[1]; f1[0] = x[2]; f1[1] = x[3];
+      } else if constexpr (S::FMT == FSA_QC_INT8) {
+        f0[0] = __byte_perm(x[0], x[1], 0x5410); f0[1] = __byte_perm(x[0], x[1], 0x7632);
+        f1[0] = __byte_perm(x[2], x[3], 0x5410); f1[1] = __byte_perm(x[2], x[3], 0x7632);
+      } else {
+        f0[0] = by16(__byte_perm(x[0], x[2], 0x5410)); f0[1] = __byte_perm(x[0], x[2], 0x7632);
+        f1[0] = by16(__byte_perm(x[1], x[3], 0x5410)); f1[1] = __byte_perm(x[1], x[3], 0x7632);
+      }
+    }
+    const float mine = up * p.scale_log2 * (1.f / S::K_UNIT);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) q.scale[nt][x] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + x));
+    if constexpr (S::ADDED != 0.f) {
+#pragma unroll
+      for (int g = 0; g < S::GROUPS; ++g) {
+        float sum = sums[g] * S::K_UNIT;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) q.sum[g][nt][x] = __shfl_sync(0xffffffffu, sum, 4 * (2 * c + x));
+      }
+    }
+  }
+}
+
+// What a warp knows about an item so far. Lanes: value columns of lane / 4, query heads 2 (lane % 4) and the next.
+template <typename S>
+struct State {
+  float o[S::MTILES][S::NT][4];
+  float centre[S::INT4 ? S::GROUPS : 1][S::NT][2];  // sum p z of this lane's keys
+  float m[S::NT][2], l[S::NT][2];                   // reference maximum; sum of this lane's keys
+  float v_inv;                                      // power of two that value scales are multiplied by; 0: none chosen yet
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int nt = 0; nt < S::NT; ++nt) {
+#pragma unroll
+      for (int t = 0; t < S::MTILES; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][nt][i] = 0.f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        m[nt][x] = -CUDART_INF_F;
+        l[nt][x] = 0.f;
+#pragma unroll
+        for (int g = 0; g < (S::INT4 ? S::GROUPS : 1); ++g) centre[g][nt][x] = 0.f;
+      }
+    }
+    v_inv = 0.f;
+  }
+};
+
+__device__ __forceinline__ float scale_of(uint32_t word, bool int4) { return __uint_as_float(int4 ? word << 16 : word); }
+__device__ __forceinline__ float centre_of(uint32_t word) { return __uint_as_float(word & 0xffff0000u); }
+
+// Moves the reference maxima to what the tile brings, and the power of two of the value scales.
+template <typename S>
+__device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[S::NT][4], float most_scale) {
+#pragma unroll
+  for (int d = 4; d < 32; d <<= 1) most_scale = fmaxf(most_scale, __shfl_xor_sync(0xffffffffu, most_scale, d));
+  float ratio = 1.f;
+  if (st.v_inv == 0.f || most_scale * st.v_inv > MOST_SCALE) {
+    int e = (int)(__float_as_uint(most_scale) >> 23) - 127;
+    e = min(max(e, -126), 126);
+    const float now = __uint_as_float((uint32_t)(127 - e) << 23);
+    if (st.v_inv != 0.f) ratio = now / st.v_inv;  // both powers of two
+    st.v_inv = now;
+  }
+#pragma unroll
+  for (int nt = 0; nt < S::NT; ++nt) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float m = fmaxf(fmaxf(s[0][nt][x], s[0][nt][x + 2]), fmaxf(s[1][nt][x], s[1][nt][x + 2]));
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      m = fmaxf(m, st.m[nt][x]);
+      const float by = m == -CUDART_INF_F ? 1.f : exp2_fast(st.m[nt][x] - m);
+      st.m[nt][x] = m;
+      st.l[nt][x] *= by;
+#pragma unroll
+      for (int g = 0; g < (S::INT4 ? S::GROUPS : 1); ++g) st.centre[g][nt][x] *= by;
+#pragma unroll
+      for (int t = 0; t < S::MTILES; ++t) {
+        st.o[t][nt][x] *= by * ratio;
+        st.o[t][nt][x + 2] *= by * ratio;
+      }
+    }
+  }
+}
+
+// One tile: its two halves of sixteen keys.
+template <typename S>
+__device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uint8_t* stage, const uint8_t* extra, uint32_t rows, int lane) {
+  const int r = lane >> 2, c = lane & 3;
+  uint32_t a_words[4][S::GROUPS], b_words[4][S::GROUPS];  // scales of rows r, r + 8, ..
+  const uint32_t* scales = reinterpret_cast<const uint32_t*>(extra);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int g = 0; g < S::GROUPS; ++g) {
+      a_words[i][g] = scales[(r + 8 * i) * S::GROUPS + g];
+      b_words[i][g] = scales[(TILE + r + 8 * i) * S::GROUPS + g];
+    }
+  // ---- scores: keys r and r + 8 of each half, heads 2 c and 2 c + 1 of each block --------------------------------------
+  float s[2][S::NT][4];
+  constexpr int KWORDS = S::RB / 16 / S::GROUPS;  // of a group, of a lane
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[half][nt][i] = 0.f;
+#pragma unroll
+    for (int g = 0; g < S::GROUPS; ++g) {
+      uint32_t w[2][KWORDS];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = 16 * half + r + 8 * i;
+        if constexpr (!S::INT4) {
+#pragma unroll
+          for (int j = 0; j < KWORDS / 4; ++j) {
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + place_of<S>(row, S::RB == 128 ? 2 * c + j : c));
+            w[i][4 * j] = x.x; w[i][4 * j + 1] = x.y; w[i][4 * j + 2] = x.z; w[i][4 * j + 3] = x.w;
+          }
+        } else if constexpr (KWORDS == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(stage + place_of<S>(row, 2 * g + (c >> 1)) + 8 * (c & 1));
+          w[i][0] = x.x; w[i][1] = x.y;
+        } else {
+          w[i][0] = *reinterpret_cast<const uint32_t*>(stage + place_of<S>(row, g) + 4 * c);
+        }
+      }
+      float acc[S::NT][4];
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[nt][i] = S::ADDED == 0.f ? 0.f : -S::ADDED * q.sum[g][nt][i & 1];
+#pragma unroll
+      for (int j = 0; j < KWORDS; ++j) {
+        if constexpr (!S::INT4) {
+          uint32_t lo0, hi0, lo1, hi1;
+          widen4<S::FMT>(w[0][j], &lo0, &hi0);
+          widen4<S::FMT>(w[1][j], &lo1, &hi1);
+#pragma unroll
+          for (int nt = 0; nt < S::NT; ++nt) mma(acc[nt], lo0, lo1, hi0, hi1, q.f[nt][j][0], q.f[nt][j][1]);
+        } else {
+          uint32_t x0[4], x1[4];
+          widen8(w[0][j], x0);
+          widen8(w[1][j], x1);
+          const int k = 2 * (g * KWORDS + j);
+#pragma unroll
+          for (int nt = 0; nt < S::NT; ++nt) {
+            mma(acc[nt], x0[0], x1[0], x0[1], x1[1], q.f[nt][k][0], q.f[nt][k][1]);
+            mma(acc[nt], x0[2], x1[2], x0[3], x1[3], q.f[nt][k + 1][0], q.f[nt][k + 1][1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t word = a_words[2 * half + (i >> 1)][g];
+          const float by = scale_of(word, S::INT4);
+          if constexpr (S::INT4)
+            s[half][nt][i] = fmaf(acc[nt][i], by, fmaf(q.sum[g][nt][i & 1], centre_of(word), s[half][nt][i]));
+          else
+            s[half][nt][i] = acc[nt][i] * by;
+        }
+    }
+#pragma unroll
+    for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[half][nt][i] *= q.scale[nt][i & 1];
+  }
+  const bool partial = __any_sync(ALL, rows != ALL);
+  if (partial) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(rows >> (16 * half + r + 8 * (i >> 1)) & 1)) s[half][nt][i] = -CUDART_INF_F;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int g = 0; g < S::GROUPS; ++g)
+        if (!(rows >> (r + 8 * i) & 1)) b_words[i][g] = 0;
+    if constexpr (S::FMT == FSA_QC_E4M3) {  // what lies in rows that are not there may be no number
+      if (!(rows >> lane & 1)) {
+#pragma unroll
+        for (int ch = 0; ch < S::CH; ++ch) *reinterpret_cast<uint4*>(stage + S::TILE_BYTES + place_of<S>(lane, ch)) = uint4{};
+      }
+      fence_proxy_async_smem();  // in front of TMA's next writes
+      __syncwarp();
+    }
+  }
+  bool move = false;
+#pragma unroll
+  for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      move = move || fmaxf(fmaxf(s[0][nt][x], s[0][nt][x + 2]), fmaxf(s[1][nt][x], s[1][nt][x + 2])) > st.m[nt][x] + LAG;
+  float most_scale = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int g = 0; g < S::GROUPS; ++g) most_scale = fmaxf(most_scale, scale_of(b_words[i][g], S::INT4));
+  move = move || most_scale * st.v_inv > MOST_SCALE;
+  if (__any_sync(ALL, move)) move_reference<S>(st, s, most_scale);
+
+  // ---- probabilities -------------------------------------------------------------------------------------------------
+#pragma unroll
+  for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float m = st.m[nt][x] == -CUDART_INF_F ? 0.f : st.m[nt][x];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float& e = s[i >> 1][nt][x + 2 * (i & 1)];
+        e = exp2_fast(e - m);
+        st.l[nt][x] += e;
+        if constexpr (S::INT4) {
+#pragma unroll
+          for (int g = 0; g < S::GROUPS; ++g) st.centre[g][nt][x] = fmaf(e, centre_of(b_words[i][g]), st.centre[g][nt][x]);
+        }
+      }
+    }
+  // ---- outputs: value bytes of lane / 4 and that + 8 of each piece, keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 of each half ------------
+  // Row of a half that the lane names to the transposing load: such that what comes out in a register is keys (2 c, 2 c + 8, 2 c + 1, 2 c + 9), or of
+  // e4m3, whose conversion takes neighbouring bytes, (2 c, 2 c + 1, 2 c + 8, 2 c + 9).
+  const int kappa = lane & 15, first = S::FMT == FSA_QC_E4M3 ? kappa : kappa >> 1, second = S::FMT == FSA_QC_E4M3 ? kappa >> 1 : kappa;
+  const int v_row = 16 * (lane >> 4) + 2 * (kappa >> 2) + (first & 1) + 8 * (second & 1);
+  const uint32_t values = smem_u32(stage + S::TILE_BYTES) + place_of<S>(v_row, 0);
+  constexpr int PIECES = S::CH / S::GROUPS;  // of sixteen bytes, of a group
+#pragma unroll
+  for (int g = 0; g < S::GROUPS; ++g) {
+    // Probabilities times scales, of fp16 results with what the rounding to fp16 leaves (else it would be as large as the result's own).
+    uint32_t pb[2][S::NT][2], rest[2][S::HALF ? S::NT : 1][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float by = scale_of(b_words[i][g], S::INT4) * st.v_inv;
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt) {
+        const float x = s[i >> 1][nt][2 * (i & 1)] * by, y = s[i >> 1][nt][2 * (i & 1) + 1] * by;
+        const uint32_t two = pack2<__half>(x, y);
+        pb[i >> 1][nt][i & 1] = transposed(two);
+        if constexpr (S::HALF) {
+          const __half2 h = *reinterpret_cast<const __half2*>(&two);
+          rest[i >> 1][nt][i & 1] = transposed(pack2<__half>(x - __low2float(h), y - __high2float(h)));
+        }
+      }
+    }
+    auto add = [&](int t, int half, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+      // less what was added to the codes: the same products with that, which no rounding of probabilities changes
+      constexpr uint32_t LESS0 = S::INT4 ? 0x80088008u : 0x80808080u, LESS1 = 0x80808080u;
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt) {
+        mma(st.o[t][nt], a0, a1, a2, a3, pb[half][nt][0], pb[half][nt][1]);
+        if constexpr (S::ADDED != 0.f) mma(st.o[t][nt], LESS0, LESS1, LESS0, LESS1, pb[half][nt][0], pb[half][nt][1]);
+        if constexpr (S::HALF) {
+          mma(st.o[t][nt], a0, a1, a2, a3, rest[half][nt][0], rest[half][nt][1]);
+          if constexpr (S::ADDED != 0.f) mma(st.o[t][nt], LESS0, LESS1, LESS0, LESS1, rest[half][nt][0], rest[half][nt][1]);
+        }
+      }
+    };
+#pragma unroll
+    for (int piece = g * PIECES; piece < (g + 1) * PIECES; ++piece) {
+      uint32_t w[4];
+      load_transposed(values ^ (piece * 16), w);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if constexpr (!S::INT4) {
+          uint32_t lo0, hi0, lo1, hi1;
+          widen4<S::FMT>(w[2 * half], &lo0, &hi0);
+          widen4<S::FMT>(w[2 * half + 1], &lo1, &hi1);
+          add(piece, half, lo0, lo1, hi0, hi1);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint32_t f[4];  // even and odd columns of keys 2 c and 2 c + 1, of 2 c + 8 and 2 c + 9
+            widen8(w[2 * half + k], f);
+            add(2 * piece + k, half, f[0], f[1], f[2], f[3]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// Sums over the lanes that share heads, and the outputs in the values' own units, two neighbouring columns in each pair (column_of).
+template <typename S>
+__device__ __forceinline__ void settle(State<S>& st, int lane) {
+  const float by = st.v_inv == 0.f ? 1.f : 1.f / st.v_inv;
+#pragma unroll
+  for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) st.l[nt][x] += __shfl_xor_sync(0xffffffffu, st.l[nt][x], d);
+      if constexpr (S::INT4) {
+#pragma unroll
+        for (int g = 0; g < S::GROUPS; ++g)
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) st.centre[g][nt][x] += __shfl_xor_sync(0xffffffffu, st.centre[g][nt][x], d);
+      }
+#pragma unroll
+      for (int t = 0; t < S::MTILES; ++t) {
+        const float z = S::INT4 ? st.centre[S::INT4 ? t / (S::GS / 16) : 0][nt][x] : 0.f;
+        float a = fmaf(st.o[t][nt][x], by * (1.f / S::UNIT), z), b = fmaf(st.o[t][nt][x + 2], by * (1.f / S::K_UNIT), z);
+        if constexpr (!S::INT4) {  // columns r and r + 8: even rows take the neighbour's first, odd ones its second
+          const float other = __shfl_xor_sync(ALL, lane & 4 ? a : b, 4);
+          if (lane & 4) a = other; else b = other;
+        }
+        st.o[t][nt][x] = a;
+        st.o[t][nt][x + 2] = b;
+      }
+    }
+}
+
+// The first of this lane's two columns in tile t, once settled.
+template <typename S>
+__device__ __forceinline__ int column_of(int t, int r) {
+  return 16 * t + (S::INT4 ? 2 * r : (r & 6) + 8 * (r & 1));
+}
+
+__device__ __forceinline__ void store_two(const QuantDecParams& p, bool half, uint16_t* row, int col, float a, float b) {
+  if (col < p.c.head_dim) *reinterpret_cast<uint32_t*>(row + col) = half ? pack2<__half>(a, b) : pack2<__nv_bfloat16>(a, b);
+}
+
+// A whole item.
+template <typename S>
+__device__ __forceinline__ void write_out(const QuantDecParams& p, const State<S>& st, int b, int item, int lane) {
+  const int r = lane >> 2, c = lane & 3, h = item / p.blocks, first = (item - h * p.blocks) * S::HEADS;
+#pragma unroll
+  for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int head = first + nt * 8 + 2 * c + x;
+      if (head >= p.group_heads) continue;
+      const float l = st.l[nt][x], by = l == 0.f ? 0.f : 1.f / l;
+      const long long hq = (long long)h * p.group_heads + head;
+      uint16_t* row = reinterpret_cast<uint16_t*>(p.out) + b * p.o_sb + hq * p.o_sh;
+#pragma unroll
+      for (int t = 0; t < S::MTILES; ++t) store_two(p, S::HALF, row, column_of<S>(t, r), st.o[t][nt][x] * by, st.o[t][nt][x + 2] * by);
+      if (r == 0) p.lse[b * p.l_sb + hq * p.l_sh] = l == 0.f ? -CUDART_INF_F : (st.m[nt][x] + log2f(l)) * CUDART_LN2_F;
+    }
+}
+
+// A part of one: outputs as they are, maxima, sums.
+template <typename S>
+__device__ __forceinline__ void write_piece(float* to, const State<S>& st, int lane) {
+  const int r = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int head = nt * 8 + 2 * c + x;
+#pragma unroll
+      for (int t = 0; t < S::MTILES; ++t)
+        *reinterpret_cast<float2*>(to + head * S::HD + column_of<S>(t, r)) = make_float2(st.o[t][nt][x], st.o[t][nt][x + 2]);
+      if (r == 0) {
+        to[S::HEADS * S::HD + head] = st.m[nt][x];
+        to[S::HEADS * (S::HD + 1) + head] = st.l[nt][x];
+      }
+    }
+}
+
+// Four columns of a head out of several parts. `part(i)`: where part i lies.
+template <int HD, int HEADS, typename F>
+__device__ __forceinline__ float4 join(int parts, int head, int col, F&& part, float* m_out, float* l_out) {
+  float m = -CUDART_INF_F;
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[HEADS * HD + head]);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int i = 0; i < parts; ++i) {
+    const float* x = part(i);
+    const float mi = x[HEADS * HD + head], by = mi == -CUDART_INF_F ? 0.f : exp2_fast(mi - m);  // (0 times a NaN is one)
+    const float4 v = *reinterpret_cast<const float4*>(x + head * HD + col);
+    o.x = fmaf(v.x, by, o.x);
+    o.y = fmaf(v.y, by, o.y);
+    o.z = fmaf(v.z, by, o.z);
+    o.w = fmaf(v.w, by, o.w);
+    l = fmaf(x[HEADS * (HD + 1) + head], by, l);
+  }
+  *m_out = m;
+  *l_out = l;
+  return o;
+}
+
+__device__ __forceinline__ void finish(const QuantDecParams& p, bool half, int b, int item, int heads, int head, int col, float4 o, float m, float l) {
+  const int h = item / p.blocks, at = (item - h * p.blocks) * heads + head;
+  if (at >= p.group_heads) return;
+  const float by = l == 0.f ? 0.f : 1.f / l;
+  const long long hq = (long long)h * p.group_heads + at;
+  uint16_t* row = reinterpret_cast<uint16_t*>(p.out) + b * p.o_sb + hq * p.o_sh;
+  store_two(p, half, row, col, o.x * by, o.y * by);
+  store_two(p, half, row, col + 2, o.z * by, o.w * by);
+  if (col == 0) p.lse[b * p.l_sb + hq * p.l_sh] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * CUDART_LN2_F;
+}
+
+template <typename S, bool GATHER>
+__global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __grid_constant__ QuantDecParams p) {
+  after_previous();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ uint64_t full_s[S::WARPS][S::STAGES];
+  __shared__ int abort_s;
+  // what a warp's first piece (of an item that began before it) and its last one (of an item that goes on behind it) are
+  __shared__ const float* part_s[S::WARPS][2];
+  __shared__ int2 item_s[S::WARPS];  // of the last piece: sequence, item
+  __shared__ int ends_s[S::WARPS];   // whether the first piece's item ends in this warp
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
+
+  uint64_t* full = full_s[warp];
+  // a stage is there when its codes are (lane 0, with TMA's bytes) and its scales (the same, or each lane's copies)
+  if (lane < S::STAGES) mbar_init(full + lane, p.scales_by_tma ? 1 : 33);
+  if (tid == 0) abort_s = 0;
+  mbar_fence_init();
+  if (lane == 0) {
+    part_s[warp][0] = part_s[warp][1] = nullptr;
+    ends_s[warp] = 0;
+  }
+  __syncthreads();
+
+  // ---- where this warp begins ------------------------------------------------------------------------------------------
+  // The first `warps` warps of the grid have equal pieces of the list, of at least a tile; the others none. Every warp adds up the
+  // lengths by itself, a lane those of neighbouring sequences: no warp waits for another before it has its first tiles under way.
+  const long long g_warp = (long long)blockIdx.x * S::WARPS + warp;
+  Walk<GATHER> walk;
+  int mine = 0;
+  {
+    auto tiles_at = [&](int b) { return tiles_of(GATHER ? p.topk : keys_of(p, b)); };
+    const bool alike = GATHER || !p.used;
+    const int per = (p.batch + 31) / 32, b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
+    long long own = 0;
+    if (alike) own = (long long)(b1 - b0) * tiles_at(0);
+    else for (int b = b0; b < b1; ++b) own += tiles_at(b);
+    long long upto = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(ALL, upto, d);
+      if (lane >= d) upto += o;
+    }
+    const long long total = __shfl_sync(ALL, upto, 31) * p.items, warps = min(total, (long long)p.ctas * S::WARPS);
+    if (g_warp < warps) {
+      const long long at = total * g_warp / warps;
+      mine = (int)min(total * (g_warp + 1) / warps - at, 0x7fffffffll);
+      long long from = (upto - own) * p.items;
+      const bool have = at >= from && at < upto * p.items;
+      int where[3] = {0, 0, 0};
+      if (have) {
+        int b = b0, tiles = tiles_at(b);
+        if (alike) {
+          const long long skip = (at - from) / ((long long)tiles * p.items);
+          b += (int)skip;
+          from += skip * tiles * p.items;
+        } else {
+          while (at >= from + (long long)tiles * p.items) {
+            from += (long long)tiles * p.items;
+            tiles = tiles_at(++b);
+          }
+        }
+        where[0] = b;
+        where[1] = (int)((at - from) / tiles);
+        where[2] = (int)((at - from) % tiles);
+      }
+      const int src = __ffs(__ballot_sync(ALL, have)) - 1;
+      walk.b = __shfl_sync(ALL, where[0], src);
+      walk.i = __shfl_sync(ALL, where[1], src);
+      walk.t = __shfl_sync(ALL, where[2], src);
+    }
+  }
+
+  // ---- this warp's tiles -----------------------------------------------------------------------------------------------
+  uint8_t* ring = smem + warp * S::RING;
+  uint8_t* extras = ring + S::STAGES * S::CODES;
+  float* own_pieces = p.pieces + (long long)blockIdx.x * 2 * S::PIECE;
+  if (mine > 0) {
+    walk.sequence(p);
+    walk.left = walk.tiles - walk.t;
+    int sent = 0, into = 0, chosen_next = -1;  // into: the stage that the next copies take
+    Place place;
+    if constexpr (GATHER) {
+      place = look_up(p, walk, chosen(p, walk, lane));
+      Walk<GATHER> ahead = walk;
+      ahead.next(p);
+      chosen_next = chosen(p, ahead, lane);
+    } else {
+      place = look_up(p, walk, 0);
+    }
+    auto send = [&]() {
+      if (sent == mine) return;
+      fetch<S, GATHER>(p, walk, place, ring + into * S::CODES, extras + into * S::EXTRA, full + into, lane);
+      into = into + 1 == S::STAGES ? 0 : into + 1;
+      if (++sent == mine) return;
+      walk.next(p);
+      place = look_up(p, walk, chosen_next);
+      if constexpr (GATHER) {
+        Walk<GATHER> ahead = walk;
+        ahead.next(p);
+        chosen_next = chosen(p, ahead, lane);
+      }
+    };
+    int2 item = make_int2(walk.b, walk.i);
+    int left = walk.left, done = 0, at = 0;
+    uint32_t phase = 0;
+    bool whole = walk.t == 0;  // the item began in this warp
+    for (int i = 0; i < S::STAGES - 1; ++i) send();
+    Queries<S> q;
+    State<S> st;
+    load_queries<S>(p, item.x, item.y, lane, q);
+    auto arrived = [&]() { return mbar_wait_uniform(full + at, phase, &abort_s); };
+    bool ok = true;
+    for (;;) {
+      st.clear();
+      const int n = min(left, mine - done);
+      for (int i = 0; i < n; ++i) {
+        // all lanes see the tile, and are done with the one whose place the next copies take
+        ok = arrived();
+        if (!ok) break;
+        __syncwarp();
+        send();
+        uint8_t* extra = extras + at * S::EXTRA;
+        take_tile<S>(st, q, ring + at * S::CODES, extra, *reinterpret_cast<const uint32_t*>(extra + 2 * S::SCALE_BYTES), lane);
+        ++done;
+        if (++at == S::STAGES) {
+          at = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      const bool ends = n == left, last = done == mine;
+      settle<S>(st, lane);
+      if (whole && ends) {
+        write_out<S>(p, st, item.x, item.y, lane);
+      } else {
+        // the ring is free behind the last tile; a first piece that is done before goes through the workspace
+        float* to = last ? reinterpret_cast<float*>(ring) : p.pieces + ((long long)p.ctas * 2 + g_warp) * S::PIECE;
+        __syncwarp();
+        write_piece<S>(to, st, lane);
+        if (lane == 0) {
+          part_s[warp][whole] = to;
+          if (whole)
+            item_s[warp] = item;
+          else
+            ends_s[warp] = ends;
+        }
+      }
+      if (last) break;
+      whole = true;
+      ok = arrived();  // the next item says what it is
+      if (!ok) break;
+      const int4 what = *reinterpret_cast<const int4*>(extras + at * S::EXTRA + 2 * S::SCALE_BYTES);
+      left = uniform(what.y);
+      item = make_int2(what.z, what.w);
+      load_queries<S>(p, item.x, item.y, lane, q);
+    }
+    if (!ok) {  // a wait ran out: say so, and wait for what else is under way
+      report_status(p.status, STATUS_WAIT);
+      for (int i = done + 1; i < sent; ++i) mbar_wait_uniform(full + i % S::STAGES, i / S::STAGES & 1, &abort_s);
+    }
+  }
+  __syncthreads();
+  if (abort_s) {  // a wait ran out: nothing to join
+    if (tid == 0) p.shared[blockIdx.x] = make_int2(0, -1);
+    return;
+  }
+
+  // ---- items that several warps share ------------------------------------------------------------------------------------
+  // Runs of pieces of one item, in the order of the warps.
+  int2 told = make_int2(0, -1);
+  int from = -1, kind = 0;  // the run's first warp and which of its pieces
+  auto close = [&](int last, bool ends) {
+    const int w0 = from, k0 = kind;
+    auto part = [&](int i) { return i == 0 ? part_s[w0][k0] : part_s[w0 + i][0]; };
+    const int2 item = k0 ? item_s[w0] : make_int2(0, 0);
+    const bool whole = k0 && ends;
+    float* to = own_pieces + (k0 ? S::PIECE : 0);
+    for (int j = tid; j < S::HEADS * S::HD / 4; j += S::THREADS) {
+      const int head = j / (S::HD / 4), col = 4 * (j % (S::HD / 4));
+      float m, l;
+      const float4 o = join<S::HD, S::HEADS>(last - w0 + 1, head, col, part, &m, &l);
+      if (whole) {
+        finish(p, S::HALF, item.x, item.y, S::HEADS, head, col, o, m, l);
+      } else {
+        *reinterpret_cast<float4*>(to + head * S::HD + col) = o;
+        if (col == 0) {
+          to[S::HEADS * S::HD + head] = m;
+          to[S::HEADS * (S::HD + 1) + head] = l;
+        }
+      }
+    }
+    if (!k0) told.x = ends ? 1 : 2;
+    else if (!ends) told.y = item.x * p.items + item.y;
+    from = -1;
+  };
+  int last = 0;
+  for (int w = 0; w < S::WARPS; ++w) {
+    if (part_s[w][0]) {
+      if (from < 0) {
+        from = w;
+        kind = 0;
+      }
+      last = w;
+      if (ends_s[w]) close(w, true);
+    }
+    if (part_s[w][1]) {
+      from = last = w;
+      kind = 1;
+    }
+  }
+  if (from >= 0) close(last, false);
+  if (tid == 0) p.shared[blockIdx.x] = told;
+}
+
+// Items that several CTAs share: a block takes a quarter of the columns of the item that begins in its CTA, if it goes on in others.
+constexpr int MERGE_THREADS = 128, SLICES = 4;
+
+template <int HD, int HEADS, bool HALF>
+__global__ void __launch_bounds__(MERGE_THREADS) quant_merge_kernel(const __grid_constant__ QuantDecParams p) {
+  after_previous();
+  __shared__ int end_s;
+  const int cta = blockIdx.x / SLICES, slice = blockIdx.x % SLICES;
+  const int item = p.shared[cta].y;
+  if (item < 0) return;
+  if (threadIdx.x == 0) end_s = p.ctas;
+  __syncthreads();
+  for (int c0 = cta + 1; c0 < p.ctas; c0 += MERGE_THREADS) {
+    const int c = c0 + threadIdx.x;
+    const bool ends = c < p.ctas && p.shared[c].x == 1;
+    if (ends) atomicMin(&end_s, c);
+    if (__syncthreads_or(ends)) break;
+  }
+  constexpr int PIECE = HEADS * (HD + 2);
+  const int last = min(end_s, p.ctas - 1);
+  auto part = [&](int i) { return p.pieces + ((long long)(cta + i) * 2 + (i == 0)) * PIECE; };
+  constexpr int WIDE = HD / 4 / SLICES;  // groups of four columns of a slice
+  for (int j = threadIdx.x; j < HEADS * WIDE; j += MERGE_THREADS) {
+    const int head = j / WIDE, col = 4 * (slice * WIDE + j % WIDE);
+    float m, l;
+    const float4 o = join<HD, HEADS>(last - cta + 1, head, col, part, &m, &l);
+    finish(p, HALF, item / p.items, item % p.items, HEADS, head, col, o, m, l);
+  }
+}
+
+// ----------------------------------------------------------------------------------------------
+// Launches
+// ----------------------------------------------------------------------------------------------
+template <typename S, bool GATHER>
+cudaError_t launch_both(const QuantDecParams& p, cudaStream_t stream) {
+  static std::atomic<unsigned long long> opted_in{0};
+  auto kern = quant_decode_kernel<S, GATHER>;
+  if (cudaError_t e = smem_opt_in(kern, S::SMEM, opted_in); e != cudaSuccess) return e;
+  cudaError_t e = launch_early(kern, (unsigned)p.ctas, S::THREADS, S::SMEM, stream, 1, p);
+  if (e != cudaSuccess || p.ctas == 1) return e;
+  return launch_early(quant_merge_kernel<S::HD, S::HEADS, S::HALF>, (unsigned)(p.ctas * SLICES), MERGE_THREADS, 0, stream, 1, p);
+}
+
+// f with the shape that a cache and a number of query heads a KV head need.
+template <int FMT, typename F>
+auto for_shape(const FsaQuantCache& c, int dtype, int group_heads, F&& f) {
+  auto with_heads = [&](auto hd, auto groups) {
+    if (dtype == FSA_DT_FP16)
+      return group_heads > 8 ? f(Shape<hd(), FMT, groups(), 2, true>{}) : f(Shape<hd(), FMT, groups(), 1, true>{});
+    return group_heads > 8 ? f(Shape<hd(), FMT, groups(), 2, false>{}) : f(Shape<hd(), FMT, groups(), 1, false>{});
+  };
+  auto with_width = [&](auto hd) {
+    using std::integral_constant;
+    if constexpr (FMT != FSA_QC_INT4)
+      return with_heads(hd, integral_constant<int, 1>{});
+    else
+      return c.group == 32 ? with_heads(hd, integral_constant<int, hd() / 32>{}) : with_heads(hd, integral_constant<int, hd() / 64>{});
+  };
+  return c.head_dim <= 64 ? with_width(std::integral_constant<int, 64>{}) : with_width(std::integral_constant<int, 128>{});
+}
+
+template <int FMT>
+QuantDecShape quant_decode_shape(const FsaQuantCache& c, int dtype, int group_heads) {
+  return for_shape<FMT>(c, dtype, group_heads, [](auto s) { return QuantDecShape{decltype(s)::WARPS, decltype(s)::PIECE, decltype(s)::HEADS}; });
+}
+template <int FMT>
+cudaError_t launch_quant_decode(const QuantDecParams& p, int dtype, cudaStream_t stream) {
+  return for_shape<FMT>(p.c, dtype, p.group_heads, [&](auto s) {
+    return p.gather ? launch_both<decltype(s), true>(p, stream) : launch_both<decltype(s), false>(p, stream);
+  });
+}
+
+}  // namespace fsa
