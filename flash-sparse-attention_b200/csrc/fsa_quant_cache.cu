@@ -32,28 +32,26 @@ struct QuantPut {
   int chunk_shift; // log2 of the chunks of a group
 };
 
-__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
-// The larger magnitude as bits: NaN is above infinity, and infinity above the rest.
-__device__ __forceinline__ uint32_t largest(const float* y, uint32_t most) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) most = max(most, magnitude(y[i]));
-  return most;
+// Extremes that a NaN does not get lost in.
+__device__ __forceinline__ float larger(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float smaller(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
-constexpr uint32_t BITS_INF = 0x7f800000u, BITS_TINY = 0x00800000u;  // 2^-126
+constexpr float TINY = 1.17549435e-38f;  // 2^-126
 
 // Scale of a row whose largest magnitude is `most`, and what its values are multiplied by.
-__device__ __forceinline__ float row_scale(uint32_t most, float top, float* inverse) {
-  const float s = __fdiv_rn(__uint_as_float(most), top);
-  if (most >= BITS_INF) {
-    *inverse = 0.f;
-    return __uint_as_float(0x7fffffffu);
-  }
-  if (__float_as_uint(s) < BITS_TINY) {
-    *inverse = 0.f;
-    return 0.f;
-  }
+__device__ __forceinline__ float row_scale(float most, float top, float* inverse) {
+  const float s = __fdiv_rn(most, top);
+  *inverse = 0.f;
+  if (!(most < INFINITY)) return NAN;
+  if (s < TINY) return 0.f;
   *inverse = __frcp_rn(s);
   return s;
 }
@@ -63,18 +61,18 @@ __device__ __forceinline__ uint2 codes8(const float* y, float inverse, bool fini
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    uint32_t r = 0;
     if constexpr (FMT == FSA_QC_INT8) {
+      // clamped and rounded to the nearest even integer by an addition that leaves no bits for less; the low byte is the code
+      uint32_t n[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = fminf(fmaxf(__fmul_rn(y[4 * i + j], inverse), -127.f), 127.f);
-        r |= (uint32_t)(__float2int_rn(x) & 0xff) << (8 * j);
-      }
+      for (int j = 0; j < 4; ++j)
+        n[j] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(y[4 * i + j], inverse), -127.f), 127.f), 12582912.f));
+      w[i] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
     } else {
-      r = pack4_fp8<__nv_fp8_e4m3>(__fmul_rn(y[4 * i], inverse), __fmul_rn(y[4 * i + 1], inverse), __fmul_rn(y[4 * i + 2], inverse),
-                                   __fmul_rn(y[4 * i + 3], inverse));
+      w[i] = pack4_fp8<__nv_fp8_e4m3>(__fmul_rn(y[4 * i], inverse), __fmul_rn(y[4 * i + 1], inverse), __fmul_rn(y[4 * i + 2], inverse),
+                                      __fmul_rn(y[4 * i + 3], inverse));
     }
-    w[i] = finite ? r : 0u;
+    if (!finite) w[i] = 0;
   }
   return make_uint2(w[0], w[1]);
 }
@@ -84,30 +82,31 @@ struct Pair4 {
   uint32_t word;
   float z, inverse;
 };
-__device__ __forceinline__ Pair4 group_pair(float low, float high, bool finite) {
+__device__ __forceinline__ Pair4 group_pair(float low, float high) {
   Pair4 p;
   const float width = __fdiv_rn(__fsub_rn(high, low), 15.f);
   float s = __bfloat162float(__float2bfloat16_rn(width));
-  if (__float_as_uint(s) < BITS_TINY) s = 0.f;
+  if (s < TINY) s = 0.f;
   p.z = __bfloat162float(__float2bfloat16_rn(__fadd_rn(low, 8.f * s)));
   p.inverse = s > 0.f ? __frcp_rn(s) : 0.f;
-  if (!finite || magnitude(s) >= BITS_INF || magnitude(p.z) >= BITS_INF) {
+  p.word = (__float_as_uint(s) >> 16) | (__float_as_uint(p.z) & 0xffff0000u);
+  if (!(s < INFINITY) || !(fabsf(p.z) < INFINITY)) {  // an infinity or a NaN among the values
     p.word = 0x7fff7fffu;
-    p.z = 0.f;
-    p.inverse = 0.f;
-  } else {
-    p.word = (__float_as_uint(s) >> 16) | (__float_as_uint(p.z) & 0xffff0000u);
+    p.z = NAN;
   }
   return p;
 }
 __device__ __forceinline__ uint32_t codes4(const float* y, const Pair4& p) {
-  uint32_t r = 0;
+  // as above, and eight such numbers put together by their sum, less what they have in common
+  constexpr uint32_t COMMON = 0x4b400000u;  // 12582912
+  uint32_t r = 0, common = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const float x = rintf(__fmul_rn(__fsub_rn(y[i], p.z), p.inverse));
-    r |= (uint32_t)(8 + (int)fminf(fmaxf(x, -8.f), 7.f)) << (4 * i);
+    const float x = fminf(fmaxf(__fmul_rn(__fsub_rn(y[i], p.z), p.inverse), -8.f), 7.f);
+    r += __float_as_uint(__fadd_rn(x, 12582920.f)) << (4 * i);
+    common += COMMON << (4 * i);
   }
-  return r;
+  return r - common;
 }
 
 // Quantises a row that `lanes` neighbouring lanes hold (all of the warp come here) and stores it if `live`.
@@ -115,42 +114,37 @@ template <int FMT>
 __device__ __forceinline__ void put_row(const QuantPut& p, const float* ya, const float* yb, int a, int b, bool has_a, bool has_b, bool live, int u,
                                         uint8_t* codes, uint32_t* scales) {
   if constexpr (FMT != FSA_QC_INT4) {
-    uint32_t most = 0;
-    if (has_a) most = largest(ya, most);
-    if (has_b) most = largest(yb, most);
-    for (int d = p.lanes >> 1; d; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+    float most = 0.f;  // (columns that this lane does not have are zeros)
+#pragma unroll
+    for (int i = 0; i < V; ++i) most = larger(most, larger(fabsf(ya[i]), fabsf(yb[i])));
+    for (int d = p.lanes >> 1; d; d >>= 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, d));
     float inverse;
     const float s = row_scale(most, FMT == FSA_QC_INT8 ? 127.f : 448.f, &inverse);
     if (!live) return;
-    const bool finite = most < BITS_INF;
+    const bool finite = most < INFINITY;
     if (has_a) *reinterpret_cast<uint2*>(codes + a) = codes8<FMT>(ya, inverse, finite);
     if (has_b) *reinterpret_cast<uint2*>(codes + b) = codes8<FMT>(yb, inverse, finite);
     if (u == 0) *scales = __float_as_uint(s);
   } else {
-    float low_a = INFINITY, high_a = -INFINITY, low_b = INFINITY, high_b = -INFINITY;
-    uint32_t most_a = 0, most_b = 0;
+    float low_a = ya[0], high_a = ya[0], low_b = yb[0], high_b = yb[0];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      low_a = fminf(low_a, ya[i]);
-      high_a = fmaxf(high_a, ya[i]);
-      low_b = fminf(low_b, yb[i]);
-      high_b = fmaxf(high_b, yb[i]);
+    for (int i = 1; i < V; ++i) {
+      low_a = smaller(low_a, ya[i]);
+      high_a = larger(high_a, ya[i]);
+      low_b = smaller(low_b, yb[i]);
+      high_b = larger(high_b, yb[i]);
     }
-    most_a = largest(ya, 0);
-    most_b = largest(yb, 0);
     const int ga = has_a ? a / V >> p.chunk_shift : -1, gb = has_b ? b / V >> p.chunk_shift : -1;
     for (int g = 0; g < p.groups; ++g) {
-      float low = fminf(ga == g ? low_a : INFINITY, gb == g ? low_b : INFINITY);
-      float high = fmaxf(ga == g ? high_a : -INFINITY, gb == g ? high_b : -INFINITY);
-      bool wrong = (ga == g && most_a >= BITS_INF) || (gb == g && most_b >= BITS_INF);
+      float low = smaller(ga == g ? low_a : INFINITY, gb == g ? low_b : INFINITY);
+      float high = larger(ga == g ? high_a : -INFINITY, gb == g ? high_b : -INFINITY);
       for (int d = p.lanes >> 1; d; d >>= 1) {
-        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, d));
-        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+        low = smaller(low, __shfl_xor_sync(0xffffffffu, low, d));
+        high = larger(high, __shfl_xor_sync(0xffffffffu, high, d));
       }
-      const unsigned all = __ballot_sync(0xffffffffu, wrong);
-      wrong = (all >> ((threadIdx.x & 31) & ~(p.lanes - 1)) & ((1u << p.lanes) - 1)) != 0;
       if (!live) continue;
-      const Pair4 pair = group_pair(low, high, !wrong);
+      const Pair4 pair = group_pair(low, high);
+      const bool wrong = isnan(pair.z);
       if (ga == g) *reinterpret_cast<uint32_t*>(codes + a / 2) = wrong ? 0x88888888u : codes4(ya, pair);
       if (gb == g) *reinterpret_cast<uint32_t*>(codes + b / 2) = wrong ? 0x88888888u : codes4(yb, pair);
       if (u == 0) scales[g] = pair.word;
@@ -246,6 +240,7 @@ __device__ __forceinline__ void store_row(const QuantPut& p, long long bi, long 
     if (has_b) store16<T, V>(out, b, yb);
   }
   const bool live = t.live && h >= q.heads_q;
+  if (!__any_sync(0xffffffffu, live)) return;
   uint8_t* codes = nullptr;
   uint32_t* scales = nullptr;
   if (live) {
@@ -323,9 +318,10 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const __grid_consta
 
 // Few tokens, pages assigned: a block per sequence finds its slots, stores its rows and advances its length, in one launch.
 constexpr int STEP_PAGES = 4;  // that the new rows of a sequence may touch
+constexpr int STEP_THREADS = 512;
 
 template <typename T, int FMT, bool IL>
-__global__ void __launch_bounds__(1024) quant_step_kernel(const __grid_constant__ QuantPut p) {
+__global__ void __launch_bounds__(STEP_THREADS) quant_step_kernel(const __grid_constant__ QuantPut p) {
   after_previous();
   const AppendParams& q = p.a;
   const int b = blockIdx.x, heads = q.heads_q + 2 * q.heads_kv, items = q.new_tokens * heads * p.lanes;
@@ -384,6 +380,8 @@ struct QuantGet {
   long long ko_sb, ko_ss, ko_sh, vo_sb, vo_ss, vo_sh;
   int batch, seqlen, total, pieces;  // pieces: of sixteen columns, of a head
   int group_shift;                   // log2 of the pieces of a group
+  int of_head;                       // 2^16 / pieces, rounded up
+  int step_tokens, step_rest;        // READ_THREADS in tokens and pieces
 };
 
 // Sixteen values.
@@ -393,21 +391,22 @@ __device__ __forceinline__ void widen(uint4 raw, uint32_t scale, float* y) {
   if constexpr (FMT == FSA_QC_INT4) {
     const float s = __uint_as_float(scale << 16), z = __uint_as_float(scale & 0xffff0000u);
 #pragma unroll
-    for (int i = 0; i < COLUMNS; ++i) y[i] = __fmaf_rn((float)((int)(w[i >> 3] >> (4 * (i & 7)) & 15u) - 8), s, z);
+    for (int i = 0; i < COLUMNS; ++i)  // 2^23 + code, less that and 8
+      y[i] = __fmaf_rn(__uint_as_float(0x4b000000u | (w[i >> 3] >> (4 * (i & 7)) & 15u)) - 8388616.f, s, z);
+  } else if constexpr (FMT == FSA_QC_INT8) {
+    const float s = __uint_as_float(scale);
+#pragma unroll
+    for (int i = 0; i < COLUMNS; ++i)  // 2^23 + 128 + code
+      y[i] = __fmul_rn(__uint_as_float(__byte_perm(w[i >> 2] ^ 0x80808080u, 0x4b000000u, 0x7650 | (i & 3))) - 8388736.f, s);
   } else {
     const float s = __uint_as_float(scale);
 #pragma unroll
-    for (int i = 0; i < COLUMNS; ++i) {
-      const uint32_t code = w[i >> 2] >> (8 * (i & 3)) & 0xffu;
-      float x;
-      if constexpr (FMT == FSA_QC_INT8) {
-        x = (float)(int8_t)code;
-      } else {
-        __nv_fp8_e4m3 f;
-        f.__x = (unsigned char)code;
-        x = (float)f;
-      }
-      y[i] = __fmul_rn(x, s);
+    for (int i = 0; i < COLUMNS; i += 2) {
+      uint32_t two;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"((uint16_t)(w[i >> 2] >> (8 * (i & 2)))));
+      const __half2 h = *reinterpret_cast<const __half2*>(&two);
+      y[i] = __fmul_rn(__low2float(h), s);
+      y[i + 1] = __fmul_rn(__high2float(h), s);
     }
   }
 }
@@ -415,21 +414,25 @@ __device__ __forceinline__ void widen(uint4 raw, uint32_t scale, float* y) {
 template <typename T, int FMT>
 __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const __grid_constant__ QuantGet p) {
   after_previous();
-  __shared__ long long block_of[READ_TOKENS];
-  __shared__ int slot_of[READ_TOKENS];  // -1: zeros
+  // of each token: where its rows' codes and scales begin (-1: zeros), and its result's
+  __shared__ long long code_at[READ_TOKENS], scale_at[READ_TOKENS], out_at[READ_TOKENS];
   const unsigned t0 = (blockIdx.x >> 1) * (unsigned)READ_TOKENS;
   const int here = (int)min((unsigned)READ_TOKENS, (unsigned)p.total - t0);
+  const bool is_v = blockIdx.x & 1;
   if (threadIdx.x < here) {
     const unsigned t = t0 + threadIdx.x;
     int seq, slot;
     bool in = true;
+    long long to;
     if (p.cu) {
       seq = sequence_of(p.cu, p.batch, (int)t);
       in = seq < p.batch;
       slot = in ? (int)t - p.cu[seq] : 0;
+      to = t * (is_v ? p.vo_ss : p.ko_ss);
     } else {
       seq = (int)(t / (unsigned)p.seqlen);
       slot = (int)(t - seq * (unsigned)p.seqlen);
+      to = seq * (is_v ? p.vo_sb : p.ko_sb) + slot * (is_v ? p.vo_ss : p.ko_ss);
     }
     const long long cap = p.c.page_table ? (long long)p.c.max_pages * p.c.page_size : p.c.capacity;
     in = in && slot >= 0 && slot < cap && (!p.used || slot < p.used[seq]);
@@ -442,57 +445,61 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const __grid_c
         report_status(p.status, STATUS_NO_ROOM);
       }
     }
-    block_of[threadIdx.x] = block;
-    slot_of[threadIdx.x] = in ? slot : -1;
+    code_at[threadIdx.x] = in ? block * (is_v ? p.c.v_stride_b : p.c.k_stride_b) + slot * (is_v ? p.c.v_stride_s : p.c.k_stride_s) : -1;
+    scale_at[threadIdx.x] = block * (is_v ? p.c.vs_stride_b : p.c.ks_stride_b) + slot * (is_v ? p.c.vs_stride_s : p.c.ks_stride_s);
+    out_at[threadIdx.x] = to;
   }
   __syncthreads();
-  const int per_token = p.pieces * p.c.heads_kv, items = here * per_token;
-  const bool is_v = blockIdx.x & 1;
-  const long long sb = is_v ? p.c.v_stride_b : p.c.k_stride_b, ss = is_v ? p.c.v_stride_s : p.c.k_stride_s, sh = is_v ? p.c.v_stride_h : p.c.k_stride_h;
-  const long long ws = is_v ? p.c.vs_stride_b : p.c.ks_stride_b, wt = is_v ? p.c.vs_stride_s : p.c.ks_stride_s, wh = is_v ? p.c.vs_stride_h : p.c.ks_stride_h;
-  const long long ob = is_v ? p.vo_sb : p.ko_sb, os = is_v ? p.vo_ss : p.ko_ss, oh = is_v ? p.vo_sh : p.ko_sh;
+  const int per_token = p.pieces * p.c.heads_kv;
+  const long long sh = is_v ? p.c.v_stride_h : p.c.k_stride_h, wh = is_v ? p.c.vs_stride_h : p.c.ks_stride_h, oh = is_v ? p.vo_sh : p.ko_sh;
   const uint8_t* codes = reinterpret_cast<const uint8_t*>(is_v ? p.c.v : p.c.k);
   const uint32_t* scales = reinterpret_cast<const uint32_t*>(is_v ? p.c.v_scales : p.c.k_scales);
   T* out = reinterpret_cast<T*>(is_v ? p.v_out : p.k_out);
+  // Piece e of head h of token t: a thread's pieces are READ_THREADS apart, which it counts out without dividing.
   constexpr int BATCH = 4;  // pieces a thread has under way
-  for (int i0 = threadIdx.x; i0 < items; i0 += BATCH * READ_THREADS) {
+  int t = threadIdx.x / per_token, rest = threadIdx.x - t * per_token;
+  while (t < here) {
     uint4 raw[BATCH];
     uint32_t scale[BATCH];
+    T* to[BATCH];
 #pragma unroll
     for (int j = 0; j < BATCH; ++j) {
-      const int i = i0 + j * READ_THREADS;
       raw[j] = uint4{};
       scale[j] = 0;
-      if (i >= items) continue;
-      const int t = i / per_token, rest = i - t * per_token, h = rest / p.pieces, e = rest - h * p.pieces;
-      const int slot = slot_of[t];
-      if (slot < 0) continue;
-      const uint8_t* row = codes + block_of[t] * sb + slot * ss + h * sh;
-      if constexpr (FMT == FSA_QC_INT4) {
-        const uint2 half = __ldg(reinterpret_cast<const uint2*>(row) + e);
-        raw[j].x = half.x;
-        raw[j].y = half.y;
-      } else {
-        raw[j] = __ldg(reinterpret_cast<const uint4*>(row) + e);
+      to[j] = nullptr;
+      if (t < here) {
+        const int h = rest * p.of_head >> 16, e = rest - h * p.pieces;
+        const long long at = code_at[t];
+        if (at >= 0) {
+          const uint8_t* row = codes + at + h * sh;
+          if constexpr (FMT == FSA_QC_INT4) {
+            const uint2 half = __ldcs(reinterpret_cast<const uint2*>(row) + e);
+            raw[j].x = half.x;
+            raw[j].y = half.y;
+          } else {
+            raw[j] = __ldcs(reinterpret_cast<const uint4*>(row) + e);
+          }
+          scale[j] = __ldg(scales + scale_at[t] + h * wh + (FMT == FSA_QC_INT4 ? e >> p.group_shift : 0));
+        }
+        to[j] = out + out_at[t] + h * oh + e * COLUMNS;
+        t += p.step_tokens;
+        rest += p.step_rest;
+        if (rest >= per_token) {
+          rest -= per_token;
+          ++t;
+        }
       }
-      scale[j] = __ldg(scales + block_of[t] * ws + slot * wt + h * wh + (FMT == FSA_QC_INT4 ? e >> p.group_shift : 0));
     }
 #pragma unroll
     for (int j = 0; j < BATCH; ++j) {
-      const int i = i0 + j * READ_THREADS;
-      if (i >= items) continue;
-      const int t = i / per_token, rest = i - t * per_token, h = rest / p.pieces, e = rest - h * p.pieces;
+      if (!to[j]) continue;
       float y[COLUMNS];
       widen<FMT>(raw[j], scale[j], y);
-      const unsigned tok = t0 + (unsigned)t;
-      long long bi = 0, si = tok;
-      if (!p.cu) {
-        bi = tok / (unsigned)p.seqlen;
-        si = tok - bi * p.seqlen;
-      }
-      T* to = out + bi * ob + si * os + h * oh + e * COLUMNS;
-      store16<T, V>(to, 0, y);
-      store16<T, V>(to, V, y + V);
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = pack2<T>(y[2 * i], y[2 * i + 1]);
+      __stcs(reinterpret_cast<uint4*>(to[j]), make_uint4(w[0], w[1], w[2], w[3]));
+      __stcs(reinterpret_cast<uint4*>(to[j]) + 1, make_uint4(w[4], w[5], w[6], w[7]));
     }
   }
 }
@@ -612,7 +619,7 @@ extern "C" int fsa_kv_append_quantized(const FsaKvAppendQuantArgs* a, void* stre
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (in_one_step(a)) {
     const long long items = (long long)a->new_tokens * heads * p.lanes;
-    const int threads = items >= 1024 ? 1024 : (int)((items + 31) & ~31ll);
+    const int threads = items >= STEP_THREADS ? STEP_THREADS : (int)((items + 31) & ~31ll);
     const cudaError_t e = for_format(a->dtype, c.format, [&](auto t, auto fmt) {
       return a->interleaved ? launch_early(quant_step_kernel<decltype(t), fmt(), true>, (unsigned)a->batch, threads, 0, stream, 1, p)
                             : launch_early(quant_step_kernel<decltype(t), fmt(), false>, (unsigned)a->batch, threads, 0, stream, 1, p);
@@ -665,6 +672,11 @@ extern "C" int fsa_kv_read_quantized(const FsaKvReadQuantArgs* a, void* stream_)
   p.total = (int)total;
   p.pieces = c.head_dim / COLUMNS;
   p.group_shift = c.group == 32 ? 1 : 2;
+  const int per_token = p.pieces * c.heads_kv;
+  if (per_token > 8192) return FSA_ERR_UNSUPPORTED;  // what of_head divides exactly
+  p.of_head = (65536 + p.pieces - 1) / p.pieces;
+  p.step_tokens = READ_THREADS / per_token;
+  p.step_rest = READ_THREADS % per_token;
   const unsigned blocks = (unsigned)((total + READ_TOKENS - 1) / READ_TOKENS);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const cudaError_t e = for_format(a->dtype, c.format, [&](auto t, auto fmt) {
