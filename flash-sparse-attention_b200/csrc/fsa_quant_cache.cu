@@ -27,7 +27,7 @@ struct QuantPut {
   AppendParams a;  // places, rows and strides; the cache's own are below
   AxisMap m;       // positions given token by token (ids null: those of the slots)
   FsaQuantCache c;
-  int lanes;       // of a row
+  int lanes, lane_shift;  // of a row, and its log2
   int groups;      // of a row: words of scales
   int chunk_shift; // log2 of the chunks of a group
 };
@@ -134,21 +134,34 @@ __device__ __forceinline__ void put_row(const QuantPut& p, const float* ya, cons
       low_b = smaller(low_b, yb[i]);
       high_b = larger(high_b, yb[i]);
     }
+    // Lane u finds the pair of group u for all.
     const int ga = has_a ? a / V >> p.chunk_shift : -1, gb = has_b ? b / V >> p.chunk_shift : -1;
-    for (int g = 0; g < p.groups; ++g) {
+    float low_u = 0.f, high_u = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      if (g >= p.groups) break;
       float low = smaller(ga == g ? low_a : INFINITY, gb == g ? low_b : INFINITY);
       float high = larger(ga == g ? high_a : -INFINITY, gb == g ? high_b : -INFINITY);
       for (int d = p.lanes >> 1; d; d >>= 1) {
         low = smaller(low, __shfl_xor_sync(0xffffffffu, low, d));
         high = larger(high, __shfl_xor_sync(0xffffffffu, high, d));
       }
-      if (!live) continue;
-      const Pair4 pair = group_pair(low, high);
-      const bool wrong = isnan(pair.z);
-      if (ga == g) *reinterpret_cast<uint32_t*>(codes + a / 2) = wrong ? 0x88888888u : codes4(ya, pair);
-      if (gb == g) *reinterpret_cast<uint32_t*>(codes + b / 2) = wrong ? 0x88888888u : codes4(yb, pair);
-      if (u == 0) scales[g] = pair.word;
+      if (u == g) {
+        low_u = low;
+        high_u = high;
+      }
     }
+    const Pair4 mine = group_pair(low_u, high_u);
+    const int first = (threadIdx.x & 31) - u;  // the row's first lane
+    Pair4 of_a, of_b;
+    of_a.z = __shfl_sync(0xffffffffu, mine.z, first + max(ga, 0));
+    of_a.inverse = __shfl_sync(0xffffffffu, mine.inverse, first + max(ga, 0));
+    of_b.z = __shfl_sync(0xffffffffu, mine.z, first + max(gb, 0));
+    of_b.inverse = __shfl_sync(0xffffffffu, mine.inverse, first + max(gb, 0));
+    if (!live) return;
+    if (has_a) *reinterpret_cast<uint32_t*>(codes + a / 2) = isnan(of_a.z) ? 0x88888888u : codes4(ya, of_a);
+    if (has_b) *reinterpret_cast<uint32_t*>(codes + b / 2) = isnan(of_b.z) ? 0x88888888u : codes4(yb, of_b);
+    if (u < p.groups) scales[u] = mine.word;
   }
 }
 
@@ -199,14 +212,11 @@ __device__ __forceinline__ void load_row(const AppendParams& p, long long bi, lo
   xb.raw = has_b ? __ldcs(reinterpret_cast<const uint4*>(src + b)) : uint4{};
 }
 
-// All lanes of the warp come here, those without a row with h < 0.
-template <typename T, int FMT, bool IL>
-__device__ __forceinline__ void store_row(const QuantPut& p, long long bi, long long si, int h, int a, int b, bool has_a, bool has_b, bool turns, int u,
-                                          const TokenPlace& t, const float* c, const float* s, const Chunk<T, V>& xa, const Chunk<T, V>& xb) {
-  const AppendParams& q = p.a;
-  const bool is_q = h >= 0 && h < q.heads_q, is_v = h >= q.heads_q + q.heads_kv;
-  float ya[V], yb[V];
-  if (turns && !is_v && t.live && t.turned) {
+// A row's two chunks as numbers, turned or as they are; zeros if it is not to be there.
+template <typename T, bool IL>
+__device__ __forceinline__ void row_values(const Chunk<T, V>& xa, const Chunk<T, V>& xb, bool turns, bool there, const float* c, const float* s, float* ya,
+                                           float* yb) {
+  if (turns && there) {
     // (each product and sum rounded: the same numbers whoever computes them)
     if constexpr (IL) {
 #pragma unroll
@@ -227,13 +237,22 @@ __device__ __forceinline__ void store_row(const QuantPut& p, long long bi, long 
       }
     }
   } else {
-    const bool there = t.live && (is_v || t.turned);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       ya[i] = there ? float(xa.e[i]) : 0.f;
       yb[i] = there ? float(xb.e[i]) : 0.f;
     }
   }
+}
+
+// All lanes of the warp come here, those without a row with h < 0.
+template <typename T, int FMT, bool IL>
+__device__ __forceinline__ void store_row(const QuantPut& p, long long bi, long long si, int h, int a, int b, bool has_a, bool has_b, bool turns, int u,
+                                          const TokenPlace& t, const float* c, const float* s, const Chunk<T, V>& xa, const Chunk<T, V>& xb) {
+  const AppendParams& q = p.a;
+  const bool is_q = h >= 0 && h < q.heads_q, is_v = h >= q.heads_q + q.heads_kv;
+  float ya[V], yb[V];
+  row_values<T, IL>(xa, xb, turns && !is_v, t.live && (is_v || t.turned), c, s, ya, yb);
   if (is_q) {
     T* out = reinterpret_cast<T*>(q.q_out) + bi * q.qo_sb + si * q.qo_ss + (long long)h * q.qo_sh;
     if (has_a) store16<T, V>(out, a, ya);
@@ -266,7 +285,8 @@ __device__ __forceinline__ void my_columns(const QuantPut& p, int u, int& a, int
   if (has_a) chunk_columns<V, IL>(p.a.r, u, a, b, has_b);
 }
 
-template <typename T, int FMT, bool IL, int HPT>
+// Few tokens: a thread has one row's share.
+template <typename T, int FMT, bool IL>
 __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const __grid_constant__ QuantPut p) {
   after_previous();
   const AppendParams& q = p.a;
@@ -276,7 +296,6 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const __grid_consta
   const bool in = t < (unsigned)q.total;
   const unsigned rest = idx - t * per_token;
   const int slot = (int)(rest / (unsigned)p.lanes), u = (int)(rest - slot * (unsigned)p.lanes);
-  const int heads = q.heads_q + 2 * q.heads_kv;
   int a, b;
   bool has_a, has_b;
   my_columns<IL>(p, u, a, b, has_a, has_b);
@@ -285,10 +304,8 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const __grid_consta
     bi = t / (unsigned)q.new_tokens;
     si = t - bi * q.new_tokens;
   }
-  Chunk<T, V> xa[HPT], xb[HPT];
-#pragma unroll
-  for (int i = 0; i < HPT; ++i)
-    if (in && slot + i * q.slots < heads) load_row<T>(q, bi, si, slot + i * q.slots, a, b, has_a, has_b, xa[i], xb[i]);
+  Chunk<T, V> xa, xb;
+  if (in) load_row<T>(q, bi, si, slot, a, b, has_a, has_b, xa, xb);
 
   TokenPlace place;
   place.live = false;
@@ -309,10 +326,95 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const __grid_consta
   const bool turns = has_a && u < q.r.turned;
   float c[V], s[V];
   if (turns && place.live && place.turned) angles_of<T, IL>(p, place, a, b, c, s);
+  store_row<T, FMT, IL>(p, bi, si, in ? slot : -1, a, b, has_a, has_b, turns, u, place, c, s, xa, xb);
+}
+
+// Many tokens: a warp takes a token, so that its place and angles are found once for all heads; 32 / lanes rows at a time.
+template <typename T, int FMT, bool IL>
+__global__ void __launch_bounds__(THREADS) quant_tokens_kernel(const __grid_constant__ QuantPut p) {
+  after_previous();
+  const AppendParams& q = p.a;
+  const unsigned t = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+  if (t >= (unsigned)q.total) return;
+  const int lane = threadIdx.x & 31, slot = lane >> p.lane_shift, u = lane & (p.lanes - 1), rows = 32 >> p.lane_shift;
+  int a, b;
+  bool has_a, has_b;
+  my_columns<IL>(p, u, a, b, has_a, has_b);
+  long long bi = 0, si = t;
+  int seq, row;
+  TokenPlace place;
+  if (q.cu) {
+    seq = sequence_of(q.cu, q.batch, (int)t);
+    place.live = seq < q.batch;
+    row = place.live ? (int)t - q.cu[seq] : 0;
+  } else {
+    seq = (int)(t / (unsigned)q.new_tokens);
+    row = (int)(t - (unsigned)seq * (unsigned)q.new_tokens);
+    bi = seq;
+    si = row;
+    place.live = true;
+  }
+  int2 at = make_int2(0, 0);
+  if (place.live) at = q.place[seq];
+  place.live = row >= 0 && row < at.y;
+  place.turned = true;
+  if (place.live) find_place(p, seq, at.x + row, bi, si, &place);
+  const bool turns = has_a && u < q.r.turned, turned = place.live && place.turned;
+  float c[V], s[V];
+  if (turns && turned) angles_of<T, IL>(p, place, a, b, c, s);
+
+  auto load = [&](const T* from, Chunk<T, V>& xa, Chunk<T, V>& xb) {
+    xa.raw = has_a ? __ldcs(reinterpret_cast<const uint4*>(from + a)) : uint4{};
+    xb.raw = has_b ? __ldcs(reinterpret_cast<const uint4*>(from + b)) : uint4{};
+  };
+  constexpr int BATCH = 4;
+  {
+    const T* from = reinterpret_cast<const T*>(q.q) + bi * q.q_sb + si * q.q_ss;
+    T* to = reinterpret_cast<T*>(q.q_out) + bi * q.qo_sb + si * q.qo_ss;
+    for (int h0 = slot; h0 < q.heads_q; h0 += BATCH * rows) {
+      Chunk<T, V> xa[BATCH], xb[BATCH];
 #pragma unroll
-  for (int i = 0; i < HPT; ++i) {
-    const int h = slot + i * q.slots;
-    store_row<T, FMT, IL>(p, bi, si, in && h < heads ? h : -1, a, b, has_a, has_b, turns, u, place, c, s, xa[i], xb[i]);
+      for (int i = 0; i < BATCH; ++i)
+        if (h0 + i * rows < q.heads_q) load(from + (long long)(h0 + i * rows) * q.q_sh, xa[i], xb[i]);
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        if (h0 + i * rows >= q.heads_q) continue;
+        float ya[V], yb[V];
+        row_values<T, IL>(xa[i], xb[i], turns, turned, c, s, ya, yb);
+        T* out = to + (long long)(h0 + i * rows) * q.qo_sh;
+        if (has_a) store16<T, V>(out, a, ya);
+        if (has_b) store16<T, V>(out, b, yb);
+      }
+    }
+  }
+  if (!place.live) return;  // (the token's warp as one)
+  const FsaQuantCache& k = p.c;
+#pragma unroll 1
+  for (int is_v = 0; is_v < 2; ++is_v) {
+    const T* from = is_v ? reinterpret_cast<const T*>(q.v) + bi * q.v_sb + si * q.v_ss : reinterpret_cast<const T*>(q.k) + bi * q.k_sb + si * q.k_ss;
+    const long long sh = is_v ? q.v_sh : q.k_sh, ch = is_v ? k.v_stride_h : k.k_stride_h, wh = is_v ? k.vs_stride_h : k.ks_stride_h;
+    uint8_t* codes = is_v ? reinterpret_cast<uint8_t*>(k.v) + place.block * k.v_stride_b + place.slot * k.v_stride_s
+                          : reinterpret_cast<uint8_t*>(k.k) + place.block * k.k_stride_b + place.slot * k.k_stride_s;
+    uint32_t* scales = is_v ? reinterpret_cast<uint32_t*>(k.v_scales) + place.block * k.vs_stride_b + place.slot * k.vs_stride_s
+                            : reinterpret_cast<uint32_t*>(k.k_scales) + place.block * k.ks_stride_b + place.slot * k.ks_stride_s;
+    constexpr int PAIR = 2;
+    for (int h0 = 0; h0 < q.heads_kv; h0 += PAIR * rows) {  // all lanes: those of a row talk to one another
+      Chunk<T, V> xa[PAIR], xb[PAIR];
+#pragma unroll
+      for (int i = 0; i < PAIR; ++i) {
+        const int h = h0 + i * rows + slot;
+        xa[i].raw = xb[i].raw = uint4{};
+        if (h < q.heads_kv) load(from + h * sh, xa[i], xb[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < PAIR; ++i) {
+        if (h0 + i * rows >= q.heads_kv) continue;
+        const int h = h0 + i * rows + slot;
+        float ya[V], yb[V];
+        row_values<T, IL>(xa[i], xb[i], turns && !is_v, is_v || place.turned, c, s, ya, yb);
+        put_row<FMT>(p, ya, yb, a, b, has_a, has_b, h < q.heads_kv, u, codes + h * ch, scales + h * wh);
+      }
+    }
   }
 }
 
@@ -528,6 +630,8 @@ bool in_one_step(const FsaKvAppendQuantArgs* a) {
   return !a->cache.page_table || (a->new_tokens - 1) / a->cache.page_size + 2 <= STEP_PAGES;
 }
 
+constexpr long long MANY_TOKENS = 148 * 16;  // from which on a warp a token fills the GPU
+
 bool multiples_of(int64_t n, std::initializer_list<int64_t> values) {
   for (int64_t v : values)
     if (v % n) return false;
@@ -586,7 +690,7 @@ extern "C" int fsa_kv_append_quantized(const FsaKvAppendQuantArgs* a, void* stre
     make_axis_map(&p.m, a->axis_bits, a->position_ids, a->position_stride_a, a->position_stride_b, a->position_stride_s, a->axes,
                   a->position_ids_int64, a->table_rows);
   p.c = c;
-  for (p.lanes = 1; p.lanes < r.units;) p.lanes *= 2;
+  for (p.lanes = 1, p.lane_shift = 0; p.lanes < r.units; ++p.lane_shift) p.lanes *= 2;
   p.groups = quant_row_words(c);
   p.chunk_shift = c.group == 32 ? 2 : 3;
   q.q = a->q; q.k = a->k_new; q.v = a->v_new;
@@ -626,10 +730,10 @@ extern "C" int fsa_kv_append_quantized(const FsaKvAppendQuantArgs* a, void* stre
     });
     return e == cudaSuccess ? FSA_OK : FSA_ERR_LAUNCH;
   }
-  const bool many = total * heads * p.lanes >= 148ll * 2048;
-  q.slots = many ? (heads + HEADS_PER_THREAD - 1) / HEADS_PER_THREAD : heads;
-  const long long blocks = (total * q.slots * p.lanes + THREADS - 1) / THREADS;
-  if (blocks * THREADS > 0xffffffffll) return FSA_ERR_UNSUPPORTED;  // threads are counted in 32 bits
+  const bool many = total >= MANY_TOKENS;
+  q.slots = heads;
+  const long long blocks = many ? (total + THREADS / 32 - 1) / (THREADS / 32) : (total * heads * p.lanes + THREADS - 1) / THREADS;
+  if (!many && total * heads * p.lanes > 0x7fffffffll) return FSA_ERR_UNSUPPORTED;  // threads are counted in 32 bits
   // a warp looks at a sequence's slots where it may have many
   const int lanes = c.page_table && total / c.page_size > 2ll * a->batch ? 32 : 1;
   cudaError_t e = launch_append_place(q, lanes, stream);
@@ -637,10 +741,10 @@ extern "C" int fsa_kv_append_quantized(const FsaKvAppendQuantArgs* a, void* stre
   e = for_format(a->dtype, c.format, [&](auto t, auto fmt) {
     using T = decltype(t);
     if (a->interleaved)
-      return many ? launch_early(quant_rows_kernel<T, fmt(), true, HEADS_PER_THREAD>, (unsigned)blocks, THREADS, 0, stream, 1, p)
-                  : launch_early(quant_rows_kernel<T, fmt(), true, 1>, (unsigned)blocks, THREADS, 0, stream, 1, p);
-    return many ? launch_early(quant_rows_kernel<T, fmt(), false, HEADS_PER_THREAD>, (unsigned)blocks, THREADS, 0, stream, 1, p)
-                : launch_early(quant_rows_kernel<T, fmt(), false, 1>, (unsigned)blocks, THREADS, 0, stream, 1, p);
+      return many ? launch_early(quant_tokens_kernel<T, fmt(), true>, (unsigned)blocks, THREADS, 0, stream, 1, p)
+                  : launch_early(quant_rows_kernel<T, fmt(), true>, (unsigned)blocks, THREADS, 0, stream, 1, p);
+    return many ? launch_early(quant_tokens_kernel<T, fmt(), false>, (unsigned)blocks, THREADS, 0, stream, 1, p)
+                : launch_early(quant_rows_kernel<T, fmt(), false>, (unsigned)blocks, THREADS, 0, stream, 1, p);
   });
   return e == cudaSuccess ? FSA_OK : FSA_ERR_LAUNCH;
 }
