@@ -11,7 +11,7 @@
 //
 // Both directions are bound by memory. Append: a group of 2, 4 or 8 (the next power of two of head_dim / 16) neighbouring lanes holds a row, two
 // chunks of eight columns each - the partners of each other's pairs - and finds the row's or its groups' extremes by shuffles; nothing goes
-// through shared memory. Read: a block takes 32 tokens, looks their slots up once, and every thread widens sixteen columns at a time.
+// through shared memory. Read: a block takes eight tokens, looks their slots up once, and every thread widens sixteen columns at a time.
 #include <initializer_list>
 
 #include "fsa_axes.cuh"
@@ -110,14 +110,17 @@ __device__ __forceinline__ uint32_t codes4(const float* y, const Pair4& p) {
 }
 
 // Quantises a row that `lanes` neighbouring lanes hold (all of the warp come here) and stores it if `live`.
-template <int FMT>
+template <int FORM>
 __device__ __forceinline__ void put_row(const QuantPut& p, const float* ya, const float* yb, int a, int b, bool has_a, bool has_b, bool live, int u,
                                         uint8_t* codes, uint32_t* scales) {
+  constexpr int FMT = FORM & 3, GROUPS = FORM >> 2;  // at most so many groups
   if constexpr (FMT != FSA_QC_INT4) {
     float most = 0.f;  // (columns that this lane does not have are zeros)
 #pragma unroll
     for (int i = 0; i < V; ++i) most = larger(most, larger(fabsf(ya[i]), fabsf(yb[i])));
-    for (int d = p.lanes >> 1; d; d >>= 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, d));
+#pragma unroll
+    for (int d = 4; d; d >>= 1)
+      if (d < p.lanes) most = larger(most, __shfl_xor_sync(0xffffffffu, most, d));
     float inverse;
     const float s = row_scale(most, FMT == FSA_QC_INT8 ? 127.f : 448.f, &inverse);
     if (!live) return;
@@ -138,14 +141,15 @@ __device__ __forceinline__ void put_row(const QuantPut& p, const float* ya, cons
     const int ga = has_a ? a / V >> p.chunk_shift : -1, gb = has_b ? b / V >> p.chunk_shift : -1;
     float low_u = 0.f, high_u = 0.f;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      if (g >= p.groups) break;
+    for (int g = 0; g < GROUPS; ++g) {
       float low = smaller(ga == g ? low_a : INFINITY, gb == g ? low_b : INFINITY);
       float high = larger(ga == g ? high_a : -INFINITY, gb == g ? high_b : -INFINITY);
-      for (int d = p.lanes >> 1; d; d >>= 1) {
-        low = smaller(low, __shfl_xor_sync(0xffffffffu, low, d));
-        high = larger(high, __shfl_xor_sync(0xffffffffu, high, d));
-      }
+#pragma unroll
+      for (int d = 4; d; d >>= 1)
+        if (d < p.lanes) {
+          low = smaller(low, __shfl_xor_sync(0xffffffffu, low, d));
+          high = larger(high, __shfl_xor_sync(0xffffffffu, high, d));
+        }
       if (u == g) {
         low_u = low;
         high_u = high;
@@ -246,7 +250,7 @@ __device__ __forceinline__ void row_values(const Chunk<T, V>& xa, const Chunk<T,
 }
 
 // All lanes of the warp come here, those without a row with h < 0.
-template <typename T, int FMT, bool IL>
+template <typename T, int FORM, bool IL>
 __device__ __forceinline__ void store_row(const QuantPut& p, long long bi, long long si, int h, int a, int b, bool has_a, bool has_b, bool turns, int u,
                                           const TokenPlace& t, const float* c, const float* s, const Chunk<T, V>& xa, const Chunk<T, V>& xb) {
   const AppendParams& q = p.a;
@@ -273,7 +277,7 @@ __device__ __forceinline__ void store_row(const QuantPut& p, long long bi, long 
       scales = reinterpret_cast<uint32_t*>(k.k_scales) + t.block * k.ks_stride_b + t.slot * k.ks_stride_s + hk * k.ks_stride_h;
     }
   }
-  put_row<FMT>(p, ya, yb, a, b, has_a, has_b, live, u, codes, scales);
+  put_row<FORM>(p, ya, yb, a, b, has_a, has_b, live, u, codes, scales);
 }
 
 // This lane's columns of a row.
@@ -286,7 +290,7 @@ __device__ __forceinline__ void my_columns(const QuantPut& p, int u, int& a, int
 }
 
 // Few tokens: a thread has one row's share.
-template <typename T, int FMT, bool IL>
+template <typename T, int FORM, bool IL>
 __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const __grid_constant__ QuantPut p) {
   after_previous();
   const AppendParams& q = p.a;
@@ -326,12 +330,15 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const __grid_consta
   const bool turns = has_a && u < q.r.turned;
   float c[V], s[V];
   if (turns && place.live && place.turned) angles_of<T, IL>(p, place, a, b, c, s);
-  store_row<T, FMT, IL>(p, bi, si, in ? slot : -1, a, b, has_a, has_b, turns, u, place, c, s, xa, xb);
+  store_row<T, FORM, IL>(p, bi, si, in ? slot : -1, a, b, has_a, has_b, turns, u, place, c, s, xa, xb);
 }
 
-// Many tokens: a warp takes a token, so that its place and angles are found once for all heads; 32 / lanes rows at a time.
-template <typename T, int FMT, bool IL>
-__global__ void __launch_bounds__(THREADS) quant_tokens_kernel(const __grid_constant__ QuantPut p) {
+// Many tokens: a warp takes a token, so that its place and angles are found once for all heads; 32 / lanes rows at a time. (41 k packed tokens, 48
+// heads of 128, 4 bits: threads with four rows of a token each 387 us; this with 104 registers 245, with five blocks an SM 206, with six, which
+// spills, 243; keys and values of eight heads loaded ahead of everything, at 166 registers, 281. Without queries 121: the quantising itself, about
+// 350 instructions for four rows.)
+template <typename T, int FORM, bool IL>
+__global__ void __launch_bounds__(THREADS, 5) quant_tokens_kernel(const __grid_constant__ QuantPut p) {
   after_previous();
   const AppendParams& q = p.a;
   const unsigned t = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
@@ -341,33 +348,37 @@ __global__ void __launch_bounds__(THREADS) quant_tokens_kernel(const __grid_cons
   bool has_a, has_b;
   my_columns<IL>(p, u, a, b, has_a, has_b);
   long long bi = 0, si = t;
-  int seq, row;
-  TokenPlace place;
-  if (q.cu) {
-    seq = sequence_of(q.cu, q.batch, (int)t);
-    place.live = seq < q.batch;
-    row = place.live ? (int)t - q.cu[seq] : 0;
-  } else {
+  int seq = 0, row = (int)t;
+  if (!q.cu) {
     seq = (int)(t / (unsigned)q.new_tokens);
     row = (int)(t - (unsigned)seq * (unsigned)q.new_tokens);
     bi = seq;
     si = row;
-    place.live = true;
   }
-  int2 at = make_int2(0, 0);
-  if (place.live) at = q.place[seq];
-  place.live = row >= 0 && row < at.y;
-  place.turned = true;
-  if (place.live) find_place(p, seq, at.x + row, bi, si, &place);
-  const bool turns = has_a && u < q.r.turned, turned = place.live && place.turned;
-  float c[V], s[V];
-  if (turns && turned) angles_of<T, IL>(p, place, a, b, c, s);
-
   auto load = [&](const T* from, Chunk<T, V>& xa, Chunk<T, V>& xb) {
     xa.raw = has_a ? __ldcs(reinterpret_cast<const uint4*>(from + a)) : uint4{};
     xb.raw = has_b ? __ldcs(reinterpret_cast<const uint4*>(from + b)) : uint4{};
   };
-  constexpr int BATCH = 4;
+  TokenPlace place;
+  place.live = true;
+  place.turned = true;
+  if (q.cu) {  // the sequence that the token is in: bounds at or in front of it, counted by all lanes
+    int behind = 0;
+    for (int b0 = 0; b0 <= q.batch; b0 += 32) behind += __popc(__ballot_sync(0xffffffffu, b0 + lane <= q.batch && q.cu[b0 + lane] <= row));
+    seq = behind - 1;  // (of empty sequences the last)
+    place.live = seq >= 0 && seq < q.batch;
+    if (place.live) row -= q.cu[seq];
+  }
+  if (place.live) {
+    const int2 at = q.place[seq];
+    place.live = row < at.y;
+    if (place.live) find_place(p, seq, at.x + row, bi, si, &place);
+  }
+  const bool turns = has_a && u < q.r.turned, turned = place.live && place.turned;
+  float c[V], s[V];
+  if (turns && turned) angles_of<T, IL>(p, place, a, b, c, s);
+
+  constexpr int BATCH = 4, PAIR = 2;  // rows of queries, and of keys or values, that a lane has under way
   {
     const T* from = reinterpret_cast<const T*>(q.q) + bi * q.q_sb + si * q.q_ss;
     T* to = reinterpret_cast<T*>(q.q_out) + bi * q.qo_sb + si * q.qo_ss;
@@ -397,7 +408,7 @@ __global__ void __launch_bounds__(THREADS) quant_tokens_kernel(const __grid_cons
                           : reinterpret_cast<uint8_t*>(k.k) + place.block * k.k_stride_b + place.slot * k.k_stride_s;
     uint32_t* scales = is_v ? reinterpret_cast<uint32_t*>(k.v_scales) + place.block * k.vs_stride_b + place.slot * k.vs_stride_s
                             : reinterpret_cast<uint32_t*>(k.k_scales) + place.block * k.ks_stride_b + place.slot * k.ks_stride_s;
-    constexpr int PAIR = 2;
+#pragma unroll 1
     for (int h0 = 0; h0 < q.heads_kv; h0 += PAIR * rows) {  // all lanes: those of a row talk to one another
       Chunk<T, V> xa[PAIR], xb[PAIR];
 #pragma unroll
@@ -412,7 +423,7 @@ __global__ void __launch_bounds__(THREADS) quant_tokens_kernel(const __grid_cons
         const int h = h0 + i * rows + slot;
         float ya[V], yb[V];
         row_values<T, IL>(xa[i], xb[i], turns && !is_v, is_v || place.turned, c, s, ya, yb);
-        put_row<FMT>(p, ya, yb, a, b, has_a, has_b, h < q.heads_kv, u, codes + h * ch, scales + h * wh);
+        put_row<FORM>(p, ya, yb, a, b, has_a, has_b, h < q.heads_kv, u, codes + h * ch, scales + h * wh);
       }
     }
   }
@@ -422,7 +433,7 @@ __global__ void __launch_bounds__(THREADS) quant_tokens_kernel(const __grid_cons
 constexpr int STEP_PAGES = 4;  // that the new rows of a sequence may touch
 constexpr int STEP_THREADS = 512;
 
-template <typename T, int FMT, bool IL>
+template <typename T, int FORM, bool IL>
 __global__ void __launch_bounds__(STEP_THREADS) quant_step_kernel(const __grid_constant__ QuantPut p) {
   after_previous();
   const AppendParams& q = p.a;
@@ -463,14 +474,17 @@ __global__ void __launch_bounds__(STEP_THREADS) quant_step_kernel(const __grid_c
     const bool turns = has_a && u < q.r.turned && h < q.heads_q + q.heads_kv;
     float c[V], s[V];
     if (turns && place.live && place.turned) angles_of<T, IL>(p, place, ca, cb, c, s);
-    store_row<T, FMT, IL>(p, b, row, in ? h : -1, ca, cb, has_a, has_b, turns, u, place, c, s, xa, xb);
+    store_row<T, FORM, IL>(p, b, row, in ? h : -1, ca, cb, has_a, has_b, turns, u, place, c, s, xa, xb);
   }
 }
 
 // ----------------------------------------------------------------------------------------------
 // Reading back
 // ----------------------------------------------------------------------------------------------
-constexpr int READ_TOKENS = 32, READ_THREADS = 256, COLUMNS = 16;
+// Small blocks with little under way each: what a read writes is two to four times what it fetches, and the GPU takes writes alone at 3.9 TB/s. 58 k
+// tokens of 8 heads of 128, int8: 32 tokens, 256 threads, four pieces a thread under way 84.4 us; 128 threads 77.2; two pieces 71.3; 16 tokens
+// 66.3; 8 tokens 64.5, with one piece 63.7 (4 bits: 56 k tokens 62.8, 59.3, 56.4, 51.8, 53.3, 58.8).
+constexpr int READ_TOKENS = 8, READ_THREADS = 128, COLUMNS = 16;
 
 struct QuantGet {
   FsaQuantCache c;
@@ -558,7 +572,7 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const __grid_c
   const uint32_t* scales = reinterpret_cast<const uint32_t*>(is_v ? p.c.v_scales : p.c.k_scales);
   T* out = reinterpret_cast<T*>(is_v ? p.v_out : p.k_out);
   // Piece e of head h of token t: a thread's pieces are READ_THREADS apart, which it counts out without dividing.
-  constexpr int BATCH = 4;  // pieces a thread has under way
+  constexpr int BATCH = 2;  // pieces a thread has under way
   int t = threadIdx.x / per_token, rest = threadIdx.x - t * per_token;
   while (t < here) {
     uint4 raw[BATCH];
@@ -609,13 +623,15 @@ __global__ void __launch_bounds__(READ_THREADS) quant_read_kernel(const __grid_c
 // ----------------------------------------------------------------------------------------------
 // Launches
 // ----------------------------------------------------------------------------------------------
+// f with the type and the format (and, in bits above, how many groups a row may have).
 template <typename F>
-cudaError_t for_format(int dtype, int format, F&& f) {
+cudaError_t for_format(int dtype, const FsaQuantCache& c, F&& f) {
   auto with_format = [&](auto t) {
-    switch (format) {
-      case FSA_QC_INT8: return f(t, std::integral_constant<int, FSA_QC_INT8>{});
-      case FSA_QC_E4M3: return f(t, std::integral_constant<int, FSA_QC_E4M3>{});
-      default: return f(t, std::integral_constant<int, FSA_QC_INT4>{});
+    using std::integral_constant;
+    switch (c.format) {
+      case FSA_QC_INT8: return f(t, integral_constant<int, FSA_QC_INT8>{});
+      case FSA_QC_E4M3: return f(t, integral_constant<int, FSA_QC_E4M3>{});
+      default: return c.group == 32 ? f(t, integral_constant<int, FSA_QC_INT4 + 4 * 4>{}) : f(t, integral_constant<int, FSA_QC_INT4 + 4 * 2>{});
     }
   };
   return dtype == FSA_DT_BF16 ? with_format(__nv_bfloat16{}) : with_format(__half{});
@@ -724,7 +740,7 @@ extern "C" int fsa_kv_append_quantized(const FsaKvAppendQuantArgs* a, void* stre
   if (in_one_step(a)) {
     const long long items = (long long)a->new_tokens * heads * p.lanes;
     const int threads = items >= STEP_THREADS ? STEP_THREADS : (int)((items + 31) & ~31ll);
-    const cudaError_t e = for_format(a->dtype, c.format, [&](auto t, auto fmt) {
+    const cudaError_t e = for_format(a->dtype, c, [&](auto t, auto fmt) {
       return a->interleaved ? launch_early(quant_step_kernel<decltype(t), fmt(), true>, (unsigned)a->batch, threads, 0, stream, 1, p)
                             : launch_early(quant_step_kernel<decltype(t), fmt(), false>, (unsigned)a->batch, threads, 0, stream, 1, p);
     });
@@ -738,7 +754,7 @@ extern "C" int fsa_kv_append_quantized(const FsaKvAppendQuantArgs* a, void* stre
   const int lanes = c.page_table && total / c.page_size > 2ll * a->batch ? 32 : 1;
   cudaError_t e = launch_append_place(q, lanes, stream);
   if (e != cudaSuccess) return FSA_ERR_LAUNCH;
-  e = for_format(a->dtype, c.format, [&](auto t, auto fmt) {
+  e = for_format(a->dtype, c, [&](auto t, auto fmt) {
     using T = decltype(t);
     if (a->interleaved)
       return many ? launch_early(quant_tokens_kernel<T, fmt(), true>, (unsigned)blocks, THREADS, 0, stream, 1, p)
@@ -783,8 +799,8 @@ extern "C" int fsa_kv_read_quantized(const FsaKvReadQuantArgs* a, void* stream_)
   p.step_rest = READ_THREADS % per_token;
   const unsigned blocks = (unsigned)((total + READ_TOKENS - 1) / READ_TOKENS);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const cudaError_t e = for_format(a->dtype, c.format, [&](auto t, auto fmt) {
-    return launch_early(quant_read_kernel<decltype(t), fmt()>, 2 * blocks, READ_THREADS, 0, stream, 1, p);
+  const cudaError_t e = for_format(a->dtype, c, [&](auto t, auto fmt) {
+    return launch_early(quant_read_kernel<decltype(t), (fmt() & 3)>, 2 * blocks, READ_THREADS, 0, stream, 1, p);
   });
   return e == cudaSuccess ? FSA_OK : FSA_ERR_LAUNCH;
 }
