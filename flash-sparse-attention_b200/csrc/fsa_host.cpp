@@ -17,7 +17,9 @@
 #include <torch/version.h>
 
 #include <cmath>
+#include <cstring>
 #include <optional>
+#include <vector>
 
 #include "../../include/fsa_b200.h"
 
@@ -32,6 +34,12 @@ decltype(&fsa_kv_append_rotary_workspace_ints) g_append_ints = nullptr;
 decltype(&fsa_kv_append_rotary) g_append = nullptr;
 decltype(&fsa_shared_prefix_workspace_bytes) g_prefix_bytes = nullptr;
 decltype(&fsa_decode_shared_prefix) g_prefix = nullptr;
+decltype(&fsa_rotary_axes) g_axes = nullptr;
+decltype(&fsa_kv_append_quantized_workspace_ints) g_qappend_ints = nullptr;
+decltype(&fsa_kv_append_quantized) g_qappend = nullptr;
+decltype(&fsa_kv_read_quantized) g_qread = nullptr;
+decltype(&fsa_decode_quantized_workspace_bytes) g_qdecode_bytes = nullptr;
+decltype(&fsa_decode_quantized) g_qdecode = nullptr;
 constexpr int MAX_DEVICES = 64;
 at::Tensor* g_status[MAX_DEVICES] = {};  // registered by the package, one int32 word per device, never replaced
 int g_sms[MAX_DEVICES] = {};
@@ -879,6 +887,506 @@ PyObject* shared_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- rotary positions with several axes, caches with scales of their rows -----------------------------------------------
+
+bool here(const at::Device& dev) {
+  return dev.is_cuda() && dev.index() >= 0 && dev.index() < MAX_DEVICES && g_status[dev.index()] && c10::cuda::current_device() == dev.index();
+}
+bool is16(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+// Rows on top of one another, backwards or without a stride.
+bool expanded(const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) <= 0) return true;
+  return false;
+}
+// The axes of the pairs, as rotary_axes.py::axis_bits lays them out.
+bool get_bits(PyObject* o, uint32_t* bits) {
+  if (!PyBytes_CheckExact(o) || PyBytes_GET_SIZE(o) != 32) return false;
+  std::memcpy(bits, PyBytes_AS_STRING(o), 32);
+  return true;
+}
+// (axis, batch, token) strides of positions for rows of these leading sizes; false where they do not fit.
+bool positions_ok(const Tensor& ids, int64_t axes, int64_t dims, at::IntArrayRef lead, const at::Device& dev, int64_t* sa, int64_t* sb, int64_t* ss) {
+  if ((ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) || ids.device() != dev || ids.dim() != dims + 1 || ids.size(0) != axes) return false;
+  if (dims == 1) {
+    if (ids.size(1) != lead[0]) return false;
+    *sb = 0;
+    *ss = ids.stride(1);
+  } else {
+    if ((ids.size(1) != 1 && ids.size(1) != lead[0]) || ids.size(2) != lead[1]) return false;
+    *sb = ids.size(1) > 1 ? ids.stride(1) : 0;
+    *ss = ids.stride(2);
+  }
+  *sa = ids.stride(0);
+  return true;
+}
+
+struct AxesCall {
+  Tensor cos, sin, ids;
+  uint32_t bits[8];
+  int64_t axes = 0;
+  bool interleaved = false, transposed = false;
+};
+
+// One launch for the tensors that are defined (one of them is).
+void axes_launch(const AxesCall& c, const Tensor& q_in, const Tensor& k_in, Tensor* q_out, Tensor* k_out) {
+  const Tensor& any = q_in.defined() ? q_in : k_in;
+  const int dev = any.device().index();
+  const Tensor q = q_in.defined() ? rows_of(q_in) : q_in, k = k_in.defined() ? rows_of(k_in) : k_in;
+  FsaRotaryAxesArgs x = {};
+  auto put = [](const Tensor& t, int64_t* sb, int64_t* ss, int64_t* sh) {
+    *sb = t.dim() == 3 ? 0 : t.stride(0);
+    *ss = t.stride(-3);
+    *sh = t.stride(-2);
+  };
+  if (q.defined()) {
+    *q_out = at::empty(q.sizes(), q.options());
+    x.q = q.data_ptr();
+    x.q_out = q_out->data_ptr();
+    x.heads_q = (int)q.size(-2);
+    put(q, &x.q_stride_b, &x.q_stride_s, &x.q_stride_h);
+    put(*q_out, &x.q_out_stride_b, &x.q_out_stride_s, &x.q_out_stride_h);
+  }
+  if (k.defined()) {
+    *k_out = at::empty(k.sizes(), k.options());
+    x.k = k.data_ptr();
+    x.k_out = k_out->data_ptr();
+    x.heads_k = (int)k.size(-2);
+    put(k, &x.k_stride_b, &x.k_stride_s, &x.k_stride_h);
+    put(*k_out, &x.k_out_stride_b, &x.k_out_stride_s, &x.k_out_stride_h);
+  }
+  if ((q.defined() ? q.numel() : 0) + (k.defined() ? k.numel() : 0) == 0) return;
+  x.cos = c.cos.data_ptr();
+  x.sin = c.sin.data_ptr();
+  x.position_ids = c.ids.data_ptr();
+  x.position_ids_int64 = c.ids.scalar_type() == at::kLong;
+  TORCH_CHECK(positions_ok(c.ids, c.axes, any.dim() - 2, any.sizes(), any.device(), &x.position_stride_a, &x.position_stride_b, &x.position_stride_s),
+              "position_ids must have one entry per axis and token");
+  x.status = ptr<int32_t>(*g_status[dev]);
+  x.table_stride = c.cos.stride(0);
+  x.table_rows = (int)c.cos.size(0);
+  x.rotary_dim = (int)(2 * c.cos.size(1));
+  x.table_dtype = table_code(c.cos.scalar_type());
+  std::memcpy(x.axis_bits, c.bits, 32);
+  x.axes = (int)c.axes;
+  x.batch = any.dim() == 4 ? (int)any.size(0) : 1;
+  x.seqlen = (int)any.size(-3);
+  x.head_dim = (int)any.size(-1);
+  x.dtype = dtype_code(any.scalar_type());
+  x.interleaved = c.interleaved;
+  x.transposed = c.transposed;
+  const int rc = g_axes(&x, c10::cuda::getCurrentCUDAStream(dev).stream());
+  TORCH_CHECK(rc == FSA_OK, "fsa_rotary_axes failed (code ", rc, ")");
+}
+
+// As RotaryFn: the gradient is the transposed rotation, which is a rotation again.
+struct AxesFn : torch::autograd::Function<AxesFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const std::optional<Tensor>& q_in,
+                                                const std::optional<Tensor>& k_in, const AxesCall& c) {
+    const Tensor q = q_in.value_or(Tensor()), k = k_in.value_or(Tensor());
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({c.cos, c.sin, c.ids});
+    ctx->saved_data["form"] =
+        int64_t(c.interleaved) | int64_t(c.transposed) << 1 | int64_t(q.defined()) << 2 | int64_t(k.defined()) << 3 | c.axes << 4;
+    std::vector<int64_t> bits(c.bits, c.bits + 8);
+    ctx->saved_data["bits"] = bits;
+    return launch(q, k, c);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t form = ctx->saved_data["form"].toInt();
+    const auto bits = ctx->saved_data["bits"].toIntVector();
+    AxesCall c;
+    c.cos = saved[0];
+    c.sin = saved[1];
+    c.ids = saved[2];
+    for (int i = 0; i < 8; ++i) c.bits[i] = (uint32_t)bits[i];
+    c.axes = form >> 4;
+    c.interleaved = (form & 1) != 0;
+    c.transposed = (form & 2) == 0;
+    Tensor in[2];
+    size_t n = 0;
+    for (int i = 0; i < 2; ++i)
+      if (form & (4 << i)) {
+        if (ctx->needs_input_grad(n)) in[i] = grads[n];  // (tensors that are left out have no edge)
+        ++n;
+      }
+    torch::autograd::variable_list out(3);  // one entry for every argument of forward
+    if (!in[0].defined() && !in[1].defined()) return out;
+    const auto turned = turn(in[0], in[1], c);
+    n = 0;
+    for (int i = 0; i < 2; ++i)
+      if (in[i].defined()) out[i] = turned[n++];
+    return out;
+  }
+  static torch::autograd::variable_list launch(const Tensor& q, const Tensor& k, const AxesCall& c) {
+    Tensor q_out, k_out;
+    axes_launch(c, q, k, &q_out, &k_out);
+    if (!k.defined()) return {q_out};
+    if (!q.defined()) return {k_out};
+    return {q_out, k_out};
+  }
+  static torch::autograd::variable_list turn(const Tensor& q, const Tensor& k, const AxesCall& c) {
+    auto seen = [](const Tensor& t) { return t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined()); };
+    auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+    return seen(q) || seen(k) ? apply(maybe(q), maybe(k), c) : launch(q, k, c);
+  }
+};
+
+// rotary_axes(q, k, cos, sin, position_ids, axes of the pairs, number of axes, interleaved) -> q or (q, k), or None. k may be None.
+PyObject* rotary_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 8 || !g_axes) return none();
+  HANDLE_TH_ERRORS
+    Tensor q, k;
+    AxesCall c;
+    if (a[0] == Py_None || a[2] == Py_None || a[3] == Py_None || a[4] == Py_None || !opt_tensor(a[0], &q) || !opt_tensor(a[1], &k) ||
+        !opt_tensor(a[2], &c.cos) || !opt_tensor(a[3], &c.sin) || !opt_tensor(a[4], &c.ids) || !get_bits(a[5], c.bits) || !get_int(a[6], &c.axes) ||
+        !PyBool_Check(a[7]))
+      return none();
+    c.interleaved = a[7] == Py_True;
+    const at::Device dev = q.device();
+    if ((q.dim() != 3 && q.dim() != 4) || !here(dev) || !is16(q.scalar_type())) return none();
+    const int64_t d = q.size(-1);
+    if (q.numel() == 0 || d > 256 || q.numel() / (q.size(-2) * d) > INT32_MAX || !tables_ok(c.cos, c.sin, d, dev)) return none();
+    if (k.defined()) {
+      if (k.dim() != q.dim() || k.scalar_type() != q.scalar_type() || k.device() != dev || k.size(-1) != d || k.numel() == 0) return none();
+      for (int64_t i = 0; i < q.dim() - 2; ++i)
+        if (k.size(i) != q.size(i)) return none();
+    }
+    int64_t sa, sb, ss;
+    if (c.axes < 2 || !positions_ok(c.ids, c.axes, q.dim() - 2, q.sizes(), dev, &sa, &sb, &ss)) return none();
+    std::optional<NoGil> no_gil(std::in_place);
+    auto out = AxesFn::turn(q, k, c);
+    no_gil.reset();
+    return k.defined() ? pair(std::move(out[0]), std::move(out[1])) : THPVariable_Wrap(std::move(out[0]));
+  END_HANDLE_TH_ERRORS
+}
+
+// The library's view of a cache (quantized_kvcache.py::check_quantized_cache, fill_quantized_cache); false where it is not an ordinary one.
+bool quant_cache(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& table, int64_t batch, const at::Device& dev,
+                 FsaQuantCache* c) {
+  for (const Tensor* t : {&kc, &vc, &ks, &vs})
+    if (!t->defined() || t->device() != dev || expanded(*t)) return false;
+  if (kc.dim() != 4 || kc.sizes() != vc.sizes() || kc.scalar_type() != vc.scalar_type() || kc.numel() == 0) return false;
+  const bool int4 = kc.scalar_type() == at::kByte;
+  if (int4) c->format = FSA_QC_INT4;
+  else if (kc.scalar_type() == at::kChar) c->format = FSA_QC_INT8;
+  else if (kc.scalar_type() == at::kFloat8_e4m3fn) c->format = FSA_QC_E4M3;
+  else return false;
+  const int64_t d = kc.size(3) * (int4 ? 2 : 1);
+  if (d > 128 || d % 16) return false;
+  if (ks.sizes() != vs.sizes() || ks.scalar_type() != vs.scalar_type() || ks.dim() != (int4 ? 5 : 4)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (ks.size(i) != kc.size(i)) return false;
+  const int64_t per = int4 ? 2 : 1;
+  if (int4) {
+    const int64_t groups = ks.size(3);
+    if (ks.scalar_type() != at::kBFloat16 || ks.size(4) != 2 || groups <= 0 || d % groups || (d / groups != 32 && d / groups != 64)) return false;
+    c->group = (int)(d / groups);
+  } else if (ks.scalar_type() != at::kFloat || ks.size(3) != 1) {
+    return false;
+  }
+  auto strides = [&](const Tensor& t, int64_t unit, int64_t divide, int64_t* sb, int64_t* ss, int64_t* sh) {
+    int64_t* const to[3] = {sb, ss, sh};
+    for (int i = 0; i < 3; ++i) {
+      const int64_t s = t.size(i) == 1 ? 0 : t.stride(i);
+      if (s % unit) return false;
+      *to[i] = s / divide;
+    }
+    return true;
+  };
+  for (const Tensor* t : {&kc, &vc})
+    if (t->stride(3) != 1 || (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15)) return false;
+  for (const Tensor* t : {&ks, &vs})
+    if (int4 && (t->stride(4) != 1 || (t->size(3) > 1 && t->stride(3) != 2) || (reinterpret_cast<uintptr_t>(t->data_ptr()) & 3))) return false;
+  if (!strides(kc, 16, 1, &c->k_stride_b, &c->k_stride_s, &c->k_stride_h) || !strides(vc, 16, 1, &c->v_stride_b, &c->v_stride_s, &c->v_stride_h) ||
+      !strides(ks, per, per, &c->ks_stride_b, &c->ks_stride_s, &c->ks_stride_h) || !strides(vs, per, per, &c->vs_stride_b, &c->vs_stride_s, &c->vs_stride_h))
+    return false;
+  c->k = kc.data_ptr();
+  c->v = vc.data_ptr();
+  c->k_scales = ks.data_ptr();
+  c->v_scales = vs.data_ptr();
+  c->heads_kv = (int)kc.size(2);
+  c->head_dim = (int)d;
+  if (table.defined()) {
+    if (!int_ok(table, dev, 2) || expanded(table) || table.size(0) != batch || table.size(1) <= 0 || (table.size(1) > 1 && table.stride(1) != 1)) return false;
+    c->page_table = ptr<int32_t>(table);
+    c->page_table_stride = table.stride(0);
+    c->num_pages = (int)kc.size(0);
+    c->page_size = (int)kc.size(1);
+    c->max_pages = (int)table.size(1);
+  } else {
+    if (kc.size(0) != batch) return false;
+    c->capacity = (int)kc.size(1);
+  }
+  return true;
+}
+// Rows of 16 bits on 16-byte boundaries (quantized_kvcache.py::rows_ok), and their strides, of dimensions of one none.
+bool rows16(const Tensor& t, int64_t* sb, int64_t* ss, int64_t* sh) {
+  if (t.stride(-1) != 1 || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15)) return false;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) % 8) return false;
+  auto at = [&](int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); };
+  *sb = t.dim() == 3 ? 0 : at(0);
+  *ss = at(-3);
+  *sh = at(-2);
+  return true;
+}
+
+// append_quantized(q, k_new, v_new, k_cache, v_cache, k_scales, v_scales, seqused_k, cos, sin, page_table, free_pages, free_count, cu_seqlens_new,
+//                  seqlen_offsets, position_ids, axes of the pairs, number of axes, interleaved, advance, out)
+//   -> the turned queries (True without queries), an error code, or None
+PyObject* append_quantized(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 21 || !g_qappend || !g_qappend_ints) return none();
+  HANDLE_TH_ERRORS
+    Tensor q, k, v, kc, vc, ks, vs, used, cos, sin, table, free, count, cu, offsets, ids, out;
+    Tensor* const into[21] = {&q,     &k,    &v,     &kc, &vc,     &ks,  &vs,     &used,   &cos,    &sin, &table,
+                              &free, &count, &cu, nullptr, &ids, nullptr, nullptr, nullptr, nullptr, &out};
+    for (int i = 0; i < 21; ++i)
+      if (into[i] && !opt_tensor(a[i], into[i])) return none();
+    int64_t offset, axes = 0;
+    if (!k.defined() || !v.defined() || !kc.defined() || !used.defined() || !get_offsets(a[14], &offset, &offsets) || !PyBool_Check(a[18]) ||
+        !PyBool_Check(a[19]))
+      return none();
+    const int64_t dims = cu.defined() ? 3 : 4;
+    if (k.dim() != dims || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || !is16(k.scalar_type())) return none();
+    const at::Device dev = k.device();
+    if (!here(dev)) return none();
+    for (int i = 0; i < 21; ++i)
+      if (into[i] && into[i]->defined() && into[i]->device() != dev) return none();
+    if (used.scalar_type() != at::kInt || used.dim() != 1 || !used.is_contiguous() || used.numel() == 0 || k.numel() == 0) return none();
+    const int64_t batch = used.numel(), d = k.size(-1);
+    FsaKvAppendQuantArgs x = {};
+    if (!quant_cache(kc, vc, ks, vs, table, batch, dev, &x.cache) || x.cache.heads_kv != k.size(-2) || x.cache.head_dim != d) return none();
+    if (cu.defined() ? (cu.scalar_type() != at::kInt || cu.dim() != 1 || !cu.is_contiguous() || cu.size(0) != batch + 1) : k.size(0) != batch) return none();
+    if (cos.defined() != sin.defined()) return none();
+    if (!cos.defined()) {
+      if (q.defined() || a[14] != Py_None || ids.defined() || a[16] != Py_None) return none();
+    } else {
+      if (!tables_ok(cos, sin, d, dev) || cos.size(1) % 8) return none();
+      const int64_t stride = cos.size(0) == 1 ? 0 : cos.stride(0);
+      if (cos.scalar_type() == at::kFloat &&
+          (((reinterpret_cast<uintptr_t>(cos.data_ptr()) | reinterpret_cast<uintptr_t>(sin.data_ptr())) & 15) || stride % 4))
+        return none();
+      x.cos = cos.data_ptr();
+      x.sin = sin.data_ptr();
+      x.table_rows = (int)cos.size(0);
+      x.rotary_dim = (int)(2 * cos.size(1));
+      x.table_stride = stride;
+      x.table_dtype = table_code(cos.scalar_type());
+    }
+    if (ids.defined() != (a[16] != Py_None)) return none();
+    if (ids.defined()) {
+      if (a[14] != Py_None || !get_bits(a[16], x.axis_bits) || !get_int(a[17], &axes) ||
+          !positions_ok(ids, axes, dims - 2, k.sizes(), dev, &x.position_stride_a, &x.position_stride_b, &x.position_stride_s))
+        return none();
+      x.position_ids = ids.data_ptr();
+      x.position_ids_int64 = ids.scalar_type() == at::kLong;
+      x.axes = (int)axes;
+    }
+    if (!offsets_ok(offsets, batch, dev)) return none();
+    if (free.defined() != count.defined() || (free.defined() && (!table.defined() || free.scalar_type() != at::kInt || !free.is_contiguous() ||
+                                                                   count.scalar_type() != at::kInt || count.numel() != 1)))
+      return none();
+    if (free.defined() && expanded(free)) return none();
+    if (!rows16(k, &x.k_stride_b, &x.k_stride_s, &x.k_stride_h) || !rows16(v, &x.v_stride_b, &x.v_stride_s, &x.v_stride_h)) return none();
+    if (q.defined()) {
+      if (q.dim() != dims || q.scalar_type() != k.scalar_type() || q.size(-1) != d || q.size(-2) <= 0 || q.size(-2) % k.size(-2)) return none();
+      for (int64_t i = 0; i < dims - 2; ++i)
+        if (q.size(i) != k.size(i)) return none();
+      if (!rows16(q, &x.q_stride_b, &x.q_stride_s, &x.q_stride_h)) return none();
+    }
+    if (out.defined() && (!q.defined() || out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || expanded(out))) return none();
+    std::optional<NoGil> no_gil(std::in_place);
+    if (q.defined()) {
+      if (!out.defined()) out = at::empty(q.sizes(), q.options());
+      if (!rows16(out, &x.q_out_stride_b, &x.q_out_stride_s, &x.q_out_stride_h)) {
+        no_gil.reset();
+        return none();
+      }
+      x.q = q.data_ptr();
+      x.q_out = out.data_ptr();
+      x.heads_q = (int)q.size(-2);
+    }
+    x.k_new = k.data_ptr();
+    x.v_new = v.data_ptr();
+    x.seqused_k = ptr<int32_t>(used);
+    x.free_pages = ptr<int32_t>(free);
+    x.free_count = ptr<int32_t>(count);
+    x.cu_seqlens_new = ptr<int32_t>(cu);
+    x.seqlen_offsets = ptr<int32_t>(offsets);
+    x.status = ptr<int32_t>(*g_status[dev.index()]);
+    x.batch = (int)batch;
+    if (cu.defined())
+      x.total = (int)k.size(0);
+    else
+      x.new_tokens = (int)k.size(1);
+    x.offset = (int)offset;
+    x.dtype = dtype_code(k.scalar_type());
+    x.interleaved = a[18] == Py_True;
+    x.advance = a[19] == Py_True;
+    const int64_t ints = g_qappend_ints(&x);
+    Tensor place;
+    if (ints > 0) place = at::empty({ints}, used.options());
+    x.place_ws = ptr<int32_t>(place);
+    const int rc = g_qappend(&x, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+    if (rc == FSA_OK) {
+      for (const Tensor* t : {&kc, &vc, &ks, &vs}) written(*t);
+      if (x.advance) written(used);
+      if (free.defined()) {
+        written(table);
+        written(count);
+      }
+      if (a[20] != Py_None) written(out);
+    }
+    no_gil.reset();
+    if (rc != FSA_OK) return PyLong_FromLong(rc);
+    if (!q.defined()) Py_RETURN_TRUE;
+    if (a[20] != Py_None) {
+      Py_INCREF(a[20]);
+      return a[20];
+    }
+    return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// read_quantized(k_cache, v_cache, k_scales, v_scales, seqused_k, page_table, cu_seqlens, max_seqlen, total, bf16) -> (k, v), an error code, or None
+PyObject* read_quantized(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10 || !g_qread) return none();
+  HANDLE_TH_ERRORS
+    Tensor kc, vc, ks, vs, used, table, cu;
+    Tensor* const into[7] = {&kc, &vc, &ks, &vs, &used, &table, &cu};
+    for (int i = 0; i < 7; ++i)
+      if (!opt_tensor(a[i], into[i])) return none();
+    int64_t rows = 0;
+    if (!kc.defined() || !PyBool_Check(a[9]) || cu.defined() != (a[7] == Py_None) || cu.defined() != (a[8] != Py_None) ||
+        !get_int(cu.defined() ? a[8] : a[7], &rows) || rows <= 0)
+      return none();
+    const at::Device dev = kc.device();
+    if (!here(dev)) return none();
+    if (cu.defined() && (cu.scalar_type() != at::kInt || cu.dim() != 1 || cu.numel() < 2 || !cu.is_contiguous() || cu.device() != dev)) return none();
+    if (kc.dim() != 4) return none();
+    const int64_t batch = cu.defined() ? cu.numel() - 1 : (table.defined() && table.dim() > 0 ? table.size(0) : kc.size(0));
+    FsaKvReadQuantArgs x = {};
+    if (!quant_cache(kc, vc, ks, vs, table, batch, dev, &x.cache)) return none();
+    if (used.defined() && (used.scalar_type() != at::kInt || used.dim() != 1 || used.size(0) != batch || !used.is_contiguous() || used.device() != dev)) return none();
+    std::optional<NoGil> no_gil(std::in_place);
+    const auto options = kc.options().dtype(a[9] == Py_True ? at::kBFloat16 : at::kHalf);
+    const int64_t h = x.cache.heads_kv, d = x.cache.head_dim;
+    const auto shape = cu.defined() ? std::vector<int64_t>{rows, h, d} : std::vector<int64_t>{batch, rows, h, d};
+    Tensor k = at::empty(shape, options), v = at::empty(shape, options);
+    x.k_out = k.data_ptr();
+    x.v_out = v.data_ptr();
+    if (!cu.defined()) x.k_out_stride_b = x.v_out_stride_b = rows * h * d;
+    x.k_out_stride_s = x.v_out_stride_s = h * d;
+    x.k_out_stride_h = x.v_out_stride_h = d;
+    x.seqused_k = ptr<int32_t>(used);
+    x.cu_seqlens = ptr<int32_t>(cu);
+    x.status = ptr<int32_t>(*g_status[dev.index()]);
+    x.batch = (int)batch;
+    (cu.defined() ? x.total : x.seqlen) = (int)rows;
+    x.dtype = a[9] == Py_True ? FSA_DT_BF16 : FSA_DT_FP16;
+    const int rc = g_qread(&x, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+    no_gil.reset();
+    if (rc != FSA_OK) return PyLong_FromLong(rc);
+    return pair(std::move(k), std::move(v));
+  END_HANDLE_TH_ERRORS
+}
+
+// decode_quantized(q, k, v, k_scales, v_scales, softmax_scale, page_table, gather_kv_indices, seqused_k, out, lse) -> (out, lse), an error code, or None
+PyObject* decode_quantized(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 11 || !g_qdecode || !g_qdecode_bytes) return none();
+  HANDLE_TH_ERRORS
+    Tensor q, k, v, ks, vs, table, gather, used, out, lse;
+    Tensor* const into[11] = {&q, &k, &v, &ks, &vs, nullptr, &table, &gather, &used, &out, &lse};
+    for (int i = 0; i < 11; ++i)
+      if (into[i] && !opt_tensor(a[i], into[i])) return none();
+    if (!q.defined() || q.dim() != 3 || !is16(q.scalar_type())) return none();
+    const at::Device dev = q.device();
+    if (!here(dev)) return none();
+    const int64_t batch = q.size(0), hq = q.size(1), d = q.size(2);
+    FsaQuantDecodeArgs x = {};
+    if (batch <= 0 || hq <= 0 || !quant_cache(k, v, ks, vs, table, batch, dev, &x.cache) || hq % x.cache.heads_kv || x.cache.head_dim != d) return none();
+    const int page = x.cache.page_size;
+    if (table.defined() && page != 32 && page != 64 && page != 128 && page != 256) return none();
+    int64_t none_b;
+    if (!rows16(q, &none_b, &x.q_stride_b, &x.q_stride_h)) return none();
+    if (used.defined() && (used.scalar_type() != at::kInt || used.dim() != 1 || used.size(0) != batch || !used.is_contiguous() || used.device() != dev)) return none();
+    if (gather.defined()) {
+      if (gather.scalar_type() != at::kInt || gather.dim() != 2 || gather.size(0) != batch || gather.device() != dev || gather.size(1) <= 0 ||
+          gather.size(1) > INT32_MAX || (gather.size(1) > 1 && gather.stride(1) != 1))
+        return none();
+      x.gather_kv_indices = ptr<int32_t>(gather);
+      x.topk = (int)gather.size(1);
+      x.gather_stride = gather.stride(0);
+    }
+    if (out.defined() && (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || out.device() != dev || out.stride(2) != 1 || expanded(out) ||
+                          (reinterpret_cast<uintptr_t>(out.data_ptr()) & 3) || (batch > 1 && out.stride(0) % 2) || (hq > 1 && out.stride(1) % 2)))
+      return none();
+    if (lse.defined() && (lse.dim() != 2 || lse.size(0) != batch || lse.size(1) != hq || lse.scalar_type() != at::kFloat || lse.device() != dev ||
+                          (hq > 1 && lse.stride(1) != 1) || expanded(lse)))
+      return none();
+    double scale;
+    if (!opt_double(a[5], 1.0 / std::sqrt((double)d), &scale) || !(scale > 0.0) || std::isinf(scale)) return none();
+    std::optional<NoGil> no_gil(std::in_place);
+    if (!out.defined()) out = at::empty({batch, hq, d}, q.options());
+    if (!lse.defined()) lse = at::empty({batch, hq}, q.options().dtype(at::kFloat));
+    x.q = q.data_ptr();
+    x.out = out.data_ptr();
+    x.lse = ptr<float>(lse);
+    x.o_stride_b = batch > 1 ? out.stride(0) : 0;
+    x.o_stride_h = hq > 1 ? out.stride(1) : 0;
+    x.lse_stride_b = batch > 1 ? lse.stride(0) : 0;
+    x.lse_stride_h = hq > 1 ? lse.stride(1) : 0;
+    x.seqused_k = ptr<int32_t>(used);
+    x.status = ptr<int32_t>(*g_status[dev.index()]);
+    x.batch = (int)batch;
+    x.heads_q = (int)hq;
+    x.dtype = dtype_code(q.scalar_type());
+    x.softmax_scale = (float)scale;
+    int64_t bytes = g_qdecode_bytes(&x);
+    int rc = bytes < 0 ? (int)bytes : FSA_OK;
+    Tensor room;
+    if (rc == FSA_OK) {
+      room = at::empty({bytes / 4}, q.options().dtype(at::kFloat));
+      x.ws = room.data_ptr();
+      rc = g_qdecode(&x, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+    }
+    if (rc == FSA_OK) {
+      if (a[9] != Py_None) written(out);
+      if (a[10] != Py_None) written(lse);
+    }
+    no_gil.reset();
+    if (rc != FSA_OK) return PyLong_FromLong(rc);
+    if (a[9] == Py_None && a[10] == Py_None) return pair(std::move(out), std::move(lse));
+    PyObject* o = a[9] != Py_None ? (Py_INCREF(a[9]), a[9]) : THPVariable_Wrap(std::move(out));
+    PyObject* l = a[10] != Py_None ? (Py_INCREF(a[10]), a[10]) : THPVariable_Wrap(std::move(lse));
+    PyObject* both = o && l ? PyTuple_Pack(2, o, l) : nullptr;
+    Py_XDECREF(o);
+    Py_XDECREF(l);
+    return both;
+  END_HANDLE_TH_ERRORS
+}
+
+// init_quantized(addresses of fsa_rotary_axes, fsa_kv_append_quantized_workspace_ints, fsa_kv_append_quantized, fsa_kv_read_quantized,
+//                fsa_decode_quantized_workspace_bytes, fsa_decode_quantized)
+PyObject* init_quantized(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "init_quantized takes six addresses");
+    return nullptr;
+  }
+  void* at[6] = {};
+  for (Py_ssize_t i = 0; i < n && !PyErr_Occurred(); ++i) at[i] = PyLong_AsVoidPtr(a[i]);
+  if (PyErr_Occurred()) return nullptr;
+  g_axes = reinterpret_cast<decltype(g_axes)>(at[0]);
+  g_qappend_ints = reinterpret_cast<decltype(g_qappend_ints)>(at[1]);
+  g_qappend = reinterpret_cast<decltype(g_qappend)>(at[2]);
+  g_qread = reinterpret_cast<decltype(g_qread)>(at[3]);
+  g_qdecode_bytes = reinterpret_cast<decltype(g_qdecode_bytes)>(at[4]);
+  g_qdecode = reinterpret_cast<decltype(g_qdecode)>(at[5]);
+  return none();
+}
+
 // init_cache(addresses of fsa_rotary, fsa_kv_append_rotary_workspace_ints, fsa_kv_append_rotary, fsa_shared_prefix_workspace_bytes,
 //            fsa_decode_shared_prefix)
 PyObject* init_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -946,6 +1454,11 @@ PyMethodDef methods[] = {
     {"init_cache", reinterpret_cast<PyCFunction>(init_cache), METH_FASTCALL, nullptr},
     {"rotary", reinterpret_cast<PyCFunction>(rotary), METH_FASTCALL, nullptr},
     {"append", reinterpret_cast<PyCFunction>(append), METH_FASTCALL, nullptr},
+    {"init_quantized", reinterpret_cast<PyCFunction>(init_quantized), METH_FASTCALL, nullptr},
+    {"rotary_axes", reinterpret_cast<PyCFunction>(rotary_axes), METH_FASTCALL, nullptr},
+    {"append_quantized", reinterpret_cast<PyCFunction>(append_quantized), METH_FASTCALL, nullptr},
+    {"read_quantized", reinterpret_cast<PyCFunction>(read_quantized), METH_FASTCALL, nullptr},
+    {"decode_quantized", reinterpret_cast<PyCFunction>(decode_quantized), METH_FASTCALL, nullptr},
     {"shared_prefix", reinterpret_cast<PyCFunction>(shared_prefix), METH_FASTCALL, nullptr},
     {"decode_num_splits", reinterpret_cast<PyCFunction>(decode_num_splits), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -664,6 +664,9 @@ def _load_host(lib):
         host.init_cache(*(ctypes.cast(f, c_void_p).value for f in (
             lib.fsa_rotary, lib.fsa_kv_append_rotary_workspace_ints, lib.fsa_kv_append_rotary, lib.fsa_shared_prefix_workspace_bytes,
             lib.fsa_decode_shared_prefix)))
+        host.init_quantized(*(ctypes.cast(f, c_void_p).value for f in (
+            lib.fsa_rotary_axes, lib.fsa_kv_append_quantized_workspace_ints, lib.fsa_kv_append_quantized, lib.fsa_kv_read_quantized,
+            lib.fsa_decode_quantized_workspace_bytes, lib.fsa_decode_quantized)))
     except (ImportError, AttributeError, TypeError) as e:  # TypeError: a launcher that takes other addresses
         _host = None
         warnings.warn("flash_sparse_attn/_host.so is missing or does not load; calls go through the slower Python launchers until "

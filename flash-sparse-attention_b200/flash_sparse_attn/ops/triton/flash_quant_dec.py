@@ -50,6 +50,13 @@ def attn_decode_quantized(query, key, value, key_scales, value_scales, softmax_s
                                                              gather_kv_indices, seqused_k, out, lse, skip_checks)
     if not query.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
+    host = _lib.native()
+    if host is not None:
+        res = host.decode_quantized(query, key, value, key_scales, value_scales, softmax_scale, page_table, gather_kv_indices, seqused_k, out, lse)
+        if res is not None:
+            if type(res) is int:
+                _lib.check(res, "fsa_decode_quantized")
+            return res
     if not skip_checks:
         _check(query, key, value, key_scales, value_scales, softmax_scale, page_table, gather_kv_indices, seqused_k, out, lse)
     device = query.device

@@ -148,6 +148,11 @@ def apply_rotary_axes_func(
     if not query.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
     sections = tuple(sections)
+    host = _lib.native() if _unseen() and isinstance(cos, torch.Tensor) and cos.ndim == 2 else None
+    if host is not None:
+        res = host.rotary_axes(query, key, cos, sin, position_ids, axis_bits(sections, cos.shape[1], bool(axes_dealt)), len(sections), bool(interleaved))
+        if res is not None:
+            return res
     if not skip_checks:
         _check(query, key, cos, sin, position_ids, sections)
     bits = axis_bits(sections, cos.shape[1], bool(axes_dealt))

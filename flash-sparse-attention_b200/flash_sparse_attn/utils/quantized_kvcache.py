@@ -193,6 +193,17 @@ def append_kv_quantized(query: Optional[torch.Tensor], key_new: torch.Tensor, va
     if not key_new.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
     sections = None if sections is None else tuple(sections)
+    host = _lib.native()
+    if host is not None:
+        axes = sections is not None and isinstance(cos, torch.Tensor) and cos.ndim == 2
+        res = host.append_quantized(query, key_new, value_new, key_cache, value_cache, key_scales, value_scales, seqused_k, cos, sin, page_table,
+                                    free_pages, free_count, cu_seqlens_new, seqlen_offsets, position_ids,
+                                    axis_bits(sections, cos.shape[1], bool(axes_dealt)) if axes else None, len(sections) if axes else 0,
+                                    bool(interleaved), bool(advance), out)
+        if res is not None:
+            if type(res) is int:
+                _lib.check(res, "fsa_kv_append_quantized")
+            return None if res is True else res
     if not skip_checks:
         _check_append(query, key_new, value_new, key_cache, value_cache, key_scales, value_scales, seqused_k, cos, sin, page_table,
                       free_pages, free_count, cu_seqlens_new, seqlen_offsets, position_ids, sections, out)
@@ -296,6 +307,14 @@ def read_kv_quantized(key_cache: torch.Tensor, value_cache: torch.Tensor, key_sc
                                                          max_seqlen, total, dtype, out, skip_checks)
     if not key_cache.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
+    host = _lib.native() if out is None and dtype in _F16 else None
+    if host is not None:
+        res = host.read_quantized(key_cache, value_cache, key_scales, value_scales, seqused_k, page_table, cu_seqlens, max_seqlen, total,
+                                  dtype == torch.bfloat16)
+        if res is not None:
+            if type(res) is int:
+                _lib.check(res, "fsa_kv_read_quantized")
+            return res
     if not skip_checks:
         _check_read(key_cache, value_cache, key_scales, value_scales, seqused_k, page_table, cu_seqlens, max_seqlen, total, dtype, out)
     device = key_cache.device
