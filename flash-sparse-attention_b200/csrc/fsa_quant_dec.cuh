@@ -663,22 +663,47 @@ __device__ __forceinline__ void write_piece(float* to, const State<S>& st, int l
     }
 }
 
-// Four columns of a head out of several parts. `part(i)`: where part i lies.
+// Four columns of a head out of several parts. `part(i)`: where part i lies. Eight parts are fetched at a time: one by one their latencies were most of
+// what a merge took.
 template <int HD, int HEADS, typename F>
 __device__ __forceinline__ float4 join(int parts, int head, int col, F&& part, float* m_out, float* l_out) {
-  float m = -CUDART_INF_F;
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[HEADS * HD + head]);
+  constexpr int AT_ONCE = 8;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float* x = part(i);
-    const float mi = x[HEADS * HD + head], by = mi == -CUDART_INF_F ? 0.f : exp2_fast(mi - m);  // (0 times a NaN is one)
-    const float4 v = *reinterpret_cast<const float4*>(x + head * HD + col);
-    o.x = fmaf(v.x, by, o.x);
-    o.y = fmaf(v.y, by, o.y);
-    o.z = fmaf(v.z, by, o.z);
-    o.w = fmaf(v.w, by, o.w);
-    l = fmaf(x[HEADS * (HD + 1) + head], by, l);
+  float m = -CUDART_INF_F, l = 0.f;
+  for (int i0 = 0; i0 < parts; i0 += AT_ONCE) {
+    float mi[AT_ONCE], li[AT_ONCE];
+    float4 v[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      mi[i] = -CUDART_INF_F;
+      li[i] = 0.f;
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i0 + i < parts) {
+        const float* x = part(i0 + i);
+        mi[i] = x[HEADS * HD + head];
+        li[i] = x[HEADS * (HD + 1) + head];
+        v[i] = *reinterpret_cast<const float4*>(x + head * HD + col);
+      }
+    }
+    float now = m;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) now = fmaxf(now, mi[i]);
+    const float before = m == -CUDART_INF_F ? 0.f : exp2_fast(m - now);  // (0 times a NaN is one)
+    m = now;
+    l *= before;
+    o.x *= before;
+    o.y *= before;
+    o.z *= before;
+    o.w *= before;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const float by = mi[i] == -CUDART_INF_F ? 0.f : exp2_fast(mi[i] - m);
+      o.x = fmaf(v[i].x, by, o.x);
+      o.y = fmaf(v[i].y, by, o.y);
+      o.z = fmaf(v[i].z, by, o.z);
+      o.w = fmaf(v[i].w, by, o.w);
+      l = fmaf(li[i], by, l);
+    }
   }
   *m_out = m;
   *l_out = l;
@@ -712,6 +737,14 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
   uint64_t* full = full_s[warp];
   // a stage is there when its codes are (lane 0, with TMA's bytes) and its scales (the same, or each lane's copies)
   if (lane < S::STAGES) mbar_init(full + lane, p.scales_by_tma ? 1 : 33);
+  if (!GATHER && tid == 0) {
+    tma_prefetch_desc(&p.map_k);
+    tma_prefetch_desc(&p.map_v);
+    if (p.scales_by_tma) {
+      tma_prefetch_desc(&p.map_ks);
+      tma_prefetch_desc(&p.map_vs);
+    }
+  }
   if (tid == 0) abort_s = 0;
   mbar_fence_init();
   if (lane == 0) {

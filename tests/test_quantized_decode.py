@@ -15,18 +15,19 @@ TOP = {"int8": 127, "e4m3": 448, "int4": 8}
 
 
 def reference(q, keys, vals, scale):
-    """q [B, Hq, D]; keys, vals: one [n, Hkv, D] per sequence in 64 bits. Result, log-sum-exp and sum |p v|, on the CPU."""
+    """q [B, Hq, D]; keys, vals: one [n, Hkv, D] per sequence in 64 bits. Result, log-sum-exp and sum |p v|, worked out where the queries are."""
     b, hq, d = q.shape
-    out, lse, size = (torch.zeros(b, hq, n, dtype=torch.float64) for n in (d, 1, d))
+    out, lse, size = (torch.zeros(b, hq, n, dtype=torch.float64, device=q.device) for n in (d, 1, d))
     lse -= torch.inf
     for i in range(b):
         if keys[i].shape[0] == 0:
             continue
-        s = torch.einsum("hgd,nhd->hgn", q[i].double().cpu().view(keys[i].shape[1], -1, d), keys[i]) * scale
+        k, v = (x.permute(1, 0, 2).to(q.device) for x in (keys[i], vals[i]))  # [Hkv, n, D]
+        s = q[i].double().view(k.shape[0], -1, d) @ k.transpose(1, 2) * scale
         p = torch.softmax(s, -1)
-        out[i], size[i] = (torch.einsum("hgn,nhd->hgd", p, v).reshape(hq, d) for v in (vals[i], vals[i].abs()))
+        out[i], size[i] = (torch.matmul(p, x).reshape(hq, d) for x in (v, v.abs()))
         lse[i] = torch.logsumexp(s, -1).reshape(hq, 1)
-    return out, lse[..., 0], size
+    return out.cpu(), lse[..., 0].cpu(), size.cpu()
 
 
 def check(out, lse, q, keys, vals, reach_k, reach_v, scale=None):
@@ -143,8 +144,8 @@ def test_ways_that_work_is_shared_out(kind):
     run([5] * 300, 8, 2, 64, kind)                          # many items a warp
     run([40, 0, 0, 3000, 1, 0, 17] * 9, 8, 2, 128, kind)    # short and long side by side
     run([0] * 7, 8, 2, 128, kind)                           # nothing
-    run([100] * 2000, 2, 1, 64, kind, twice=False)          # more sequences than threads
-    run([9000, 4] + [0] * 500, 4, 4, 64, kind, page=256)
+    run([100] * 2000, 2, 1, 64, kind, twice=False)          # more sequences than lanes, many each
+    run([9000, 4] + [0] * 30, 4, 4, 64, kind, page=256)
     run([3], 4, 1, 64, kind, capacity=5000)                 # room for more than there is
 
 
