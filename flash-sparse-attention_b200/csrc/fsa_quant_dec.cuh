@@ -663,11 +663,10 @@ __device__ __forceinline__ void write_piece(float* to, const State<S>& st, int l
     }
 }
 
-// Four columns of a head out of several parts. `part(i)`: where part i lies. Eight parts are fetched at a time: one by one their latencies were most of
-// what a merge took.
-template <int HD, int HEADS, typename F>
+// Four columns of a head out of several parts. `part(i)`: where part i lies. AT_ONCE parts are fetched at a time: one by one their latencies were
+// most of what a merge took.
+template <int HD, int HEADS, int AT_ONCE, typename F>
 __device__ __forceinline__ float4 join(int parts, int head, int col, F&& part, float* m_out, float* l_out) {
-  constexpr int AT_ONCE = 8;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float m = -CUDART_INF_F, l = 0.f;
   for (int i0 = 0; i0 < parts; i0 += AT_ONCE) {
@@ -731,7 +730,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
   // what a warp's first piece (of an item that began before it) and its last one (of an item that goes on behind it) are
   __shared__ const float* part_s[S::WARPS][2];
   __shared__ int2 item_s[S::WARPS];  // of the last piece: sequence, item
-  __shared__ int ends_s[S::WARPS];   // whether the first piece's item ends in this warp
+  __shared__ unsigned pieces_s[3];
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
   uint64_t* full = full_s[warp];
@@ -746,11 +745,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     }
   }
   if (tid == 0) abort_s = 0;
+  if (tid < 3) pieces_s[tid] = 0;
   mbar_fence_init();
-  if (lane == 0) {
-    part_s[warp][0] = part_s[warp][1] = nullptr;
-    ends_s[warp] = 0;
-  }
   __syncthreads();
 
   // ---- where this warp begins ------------------------------------------------------------------------------------------
@@ -846,13 +842,14 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     int left = walk.left, done = 0, at = 0;
     uint32_t phase = 0;
     bool whole = walk.t == 0;  // the item began in this warp
+#pragma unroll 1
     for (int i = 0; i < S::STAGES - 1; ++i) send();
     Queries<S> q;
     State<S> st;
-    load_queries<S>(p, item.x, item.y, lane, q);
     auto arrived = [&]() { return mbar_wait_uniform(full + at, phase, &abort_s); };
     bool ok = true;
     for (;;) {
+      load_queries<S>(p, item.x, item.y, lane, q);
       st.clear();
       const int n = min(left, mine - done);
       for (int i = 0; i < n; ++i) {
@@ -881,10 +878,11 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
         write_piece<S>(to, st, lane);
         if (lane == 0) {
           part_s[warp][whole] = to;
+          atomicOr(&pieces_s[whole], 1u << warp);
           if (whole)
             item_s[warp] = item;
-          else
-            ends_s[warp] = ends;
+          else if (ends)
+            atomicOr(&pieces_s[2], 1u << warp);
         }
       }
       if (last) break;
@@ -894,7 +892,6 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
       const int4 what = *reinterpret_cast<const int4*>(extras + at * S::EXTRA + 2 * S::SCALE_BYTES);
       left = uniform(what.y);
       item = make_int2(what.z, what.w);
-      load_queries<S>(p, item.x, item.y, lane, q);
     }
     if (!ok) {  // a wait ran out: say so, and wait for what else is under way
       report_status(p.status, STATUS_WAIT);
@@ -909,48 +906,41 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
 
   // ---- items that several warps share ------------------------------------------------------------------------------------
   // Runs of pieces of one item, in the order of the warps.
+  const unsigned firsts = pieces_s[0], lasts = pieces_s[1], ends_in = pieces_s[2];  // a bit a warp: first piece, last piece, the first one's item ends
   int2 told = make_int2(0, -1);
-  int from = -1, kind = 0;  // the run's first warp and which of its pieces
-  auto close = [&](int last, bool ends) {
-    const int w0 = from, k0 = kind;
-    auto part = [&](int i) { return i == 0 ? part_s[w0][k0] : part_s[w0 + i][0]; };
-    const int2 item = k0 ? item_s[w0] : make_int2(0, 0);
-    const bool whole = k0 && ends;
+  const int highest = 31 - __clz(firsts | lasts);
+  // a run goes from a warp's last piece (an item that begins there), or from the CTA's first piece of all, to the next warp in which an item ends
+#pragma unroll 1
+  for (int w0 = firsts & 1 ? -1 : (lasts ? __ffs(lasts) - 1 : 32); w0 < 32;) {
+    const int k0 = w0 >= 0, begin = max(w0, 0);
+    const unsigned later = ends_in & (k0 ? ~0u << begin << 1 : ~0u);
+    const bool ends = later != 0, whole = k0 && ends;
+    const int last = ends ? __ffs(later) - 1 : highest;
+    auto part = [&](int i) { return i == 0 ? part_s[begin][k0] : part_s[begin + i][0]; };
+    const int2 item = k0 ? item_s[begin] : make_int2(0, 0);
     float* to = own_pieces + (k0 ? S::PIECE : 0);
-    for (int j = tid; j < S::HEADS * S::HD / 4; j += S::THREADS) {
-      const int head = j / (S::HD / 4), col = 4 * (j % (S::HD / 4));
-      float m, l;
-      const float4 o = join<S::HD, S::HEADS>(last - w0 + 1, head, col, part, &m, &l);
-      if (whole) {
-        finish(p, S::HALF, item.x, item.y, S::HEADS, head, col, o, m, l);
-      } else {
-        *reinterpret_cast<float4*>(to + head * S::HD + col) = o;
-        if (col == 0) {
-          to[S::HEADS * S::HD + head] = m;
-          to[S::HEADS * (S::HD + 1) + head] = l;
+    {
+#pragma unroll 1
+      for (int j = tid; j < S::HEADS * S::HD / 4; j += S::THREADS) {
+        const int head = j / (S::HD / 4), col = 4 * (j % (S::HD / 4));
+        float m, l;
+        const float4 o = join<S::HD, S::HEADS, 8>(last - begin + 1, head, col, part, &m, &l);
+        if (whole) {
+          finish(p, S::HALF, item.x, item.y, S::HEADS, head, col, o, m, l);
+        } else {
+          *reinterpret_cast<float4*>(to + head * S::HD + col) = o;
+          if (col == 0) {
+            to[S::HEADS * S::HD + head] = m;
+            to[S::HEADS * (S::HD + 1) + head] = l;
+          }
         }
       }
+      if (!k0) told.x = ends ? 1 : 2;
+      else if (!ends) told.y = item.x * p.items + item.y;
     }
-    if (!k0) told.x = ends ? 1 : 2;
-    else if (!ends) told.y = item.x * p.items + item.y;
-    from = -1;
-  };
-  int last = 0;
-  for (int w = 0; w < S::WARPS; ++w) {
-    if (part_s[w][0]) {
-      if (from < 0) {
-        from = w;
-        kind = 0;
-      }
-      last = w;
-      if (ends_s[w]) close(w, true);
-    }
-    if (part_s[w][1]) {
-      from = last = w;
-      kind = 1;
-    }
+    const unsigned next = lasts & (k0 ? ~0u << begin << 1 : ~0u);
+    w0 = next ? __ffs(next) - 1 : 32;
   }
-  if (from >= 0) close(last, false);
   if (tid == 0) p.shared[blockIdx.x] = told;
 }
 
@@ -979,7 +969,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) quant_merge_kernel(const __grid
   for (int j = threadIdx.x; j < HEADS * WIDE; j += MERGE_THREADS) {
     const int head = j / WIDE, col = 4 * (slice * WIDE + j % WIDE);
     float m, l;
-    const float4 o = join<HD, HEADS>(last - cta + 1, head, col, part, &m, &l);
+    const float4 o = join<HD, HEADS, 8>(last - cta + 1, head, col, part, &m, &l);
     finish(p, HALF, item / p.items, item % p.items, HEADS, head, col, o, m, l);
   }
 }
