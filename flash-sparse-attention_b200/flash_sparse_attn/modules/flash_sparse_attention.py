@@ -10,13 +10,14 @@ handed a transposed view, for which its own ``.contiguous()`` is a no-op, and au
 back through the same views. Beyond the reference's layer, ``forward`` takes the tables of rotary positions.
 """
 
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
 
 from flash_sparse_attn.ops.triton.interface import flash_gated_attn_func
 from flash_sparse_attn.ops.triton.rotary import apply_rotary_func
+from flash_sparse_attn.ops.triton.rotary_axes import apply_rotary_axes_func
 
 
 class FlashSparseAttentionConfig:
@@ -67,14 +68,19 @@ class FlashSparseAttention(nn.Module):
         return torch.matmul(weight, hidden_states.transpose(1, 2))
 
     def forward(self, hidden_states: torch.Tensor, rotary: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
-                position_ids: Optional[torch.Tensor] = None, rotary_interleaved: bool = False, **kwargs):
+                position_ids: Optional[torch.Tensor] = None, rotary_interleaved: bool = False,
+                rotary_sections: Optional[Sequence[int]] = None, rotary_axes_dealt: bool = False, **kwargs):
         """``rotary``: the tables ``(cos, sin)`` of ``apply_rotary_func``; queries and keys are then turned by their positions (or by
-        ``position_ids``), and the keys that are returned are the turned ones."""
+        ``position_ids``), and the keys that are returned are the turned ones. With ``rotary_sections`` (and ``rotary_axes_dealt``) the
+        positions have several axes, ``position_ids [axes, batch, positions]``: the step is then ``apply_rotary_axes_func``."""
         bsz, seq_len, _ = hidden_states.size()
         query_states = self.q_proj(hidden_states).view(bsz, seq_len, self.num_attention_heads, self.head_dim)
         key_states = self.k_proj(hidden_states).view(bsz, seq_len, self.num_key_value_heads, self.head_dim)
         value_states = self.v_proj(hidden_states).view(bsz, seq_len, self.num_key_value_heads, self.head_dim)
-        if rotary is not None:
+        if rotary is not None and rotary_sections is not None:
+            query_states, key_states = apply_rotary_axes_func(query_states, key_states, *rotary, position_ids, rotary_sections,
+                                                              axes_dealt=rotary_axes_dealt, interleaved=rotary_interleaved)
+        elif rotary is not None:
             query_states, key_states = apply_rotary_func(query_states, key_states, *rotary, position_ids=position_ids,
                                                          interleaved=rotary_interleaved)
         # [B, H, S] buffers, passed as the [B, S, H] views the operator's signature asks for
