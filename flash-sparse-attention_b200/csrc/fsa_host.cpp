@@ -1074,7 +1074,7 @@ bool quant_cache(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Ten
   else if (kc.scalar_type() == at::kFloat8_e4m3fn) c->format = FSA_QC_E4M3;
   else return false;
   const int64_t d = kc.size(3) * (int4 ? 2 : 1);
-  if (d > 128 || d % 16) return false;
+  if (d > 128 || d % 16 || kc.size(0) > INT32_MAX || kc.size(1) > INT32_MAX || kc.size(2) > INT32_MAX) return false;
   if (ks.sizes() != vs.sizes() || ks.scalar_type() != vs.scalar_type() || ks.dim() != (int4 ? 5 : 4)) return false;
   for (int i = 0; i < 3; ++i)
     if (ks.size(i) != kc.size(i)) return false;

@@ -84,7 +84,7 @@ struct Pair4 {
 };
 __device__ __forceinline__ Pair4 group_pair(float low, float high) {
   Pair4 p;
-  const float width = __fdiv_rn(__fsub_rn(high, low), 15.f);
+  const float width = __fdiv_rn(__fsub_rn(0.5f * high, 0.5f * low), 7.5f);  // (halves: the difference may be beyond fp32)
   float s = __bfloat162float(__float2bfloat16_rn(width));
   if (s < TINY) s = 0.f;
   p.z = __bfloat162float(__float2bfloat16_rn(__fadd_rn(low, 8.f * s)));
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, 5) quant_tokens_kernel(const __grid_c
   }
   if (place.live) {
     const int2 at = q.place[seq];
-    place.live = row < at.y;
+    place.live = row >= 0 && row < at.y;
     if (place.live) find_place(p, seq, at.x + row, bi, si, &place);
   }
   const bool turns = has_a && u < q.r.turned, turned = place.live && place.turned;

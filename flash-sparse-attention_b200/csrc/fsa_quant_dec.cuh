@@ -5,9 +5,10 @@
 //   s_jh = c sum_g (q_hg . (k^_jg - 8)) a_jg + (sum q_hg) z_jg     4 bits, group by group
 //   o_h  = sum_j p_jh b_j v^_j / sum_j p_jh,  p_jh = 2^(s_jh - m_h)
 // so no value is ever rounded on its way: codes are exact in fp16, products and sums are those of the matrix instructions in fp32, scales are
-// applied to scores and to probabilities. The queries enter as fp16 too: a bf16 row is multiplied by a power of two that brings its largest
-// element to [1, 2) (exact but for elements 2^-14 below it, whose lost bits are below the fp32 sum's own), probabilities as fp16 (2^-12) times b_j times a power
-// of two that keeps them in range. Running maxima, sums and outputs are fp32.
+// applied to scores and to probabilities. The queries enter as fp16 too: a row is multiplied by a power of two that brings its largest element
+// to [2^10, 2^11) (exact but for elements 2^-24 and more below it, which lose less than 2^-34 of the largest), probabilities times b_j times a power
+// of two that keeps them in range are rounded to fp16 (2^-11; of fp16 results what that leaves goes in as well). Running maxima, sums and outputs
+// are fp32.
 //
 // Bound by memory: a key is read once, at 2 * 8 * (heads per KV head) operations a byte. What a warp does with a tile of 32 keys has to fit
 // into the time that its bytes take, so: products run transposed (keys or value columns on the M = 16 side of mma.m16n8k16, up to eight query
@@ -604,7 +605,8 @@ __device__ __forceinline__ void settle(State<S>& st, int lane) {
 #pragma unroll
       for (int t = 0; t < S::MTILES; ++t) {
         const float z = S::INT4 ? st.centre[S::INT4 ? t / (S::GS / 16) : 0][nt][x] : 0.f;
-        float a = fmaf(st.o[t][nt][x], by * (1.f / S::UNIT), z), b = fmaf(st.o[t][nt][x + 2], by * (1.f / S::K_UNIT), z);
+        // (one after the other: of values from 2^111 on their product is beyond fp32)
+        float a = fmaf(st.o[t][nt][x] * (1.f / S::UNIT), by, z), b = fmaf(st.o[t][nt][x + 2] * (1.f / S::K_UNIT), by, z);
         if constexpr (!S::INT4) {  // columns r and r + 8: even rows take the neighbour's first, odd ones its second
           const float other = __shfl_xor_sync(ALL, lane & 4 ? a : b, 4);
           if (lane & 4) a = other; else b = other;

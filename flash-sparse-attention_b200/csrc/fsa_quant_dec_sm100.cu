@@ -19,7 +19,7 @@ int plan(const FsaQuantDecodeArgs* a, QuantDecParams* p, int* warps, int* piece)
   const FsaQuantCache& c = a->cache;
   const int rc = check_quant_cache(c);
   if (rc != FSA_OK) return rc;
-  if (a->batch <= 0 || a->heads_q <= 0 || a->heads_q % c.heads_kv || a->topk < 0) return FSA_ERR_INVALID_ARG;
+  if (a->batch <= 0 || a->heads_q <= 0 || a->heads_q % c.heads_kv || a->topk < 0 || a->topk > 0x7fffff00) return FSA_ERR_INVALID_ARG;
   // the keys of a tile lie in one page
   if (c.page_table && (c.page_size < QUANT_TILE || (c.page_size & (c.page_size - 1)))) return FSA_ERR_UNSUPPORTED;
   for (p->page_shift = 0; c.page_table && 1 << p->page_shift < c.page_size;) ++p->page_shift;

@@ -58,6 +58,7 @@ def check_quantized_cache(key_cache, value_cache, key_scales, value_scales, page
     head_dim = key_cache.shape[3] * (2 if int4 else 1)
     assert 0 < head_dim <= MAX_HEAD_DIM and head_dim % 16 == 0, f"head_dim must be a multiple of 16 up to {MAX_HEAD_DIM}"
     assert key_cache.shape[0] > 0 and key_cache.shape[1] > 0 and key_cache.shape[2] > 0, "the cache must not be empty"
+    assert max(key_cache.shape) < 2**31, "blocks and slots must be below 2^31"
     for t in (key_scales, value_scales):
         assert t.shape[:3] == key_cache.shape[:3], "scales must have the blocks, slots and heads of the codes"
         if int4:

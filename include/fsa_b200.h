@@ -724,7 +724,7 @@ int fsa_kv_append_quantized(const FsaKvAppendQuantArgs* args, void* stream);
  * The values of such a cache in 16 bits, computed in fp32 and rounded once: the first seqused_k[b] slots of every sequence (null: all) as
  * rows [batch, seqlen, heads_kv, head_dim], zeros behind them, or packed [total, heads_kv, head_dim] where cu_seqlens says; packed rows
  * outside every sequence and behind its last slot are zeros. Slots on a page outside the pool read as zeros and set the status word to 3.
- * Results on 16-byte boundaries.
+ * Results on 16-byte boundaries; heads_kv * head_dim up to 131072.
  */
 typedef struct FsaKvReadQuantArgs {
   FsaQuantCache cache;
@@ -745,7 +745,8 @@ int fsa_kv_read_quantized(const FsaKvReadQuantArgs* args, void* stream);
  * all), or against the slots that gather_kv_indices [batch, topk] names (entries outside [0, seqused_k[b]) are left out). Scores, the
  * statistics and sums are fp32; a sequence without keys gets zeros and a log-sum-exp of -inf. Keys on a page outside the pool are left
  * out and set the status word to 3. The work is cut evenly over the GPU whatever the lengths; pieces meet in `ws`, of
- * fsa_decode_quantized_workspace_bytes bytes, one per call under way. Rows of q and out on 16-byte boundaries.
+ * fsa_decode_quantized_workspace_bytes bytes, one per call under way. Pages of a power of two of slots, at least 32; rows of q on 16-byte
+ * boundaries, of out on 4-byte ones. Elements of queries, keys and values above 2^100 may count as infinite.
  */
 typedef struct FsaQuantDecodeArgs {
   FsaQuantCache cache;

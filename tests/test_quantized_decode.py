@@ -200,6 +200,20 @@ def test_size_of_values(kind, factor):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["int8", "int4", "e4m3"])
+def test_values_near_the_top_of_bf16(kind):
+    """Values around 2^113: the same numbers as small ones in other units."""
+    import flash_sparse_attn as fsa
+
+    q = normal(1, 2, 4, 64)
+    k, v, ks, vs = make_cache(3, 2, 70, 2, 64, kind)
+    one = fsa.flash_dense_attn_with_quantized_kvcache_func(q, k, v, ks, vs)
+    two = fsa.flash_dense_attn_with_quantized_kvcache_func(q, k, v, ks, (vs.float() * 2.0**112).to(vs.dtype))
+    done()
+    assert two.abs().max() > 2.0**110 and torch.equal(one.float(), two.float() * 2.0**-112)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "int4", "e4m3"])
 def test_infinities_and_nan_stay_in_their_row(kind):
     """A stored row that stands for NaN makes the results of the sequence that attends to it NaN, and no others."""
     import flash_sparse_attn as fsa

@@ -295,6 +295,23 @@ def test_special_rows(kind, group, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3", "int4"])
+def test_rows_from_end_to_end_of_bf16(kind):
+    """The largest and the least number of a row: their difference is beyond fp32, neither is an infinity."""
+    from flash_sparse_attn.utils.kvcache import append_kv_quantized, empty_kv_quantized, read_kv_quantized
+
+    cache = empty_kv_quantized(1, 4, 1, 64, KINDS[kind])
+    used = torch.zeros(1, dtype=torch.int32, device=DEV)
+    x = (torch.linspace(-3e38, 3e38, 64, device=DEV, dtype=torch.float64).to(torch.bfloat16)).view(1, 1, 1, 64)
+    append_kv_quantized(None, x, x, *cache, used)
+    got, _ = read_kv_quantized(*cache, used, max_seqlen=1)
+    done()
+    # half a step (of 15 over 6e38, of 254, or e4m3's 2^-4 of the value), and 2^-8 of 3e38 for each of the roundings of s (eight times), z and the result
+    step = {"int4": 2e37 + 10 * 2.0**-8 * 3e38, "int8": 1.2e36 + 2.0**-8 * 3e38, "e4m3": 2.0**-4 * 3e38 + 2.0**-8 * 3e38}[kind]
+    assert ((got.double() - x.double()).abs() <= step).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("kind,d,group", FORMS)
 def test_reading_back(kind, d, group, dtype):
