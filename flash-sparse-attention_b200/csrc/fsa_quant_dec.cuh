@@ -16,11 +16,14 @@
 // values are transposed on their way out of shared memory (ldmatrix on bytes); and codes become fp16 numbers by being taken for the bits of one:
 // n below 1024 in the low bits is the subnormal n 2^-24, which the matrix instructions multiply exactly. Codes are made positive for that (+128, of 4
 // bits they are), and what this adds is taken off where it cannot grow: of scores, a sum over columns, in the first accumulator (-128 2^-24 sum q);
-// of outputs, whose sums over keys run on and on, by a product of the same probabilities with the constant, tile by tile.
+// of outputs, whose sums over keys run on and on, by a product of the same probabilities with the constant, tile by tile, once for the columns of a
+// group (once for each sixteen columns: 8 x 100000 keys in 4 bits 113.5 us, so 112).
 //
 // The work is one list of tiles (sequence, KV head and block of query heads, 32 keys), cut into equal pieces for all warps of the grid whatever the
 // lengths are. A warp streams its piece through a ring of its own in shared memory: TMA brings a tile's codes (cp.async, where positions are
-// chosen one by one), the warp's own mbarriers say when, and no barrier of the CTA is in the loop. A piece that is a whole item is written out, the
+// chosen one by one), the warp's own mbarriers say when, and no barrier of the CTA is in the loop. Whole tiles that follow in a page (or in a contiguous
+// cache) are counted out when the first is sent, so that the walk and the page table are gone to once for all of them (8 x 100000 keys in 4 bits 112 us,
+// so 109). A piece that is a whole item is written out, the
 // others meet inside the CTA and then, for items that several CTAs share, in quant_merge_kernel.
 #pragma once
 #include <math_constants.h>
@@ -81,6 +84,11 @@ __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void add2(float* d, const float* a) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(d[0]), "+f"(d[1])
+      : "f"(a[0]), "f"(a[1]));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   uint32_t r;
@@ -176,29 +184,47 @@ __device__ __forceinline__ Place look_up(const QuantDecParams& p, const Walk<GAT
   return at;
 }
 
-// Sends for a tile. Pages hold a multiple of 32 slots, so that without gather the keys of a tile lie in one.
-template <typename S, bool GATHER>
-__device__ __forceinline__ void fetch(const QuantDecParams& p, const Walk<GATHER>& w, const Place& at, uint8_t* stage, uint8_t* extra, uint64_t* full,
-                                      int lane) {
-  const FsaQuantCache& c = p.c;
-  const int h = p.blocks == 1 ? w.i : w.i / p.blocks;
-  const int block = GATHER ? at.block : uniform(at.block);
-  const bool there = at.position >= 0, known = there && (unsigned)block < (unsigned)p.cache_blocks;
-  if (there && !known) report_status(p.status, STATUS_BAD_PAGE);
-  const int slot = c.page_table ? at.position & (c.page_size - 1) : at.position;
+// A tile on its way: `left` of item (b, i) with this one; of a KV head h; rows: a bit each that is there. Where positions are chosen, block and slot
+// are those of the lane's row.
+struct Tile {
+  int block, slot, h, left, b, i, run;  // run: whole tiles that follow side by side with it
   uint32_t rows;
+};
+
+// The tile that the walk has come to. Pages hold a multiple of 32 slots, so that without gather the keys of a tile lie in one.
+template <bool GATHER>
+__device__ __forceinline__ void find_tile(const QuantDecParams& p, const Walk<GATHER>& w, const Place& at, Tile& tile) {
+  tile.h = p.blocks == 1 ? w.i : w.i / p.blocks;
+  tile.block = GATHER ? at.block : uniform(at.block);
+  const bool there = at.position >= 0, known = there && (unsigned)tile.block < (unsigned)p.cache_blocks;
+  if (there && !known) report_status(p.status, STATUS_BAD_PAGE);
+  tile.slot = p.c.page_table ? at.position & (p.c.page_size - 1) : at.position;
+  tile.left = w.left;
+  tile.b = w.b;
+  tile.i = w.i;
+  tile.run = 0;
   if constexpr (GATHER) {
-    rows = __ballot_sync(ALL, known);
+    tile.rows = __ballot_sync(ALL, known);
   } else {
     const int left = w.count - w.t * TILE;
-    rows = !known ? 0u : (left >= TILE ? ALL : (1u << left) - 1);
+    tile.rows = !known ? 0u : (left >= TILE ? ALL : (1u << left) - 1);
+    const int end = p.c.page_table ? min(left, p.c.page_size - tile.slot) : left;
+    if (known && end >= 2 * TILE) tile.run = end / TILE - 1;
   }
+}
+
+// Sends for a tile.
+template <typename S, bool GATHER>
+__device__ __forceinline__ void fetch(const QuantDecParams& p, const Tile& tile, uint8_t* stage, uint8_t* extra, uint64_t* full, int lane) {
+  const FsaQuantCache& c = p.c;
+  const int block = tile.block, slot = tile.slot, h = tile.h;
+  const uint32_t rows = tile.rows;
   const bool lead = elect_one();
-  if (lead) *reinterpret_cast<int4*>(extra + 2 * S::SCALE_BYTES) = make_int4((int)rows, w.left, w.b, w.i);
+  if (lead) *reinterpret_cast<int4*>(extra + 2 * S::SCALE_BYTES) = make_int4((int)rows, tile.left, tile.b, tile.i);
   const bool here = rows >> lane & 1;  // this lane's row
   if constexpr (!GATHER) {
     if (lead) {
-      if (known) {
+      if (rows) {
         mbar_arrive_expect_tx(full, 2 * S::TILE_BYTES + (p.scales_by_tma ? 2 * S::SCALE_BYTES : 0));
         tma_load_4d(stage, &p.map_k, full, 0, h, slot, block);
         tma_load_4d(stage + S::TILE_BYTES, &p.map_v, full, 0, h, slot, block);
@@ -387,9 +413,9 @@ __device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[S:
   }
 }
 
-// One tile: its two halves of sixteen keys.
+// One tile: its two halves of sixteen keys. groups: that the row has (of 96 columns in groups of 32 three).
 template <typename S>
-__device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uint8_t* stage, const uint8_t* extra, uint32_t rows, int lane) {
+__device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uint8_t* stage, const uint8_t* extra, uint32_t rows, int groups, int lane) {
   const int r = lane >> 2, c = lane & 3;
   uint32_t a_words[4][S::GROUPS], b_words[4][S::GROUPS];  // scales of rows r, r + 8, ..
   const uint32_t* scales = reinterpret_cast<const uint32_t*>(extra);
@@ -411,6 +437,7 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uin
       for (int i = 0; i < 4; ++i) s[half][nt][i] = 0.f;
 #pragma unroll
     for (int g = 0; g < S::GROUPS; ++g) {
+      if (S::GS == 32 && g >= groups) continue;
       uint32_t w[2][KWORDS];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -432,7 +459,7 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uin
 #pragma unroll
       for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[nt][i] = S::ADDED == 0.f ? 0.f : -S::ADDED * q.sum[g][nt][i & 1];
+        for (int i = 0; i < 4; ++i) acc[nt][i] = S::INT4 || S::ADDED == 0.f ? 0.f : -S::ADDED * q.sum[g][nt][i & 1];
 #pragma unroll
       for (int j = 0; j < KWORDS; ++j) {
         if constexpr (!S::INT4) {
@@ -460,7 +487,7 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uin
           const uint32_t word = a_words[2 * half + (i >> 1)][g];
           const float by = scale_of(word, S::INT4);
           if constexpr (S::INT4)
-            s[half][nt][i] = fmaf(acc[nt][i], by, fmaf(q.sum[g][nt][i & 1], centre_of(word), s[half][nt][i]));
+            s[half][nt][i] = fmaf(acc[nt][i], by, fmaf(q.sum[g][nt][i & 1], fmaf(-S::ADDED, by, centre_of(word)), s[half][nt][i]));  // (the codes' 8)
           else
             s[half][nt][i] = acc[nt][i] * by;
         }
@@ -533,6 +560,7 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uin
   constexpr int PIECES = S::CH / S::GROUPS;  // of sixteen bytes, of a group
 #pragma unroll
   for (int g = 0; g < S::GROUPS; ++g) {
+    if (S::GS == 32 && g >= groups) continue;
     // Probabilities times scales, of fp16 results with what the rounding to fp16 leaves (else it would be as large as the result's own).
     uint32_t pb[2][S::NT][2], rest[2][S::HALF ? S::NT : 1][2];
 #pragma unroll
@@ -549,17 +577,29 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uin
         }
       }
     }
-    auto add = [&](int t, int half, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-      // less what was added to the codes: the same products with that, which no rounding of probabilities changes
+    if constexpr (S::ADDED != 0.f) {
+      // less what was added to the codes: the same products with that, which no rounding of probabilities changes; columns of a group share them
       constexpr uint32_t LESS0 = S::INT4 ? 0x80088008u : 0x80808080u, LESS1 = 0x80808080u;
 #pragma unroll
       for (int nt = 0; nt < S::NT; ++nt) {
-        mma(st.o[t][nt], a0, a1, a2, a3, pb[half][nt][0], pb[half][nt][1]);
-        if constexpr (S::ADDED != 0.f) mma(st.o[t][nt], LESS0, LESS1, LESS0, LESS1, pb[half][nt][0], pb[half][nt][1]);
-        if constexpr (S::HALF) {
-          mma(st.o[t][nt], a0, a1, a2, a3, rest[half][nt][0], rest[half][nt][1]);
-          if constexpr (S::ADDED != 0.f) mma(st.o[t][nt], LESS0, LESS1, LESS0, LESS1, rest[half][nt][0], rest[half][nt][1]);
+        float less[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          mma(less, LESS0, LESS1, LESS0, LESS1, pb[half][nt][0], pb[half][nt][1]);
+          if constexpr (S::HALF) mma(less, LESS0, LESS1, LESS0, LESS1, rest[half][nt][0], rest[half][nt][1]);
         }
+#pragma unroll
+        for (int t = g * (S::MTILES / S::GROUPS); t < (g + 1) * (S::MTILES / S::GROUPS); ++t) {
+          add2(st.o[t][nt], less);
+          add2(st.o[t][nt] + 2, less + 2);
+        }
+      }
+    }
+    auto add = [&](int t, int half, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt) {
+        mma(st.o[t][nt], a0, a1, a2, a3, pb[half][nt][0], pb[half][nt][1]);
+        if constexpr (S::HALF) mma(st.o[t][nt], a0, a1, a2, a3, rest[half][nt][0], rest[half][nt][1]);
       }
     };
 #pragma unroll
@@ -819,6 +859,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     walk.left = walk.tiles - walk.t;
     int sent = 0, into = 0, chosen_next = -1;  // into: the stage that the next copies take
     Place place;
+    Tile tile;
+    tile.run = 0;
     if constexpr (GATHER) {
       place = look_up(p, walk, chosen(p, walk, lane));
       Walk<GATHER> ahead = walk;
@@ -829,16 +871,25 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     }
     auto send = [&]() {
       if (sent == mine) return;
-      fetch<S, GATHER>(p, walk, place, ring + into * S::CODES, extras + into * S::EXTRA, full + into, lane);
-      into = into + 1 == S::STAGES ? 0 : into + 1;
-      if (++sent == mine) return;
-      walk.next(p);
-      place = look_up(p, walk, chosen_next);
-      if constexpr (GATHER) {
-        Walk<GATHER> ahead = walk;
-        ahead.next(p);
-        chosen_next = chosen(p, ahead, lane);
+      ++sent;
+      if (!GATHER && tile.run > 0) {
+        --tile.run;
+        --tile.left;
+        tile.slot += TILE;
+      } else {
+        find_tile(p, walk, place, tile);
+        walk.t += tile.run;
+        walk.left -= tile.run;
+        walk.next(p);
+        place = look_up(p, walk, chosen_next);
+        if constexpr (GATHER) {
+          Walk<GATHER> ahead = walk;
+          ahead.next(p);
+          chosen_next = chosen(p, ahead, lane);
+        }
       }
+      fetch<S, GATHER>(p, tile, ring + into * S::CODES, extras + into * S::EXTRA, full + into, lane);
+      into = into + 1 == S::STAGES ? 0 : into + 1;
     };
     int2 item = make_int2(walk.b, walk.i);
     int left = walk.left, done = 0, at = 0;
@@ -861,7 +912,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
         __syncwarp();
         send();
         uint8_t* extra = extras + at * S::EXTRA;
-        take_tile<S>(st, q, ring + at * S::CODES, extra, *reinterpret_cast<const uint32_t*>(extra + 2 * S::SCALE_BYTES), lane);
+        take_tile<S>(st, q, ring + at * S::CODES, extra, *reinterpret_cast<const uint32_t*>(extra + 2 * S::SCALE_BYTES), p.words, lane);
         ++done;
         if (++at == S::STAGES) {
           at = 0;
