@@ -24,8 +24,10 @@
 // chosen one by one), the warp's own mbarriers say when, and no barrier of the CTA is in the loop. Whole tiles that follow in a page (or in a contiguous
 // cache) are counted out when the first is sent, so that the walk and the page table are gone to once for all of them (8 x 100000 keys in 4 bits 112 us,
 // so 109). A piece that is a whole item is written out, the
-// others meet inside the CTA and then, for items that several CTAs share, in quant_merge_kernel.
+// others meet inside the CTA and then, for items that several CTAs share, in quant_merge_kernel. Calls of few
+// tiles are cut by items instead, each for a cluster of CTAs, and meet in its shared memory: one launch.
 #pragma once
+#include <cooperative_groups.h>
 #include <math_constants.h>
 
 #include <atomic>
@@ -67,7 +69,7 @@ struct Shape {
   static constexpr int PIECE = HEADS * (HD + 2);   // floats: outputs, maxima, sums
   static constexpr int RING = (STAGES * (CODES + EXTRA) + ALIGN - 1) / ALIGN * ALIGN;
   static constexpr int SMEM = WARPS * RING + 1024;
-  static_assert(STAGES >= 2 && RING >= PIECE * 4 && SMEM <= 225 * 1024, "ring");
+  static_assert(STAGES >= 2 && RING >= 2 * PIECE * 4 && SMEM <= 225 * 1024, "ring");
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
@@ -797,7 +799,18 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
   const long long g_warp = (long long)blockIdx.x * S::WARPS + warp;
   Walk<GATHER> walk;
   int mine = 0;
-  {
+  if (p.cluster) {
+    // an item's tiles go round the CTAs of its cluster first, then round their warps
+    const int n = (int)blockIdx.x / p.cluster, w = warp * p.cluster + (int)blockIdx.x % p.cluster;
+    walk.b = n / p.items;
+    walk.i = n - walk.b * p.items;
+    const int tiles = tiles_of(GATHER ? p.topk : keys_of(p, walk.b)), warps = min(tiles, p.cluster * S::WARPS);
+    if (w < warps) {
+      const int each = tiles / warps, more = tiles - each * warps;
+      walk.t = each * w + more * w / warps;
+      mine = each * (w + 1) + more * (w + 1) / warps - walk.t;
+    }
+  } else {
     auto tiles_at = [&](int b) { return tiles_of(GATHER ? p.topk : keys_of(p, b)); };
     const bool alike = GATHER || !p.used;
     const int per = (p.batch + 31) / 32, b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
@@ -922,7 +935,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
       if (!ok) break;
       const bool ends = n == left, last = done == mine;
       settle<S>(st, lane);
-      if (whole && ends) {
+      if (whole && ends && !p.cluster) {
         write_out<S>(p, st, item.x, item.y, lane);
       } else {
         // the ring is free behind the last tile; a first piece that is done before goes through the workspace
@@ -930,9 +943,10 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
         __syncwarp();
         write_piece<S>(to, st, lane);
         if (lane == 0) {
-          part_s[warp][whole] = to;
-          atomicOr(&pieces_s[whole], 1u << warp);
-          if (whole)
+          const bool begins = whole && !p.cluster;
+          part_s[warp][begins] = to;
+          atomicOr(&pieces_s[begins], 1u << warp);
+          if (begins)
             item_s[warp] = item;
           else if (ends)
             atomicOr(&pieces_s[2], 1u << warp);
@@ -952,6 +966,34 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     }
   }
   __syncthreads();
+  if (p.cluster) {  // the CTA's warps join their pieces behind warp 0's, the cluster's CTAs a share of the columns each
+    auto cluster = cooperative_groups::this_cluster();
+    float* joined = reinterpret_cast<float*>(smem) + S::PIECE;
+    const int parts = abort_s ? 0 : __popc(pieces_s[0]), share = S::HEADS * S::HD / 4 / p.cluster, rank = (int)blockIdx.x % p.cluster;
+    const int n = (int)blockIdx.x / p.cluster;
+#pragma unroll 1
+    for (int last = 0; last < 2; ++last) {
+      auto part = [&](int i) { return last ? static_cast<const float*>(cluster.map_shared_rank(joined, i)) : part_s[i][0]; };
+      const int j0 = last ? rank * share : 0, j1 = last ? j0 + share : S::HEADS * S::HD / 4;
+#pragma unroll 1
+      for (int j = j0 + tid; j < j1; j += S::THREADS) {
+        const int head = j / (S::HD / 4), col = 4 * (j % (S::HD / 4));
+        float m, l;
+        const float4 o = join<S::HD, S::HEADS, 8>(last ? p.cluster : parts, head, col, part, &m, &l);
+        if (last) {
+          finish(p, S::HALF, n / p.items, n % p.items, S::HEADS, head, col, o, m, l);
+        } else {
+          *reinterpret_cast<float4*>(joined + head * S::HD + col) = o;
+          if (col == 0) {
+            joined[S::HEADS * S::HD + head] = m;
+            joined[S::HEADS * (S::HD + 1) + head] = l;
+          }
+        }
+      }
+      cluster.sync();  // behind the last one nobody leaves while another CTA may still read its shared memory
+    }
+    return;
+  }
   if (abort_s) {  // a wait ran out: nothing to join
     if (tid == 0) p.shared[blockIdx.x] = make_int2(0, -1);
     return;
@@ -1035,6 +1077,7 @@ cudaError_t launch_both(const QuantDecParams& p, cudaStream_t stream) {
   static std::atomic<unsigned long long> opted_in{0};
   auto kern = quant_decode_kernel<S, GATHER>;
   if (cudaError_t e = smem_opt_in(kern, S::SMEM, opted_in); e != cudaSuccess) return e;
+  if (p.cluster) return launch_early(kern, (unsigned)(p.batch * p.items * p.cluster), S::THREADS, S::SMEM, stream, p.cluster, p);
   cudaError_t e = launch_early(kern, (unsigned)p.ctas, S::THREADS, S::SMEM, stream, 1, p);
   if (e != cudaSuccess || p.ctas == 1) return e;
   return launch_early(quant_merge_kernel<S::HD, S::HEADS, S::HALF>, (unsigned)(p.ctas * SLICES), MERGE_THREADS, 0, stream, 1, p);

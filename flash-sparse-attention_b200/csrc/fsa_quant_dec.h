@@ -33,6 +33,7 @@ struct alignas(64) QuantDecParams {
   int page_shift;                   // log2 of the slots of a page
   int cache_blocks;                 // pages of the pool, or sequences
   int ctas;
+  int cluster;                      // CTAs that share an item and meet in shared memory; 0: the work is one list
   bool scales_by_tma;
   float scale_log2;
 };

@@ -14,6 +14,19 @@ extern template cudaError_t launch_quant_decode<FSA_QC_INT4>(const QuantDecParam
 
 namespace {
 
+// CTAs that take an item together and meet in shared memory, or 0: the work as one list, whose pieces meet in a kernel of their own. That kernel
+// costs 4 us, which a cluster saves (one sequence of 8 KV heads of 128, int8: 200 keys 11.1 us, so 6.6; 2000 11.2 and 7.8; 8000 14.5 and 12.7); on
+// the other side its CTAs are some of the GPU's and do not help one another, at about 1 us for each tile that a warp has more. So: as many CTAs as
+// can all run (a cluster lies in one GPC, whose SMs need not be a multiple of it: 15 clusters of 8 ran at once, 33 of 4, 74 of 2, and a second turn
+// doubles the time), and at most 4 tiles a warp where lengths are not known here and one sequence may have all the keys, else at most 3 tiles more
+// than in the list (32 sequences x 2048 chosen keys: 24.4 us, so 21.1).
+int cluster_of(long long items, long long tiles, int warps, bool alike, int sms) {
+  int c = 8;
+  while (c > 0 && (c > tiles || items * c > (c > 1 ? sms - 5 * c : sms))) c /= 2;
+  if (c == 0) return 0;
+  return (alike ? tiles * (sms - items * c) <= 3ll * c * warps * sms : tiles <= 4ll * c * warps) ? c : 0;
+}
+
 // What follows from sizes alone; a FSA_ERR_* code where they do not fit.
 int plan(const FsaQuantDecodeArgs* a, QuantDecParams* p, int* warps, int* piece) {
   const FsaQuantCache& c = a->cache;
@@ -40,7 +53,9 @@ int plan(const FsaQuantDecodeArgs* a, QuantDecParams* p, int* warps, int* piece)
   p->words = quant_row_words(c);
   const long long most = a->gather_kv_indices ? a->topk : p->keys, tiles = most > 0 ? (most + QUANT_TILE - 1) / QUANT_TILE : 1;
   const long long ctas = ((long long)p->items * a->batch * tiles + *warps - 1) / *warps;  // no warp without a tile
-  p->ctas = (int)(ctas < device_sm_count() ? ctas : device_sm_count());
+  const int sms = device_sm_count();
+  p->ctas = (int)(ctas < sms ? ctas : sms);
+  p->cluster = cluster_of((long long)p->items * a->batch, tiles, *warps, a->gather_kv_indices || !a->seqused_k, sms);
   return FSA_OK;
 }
 
@@ -57,7 +72,7 @@ extern "C" int64_t fsa_decode_quantized_workspace_bytes(const FsaQuantDecodeArgs
   int warps, piece;
   const int rc = plan(a, &p, &warps, &piece);
   if (rc != FSA_OK) return rc;
-  return shared_bytes(p) + (int64_t)p.ctas * (2 + warps) * piece * (int64_t)sizeof(float);
+  return p.cluster ? 16 : shared_bytes(p) + (int64_t)p.ctas * (2 + warps) * piece * (int64_t)sizeof(float);
 }
 
 extern "C" int fsa_decode_quantized(const FsaQuantDecodeArgs* a, void* stream_) {

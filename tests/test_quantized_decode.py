@@ -150,6 +150,19 @@ def test_ways_that_work_is_shared_out(kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,d", [("int8", 128), ("int4", 64)])
+@pytest.mark.parametrize("batch,hkv,per", [(1, 13, 4), (3, 5, 4), (16, 2, 1), (33, 1, 12), (69, 1, 4), (35, 2, 4), (148, 1, 4), (149, 1, 4)])
+def test_few_tiles_and_many_sequences(kind, d, batch, hkv, per):
+    """Items that a cluster of 8, 4, 2 or 1 takes, or the list; lengths from none up to what a cluster is given (4 tiles a warp of 8 to 12), and past it."""
+    rng = torch.Generator().manual_seed(batch)
+    for capacity in (40, 1290, 3100):
+        lens = [capacity, *torch.randint(0, capacity + 1, (batch - 1,), generator=rng).tolist()]
+        lens[batch // 2] = 0 if batch > 1 else capacity
+        run(lens, hkv * per, hkv, d, kind, twice=False)
+    run([700] * batch, hkv * per, hkv, d, kind, page=64, topk=500, twice=False)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind,group", [("int8", 64), ("e4m3", 64), ("int4", 64), ("int4", 32)])
 @pytest.mark.parametrize("page", [0, 32, 64, 128, 256])
 def test_pages_and_what_lies_behind_the_last_position(kind, group, page):
