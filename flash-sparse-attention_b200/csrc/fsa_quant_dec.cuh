@@ -10,7 +10,8 @@
 // of two that keeps them in range are rounded to fp16 (2^-11; of fp16 results what that leaves goes in as well). Running maxima, sums and outputs
 // are fp32.
 //
-// Bound by memory: a key is read once, at 2 * 8 * (heads per KV head) operations a byte. What a warp does with a tile of 32 keys has to fit
+// Bound by memory: a key is read once, at 2 * 8 * (heads per KV head) operations a byte. (int8, 64 chats of up to 8192 tokens: 100.4 us, 5.3 TB/s, 0.82 of a
+// copy's rate; 4 bits, 8 x 100000: 109 us, 4.05 TB/s, where instructions bound it, 605 a tile; one sequence of 2001 keys 6.8 us.) What a warp does with a tile of 32 keys has to fit
 // into the time that its bytes take, so: products run transposed (keys or value columns on the M = 16 side of mma.m16n8k16, up to eight query
 // heads on the N = 8 side); columns of keys are dealt to lanes so that a lane's codes are neighbours in memory (the sum over columns has no order),
 // values are transposed on their way out of shared memory (ldmatrix on bytes); and codes become fp16 numbers by being taken for the bits of one:
