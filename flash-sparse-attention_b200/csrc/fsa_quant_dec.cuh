@@ -1048,15 +1048,19 @@ __global__ void __launch_bounds__(MERGE_THREADS) quant_merge_kernel(const __grid
   after_previous();
   __shared__ int end_s;
   const int cta = blockIdx.x / SLICES, slice = blockIdx.x % SLICES;
+  if (threadIdx.x == 0) end_s = p.ctas;
+  // (what the next CTAs say is asked for with the item: two trips to memory in one)
+  auto says = [&](int c) { return c < p.ctas ? p.shared[c].x : 0; };
+  int c = cta + 1 + threadIdx.x, said = says(c);
   const int item = p.shared[cta].y;
   if (item < 0) return;
-  if (threadIdx.x == 0) end_s = p.ctas;
   __syncthreads();
   for (int c0 = cta + 1; c0 < p.ctas; c0 += MERGE_THREADS) {
-    const int c = c0 + threadIdx.x;
-    const bool ends = c < p.ctas && p.shared[c].x == 1;
+    const bool ends = said == 1;
     if (ends) atomicMin(&end_s, c);
     if (__syncthreads_or(ends)) break;
+    c += MERGE_THREADS;
+    said = says(c);
   }
   constexpr int PIECE = HEADS * (HD + 2);
   const int last = min(end_s, p.ctas - 1);
