@@ -11,7 +11,7 @@
 // are fp32.
 //
 // Bound by memory: a key is read once, at 2 * 8 * (heads per KV head) operations a byte. (int8, 64 chats of up to 8192 tokens: 100.4 us, 5.3 TB/s, 0.82 of a
-// copy's rate; 4 bits, 8 x 100000: 109 us, 4.05 TB/s, where instructions bound it, 605 a tile; one sequence of 2001 keys 6.8 us.) What a warp does with a tile of 32 keys has to fit
+// copy's rate; 4 bits, 8 x 100000: 112 us, 3.95 TB/s, where instructions bound it, 630 a tile; one sequence of 2001 keys 6.8 us.) What a warp does with a tile of 32 keys has to fit
 // into the time that its bytes take, so: products run transposed (keys or value columns on the M = 16 side of mma.m16n8k16, up to eight query
 // heads on the N = 8 side); columns of keys are dealt to lanes so that a lane's codes are neighbours in memory (the sum over columns has no order),
 // values are transposed on their way out of shared memory (ldmatrix on bytes); and codes become fp16 numbers by being taken for the bits of one:
@@ -54,8 +54,8 @@ struct Shape {
   static constexpr int RB = INT4 ? HD / 2 : HD;    // bytes of a row
   static constexpr int CH = RB / 16;
   static constexpr int KSTEPS = HD / 16, MTILES = HD / 16;
-  // One of a code's units, as it enters the products, and what was added to it. (Of 4 bits every other column enters 16 times as large: of
-  // keys the others' queries make up for it, of values the result is divided.)
+  // One of a code's units, as it enters the products, and what was added to it. (Of 4 bits every other column comes 16 times as large: of
+  // keys the others are multiplied, of values the result is divided.)
   static constexpr float UNIT = FMT == FSA_QC_E4M3 ? 1.f : 1.f / 16777216.f, K_UNIT = INT4 ? 16.f * UNIT : UNIT;
   static constexpr float ADDED = FMT == FSA_QC_E4M3 ? 0.f : (FMT == FSA_QC_INT8 ? 128.f : 8.f);
   static constexpr int HEADS = 8 * NT;
@@ -121,6 +121,18 @@ __device__ __forceinline__ void widen8(uint32_t w, uint32_t* out) {
   out[1] = w & 0x00f000f0u;
   out[2] = v & 0x000f000fu;
   out[3] = v & 0x00f000f0u;
+}
+__device__ __forceinline__ uint32_t by16(uint32_t two) {
+  const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&two), __float2half2_rn(16.f));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+// The same with all of them 16 n 2^-24: the matrix instructions align products by the exponents of their factors, of which a subnormal has the least
+// there is, and what lies 2^-24 below the largest is lost. Of scores that was up to 4e-6 (2^-24 n: log-sum-exps off by up to 9e-7 of themselves, so by
+// 1e-7); of outputs it is far below their rounding.
+__device__ __forceinline__ void widen8_high(uint32_t w, uint32_t* out) {
+  widen8(w, out);
+  out[0] = by16(out[0]);
+  out[2] = by16(out[2]);
 }
 // Two tiles of 16 rows x 16 bytes, transposed: lane's row address; registers 0, 1 hold bytes lane / 4 and that + 8 of rows 4 (lane % 4) .. + 3 of the
 // first tile, 2 and 3 of the second.
@@ -278,11 +290,6 @@ struct Queries {
   float sum[S::GROUPS][S::NT][2];
 };
 
-__device__ __forceinline__ uint32_t by16(uint32_t two) {
-  const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&two), __float2half2_rn(16.f));
-  return *reinterpret_cast<const uint32_t*>(&y);
-}
-
 template <typename S>
 __device__ __forceinline__ void load_queries(const QuantDecParams& p, int b, int item, int lane, Queries<S>& q) {
   const int r = lane >> 2, c = lane & 3, h = item / p.blocks, first = (item - h * p.blocks) * S::HEADS;
@@ -332,8 +339,8 @@ __device__ __forceinline__ void load_queries(const QuantDecParams& p, int b, int
         f0[0] = __byte_perm(x[0], x[1], 0x5410); f0[1] = __byte_perm(x[0], x[1], 0x7632);
         f1[0] = __byte_perm(x[2], x[3], 0x5410); f1[1] = __byte_perm(x[2], x[3], 0x7632);
       } else {
-        f0[0] = by16(__byte_perm(x[0], x[2], 0x5410)); f0[1] = __byte_perm(x[0], x[2], 0x7632);
-        f1[0] = by16(__byte_perm(x[1], x[3], 0x5410)); f1[1] = __byte_perm(x[1], x[3], 0x7632);
+        f0[0] = __byte_perm(x[0], x[2], 0x5410); f0[1] = __byte_perm(x[0], x[2], 0x7632);
+        f1[0] = __byte_perm(x[1], x[3], 0x5410); f1[1] = __byte_perm(x[1], x[3], 0x7632);
       }
     }
     const float mine = up * p.scale_log2 * (1.f / S::K_UNIT);
@@ -473,8 +480,8 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uin
           for (int nt = 0; nt < S::NT; ++nt) mma(acc[nt], lo0, lo1, hi0, hi1, q.f[nt][j][0], q.f[nt][j][1]);
         } else {
           uint32_t x0[4], x1[4];
-          widen8(w[0][j], x0);
-          widen8(w[1][j], x1);
+          widen8_high(w[0][j], x0);
+          widen8_high(w[1][j], x1);
           const int k = 2 * (g * KWORDS + j);
 #pragma unroll
           for (int nt = 0; nt < S::NT; ++nt) {
@@ -1084,7 +1091,7 @@ cudaError_t launch_both(const QuantDecParams& p, cudaStream_t stream) {
   if (cudaError_t e = smem_opt_in(kern, S::SMEM, opted_in); e != cudaSuccess) return e;
   if (p.cluster) return launch_early(kern, (unsigned)(p.batch * p.items * p.cluster), S::THREADS, S::SMEM, stream, p.cluster, p);
   cudaError_t e = launch_early(kern, (unsigned)p.ctas, S::THREADS, S::SMEM, stream, 1, p);
-  if (e != cudaSuccess || p.ctas == 1) return e;
+  if (e != cudaSuccess) return e;
   return launch_early(quant_merge_kernel<S::HD, S::HEADS, S::HALF>, (unsigned)(p.ctas * SLICES), MERGE_THREADS, 0, stream, 1, p);
 }
 

@@ -212,6 +212,20 @@ def test_size_of_values(kind, factor):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,group", [("int8", 64), ("e4m3", 64), ("int4", 64), ("int4", 32)])
+def test_log_sum_exps_of_few_keys_are_fp32(kind, group):
+    """The root mean square of what 2400 of them are off by: four roundings of 2^-24 (row scales, softmax scale, exponentials' sum, its logarithm) of
+    their own size, and the sum over columns, which the matrix instruction takes sixteen at a time: 2^-22 in all."""
+    import flash_sparse_attn as fsa
+
+    q, (k, v, ks, vs) = normal(1, 300, 8, 64), make_cache(2, 300, 2, 2, 64, kind, group)
+    _, lse = fsa.flash_dense_attn_with_quantized_kvcache_func(q, k, v, ks, vs, return_lse=True)
+    done()
+    want = reference(q, list(values(k, ks)), list(values(v, vs)), 0.125)[1]
+    assert (lse.double().cpu() - want).norm() <= 2.0**-22 * want.norm()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["int8", "int4", "e4m3"])
 def test_values_near_the_top_of_bf16(kind):
     """Values around 2^113: the same numbers as small ones in other units."""
