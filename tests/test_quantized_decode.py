@@ -146,6 +146,8 @@ def test_ways_that_work_is_shared_out(kind):
     run([0] * 7, 8, 2, 128, kind)                           # nothing
     run([100] * 2000, 2, 1, 64, kind, twice=False)          # more sequences than lanes, many each
     run([9000, 4] + [0] * 30, 4, 4, 64, kind, page=256)
+    run([(7 * i) % 41 for i in range(1500)], 1, 1, 64, kind, twice=False)  # lengths read side by side
+    run([0] * 300 + [6000] + [0] * 33, 2, 1, 64, kind)      # one among many without a key
     run([3], 4, 1, 64, kind, capacity=5000)                 # room for more than there is
 
 
