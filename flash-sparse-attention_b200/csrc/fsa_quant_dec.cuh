@@ -6,9 +6,10 @@
 //   o_h  = sum_j p_jh b_j v^_j / sum_j p_jh,  p_jh = 2^(s_jh - m_h)
 // so no value is ever rounded on its way: codes are exact in fp16, products and sums are those of the matrix instructions in fp32, scales are
 // applied to scores and to probabilities. The queries enter as fp16 too: a row is multiplied by a power of two that brings its largest element
-// to [2^10, 2^11) (exact but for elements 2^-24 and more below it, which lose less than 2^-34 of the largest), probabilities times b_j times a power
-// of two that keeps them in range are rounded to fp16 (2^-11; of fp16 results what that leaves goes in as well). Running maxima, sums and outputs
-// are fp32.
+// to [2^10, 2^11) (exact but for elements 2^-24 and more below it, which lose less than 2^-34 of the largest), probabilities times b_j are rounded to
+// fp16 (2^-12 of each; of fp16 results what that leaves goes in as well) in a unit of each head and group of columns that follows the largest of
+// these products so far, so that what a key adds is held by what it weighs: a large b_j that nobody attends to, a key far above the others without a
+// value, or a group of small columns beside large ones take nothing from the rest. Running maxima, sums and outputs are fp32.
 //
 // Bound by memory: a key is read once, at 2 * 8 * (heads per KV head) operations a byte. (int8, 64 chats of up to 8192 tokens: 100.4 us, 5.3 TB/s, 0.82 of a
 // copy's rate; 4 bits, 8 x 100000: 112 us, 3.95 TB/s, where instructions bound it, 630 a tile; one sequence of 2001 keys 6.8 us.) What a warp does with a tile of 32 keys has to fit
@@ -42,8 +43,13 @@ namespace fsa {
 constexpr int TILE = QUANT_TILE;
 constexpr uint32_t ALL = 0xffffffffu;
 constexpr int STATUS_WAIT = 1, STATUS_BAD_PAGE = 3;
-constexpr float LAG = 6.f;           // how far (base 2) a score may be above the reference maximum before that moves
-constexpr float MOST_SCALE = 512.f;  // and a value scale above 1: 2^6 * 2^9 is within fp16
+constexpr float LAG = 6.f;  // how far (base 2) a score may be above the reference maximum before that moves
+// Units of a probability times a value scale as fp16: where one is chosen, the largest product is brought to [2^8, 2^9), and products may grow to fp16's
+// end before it is chosen anew (2^6 of that are the lag's). What fp16 loses below its normal numbers is then at most 2^-33 of the largest for each key.
+// (One unit for all heads and groups, chosen by scales alone, costs 2 us less of 35 with four groups and nothing to speak of with one or two, but rounds
+// away what lies 2^-14 below a scale that nobody attends to.)
+constexpr int UNIT_TO = 8;
+constexpr float FINEST = 8.507059173023462e37f;  // 2^126
 
 template <int HD_, int FMT_, int GROUPS_, int NT_, bool HALF_>
 struct Shape {
@@ -96,6 +102,11 @@ __device__ __forceinline__ void add2(float* d, const float* a) {
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ float inverse_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -365,7 +376,9 @@ struct State {
   float o[S::MTILES][S::NT][4];
   float centre[S::INT4 ? S::GROUPS : 1][S::NT][2];  // sum p z of this lane's keys
   float m[S::NT][2], l[S::NT][2];                   // reference maximum; sum of this lane's keys
-  float v_inv;                                      // power of two that value scales are multiplied by; 0: none chosen yet
+  // What probabilities times value scales are multiplied by, and outputs with them: of each head, as what a key weighs is its probability times its
+  // scale, neither alone; and of each group of columns, whose scales need not be alike.
+  float unit[S::GROUPS][S::NT][2];
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int nt = 0; nt < S::NT; ++nt) {
@@ -379,28 +392,30 @@ struct State {
         l[nt][x] = 0.f;
 #pragma unroll
         for (int g = 0; g < (S::INT4 ? S::GROUPS : 1); ++g) centre[g][nt][x] = 0.f;
+#pragma unroll
+        for (int g = 0; g < S::GROUPS; ++g) unit[g][nt][x] = FINEST;
       }
     }
-    v_inv = 0.f;
   }
 };
 
 __device__ __forceinline__ float scale_of(uint32_t word, bool int4) { return __uint_as_float(int4 ? word << 16 : word); }
 __device__ __forceinline__ float centre_of(uint32_t word) { return __uint_as_float(word & 0xffff0000u); }
 
-// Moves the reference maxima to what the tile brings, and the power of two of the value scales.
 template <typename S>
-__device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[S::NT][4], float most_scale) {
+__device__ __forceinline__ void scale_outputs(State<S>& st, int g, int nt, int x, float by) {
 #pragma unroll
-  for (int d = 4; d < 32; d <<= 1) most_scale = fmaxf(most_scale, __shfl_xor_sync(0xffffffffu, most_scale, d));
-  float ratio = 1.f;
-  if (st.v_inv == 0.f || most_scale * st.v_inv > MOST_SCALE) {
-    int e = (int)(__float_as_uint(most_scale) >> 23) - 127;
-    e = min(max(e, -126), 126);
-    const float now = __uint_as_float((uint32_t)(127 - e) << 23);
-    if (st.v_inv != 0.f) ratio = now / st.v_inv;  // both powers of two
-    st.v_inv = now;
+  for (int t = g * (S::MTILES / S::GROUPS); t < (g + 1) * (S::MTILES / S::GROUPS); ++t) {
+    st.o[t][nt][x] *= by;
+    st.o[t][nt][x + 2] *= by;
   }
+}
+
+// Moves the reference maxima to what the tile brings. What has been added up shrinks by as much: the units take that up, so that sums of products stay
+// as they are and later keys are held as finely as they deserve.
+template <typename S>
+__device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[S::NT][4]) {
+  bool beyond = false;
 #pragma unroll
   for (int nt = 0; nt < S::NT; ++nt) {
 #pragma unroll
@@ -409,16 +424,54 @@ __device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[S:
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
       m = fmaxf(m, st.m[nt][x]);
-      const float by = m == -CUDART_INF_F ? 1.f : exp2_fast(st.m[nt][x] - m);
+      const bool first = st.m[nt][x] == -CUDART_INF_F;  // nothing has been added up
+      const float down = m == -CUDART_INF_F ? 0.f : st.m[nt][x] - m, by = exp2_fast(down), back = exp2_fast(-down);
       st.m[nt][x] = m;
       st.l[nt][x] *= by;
 #pragma unroll
       for (int g = 0; g < (S::INT4 ? S::GROUPS : 1); ++g) st.centre[g][nt][x] *= by;
 #pragma unroll
-      for (int t = 0; t < S::MTILES; ++t) {
-        st.o[t][nt][x] *= by * ratio;
-        st.o[t][nt][x + 2] *= by * ratio;
+      for (int g = 0; g < S::GROUPS; ++g) {
+        if (!first) st.unit[g][nt][x] *= back;
+        beyond = beyond || !(st.unit[g][nt][x] <= FINEST);
       }
+    }
+  }
+  if (__any_sync(ALL, beyond)) {
+#pragma unroll
+    for (int g = 0; g < S::GROUPS; ++g)
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float unit = st.unit[g][nt][x];
+          // (of an infinite one nothing is left: what has been added up is 2^-126 of what the tile brings, and less)
+          scale_outputs<S>(st, g, nt, x, unit <= FINEST ? 1.f : FINEST * inverse_fast(unit));
+          st.unit[g][nt][x] = fminf(unit, FINEST);
+        }
+  }
+}
+
+// Chooses the units of group g by the tile's largest products of a probability and a value scale. (Their exponents are what counts: two heads a word.)
+template <typename S>
+__device__ __forceinline__ void choose_unit(State<S>& st, int g, const float (*e)[S::NT][4], const uint32_t (*b_words)[S::GROUPS]) {
+#pragma unroll
+  for (int nt = 0; nt < S::NT; ++nt) {
+    float most[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) most[x] = fmaxf(most[x], e[i >> 1][nt][x + 2 * (i & 1)] * scale_of(b_words[i][g], S::INT4));
+    uint32_t both = __byte_perm(__float_as_uint(most[0]), __float_as_uint(most[1]), 0x7632);
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, d));
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float old = st.unit[g][nt][x];
+      const uint32_t exponent = max(both >> (7 + 16 * x) & 0xffu, 128u + UNIT_TO - 127u);  // (no unit above FINEST)
+      const float unit = fminf(old, __uint_as_float((254u + UNIT_TO - exponent) << 23));
+      scale_outputs<S>(st, g, nt, x, unit < old ? unit * inverse_fast(old) : 1.f);
+      st.unit[g][nt][x] = unit;
     }
   }
 }
@@ -536,13 +589,8 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uin
 #pragma unroll
     for (int x = 0; x < 2; ++x)
       move = move || fmaxf(fmaxf(s[0][nt][x], s[0][nt][x + 2]), fmaxf(s[1][nt][x], s[1][nt][x + 2])) > st.m[nt][x] + LAG;
-  float most_scale = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int g = 0; g < S::GROUPS; ++g) most_scale = fmaxf(most_scale, scale_of(b_words[i][g], S::INT4));
-  move = move || most_scale * st.v_inv > MOST_SCALE;
-  if (__any_sync(ALL, move)) move_reference<S>(st, s, most_scale);
+  const bool moved = __any_sync(ALL, move);
+  if (moved) move_reference<S>(st, s);
 
   // ---- probabilities -------------------------------------------------------------------------------------------------
 #pragma unroll
@@ -568,25 +616,52 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uin
   const int v_row = 16 * (lane >> 4) + 2 * (kappa >> 2) + (first & 1) + 8 * (second & 1);
   const uint32_t values = smem_u32(stage + S::TILE_BYTES) + place_of<S>(v_row, 0);
   constexpr int PIECES = S::CH / S::GROUPS;  // of sixteen bytes, of a group
+  // Probabilities times scales, of fp16 results with what the rounding to fp16 leaves (else it would be as large as the result's own); of several groups
+  // at a time, as far as registers go, since a vote is a wait.
+  constexpr int FIT = 4 / (S::NT * (S::HALF ? 2 : 1)), AT_ONCE = S::GROUPS < FIT ? S::GROUPS : FIT;
+  uint32_t pb_of[AT_ONCE][2][S::NT][2], rest_of[AT_ONCE][2][S::HALF ? S::NT : 1][2];
 #pragma unroll
   for (int g = 0; g < S::GROUPS; ++g) {
-    if (S::GS == 32 && g >= groups) continue;
-    // Probabilities times scales, of fp16 results with what the rounding to fp16 leaves (else it would be as large as the result's own).
-    uint32_t pb[2][S::NT][2], rest[2][S::HALF ? S::NT : 1][2];
+    if (g % AT_ONCE == 0) {
+      auto products = [&]() {  // whether one of them is beyond fp16 (or their sum, or is no number)
+        __half2 sum = __float2half2_rn(0.f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float by = scale_of(b_words[i][g], S::INT4) * st.v_inv;
+        for (int k = 0; k < AT_ONCE; ++k)
 #pragma unroll
-      for (int nt = 0; nt < S::NT; ++nt) {
-        const float x = s[i >> 1][nt][2 * (i & 1)] * by, y = s[i >> 1][nt][2 * (i & 1) + 1] * by;
-        const uint32_t two = pack2<__half>(x, y);
-        pb[i >> 1][nt][i & 1] = transposed(two);
-        if constexpr (S::HALF) {
-          const __half2 h = *reinterpret_cast<const __half2*>(&two);
-          rest[i >> 1][nt][i & 1] = transposed(pack2<__half>(x - __low2float(h), y - __high2float(h)));
-        }
+          for (int i = 0; i < 4; ++i) {
+            const float by = scale_of(b_words[i][g + k], S::INT4);
+#pragma unroll
+            for (int nt = 0; nt < S::NT; ++nt) {
+              const float x = s[i >> 1][nt][2 * (i & 1)] * by * st.unit[g + k][nt][0], y = s[i >> 1][nt][2 * (i & 1) + 1] * by * st.unit[g + k][nt][1];
+              const uint32_t two = pack2<__half>(x, y);
+              const __half2 h = *reinterpret_cast<const __half2*>(&two);
+              sum = __hadd2(sum, h);
+              pb_of[k][i >> 1][nt][i & 1] = two;
+              if constexpr (S::HALF) rest_of[k][i >> 1][nt][i & 1] = pack2<__half>(x - __low2float(h), y - __high2float(h));
+            }
+          }
+        return ((*reinterpret_cast<const uint32_t*>(&sum) & 0x7fff7fffu) + 0x04000400u & 0x80008000u) != 0;
+      };
+      bool choose = moved;
+      if (!choose) choose = __any_sync(ALL, products());
+      if (choose) {
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) choose_unit<S>(st, g + k, s, b_words);
+        products();
       }
     }
+    if (S::GS == 32 && g >= groups) continue;
+    uint32_t (&pb)[2][S::NT][2] = pb_of[g % AT_ONCE];
+    uint32_t (&rest)[2][S::HALF ? S::NT : 1][2] = rest_of[g % AT_ONCE];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          pb[half][nt][i] = transposed(pb[half][nt][i]);
+          if constexpr (S::HALF) rest[half][nt][i] = transposed(rest[half][nt][i]);
+        }
     if constexpr (S::ADDED != 0.f) {
       // less what was added to the codes: the same products with that, which no rounding of probabilities changes; columns of a group share them
       constexpr uint32_t LESS0 = S::INT4 ? 0x80088008u : 0x80808080u, LESS1 = 0x80808080u;
@@ -639,7 +714,6 @@ __device__ __forceinline__ void take_tile(State<S>& st, const Queries<S>& q, uin
 // Sums over the lanes that share heads, and the outputs in the values' own units, two neighbouring columns in each pair (column_of).
 template <typename S>
 __device__ __forceinline__ void settle(State<S>& st, int lane) {
-  const float by = st.v_inv == 0.f ? 1.f : 1.f / st.v_inv;
 #pragma unroll
   for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
@@ -654,6 +728,7 @@ __device__ __forceinline__ void settle(State<S>& st, int lane) {
       }
 #pragma unroll
       for (int t = 0; t < S::MTILES; ++t) {
+        const float by = inverse_fast(st.unit[t / (S::MTILES / S::GROUPS)][nt][x]);
         const float z = S::INT4 ? st.centre[S::INT4 ? t / (S::GS / 16) : 0][nt][x] : 0.f;
         // (one after the other: of values from 2^111 on their product is beyond fp32)
         float a = fmaf(st.o[t][nt][x] * (1.f / S::UNIT), by, z), b = fmaf(st.o[t][nt][x + 2] * (1.f / S::K_UNIT), by, z);
