@@ -873,14 +873,17 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
   }
   if (tid == 0) abort_s = 0;
   if (tid < 3) pieces_s[tid] = 0;
+  if (tid < 2 * S::WARPS) part_s[tid >> 1][tid & 1] = reinterpret_cast<const float*>(smem + (tid >> 1) * S::RING);
   mbar_fence_init();
   __syncthreads();
 
   // ---- where this warp begins ------------------------------------------------------------------------------------------
   // The first `warps` warps of the grid have equal pieces of the list, of at least a tile; the others none. Every warp adds up the
   // lengths by itself, a lane those of neighbouring sequences: no warp waits for another before it has its first tiles under way.
-  // (Lengths are read more than once. Should someone write them meanwhile, which spoils the results, every index still stays in bounds and every
-  // loop ends.)
+  // (Should someone write lengths meanwhile, which spoils the results, every index still stays in bounds and every loop ends. A cluster's warp reads its
+  // sequence's once, so that it has no more than one piece, which its ring holds. In the list a warp reads them more than once and may come to another
+  // cut than its neighbour: its walk ends by its own count, behind the last sequence there are no keys, and pieces that a neighbour expects and nobody
+  // wrote are looked for where there is memory.)
   const long long g_warp = (long long)blockIdx.x * S::WARPS + warp;
   Walk<GATHER> walk;
   int mine = 0;
@@ -889,12 +892,8 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
     const int n = (int)blockIdx.x / p.cluster, w = warp * p.cluster + (int)blockIdx.x % p.cluster;
     walk.b = n / p.items;
     walk.i = n - walk.b * p.items;
-    const int tiles = tiles_of(GATHER ? p.topk : keys_of(p, walk.b)), warps = min(tiles, p.cluster * S::WARPS);
-    if (w < warps) {
-      const int each = tiles / warps, more = tiles - each * warps;
-      walk.t = each * w + more * w / warps;
-      mine = each * (w + 1) + more * (w + 1) / warps - walk.t;
-    }
+    walk.sequence(p);
+    mine = quant_cluster_share(walk.tiles, p.cluster * S::WARPS, w, &walk.t);
   } else {
     auto tiles_at = [&](int b) { return tiles_of(GATHER ? p.topk : keys_of(p, b)); };
     const bool alike = GATHER || !p.used;
@@ -994,7 +993,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) quant_decode_kernel(const __gri
   uint8_t* extras = ring + S::STAGES * S::CODES;
   float* own_pieces = p.pieces + (long long)blockIdx.x * 2 * S::PIECE;
   if (mine > 0) {
-    walk.sequence(p);
+    if (!p.cluster) walk.sequence(p);
     walk.left = max(walk.tiles - walk.t, 1);
     int sent = 0, into = 0, chosen_next = -1;  // into: the stage that the next copies take
     Place place;

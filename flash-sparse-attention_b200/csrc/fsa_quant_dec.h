@@ -8,6 +8,7 @@
 #include <type_traits>
 
 #include "fsa_quant_cache.h"
+#include "fsa_quant_share.h"
 
 namespace fsa {
 
