@@ -194,9 +194,9 @@ def append_kv_quantized(query: Optional[torch.Tensor], key_new: torch.Tensor, va
     if not key_new.is_cuda:
         raise RuntimeError("flash_sparse_attn (B200 build) only runs on CUDA tensors; there is no CPU path")
     sections = None if sections is None else tuple(sections)
-    host = _lib.native()
+    axes = sections is not None and isinstance(cos, torch.Tensor) and cos.ndim == 2
+    host = _lib.native() if axes or sections is None else None  # (sections without tables are for the checks below to refuse)
     if host is not None:
-        axes = sections is not None and isinstance(cos, torch.Tensor) and cos.ndim == 2
         res = host.append_quantized(query, key_new, value_new, key_cache, value_cache, key_scales, value_scales, seqused_k, cos, sin, page_table,
                                     free_pages, free_count, cu_seqlens_new, seqlen_offsets, position_ids,
                                     axis_bits(sections, cos.shape[1], bool(axes_dealt)) if axes else None, len(sections) if axes else 0,

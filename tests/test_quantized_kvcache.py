@@ -434,6 +434,26 @@ def test_autograd_notices_what_was_written():
     assert used.item() == 1
 
 
+@pytest.mark.gpu
+def test_axes_without_tables_or_positions_are_refused():
+    """Both launchers: axes belong to tables and positions, neither goes without the others."""
+    from flash_sparse_attn.utils.kvcache import append_kv_quantized, empty_kv_quantized
+
+    cos, sin = tables(9, 32)
+    k, ids = normal(1, 2, 1, 2, 64), torch.zeros(2, 2, 1, dtype=torch.int32, device=DEV)
+    cache, used = empty_kv_quantized(2, 10, 2, 64), torch.zeros(2, dtype=torch.int32, device=DEV)
+    append_kv_quantized(None, k, k, *cache, used, cos, sin, position_ids=ids, sections=[16, 16])  # (which a native launcher wants to have seen)
+    done()
+    assert used.tolist() == [1, 1]
+    kept = [t.clone() for t in cache]
+    for kw in (dict(sections=(16, 16)), dict(sections=[16, 16], position_ids=ids), dict(position_ids=ids), dict(cos=cos, sin=sin, sections=(16, 16)),
+               dict(cos=cos, sin=sin, position_ids=ids), dict(sin=sin, sections=(16, 16), position_ids=ids), dict(cos=cos, sections=(16, 16), position_ids=ids)):
+        with pytest.raises(AssertionError):
+            append_kv_quantized(None, k, k, *cache, used, **kw)
+    done()
+    assert used.tolist() == [1, 1] and all(torch.equal(a, b) for a, b in zip(cache, kept))
+
+
 def test_refusals_on_the_cpu():
     from flash_sparse_attn import _lib
     from flash_sparse_attn.utils import quantized_kvcache as m
