@@ -73,6 +73,8 @@ class FlashSparseAttention(nn.Module):
         """``rotary``: the tables ``(cos, sin)`` of ``apply_rotary_func``; queries and keys are then turned by their positions (or by
         ``position_ids``), and the keys that are returned are the turned ones. With ``rotary_sections`` (and ``rotary_axes_dealt``) the
         positions have several axes, ``position_ids [axes, batch, positions]``: the step is then ``apply_rotary_axes_func``."""
+        assert rotary is not None or rotary_sections is None, "rotary_sections belong to rotary: without tables nothing is turned"
+        assert rotary_sections is not None or not rotary_axes_dealt, "rotary_axes_dealt belongs to rotary_sections"
         bsz, seq_len, _ = hidden_states.size()
         query_states = self.q_proj(hidden_states).view(bsz, seq_len, self.num_attention_heads, self.head_dim)
         key_states = self.k_proj(hidden_states).view(bsz, seq_len, self.num_key_value_heads, self.head_dim)

@@ -71,3 +71,13 @@ def test_layer_calls_the_operator(monkeypatch):
     assert seen["tables"] == ("cos", "sin") and seen["ids"] == "ids" and seen["sections"] == (4, 4)
     assert seen["axes_dealt"] is True and seen["interleaved"] is False
     assert (seen["q"] == 1).all() and (keys == 2).all()
+
+
+def test_layer_refuses_axes_that_turn_nothing():
+    from flash_sparse_attn.modules.flash_sparse_attention import FlashSparseAttention, FlashSparseAttentionConfig
+
+    layer, x = FlashSparseAttention(FlashSparseAttentionConfig(64, 4, 2, 16)), torch.zeros(1, 3, 64)
+    for kw in (dict(rotary_sections=(4, 4)), dict(rotary_sections=(4, 4), position_ids=torch.zeros(2, 1, 3, dtype=torch.int32)),
+               dict(rotary=(torch.ones(4, 8), torch.ones(4, 8)), rotary_axes_dealt=True), dict(rotary_axes_dealt=True)):
+        with pytest.raises(AssertionError, match="belong"):
+            layer(x, **kw)
