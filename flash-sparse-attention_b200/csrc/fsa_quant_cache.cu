@@ -87,7 +87,9 @@ __device__ __forceinline__ Pair4 group_pair(float low, float high) {
   const float width = __fdiv_rn(__fsub_rn(0.5f * high, 0.5f * low), 7.5f);  // (halves: the difference may be beyond fp32)
   float s = __bfloat162float(__float2bfloat16_rn(width));
   if (s < TINY) s = 0.f;
-  p.z = __bfloat162float(__float2bfloat16_rn(__fadd_rn(low, 8.f * s)));
+  // (of extremes near the end of fp32 8 s is beyond it, its sum with the least number is not)
+  const float z = s < 1.3292279957849159e36f ? __fadd_rn(low, 8.f * s) : 2.f * __fadd_rn(0.5f * low, 4.f * s);  // (2^120)
+  p.z = __bfloat162float(__float2bfloat16_rn(z));
   p.inverse = s > 0.f ? __frcp_rn(s) : 0.f;
   p.word = (__float_as_uint(s) >> 16) | (__float_as_uint(p.z) & 0xffff0000u);
   if (!(s < INFINITY) || !(fabsf(p.z) < INFINITY)) {  // an infinity or a NaN among the values

@@ -312,6 +312,35 @@ def test_rows_from_end_to_end_of_bf16(kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64])
+def test_four_bits_up_to_the_largest_number_of_bf16(group):
+    """Groups from -a to a, a up to the type's largest: 8 s is beyond fp32 from 0.94 of that on. Scale, middle and codes are those of the definition in 64
+    bits; nothing reads back as NaN or infinity. (The largest, 15 s - a for s rounded up by up to 2^-9, stays below where bf16 rounds to infinity for
+    these a.)"""
+    from flash_sparse_attn.utils.kvcache import append_kv_quantized, empty_kv_quantized, read_kv_quantized
+
+    top = torch.finfo(torch.bfloat16).max
+    a = torch.tensor([top, 3.35e38, 3.25e38, 3.2e38, 3.18e38, 1e38, 2.0**120, 2.0**119], dtype=torch.float64)
+    x = (torch.linspace(-1, 1, group, dtype=torch.float64).repeat(64 // group)[None] * a[:, None]).to(torch.bfloat16).to(DEV)
+    cache, used = empty_kv_quantized(1, 8, 1, 64, torch.uint8, group), torch.zeros(1, dtype=torch.int32, device=DEV)
+    append_kv_quantized(None, x.view(1, 8, 1, 64), x.flip(-1).view(1, 8, 1, 64), *cache, used)
+    got = read_kv_quantized(*cache, used, max_seqlen=8)
+    done()
+    for codes, scales, rows, values16 in ((cache[0], cache[2], x, got[0]), (cache[1], cache[3], x.flip(-1), got[1])):
+        g = rows.double().cpu().unflatten(-1, (-1, group))
+        low, high = g.amin(-1), g.amax(-1)
+        s = ((high - low) / 15).float().to(torch.bfloat16)
+        z = (low + 8 * s.double()).float().to(torch.bfloat16)
+        assert torch.equal(bits(scales[0, :, 0]), bits(torch.stack([s, z], -1)))
+        n = ((g - z.double()[..., None]) / s.double()[..., None]).round().clamp(-8, 7).flatten(-2) + 8
+        kept = torch.stack([codes & 15, codes >> 4], -1).flatten(-2)[0, :, 0].cpu()
+        assert ((kept.double() - n).abs() <= 1).all() and (kept == n).double().mean() > 0.95  # (ties, by products with 1 / s)
+        assert values16.isfinite().all()
+        step = s.double()[..., None] * (0.5 + 15 * 2.0**-8) * 1.01 + 2.0**-8 * high[..., None].abs() * 1.01  # as for special rows
+        assert ((values16[0, :, 0].double().cpu().unflatten(-1, (-1, group)) - g).abs() <= step + 2.0**-8 * g.abs()).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("kind,d,group", FORMS)
 def test_reading_back(kind, d, group, dtype):
