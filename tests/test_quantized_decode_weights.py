@@ -7,8 +7,8 @@ import math
 import pytest
 import torch
 
-from test_quantized_decode import FORMS
-from test_quantized_kvcache import KINDS, quantised
+from test_quantized_decode import FORMS, reference
+from test_quantized_kvcache import KINDS, make_cache, quantised, values
 from test_rotary import done, normal
 
 DEV = "cuda"
@@ -138,3 +138,55 @@ def test_groups_of_columns_of_very_different_size(d, group, dtype):
         v[..., columns] *= 2.0**-20
         out, _, ref, _, _, reach = attend(q, xk, v, "int4", group, scale)
         rows_close(out, ref, dtype, score_error(d, reach), columns)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [20000, 70001])
+@pytest.mark.parametrize("kind,d,group", [("int8", 128, 64), ("int4", 128, 64), ("int4", 96, 32), ("e4m3", 64, 64)])
+def test_every_tile_of_a_long_sequence_counts(kind, d, group, n):
+    """Values that average out: the result is far smaller than they are, and so is what it may be off by. bf16's rounding 2^-9, probabilities' 2^-12, the
+    matrix instructions' at most 2^-8 (2^-14 of a code's step a key where a subnormal's exponent is taken for its size, all to one side: of the
+    result's 4.6 steps / sqrt(n) in 4 bits 2^-8.2); 2^-7 in all. One tile of 32 rows that is not the right one is sqrt(64 / n), 0.03 and more, off."""
+    import flash_sparse_attn as fsa
+
+    q, cache = normal(5, 1, 8, d), make_cache(6, 1, n, 2, d, kind, group)
+    out = fsa.flash_dense_attn_with_quantized_kvcache_func(q, *cache)
+    done()
+    keys, vals = values(cache[0], cache[2])[0], values(cache[1], cache[3])[0]
+    ref = reference(q, [keys], [vals], d**-0.5)[0]
+    size = ref.norm(dim=-1)
+    assert ((out.double().cpu() - ref).norm(dim=-1) <= 2.0**-7 * size).all()
+    for tile in (0, n // 64, n // 32 - 1):  # what the bound has to see
+        wrong = vals.clone()
+        wrong[32 * tile:32 * tile + 32] = vals[:32].flip(0) if tile else vals[-32:]
+        assert ((reference(q, [keys], [wrong], d**-0.5)[0] - ref).norm(dim=-1) > 2.0**-7 * size).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,d,group", [("int8", 128, 64), ("int4", 128, 32), ("e4m3", 64, 64)])
+@pytest.mark.parametrize("chosen", [0, 9000])
+def test_every_page_of_long_sequences_counts(kind, d, group, chosen):
+    """The same for pages in any order, of sequences of several lengths, and for positions chosen among them: a page of values in another's place shows."""
+    import flash_sparse_attn as fsa
+
+    page, lens, g = 64, [20011, 4096, 11000], torch.Generator().manual_seed(3)
+    slots = -(-max(lens) // page)
+    table = torch.randperm(3 * slots + 2, generator=g)[:3 * slots].view(3, slots)
+    q, cache = normal(5, 3, 8, d), make_cache(6, 3 * slots + 2, page, 2, d, kind, group)
+    kw, pick = {}, [torch.arange(n) for n in lens]
+    if chosen:
+        at = torch.stack([torch.randperm(slots * page, generator=g)[:chosen].sort().values for _ in lens])
+        kw["gather_kv_indices"], pick = at.to(torch.int32).to(DEV), [a[a < n] for a, n in zip(at, lens)]
+    out = fsa.flash_dense_attn_with_quantized_kvcache_func(q, *cache, page_table=table.to(torch.int32).to(DEV),
+                                                           seqused_k=torch.tensor(lens, dtype=torch.int32, device=DEV), **kw)
+    done()
+    pool = [values(cache[i], cache[2 + i]) for i in range(2)]
+    keys, vals = ([x[table[i]].flatten(0, 1)[at] for i, at in enumerate(pick)] for x in pool)
+    ref = reference(q, keys, vals, d**-0.5)[0]
+    size = ref.norm(dim=-1)
+    assert ((out.double().cpu() - ref).norm(dim=-1) <= 2.0**-7 * size).all()
+    other = table.clone()
+    other[:, [0, -1]] = table[:, [1, 2]]
+    other[:, lens[1] // page - 1] = table[:, 5]
+    wrong = [pool[1][other[i]].flatten(0, 1)[at] for i, at in enumerate(pick)]
+    assert ((reference(q, keys, wrong, d**-0.5)[0] - ref).norm(dim=-1) > 2.0**-7 * size).all()
