@@ -14,9 +14,13 @@ from flash_sparse_attn.ops.triton.rotary import _rows, _strides, _unseen, check_
 _F16 = (torch.float16, torch.bfloat16)
 
 
-@lru_cache(maxsize=256)
 def axis_bits(sections: Tuple[int, ...], pairs: int, dealt: bool) -> bytes:
     """The axis of every pair, two bits each (eight words), for ``sections[a]`` pairs of axis a: run after run, or dealt out in turn."""
+    return _axis_bits(pairs, dealt, *sections)
+
+
+@lru_cache(maxsize=256, typed=True)  # (each number by itself: 16.0 is not taken for the 16 of an earlier call)
+def _axis_bits(pairs, dealt, *sections):
     assert 2 <= len(sections) <= _lib.MAX_AXES, f"sections must name two to {_lib.MAX_AXES} axes"
     assert all(type(n) is int and n > 0 for n in sections) and sum(sections) == pairs, "sections must be positive and add up to rotary_dim / 2"
     assert pairs <= 128, "rotary_dim must be less than or equal to 256"

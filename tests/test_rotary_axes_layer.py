@@ -81,3 +81,12 @@ def test_layer_refuses_axes_that_turn_nothing():
                dict(rotary=(torch.ones(4, 8), torch.ones(4, 8)), rotary_axes_dealt=True), dict(rotary_axes_dealt=True)):
         with pytest.raises(AssertionError, match="belong"):
             layer(x, **kw)
+
+
+def test_sections_are_whole_numbers_whatever_was_called_before():
+    from flash_sparse_attn.ops.triton.rotary_axes import axis_bits
+
+    assert axis_bits((1, 31), 32, False) == axis_bits((1, 31), 32, False)
+    for bad in ((1.0, 31), (True, 31), (1, 31.0)):
+        with pytest.raises(AssertionError):
+            axis_bits(bad, 32, False)
