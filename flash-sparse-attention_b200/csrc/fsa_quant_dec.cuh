@@ -7,7 +7,7 @@
 // so no value is ever rounded on its way: codes are exact in fp16, products and sums are those of the matrix instructions in fp32, scales are
 // applied to scores and to probabilities. The queries enter as fp16 too: a row is multiplied by a power of two that brings its largest element
 // to [2^10, 2^11) (exact but for elements 2^-24 and more below it, which lose less than 2^-34 of the largest), probabilities times b_j are rounded to
-// fp16 (2^-12 of each; of fp16 results what that leaves goes in as well) in a unit of each head and group of columns that follows the largest of
+// fp16 (2^-11 of each; of fp16 results what that leaves goes in as well) in a unit of each head and group of columns that follows the largest of
 // these products so far, so that what a key adds is held by what it weighs: a large b_j that nobody attends to, a key far above the others without a
 // value, or a group of small columns beside large ones take nothing from the rest. Running maxima, sums and outputs are fp32.
 //
