@@ -43,7 +43,9 @@ namespace fsa {
 constexpr int TILE = QUANT_TILE;
 constexpr uint32_t ALL = 0xffffffffu;
 constexpr int STATUS_WAIT = 1, STATUS_BAD_PAGE = 3;
-constexpr float LAG = 6.f;  // how far (base 2) a score may be above the reference maximum before that moves
+// How far (base 2) a score may be above the reference maximum before that moves. (What lies 2^-126 below the reference is lost in fp32: of probabilities
+// below 2^-120 of the largest some count as none.)
+constexpr float LAG = 6.f;
 // Units of a probability times a value scale as fp16: where one is chosen, the largest product is brought to [2^8, 2^9), and products may grow to fp16's
 // end before it is chosen anew (2^6 of that are the lag's). What fp16 loses below its normal numbers is then at most 2^-33 of the largest for each key.
 // (One unit for all heads and groups, chosen by scales alone, costs 2 us less of 35 with four groups and nothing to speak of with one or two, but rounds
@@ -415,6 +417,7 @@ __device__ __forceinline__ void scale_outputs(State<S>& st, int g, int nt, int x
 // as they are and later keys are held as finely as they deserve.
 template <typename S>
 __device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[S::NT][4]) {
+  float by[S::NT][2], back[S::NT][2];  // back: 1 where nothing has been added up
   bool beyond = false;
 #pragma unroll
   for (int nt = 0; nt < S::NT; ++nt) {
@@ -424,32 +427,32 @@ __device__ __forceinline__ void move_reference(State<S>& st, const float (*s)[S:
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
       m = fmaxf(m, st.m[nt][x]);
-      const bool first = st.m[nt][x] == -CUDART_INF_F;  // nothing has been added up
-      const float down = m == -CUDART_INF_F ? 0.f : st.m[nt][x] - m, by = exp2_fast(down), back = exp2_fast(-down);
+      const float down = m == -CUDART_INF_F ? 0.f : st.m[nt][x] - m;
+      by[nt][x] = exp2_fast(down);
+      back[nt][x] = st.m[nt][x] == -CUDART_INF_F ? 1.f : exp2_fast(-down);
       st.m[nt][x] = m;
-      st.l[nt][x] *= by;
+      st.l[nt][x] *= by[nt][x];
 #pragma unroll
-      for (int g = 0; g < (S::INT4 ? S::GROUPS : 1); ++g) st.centre[g][nt][x] *= by;
+      for (int g = 0; g < (S::INT4 ? S::GROUPS : 1); ++g) st.centre[g][nt][x] *= by[nt][x];
 #pragma unroll
-      for (int g = 0; g < S::GROUPS; ++g) {
-        if (!first) st.unit[g][nt][x] *= back;
-        beyond = beyond || !(st.unit[g][nt][x] <= FINEST);
-      }
+      for (int g = 0; g < S::GROUPS; ++g) beyond = beyond || !(st.unit[g][nt][x] * back[nt][x] <= FINEST);
     }
   }
-  if (__any_sync(ALL, beyond)) {
+  if (__any_sync(ALL, beyond)) {  // there is no finer one: what is left over shrinks after all
 #pragma unroll
     for (int g = 0; g < S::GROUPS; ++g)
 #pragma unroll
       for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float unit = st.unit[g][nt][x];
-          // (of an infinite one nothing is left: what has been added up is 2^-126 of what the tile brings, and less)
-          scale_outputs<S>(st, g, nt, x, unit <= FINEST ? 1.f : FINEST * inverse_fast(unit));
-          st.unit[g][nt][x] = fminf(unit, FINEST);
-        }
+        for (int x = 0; x < 2; ++x)
+          if (!(st.unit[g][nt][x] * back[nt][x] <= FINEST)) scale_outputs<S>(st, g, nt, x, by[nt][x] * FINEST * inverse_fast(st.unit[g][nt][x]));
   }
+#pragma unroll
+  for (int g = 0; g < S::GROUPS; ++g)
+#pragma unroll
+    for (int nt = 0; nt < S::NT; ++nt)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) st.unit[g][nt][x] = fminf(st.unit[g][nt][x] * back[nt][x], FINEST);
 }
 
 // Chooses the units of group g by the tile's largest products of a probability and a value scale. (Their exponents are what counts: two heads a word.)

@@ -563,8 +563,10 @@ def flash_dense_attn_with_quantized_kvcache_func(
     it (int8, e4m3 or 4 bits): ``query [B, Hq, D]`` (bf16 / fp16) attends to the ``seqused_k [B]`` first positions of its sequence, or to
     those of them that ``gather_kv_indices [B, topk]`` names (negative = masked). ``key / value`` are the codes ``[B, Sk, Hkv, ..]``, or
     pages ``[num_pages, page, Hkv, ..]`` + ``page_table [B, max_pages]``, ``key_scales / value_scales`` their scales. The result is that of
-    the values that codes and scales stand for, none of which is rounded on its way; the work is cut evenly over the GPU whatever
-    the lengths. ``head_dim`` a multiple of 16 up to 128; elements of queries, keys and values above 2^100 may count as infinite.
+    the values that codes and scales stand for, none of which is rounded on its way (a probability times a value's scale is, to 11 bits, for fp16
+    results to 22, in units that follow what keys weigh); the work is cut evenly over the GPU whatever the lengths. ``head_dim`` a multiple of 16 up
+    to 128, pages of 32, 64, 128 or 256 slots; elements of queries, keys and values above 2^100 may count as infinite, probabilities below 2^-120
+    of the largest as none.
 
     A row without any key is 0 with log-sum-exp ``-inf``. Keys on a page outside the pool are left out and reported by
     ``flash_sparse_attn.check_status()`` (status 3). Returns ``out [B, Hq, D]`` or ``(out, lse [B, Hq])``, without gradients; the

@@ -746,7 +746,8 @@ int fsa_kv_read_quantized(const FsaKvReadQuantArgs* args, void* stream);
  * statistics and sums are fp32; a sequence without keys gets zeros and a log-sum-exp of -inf. Keys on a page outside the pool are left
  * out and set the status word to 3. The work is cut evenly over the GPU whatever the lengths; pieces meet in `ws`, of
  * fsa_decode_quantized_workspace_bytes bytes, one per call under way. Pages of a power of two of slots, at least 32; rows of q on 16-byte
- * boundaries, of out on 4-byte ones. Elements of queries, keys and values above 2^100 may count as infinite.
+ * boundaries, of out on 4-byte ones. Elements of queries, keys and values above 2^100 may count as infinite, probabilities below 2^-120 of the
+ * largest as none.
  */
 typedef struct FsaQuantDecodeArgs {
   FsaQuantCache cache;

@@ -108,6 +108,22 @@ def test_a_key_far_above_the_others_without_a_value(kind, group, dtype, at):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,group", [("int8", 64), ("e4m3", 64), ("int4", 64), ("int4", 32)])
+@pytest.mark.parametrize("gap", [40, 46, 49, 50, 51, 52, 53, 54, 58])
+def test_a_key_far_above_small_values(kind, group, gap):
+    """Values of 2^-60 under a sink 2^40 to 2^58 above them, in the middle: products down to the end of fp32's normal numbers."""
+    d, g = 64, torch.Generator(device=DEV).manual_seed(gap)
+    q = torch.ones(BATCH, 2 * HEADS, d, device=DEV, dtype=torch.bfloat16)
+    scale = d**-0.5
+    xk, xv = (torch.randn(BATCH, HEADS, KEYS, d, generator=g, device=DEV) for _ in range(2))
+    xk *= 0.1
+    xk[:, :, 200] = gap * math.log(2) / (scale * d)
+    xv[:, :, 200] = 0
+    out, _, ref, _, _, reach = attend(q, xk, xv * 2.0**-60, kind, group, scale)
+    rows_close(out, ref, torch.bfloat16, score_error(d, reach))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("kind,group", [("int8", 64), ("e4m3", 64), ("int4", 64), ("int4", 32)])
 @pytest.mark.parametrize("up", [False, True])
