@@ -11,21 +11,21 @@
 // these products so far, so that what a key adds is held by what it weighs: a large b_j that nobody attends to, a key far above the others without a
 // value, or a group of small columns beside large ones take nothing from the rest. Running maxima, sums and outputs are fp32.
 //
-// Bound by memory: a key is read once, at 2 * 8 * (heads per KV head) operations a byte. (int8, 64 chats of up to 8192 tokens: 100.4 us, 5.3 TB/s, 0.82 of a
-// copy's rate; 4 bits, 8 x 100000: 112 us, 3.95 TB/s, where instructions bound it, 630 a tile; one sequence of 2001 keys 6.8 us.) What a warp does with a tile of 32 keys has to fit
+// Bound by memory: a key is read once, at 2 * 8 * (heads per KV head) operations a byte. (int8, 64 chats of up to 8192 tokens: 102 us, 5.2 TB/s, 0.80 of a
+// copy's rate; 4 bits, 8 x 100000: 112 us, 3.95 TB/s, where instructions bound it, 650 a tile; one sequence of 2001 keys 6.9 us.) What a warp does with a tile of 32 keys has to fit
 // into the time that its bytes take, so: products run transposed (keys or value columns on the M = 16 side of mma.m16n8k16, up to eight query
 // heads on the N = 8 side); columns of keys are dealt to lanes so that a lane's codes are neighbours in memory (the sum over columns has no order),
 // values are transposed on their way out of shared memory (ldmatrix on bytes); and codes become fp16 numbers by being taken for the bits of one:
 // n below 1024 in the low bits is the subnormal n 2^-24, which the matrix instructions multiply exactly. Codes are made positive for that (+128, of 4
 // bits they are), and what this adds is taken off where it cannot grow: of scores, a sum over columns, in the first accumulator (-128 2^-24 sum q);
 // of outputs, whose sums over keys run on and on, by a product of the same probabilities with the constant, tile by tile, once for the columns of a
-// group (once for each sixteen columns: 8 x 100000 keys in 4 bits 113.5 us, so 112).
+// group (once for each sixteen columns took 1.5 us more of 8 x 100000 keys in 4 bits).
 //
 // The work is one list of tiles (sequence, KV head and block of query heads, 32 keys), cut into equal pieces for all warps of the grid whatever the
 // lengths are. A warp streams its piece through a ring of its own in shared memory: TMA brings a tile's codes (cp.async, where positions are
 // chosen one by one), the warp's own mbarriers say when, and no barrier of the CTA is in the loop. Whole tiles that follow in a page (or in a contiguous
-// cache) are counted out when the first is sent, so that the walk and the page table are gone to once for all of them (8 x 100000 keys in 4 bits 112 us,
-// so 109). A piece that is a whole item is written out, the
+// cache) are counted out when the first is sent, so that the walk and the page table are gone to once for all of them (3 us of
+// 8 x 100000 keys in 4 bits). A piece that is a whole item is written out, the
 // others meet inside the CTA and then, for items that several CTAs share, in quant_merge_kernel. Calls of few
 // tiles are cut by items instead, each for a cluster of CTAs, and meet in its shared memory: one launch.
 #pragma once
@@ -48,8 +48,9 @@ constexpr int STATUS_WAIT = 1, STATUS_BAD_PAGE = 3;
 constexpr float LAG = 6.f;
 // Units of a probability times a value scale as fp16: where one is chosen, the largest product is brought to [2^8, 2^9), and products may grow to fp16's
 // end before it is chosen anew (2^6 of that are the lag's). What fp16 loses below its normal numbers is then at most 2^-33 of the largest for each key.
-// (One unit for all heads and groups, chosen by scales alone, costs 2 us less of 35 with four groups and nothing to speak of with one or two, but rounds
-// away what lies 2^-14 below a scale that nobody attends to.)
+// (One unit for all heads and groups, chosen by scales alone, rounds away what lies 2^-14 below a scale that nobody attends to. It takes 29.8 us where
+// this takes 32.3 of 37 ragged sequences with three groups, 146 and 160 of 8 x 100000 keys with four, 134.8 and 138.2 of 64 chats with 16 heads, and as
+// long with up to two groups and eight heads; divisions in place of inverse_fast, which each item comes to once, cost 3 to 7 us more.)
 constexpr int UNIT_TO = 8;
 constexpr float FINEST = 8.507059173023462e37f;  // 2^126
 
@@ -70,7 +71,8 @@ struct Shape {
   static constexpr int TILE_BYTES = TILE * RB, SCALE_BYTES = TILE * GROUPS * 4;
   // a stage: keys and values, and elsewhere (swizzled tiles begin where their pattern does) their scales and what the tile is
   static constexpr int CODES = 2 * TILE_BYTES, EXTRA = 2 * SCALE_BYTES + 128;
-  // (int8, 64 chats of up to 8192 tokens: 8 warps 109.5 us, 10 99.4, 12 107; 4 bits, 8 x 100000: 133, 124, 117)
+  // (When it was chosen, before the later steps: int8, 64 chats of up to 8192 tokens, 8 warps 109.5 us, 10 99.4, 12 107; 4 bits, 8 x 100000, 133, 124
+  // and 117.)
   static constexpr int WARPS = NT == 2 ? 8 : (RB == 128 ? 10 : 12), THREADS = 32 * WARPS;
   static constexpr int ALIGN = 8 * RB;             // the swizzle's pattern
   static constexpr int ROOM = 222 * 1024 / WARPS / ALIGN * ALIGN;
